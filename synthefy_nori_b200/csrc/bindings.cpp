@@ -150,6 +150,19 @@ void adamw_ema(torch::Tensor& p, const torch::Tensor& g, torch::Tensor& m, torch
                double wd, int64_t step, double ema_decay, double max_norm, double grad_scale, const c10::optional<torch::Tensor>& skip);
 std::vector<torch::Tensor> quantize_int8(const torch::Tensor& x);
 void dequantize_int8(const torch::Tensor& q, const torch::Tensor& scale, torch::Tensor& out);
+void newton_schulz(const torch::Tensor& g, torch::Tensor& out, int64_t steps, double eps, std::vector<double> coeffs,
+                   const torch::Tensor& status);
+void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mom,
+               const c10::optional<torch::Tensor>& ema, const torch::Tensor& table, std::vector<int64_t> groups,
+               double lr, double wd, double momentum, bool nesterov, int64_t steps, double eps,
+               std::vector<double> coeffs, int64_t adjust, const c10::optional<torch::Tensor>& norm_sq,
+               double max_norm, const c10::optional<torch::Tensor>& skip, double ema_decay,
+               const torch::Tensor& status);
+std::vector<torch::Tensor> layer_norm_fwd(const torch::Tensor& x, const c10::optional<torch::Tensor>& w,
+                                          const c10::optional<torch::Tensor>& b, double eps, bool out_f32);
+std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x, const torch::Tensor& mean,
+                                          const torch::Tensor& rstd, const c10::optional<torch::Tensor>& w,
+                                          bool weight_grad, bool bias_grad);
 }  // namespace nori
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -216,4 +229,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_ema", &nori::adamw_ema);
   m.def("quantize_int8", &nori::quantize_int8);
   m.def("dequantize_int8", &nori::dequantize_int8);
+  m.def("newton_schulz", &nori::newton_schulz);
+  m.def("muon_step", &nori::muon_step);
+  m.def("layer_norm_fwd", &nori::layer_norm_fwd);
+  m.def("layer_norm_bwd", &nori::layer_norm_bwd);
 }

@@ -1,0 +1,114 @@
+// Shared pieces of the LayerNorm forward and backward kernels.
+//
+//   y = (x - mean) rstd w + b,  mean and variance over a row's C values (two passes over
+//   registers: the variance sums squares of differences, never a difference of sums)
+//
+// A row belongs to TPR threads (8, a warp, or a CTA of 256), each holding VPL values in
+// chunks of VEC consecutive columns, so a row is read from memory once in each direction.
+#pragma once
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+
+#include "sm100.cuh"
+
+namespace nori {
+namespace ln {
+
+constexpr int kThreads = 256;
+constexpr int kMaxRegCols = 8192;  // 256 threads x 32 values
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) {
+  return __half2float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16(v);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// VEC consecutive values as one memory access (VEC * sizeof(T) is 2, 4, 8 or 16 bytes).
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  const Pack<T, VEC> u = *reinterpret_cast<const Pack<T, VEC>*>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = to_f32<T>(u.v[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+  Pack<T, VEC> u;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) u.v[i] = from_f32<T>(v[i]);
+  *reinterpret_cast<Pack<T, VEC>*>(p) = u;
+}
+
+// Sum over the TPR threads of a row; every one of them gets it. `sh` holds 8 floats per
+// reduction of a CTA-wide row (a fresh slot for each, so one barrier is enough).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* sh) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TPR > 32) {
+    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) v += sh[i];
+  }
+  return v;
+}
+
+// 16-byte accesses need rows that start on 16 bytes and a width that is a whole number of them.
+inline bool vec_ok(const void* p, int64_t ld, int64_t C, int64_t elem, int vec) {
+  return C % vec == 0 && (ld * elem) % (vec * elem) == 0 && reinterpret_cast<uintptr_t>(p) % (vec * elem) == 0;
+}
+
+inline const float* opt_vec(const c10::optional<torch::Tensor>& t, int64_t C, const torch::Device& dev,
+                            const char* what) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == C, what,
+              ": contiguous fp32 vector of the row width on x's device expected");
+  return t->data_ptr<float>();
+}
+
+// rows of `t`: [R, C] with unit column stride, any row stride
+inline void check_rows(const torch::Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2, what, ": a CUDA matrix [rows, cols] expected");
+  const auto s = t.scalar_type();
+  TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, what, ": fp32, bf16 or fp16 expected");
+  TORCH_CHECK(t.size(1) >= 1 && t.size(1) < (int64_t{1} << 30), what, ": 1 to 2^30 columns expected");
+  TORCH_CHECK(t.size(1) == 1 || t.stride(1) == 1, what, ": columns must be contiguous");
+  TORCH_CHECK(t.stride(0) >= 0, what, ": negative row stride");
+}
+
+}  // namespace ln
+}  // namespace nori

@@ -32,7 +32,21 @@ from torch.utils.checkpoint import checkpoint
 ACTIVATIONS = {"gelu": nn.GELU, "relu": nn.ReLU, "silu": nn.SiLU}
 
 
-class LayerNormMixedPrecision(nn.LayerNorm):
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` that runs the native kernel on CUDA tensors (``ops.layer_norm``; under
+    autocast the result is fp32, as torch's is, without a cast of the input before it)."""
+
+    def forward(self, x):
+        from synthefy_nori_b200 import ops
+
+        if (x.is_cuda and len(self.normalized_shape) == 1 and x.dim() and x.shape[-1] == self.normalized_shape[0]
+                and x.dtype in (torch.float32, torch.bfloat16, torch.float16) and ops.native_available()):
+            out = torch.float32 if torch.is_autocast_enabled("cuda") else None
+            return ops.layer_norm(x, self.weight, self.bias, self.eps, out)
+        return super().forward(x)
+
+
+class LayerNormMixedPrecision(LayerNorm):
     """LayerNorm that runs outside fp16 autocast for widths below 512."""
 
     def forward(self, x):

@@ -15,12 +15,12 @@ Scaling of the orthogonalised update (``adjust_lr``):
 - ``"nd"``: ``sqrt(max(rows, cols) / min(rows, cols))`` (the reference's ``MuonND``).
 Weight decay is decoupled: ``p *= 1 - lr * wd`` before the update.
 
-B200 layout: matrices are grouped by shape and each group is orthogonalised as one
-batch (``bmm`` over a stacked ``[G, m, n]`` tensor), so a step costs a handful of
-batched GEMMs per distinct shape instead of a chain of small launches per parameter.
-The AdamW part runs the fused ``adamw_ema`` kernel on one contiguous tail of the flat
-parameter buffer (Muon parameters are laid out first), and the EMA covers the whole
-buffer.
+B200 layout: Muon parameters come first in the flat buffer; on the GPU one
+``ops.muon_step`` call clips, updates the momentum, orthogonalises and applies every matrix
+and its EMA (``ops.MuonPlan`` holds their places), and the fused ``adamw_ema`` kernel does
+the contiguous tail.  The momentum is one buffer too, seen as a stacked ``[G, m, n]`` tensor
+per distinct shape (the checkpoint's form).  On the CPU each shape group is orthogonalised
+as one batch of ``bmm`` products in bf16.
 """
 
 from __future__ import annotations
@@ -48,7 +48,12 @@ def split_muon_adamw_params(named_parameters, *, include_embeddings: bool = Fals
 
 @torch.no_grad()
 def newton_schulz(G: torch.Tensor, steps: int = 5, eps: float = 1e-7) -> torch.Tensor:
-    """Batched quintic Newton-Schulz on ``G [..., m, n]`` (bf16 inside), returns G's dtype."""
+    """Batched quintic Newton-Schulz on ``G [..., m, n]``, returns G's dtype: the native
+    kernel on CUDA tensors, otherwise bf16 products."""
+    from synthefy_nori_b200 import ops
+
+    if G.is_cuda and ops.native_available() and steps >= 1 and G.dtype in (torch.float32, torch.bfloat16, torch.float16):
+        return ops.newton_schulz(G, steps, eps, NS_COEFFS)
     a, b, c = NS_COEFFS
     X = G.to(torch.bfloat16)
     X = X / (X.flatten(-2).norm(dim=-1)[..., None, None] + eps)
@@ -98,10 +103,24 @@ class HybridMuonAdamW:
         self.norm_sq = torch.zeros(1, device=device)
         self.step_count = 0
         groups = defaultdict(list)
-        for p in self.flat.params[: self.n_muon]:
-            groups[(p.numel() // p.shape[-1], p.shape[-1])].append(p)  # N-D: [prod(leading), last]
-        # momentum buffers stacked per shape group
-        self.groups = [(shape, ps, torch.zeros(len(ps), *shape, device=device)) for shape, ps in groups.items()]
+        for i, p in enumerate(self.flat.params[: self.n_muon]):
+            groups[(p.numel() // p.shape[-1], p.shape[-1])].append(i)  # N-D: [prod(leading), last]
+        # one momentum buffer, each shape group's part (64-aligned) seen as a stack
+        self.momentum_buf = torch.zeros(sum(-(-len(ix) * m * n // 64) * 64 for (m, n), ix in groups.items()), device=device)
+        self.groups, places, off = [], [], 0
+        for (m, n), ix in groups.items():
+            size = len(ix) * m * n
+            stack = self.momentum_buf[off : off + size].view(len(ix), m, n)
+            self.groups.append(((m, n), [self.flat.params[i] for i in ix], stack))
+            places += [((m, n), self.flat.offsets[i], off + j * m * n) for j, i in enumerate(ix)]
+            off += -(-size // 64) * 64
+        self.plan = None
+        if self.flat.data.is_cuda and ns_steps >= 1 and places:
+            from synthefy_nori_b200 import ops
+
+            if ops.native_available():
+                shapes, offsets, moffs = zip(*places)
+                self.plan = ops.MuonPlan(shapes, offsets, self.flat.data.device, moffs)
 
     @torch.no_grad()
     def step(self, grad_scale: float = 1.0, skip: torch.Tensor | None = None) -> None:
@@ -124,7 +143,16 @@ class HybridMuonAdamW:
                 self.norm_sq.copy_(grad.double().pow(2).sum().float().view(1))
             clip = (self.max_grad_norm / (self.norm_sq.sqrt() + 1e-6)).clamp(max=1.0)
         lr_m = self.muon_lr if self.muon_lr is not None else self.lr
-        for (m, n), ps, buf in self.groups:
+        native = grad.is_cuda and ops.native_available()
+        skip1 = None if skip is None else skip.reshape(1).float()
+        if self.plan is not None:
+            # a gradient norm that is not finite rejects the step, as in the AdamW kernel
+            ops.muon_step(self.plan, self.flat.data, grad, self.momentum_buf, lr=lr_m, wd=self.wd,
+                          momentum=self.momentum, nesterov=self.nesterov, steps=self.ns_steps, coeffs=NS_COEFFS,
+                          adjust_lr=self.adjust_lr, norm_sq=self.norm_sq if clip is not None else None,
+                          max_norm=self.max_grad_norm or 0.0, skip=skip1, ema=self.ema,
+                          ema_decay=self.ema_decay if self.ema_decay is not None else 0.0)
+        for (m, n), ps, buf in self.groups if self.plan is None else ():
             g = torch.stack([p.grad.reshape(m, n) for p in ps])
             if clip is not None:
                 g.mul_(clip)
@@ -146,18 +174,19 @@ class HybridMuonAdamW:
                     p.add_(upd[i].view_as(p) * (-lr_m * s * keep))
         if self.split < self.flat.numel:
             data, g = self.flat.data[self.split :], grad[self.split :]
-            if data.is_cuda and ops.native_available():
+            if native:
+                tail_ema = self.ema[self.split :] if self.plan is not None and self.ema is not None else None
                 ops.adamw_ema_step(data, g, self.m, self.v, lr=self.lr, beta1=self.betas[0], beta2=self.betas[1],
-                                   eps=self.eps, wd=self.wd, step=self.step_count, ema=None,
-                                   norm_sq=self.norm_sq if clip is not None else None, ema_decay=0.0,
-                                   max_norm=self.max_grad_norm or 0.0, grad_scale=1.0,
-                                   skip=None if skip is None else skip.reshape(1).float())
+                                   eps=self.eps, wd=self.wd, step=self.step_count, ema=tail_ema,
+                                   norm_sq=self.norm_sq if clip is not None else None,
+                                   ema_decay=self.ema_decay if tail_ema is not None else 0.0,
+                                   max_norm=self.max_grad_norm or 0.0, grad_scale=1.0, skip=skip1)
             else:
                 if keep is not None and float(keep) == 0.0:  # CPU path: a host decision costs nothing
                     pass
                 else:
                     self._adamw_torch(data, g * (clip if clip is not None else 1.0))
-        if self.ema is not None:
+        if self.ema is not None and self.plan is None:
             w = 1.0 - self.ema_decay
             self.ema.lerp_(self.flat.data, w if keep is None else keep * w)
 
