@@ -158,6 +158,7 @@ void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mo
                std::vector<double> coeffs, int64_t adjust, const c10::optional<torch::Tensor>& norm_sq,
                double max_norm, const c10::optional<torch::Tensor>& skip, double ema_decay,
                const torch::Tensor& status);
+bool muon_single_cta(int64_t rows, int64_t cols);
 std::vector<torch::Tensor> layer_norm_fwd(const torch::Tensor& x, const c10::optional<torch::Tensor>& w,
                                           const c10::optional<torch::Tensor>& b, double eps, bool out_f32);
 std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x, const torch::Tensor& mean,
@@ -231,6 +232,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dequantize_int8", &nori::dequantize_int8);
   m.def("newton_schulz", &nori::newton_schulz);
   m.def("muon_step", &nori::muon_step);
+  m.def("muon_single_cta", &nori::muon_single_cta);
   m.def("layer_norm_fwd", &nori::layer_norm_fwd);
   m.def("layer_norm_bwd", &nori::layer_norm_bwd);
 }

@@ -25,6 +25,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -102,6 +103,35 @@ __device__ __forceinline__ float load_src(const void* g, int64_t i) {
   return 0.f;
 }
 
+// Where one element of the result goes: a plain output tensor, or the weights.
+struct Sink {
+  int type;      // OutType
+  void* out;     // plain output of this matrix's batch, or null
+  int64_t base;  // first element of the matrix
+  float lr_o;    // kOutMuon: lr times the shape's factor
+};
+__device__ __forceinline__ void emit(const Sink& k, const StepArgs& s, int64_t e, float o) {
+  if (k.type == kOutMuon)
+    apply_update(s, k.base + e, o, k.lr_o);
+  else if (k.type == kOutF32)
+    static_cast<float*>(k.out)[k.base + e] = o;
+  else if (k.type == kOutBF16)
+    static_cast<__nv_bfloat16*>(k.out)[k.base + e] = __float2bfloat16(o);
+  else
+    static_cast<__half*>(k.out)[k.base + e] = __float2half_rn(o);
+}
+
+// 2^8 / norm as a product of two floats (it may lie outside fp32's range), and
+// f = norm / (norm + eps); all zero for a zero matrix.
+__device__ __forceinline__ void z_scale(double norm, double eps, float& s0, float& s1, float& f) {
+  int e = 0;
+  const double inv = norm > 0.0 ? frexp(static_cast<double>(kZScale) / norm, &e) : 0.0;
+  e = max(-250, min(250, e));
+  s0 = exp2f(static_cast<float>(e / 2));
+  s1 = static_cast<float>(inv * exp2(static_cast<double>(e - e / 2)));
+  f = static_cast<float>(norm > 0.0 ? norm / (norm + eps) : norm);
+}
+
 // ------------------------------------------------------------------ norm (and momentum)
 // Partial sums of squares of the update's input, one per (matrix, slice), in double: no fp32
 // gradient overflows or vanishes in its own norm.  With kSrcMuon the momentum buffer is
@@ -161,14 +191,9 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
   if (threadIdx.x == 0) {
     double v = 0.0;
     for (int i = 0; i < slices; ++i) v += partial[static_cast<int64_t>(mat) * slices + i];
-    const double norm = sqrt(v);
-    // the factor 2^8 / norm as a product of two floats: it may lie outside fp32's range
-    int e = 0;
-    const double inv = norm > 0.0 ? frexp(static_cast<double>(kZScale) / norm, &e) : 0.0;
-    e = max(-250, min(250, e));
-    scale[0] = exp2f(static_cast<float>(e / 2));
-    scale[1] = static_cast<float>(inv * exp2(static_cast<double>(e - e / 2)));
-    if (blockIdx.x == 0) f[mat] = static_cast<float>(norm > 0.0 ? norm / (norm + eps) : 0.0);
+    float fm;
+    z_scale(sqrt(v), eps, scale[0], scale[1], fm);
+    if (blockIdx.x == 0) f[mat] = fm;
   }
   __syncthreads();
   const float s0 = scale[0], s1 = scale[1];
@@ -510,24 +535,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             // lie, consecutive lanes being consecutive columns of a wide G
             const float xo = xi * p.a;
             const bool wide = p.rows < p.cols;
-            const float lr_o = p.out_type == kOutMuon ? p.s.lr * lr_factor(p.s.adjust, p.rows, p.cols) : 0.f;
-            const int64_t base = p.out_type == kOutMuon ? p.s.table[p.first + it.mat].off
-                                                        : static_cast<int64_t>(it.mat) * p.rows * p.cols;
-            auto emit = [&](int64_t e, float o) {
-              if (p.out_type == kOutMuon)
-                apply_update(p.s, base + e, o, lr_o);
-              else if (p.out_type == kOutF32)
-                static_cast<float*>(p.out)[base + e] = o;
-              else if (p.out_type == kOutBF16)
-                static_cast<__nv_bfloat16*>(p.out)[base + e] = __float2bfloat16(o);
-              else
-                static_cast<__half*>(p.out)[base + e] = __float2half_rn(o);
-            };
+            const Sink sink = {p.out_type, p.out,
+                               p.out_type == kOutMuon ? p.s.table[p.first + it.mat].off
+                                                      : static_cast<int64_t>(it.mat) * p.rows * p.cols,
+                               p.s.lr * lr_factor(p.s.adjust, p.rows, p.cols)};
             if (wide) {
               if (row_ok) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (col + i < p.m && i < left) emit(static_cast<int64_t>(col + i) * p.n + row, v[i] * xo);
+                  if (col + i < p.m && i < left) emit(sink, p.s, static_cast<int64_t>(col + i) * p.n + row, v[i] * xo);
               }
             } else {
 #pragma unroll
@@ -536,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int r0 = it.ti * 128 + q * 32;
               if (col + lane < p.m && lane < left) {
                 for (int rr = 0; rr < 32 && r0 + rr < p.n; ++rr)
-                  emit(static_cast<int64_t>(r0 + rr) * p.m + col + lane, tile[rr * 33 + lane]);
+                  emit(sink, p.s, static_cast<int64_t>(r0 + rr) * p.m + col + lane, tile[rr * 33 + lane]);
               }
               __syncwarp();
             }
@@ -556,6 +572,307 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ one matrix per CTA
+// Matrices that fit one SM run their whole step in one CTA, and a ragged set of them in one
+// launch.  The iterate stays in fp32 in tensor memory, where the update's MMAs add to it in
+// place (Z <- Z + Z C); its fp16 copy lies in shared memory once, as 128B-swizzled rows of 64
+// columns, and serves the Gram product (read MN-major, the sum running over rows) and the
+// update (read K-major).  A and then C take one 128-row tile beside it.  Nothing but the
+// matrix itself and its result crosses memory.  The chain of 3 x steps dependent products
+// bounds it: each is issued by one thread, waited for by all, read back by tcgen05.ld.
+constexpr int kSingleThreads = 512;
+constexpr int kSingleMaxTiles = 12;
+constexpr int kSingleStage = 16 * 32 * 17 * 4;  // one [32][17] tile per warp, in the operands' place
+
+struct Fit {
+  int n, m, mp, tiles, panels;
+  int smem, tmem;
+  bool ok;
+};
+__host__ __device__ inline Fit single_fit(int rows, int cols) {
+  Fit f;
+  f.n = rows > cols ? rows : cols;
+  f.m = rows > cols ? cols : rows;
+  f.mp = (f.m + 15) / 16 * 16;
+  f.tiles = (f.n + 127) / 128;
+  f.panels = (f.mp + 63) / 64;
+  f.smem = (f.tiles + 1) * f.panels * 16384;
+  if (f.smem < kSingleStage) f.smem = kSingleStage;
+  f.tmem = (f.tiles + 1) * f.mp;
+  f.ok = f.m <= 128 && f.tiles <= kSingleMaxTiles && f.smem <= 220 * 1024 && f.tmem <= 512;
+  return f;
+}
+
+struct SingleParams {
+  int first, rows, cols, steps;
+  double eps;
+  float a, b, c;
+  int out_type;
+  void* out;
+  StepArgs s;
+  int* status;
+};
+
+template <int SRC>
+__global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* __restrict__ g, SingleParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ uint64_t bar[1 + kSingleMaxTiles];
+  __shared__ double red[16];
+  __shared__ float sc[3];
+  __shared__ uint32_t tmem_slot;
+  if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
+  int rows = p.rows, cols = p.cols;
+  int64_t base, mbase = 0;
+  float clip = 1.f;
+  if constexpr (SRC == kSrcMuon) {
+    if (step_rejected(p.s)) return;
+    const Mat t = p.s.table[p.first + blockIdx.x];
+    rows = static_cast<int>(t.rows);
+    cols = static_cast<int>(t.cols);
+    base = t.off;
+    mbase = t.moff;
+    clip = clip_factor(p.s);
+  } else {
+    base = static_cast<int64_t>(blockIdx.x) * rows * cols;
+  }
+  const Fit fit = single_fit(rows, cols);
+  const bool wide = rows < cols;
+  const int n = fit.n, m = fit.m, mp = fit.mp, tiles = fit.tiles, chunks = mp / 16;
+  uint8_t* zh = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ac = zh + tiles * fit.panels * 16384;
+  const int zpanel = tiles * 16384;  // bytes between two 64-column panels of Z
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int q = warp & 3, grp = warp >> 2;  // lane quarter; 16-column chunks are dealt to 4 groups
+  float* stage = reinterpret_cast<float*>(zh) + warp * 32 * 17;
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < static_cast<uint32_t>(fit.tmem)) tmem_cols *= 2;
+  if (warp == 0) tmem_alloc(&tmem_slot, tmem_cols);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i <= kSingleMaxTiles; ++i) mbar_init(&bar[i], 1);
+    fence_barrier_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t tlane = tmem + (static_cast<uint32_t>(q * 32) << 16);
+
+  // the update's input, tall, raw, into tensor memory; its sum of squares
+  auto fetch = [&](int64_t e) -> float {
+    if constexpr (SRC == kSrcMuon) {
+      const float gi = p.s.grad[base + e] * clip;
+      const float mo = p.s.momentum * p.s.mom[mbase + e] + gi;
+      p.s.mom[mbase + e] = mo;
+      return p.s.nesterov ? gi + p.s.momentum * mo : mo;
+    } else {
+      return load_src<SRC>(g, base + e);
+    }
+  };
+  double acc = 0.0;
+  for (int u = grp; u < tiles * chunks; u += 4) {
+    const int t = u / chunks, c0 = u % chunks * 16, r0 = t * 128 + q * 32;
+    float v[16];
+    if (wide) {  // consecutive lanes are consecutive columns of G
+      const int r = r0 + lane;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = (r < n && c0 + i < m) ? fetch(static_cast<int64_t>(c0 + i) * n + r) : 0.f;
+    } else {     // two rows at a time, turned in shared memory
+      const int cl = lane & 15;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int rl = 2 * i + (lane >> 4);
+        v[i] = (r0 + rl < n && c0 + cl < m) ? fetch(static_cast<int64_t>(r0 + rl) * m + c0 + cl) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) stage[(2 * i + (lane >> 4)) * 17 + cl] = v[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = stage[lane * 17 + i];
+      __syncwarp();
+    }
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      acc += static_cast<double>(v[i]) * v[i];
+      r[i] = __float_as_uint(v[i]);
+    }
+    tmem_st16(tlane + t * mp + c0, r);
+  }
+  tmem_wait_st();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0) red[warp] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double v = 0.0;
+    for (int i = 0; i < 16; ++i) v += red[i];
+    z_scale(sqrt(v), p.eps, sc[0], sc[1], sc[2]);
+  }
+  __syncthreads();
+
+  // 16 columns of row r as fp16 into the swizzled rows at `panel0`
+  auto put16 = [&](uint8_t* panel0, int pstride, int r, int c0, const float* v) {
+    uint8_t* d = panel0 + (c0 >> 6) * pstride + r * 128;
+    const int k = (c0 & 63) >> 3, x = r & 7;
+    *reinterpret_cast<uint4*>(d + ((k ^ x) << 4)) = pack8(v);
+    *reinterpret_cast<uint4*>(d + (((k + 1) ^ x) << 4)) = pack8(v + 8);
+  };
+  auto get16 = [&](const uint8_t* panel0, int pstride, int r, int c0, float* v) {
+    const uint8_t* d = panel0 + (c0 >> 6) * pstride + r * 128;
+    const int k = (c0 & 63) >> 3, x = r & 7;
+    unpack8(*reinterpret_cast<const uint4*>(d + ((k ^ x) << 4)), v);
+    unpack8(*reinterpret_cast<const uint4*>(d + (((k + 1) ^ x) << 4)), v + 8);
+  };
+  auto ld16 = [&](uint32_t addr, float* v) {
+    uint32_t r[16];
+    tmem_ld16(addr, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  };
+  for (int u = grp; u < tiles * chunks; u += 4) {
+    const int t = u / chunks, c0 = u % chunks * 16;
+    float v[16];
+    ld16(tlane + t * mp + c0, v);
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = v[i] * sc[0] * sc[1];
+      r[i] = __float_as_uint(v[i]);
+    }
+    tmem_st16(tlane + t * mp + c0, r);
+    put16(zh, zpanel, t * 128 + q * 32 + lane, c0, v);
+  }
+  tmem_wait_st();
+  float xi = sc[2] * (1.f / kZScale);
+
+  const uint32_t zs = smem_u32(zh), as = smem_u32(ac);
+  const uint32_t d_a = tmem + tiles * mp;  // A's (and A^2's) accumulator
+  const uint32_t idesc_mn = idesc_f16(mp, true), idesc_k = idesc_f16(mp, false);
+  // with one panel the MMA's rows 64..127 are padding: let them read the next rows
+  const uint32_t lbo = fit.panels == 2 ? zpanel : 1024;
+  const int row = q * 32 + lane;
+  const Sink sink = {p.out_type, p.out, base, p.s.lr * lr_factor(p.s.adjust, rows, cols)};
+  uint32_t ph = 0;
+  bool ok = true;
+  for (int it = 0; it < p.steps; ++it) {
+    const bool last = it == p.steps - 1;
+    // A = xi^2 Z^T Z
+    tc_fence_before();
+    fence_proxy_async_smem();
+    if (__syncthreads_or(!ok)) break;
+    if (warp == 0 && elect_one()) {
+      tc_fence_after();
+      for (int k = 0; k < (n + 15) / 16; ++k) {
+        const uint64_t d = umma_smem_desc(zs + k * 2048, lbo, 1024, 2);
+        umma_bf16_ss(d_a, d, d, idesc_mn, k > 0 ? 1u : 0u);
+      }
+      umma_commit(&bar[0]);
+    }
+    __syncwarp();
+    ok = mbar_wait_warp(&bar[0], ph, p.status, kTimeoutEpilogue, nullptr);
+    ph ^= 1;
+    tc_fence_after();
+    for (int c = grp; c < chunks; c += 4) {
+      float v[16];
+      ld16(tlane + tiles * mp + c * 16, v);
+      const float x2 = xi * xi;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = (row < m && c * 16 + i < m) ? v[i] * x2 : 0.f;
+      put16(ac, 16384, row, c * 16, v);
+    }
+    // C = (b A + c A^2) / a
+    tc_fence_before();
+    fence_proxy_async_smem();
+    if (__syncthreads_or(!ok)) break;
+    if (warp == 0 && elect_one()) {
+      tc_fence_after();
+      for (int k = 0; k < chunks; ++k) {
+        const uint64_t d = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
+        umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
+      }
+      umma_commit(&bar[0]);
+    }
+    __syncwarp();
+    ok = mbar_wait_warp(&bar[0], ph, p.status, kTimeoutEpilogue, nullptr);
+    ph ^= 1;
+    tc_fence_after();
+    for (int c = grp; c < chunks; c += 4) {
+      float v[16], s[16];
+      ld16(tlane + tiles * mp + c * 16, v);
+      get16(ac, 16384, row, c * 16, s);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = (row < m && c * 16 + i < m) ? (p.b * s[i] + p.c * v[i]) / p.a : 0.f;
+      put16(ac, 16384, row, c * 16, v);
+    }
+    // Z += Z C, tile by tile
+    tc_fence_before();
+    fence_proxy_async_smem();
+    if (__syncthreads_or(!ok)) break;
+    if (warp == 0 && elect_one()) {
+      tc_fence_after();
+      for (int t = 0; t < tiles; ++t) {
+        for (int k = 0; k < chunks; ++k) {
+          const uint64_t da = umma_desc_kmajor_sw128(zs + (k >> 2) * zpanel + t * 16384 + (k & 3) * 32);
+          const uint64_t db = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
+          umma_bf16_ss(tmem + t * mp, da, db, idesc_k, 1u);
+        }
+        umma_commit(&bar[1 + t]);
+      }
+    }
+    __syncwarp();
+    if (last) {  // the operands' place is free once the last tile is done
+      ok = mbar_wait_warp(&bar[tiles], it & 1, p.status, kTimeoutEpilogue, nullptr);
+      if (!ok) break;
+      tc_fence_after();
+    }
+    for (int u = grp, seen = -1; u < tiles * chunks; u += 4) {
+      const int t = u / chunks, c0 = u % chunks * 16, r0 = t * 128 + q * 32;
+      if (!last && t > seen) {
+        ok = ok && mbar_wait_warp(&bar[1 + t], it & 1, p.status, kTimeoutEpilogue, nullptr);
+        seen = t;
+        tc_fence_after();
+      }
+      float v[16];
+      ld16(tlane + t * mp + c0, v);
+      if (!last) {
+        put16(zh, zpanel, r0 + lane, c0, v);
+        continue;
+      }
+      const float xo = xi * p.a;
+      if (wide) {
+        if (r0 + lane < n) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c0 + i < m) emit(sink, p.s, static_cast<int64_t>(c0 + i) * n + r0 + lane, v[i] * xo);
+        }
+      } else {
+        const int cl = lane & 15;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) stage[lane * 17 + i] = v[i] * xo;
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int rl = 2 * i + (lane >> 4);
+          if (r0 + rl < n && c0 + cl < m)
+            emit(sink, p.s, static_cast<int64_t>(r0 + rl) * m + c0 + cl, stage[rl * 17 + cl]);
+        }
+        __syncwarp();
+      }
+    }
+    xi *= p.a;
+  }
+  // every product was waited for (or a wait has run out)
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 
@@ -657,6 +974,32 @@ static void run_group(int src, const void* g, int out_type, void* out, const Ste
   }
 }
 
+// Matrices first .. first + count of a set that all fit one CTA; `smem` is the largest need.
+static void run_single(int src, const void* g, int out_type, void* out, const StepArgs& s, int64_t first,
+                       int64_t count, int rows, int cols, int smem, const Coeffs& k, const torch::Tensor& status) {
+  SingleParams p{};
+  p.first = static_cast<int>(first);
+  p.rows = rows;
+  p.cols = cols;
+  p.steps = k.steps;
+  p.eps = k.eps;
+  p.a = k.a;
+  p.b = k.b;
+  p.c = k.c;
+  p.out_type = out_type;
+  p.out = out;
+  p.s = s;
+  p.status = status.data_ptr<int>();
+  auto kernel = src == kSrcF32    ? single_kernel<kSrcF32>
+                : src == kSrcBF16 ? single_kernel<kSrcBF16>
+                : src == kSrcF16  ? single_kernel<kSrcF16>
+                                  : single_kernel<kSrcMuon>;
+  smem += 1024;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 221 * 1024));
+  kernel<<<static_cast<unsigned>(count), kSingleThreads, smem, at::cuda::getCurrentCUDAStream()>>>(g, p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
 constexpr int64_t kMaxDim = 1 << 20, kMaxBatch = 65535;
 
 static Coeffs make_coeffs(int64_t steps, double eps, const std::vector<double>& c, const char* who) {
@@ -694,6 +1037,13 @@ void newton_schulz(const torch::Tensor& g, torch::Tensor& out, int64_t steps, do
   if (g.numel() == 0) return;
   const at::cuda::CUDAGuard guard(g.device());
   const int64_t numel = g.size(1) * g.size(2);
+  const Fit fit = single_fit(static_cast<int>(g.size(1)), static_cast<int>(g.size(2)));
+  if (fit.ok) {
+    TORCH_CHECK(g.size(0) <= INT_MAX, "newton_schulz: at most 2^31 - 1 matrices");
+    run_single(src, g.data_ptr(), dst, out.data_ptr(), StepArgs{}, 0, g.size(0), static_cast<int>(g.size(1)),
+               static_cast<int>(g.size(2)), fit.smem, k, status);
+    return;
+  }
   for (int64_t b0 = 0; b0 < g.size(0); b0 += kMaxBatch) {
     const int nb = static_cast<int>(std::min(kMaxBatch, g.size(0) - b0));
     run_group(src, static_cast<const char*>(g.data_ptr()) + b0 * numel * g.element_size(), dst,
@@ -742,11 +1092,35 @@ void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mo
   s.nesterov = nesterov ? 1 : 0;
   s.adjust = static_cast<int>(adjust);
   const at::cuda::CUDAGuard guard(data.device());
-  for (size_t i = 0; i + 3 < groups.size(); i += 4)
+  // runs of groups whose matrices fit one CTA go in one launch
+  int64_t run_first = 0, run_count = 0;
+  int run_smem = 0;
+  auto flush = [&]() {
+    if (run_count > 0)
+      run_single(kSrcMuon, nullptr, kOutMuon, nullptr, s, run_first, run_count, 0, 0, run_smem, k, status);
+    run_count = 0;
+    run_smem = 0;
+  };
+  for (size_t i = 0; i + 3 < groups.size(); i += 4) {
+    const Fit fit = single_fit(static_cast<int>(groups[i + 2]), static_cast<int>(groups[i + 3]));
+    if (fit.ok) {
+      if (run_count == 0) run_first = groups[i];
+      run_count += groups[i + 1];
+      run_smem = std::max(run_smem, fit.smem);
+      continue;
+    }
+    flush();
     for (int64_t b0 = 0; b0 < groups[i + 1]; b0 += kMaxBatch)
       run_group(kSrcMuon, nullptr, kOutMuon, nullptr, s, static_cast<int>(groups[i] + b0),
                 static_cast<int>(std::min(kMaxBatch, groups[i + 1] - b0)), static_cast<int>(groups[i + 2]),
                 static_cast<int>(groups[i + 3]), k, status, data.options());
+  }
+  flush();
+}
+
+// Whether a matrix of this shape runs its whole step in one CTA.
+bool muon_single_cta(int64_t rows, int64_t cols) {
+  return muon::single_fit(static_cast<int>(rows), static_cast<int>(cols)).ok;
 }
 
 }  // namespace nori

@@ -79,8 +79,10 @@ class MuonPlan:
         by_shape: dict = {}
         for i, s in enumerate(shapes):
             by_shape.setdefault(s, []).append(i)
+        # shapes that need a whole GPU first, then the ones of a single CTA in one run, largest first
+        single = _lib().muon_single_cta
         rows, self.groups = [], []
-        for (r, c), idx in by_shape.items():
+        for (r, c), idx in sorted(by_shape.items(), key=lambda kv: (single(*kv[0]), -kv[0][0] * kv[0][1])):
             self.groups += [len(rows), len(idx), r, c]
             rows += [[offsets[i], moff[i], r, c] for i in idx]
         self.count = len(rows)
