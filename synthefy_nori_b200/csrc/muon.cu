@@ -85,16 +85,6 @@ __device__ __forceinline__ float lr_factor(int adjust, int rows, int cols) {
   return sqrtf(fmaxf(r, c) / fminf(r, c));
 }
 
-// weight (and average) of one element, given its orthogonalised update
-__device__ __forceinline__ void apply_update(const StepArgs& s, int64_t i, float o, float lr_o) {
-  const float p = s.data[i] * (1.f - s.lr * s.wd) - lr_o * o;
-  s.data[i] = p;
-  if (s.ema != nullptr) {
-    const float e = s.ema[i];
-    s.ema[i] = e + s.ema_w * (p - e);
-  }
-}
-
 template <int SRC>
 __device__ __forceinline__ float load_src(const void* g, int64_t i) {
   if constexpr (SRC == kSrcF32) return static_cast<const float*>(g)[i];
@@ -110,15 +100,68 @@ struct Sink {
   int64_t base;  // first element of the matrix
   float lr_o;    // kOutMuon: lr times the shape's factor
 };
-__device__ __forceinline__ void emit(const Sink& k, const StepArgs& s, int64_t e, float o) {
-  if (k.type == kOutMuon)
-    apply_update(s, k.base + e, o, k.lr_o);
-  else if (k.type == kOutF32)
-    static_cast<float*>(k.out)[k.base + e] = o;
-  else if (k.type == kOutBF16)
-    static_cast<__nv_bfloat16*>(k.out)[k.base + e] = __float2bfloat16(o);
-  else
-    static_cast<__half*>(k.out)[k.base + e] = __float2half_rn(o);
+// Values o[0 .. cnt) go to elements e0, e0 + stride, ...: every load of the weights is issued
+// before the first store (the compiler may not move one past the other), so a thread waits
+// for memory once, not once per element.
+template <int N>
+__device__ __forceinline__ void emit(const Sink& k, const StepArgs& s, int64_t e0, int64_t stride, int cnt,
+                                     const float* o) {
+  e0 += k.base;
+  if (k.type == kOutMuon) {
+    float p[N], e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = i < cnt ? s.data[e0 + i * stride] : 0.f;
+    if (s.ema != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = i < cnt ? s.ema[e0 + i * stride] : 0.f;
+    }
+    const float keep = 1.f - s.lr * s.wd;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      p[i] = p[i] * keep - k.lr_o * o[i];
+      if (i < cnt) s.data[e0 + i * stride] = p[i];
+    }
+    if (s.ema != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < cnt) s.ema[e0 + i * stride] = e[i] + s.ema_w * (p[i] - e[i]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i < cnt) {
+      if (k.type == kOutF32)
+        static_cast<float*>(k.out)[e0 + i * stride] = o[i];
+      else if (k.type == kOutBF16)
+        static_cast<__nv_bfloat16*>(k.out)[e0 + i * stride] = __float2bfloat16(o[i]);
+      else
+        static_cast<__half*>(k.out)[e0 + i * stride] = __float2half_rn(o[i]);
+    }
+  }
+}
+
+// The update's input at elements e0, e0 + stride, ... (the momentum brought up to date on the
+// way), loads before stores as in emit.
+template <int SRC, int N>
+__device__ __forceinline__ void fetch(const void* g, const StepArgs& s, int64_t base, int64_t mbase, float clip,
+                                      int64_t e0, int64_t stride, int cnt, float* v) {
+  if constexpr (SRC == kSrcMuon) {
+    float m[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < cnt ? s.grad[base + e0 + i * stride] * clip : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m[i] = i < cnt ? s.mom[mbase + e0 + i * stride] : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      m[i] = s.momentum * m[i] + v[i];
+      if (i < cnt) s.mom[mbase + e0 + i * stride] = m[i];
+      v[i] = s.nesterov ? v[i] + s.momentum * m[i] : m[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < cnt ? load_src<SRC>(g, base + e0 + i * stride) : 0.f;
+  }
 }
 
 // 2^8 / norm as a product of two floats (it may lie outside fp32's range), and
@@ -540,21 +583,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                       : static_cast<int64_t>(it.mat) * p.rows * p.cols,
                                p.s.lr * lr_factor(p.s.adjust, p.rows, p.cols)};
             if (wide) {
-              if (row_ok) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (col + i < p.m && i < left) emit(sink, p.s, static_cast<int64_t>(col + i) * p.n + row, v[i] * xo);
-              }
+              for (int i = 0; i < 32; ++i) v[i] *= xo;
+              const int cnt = row_ok ? min(left, p.m - col) : 0;
+              emit<16>(sink, p.s, static_cast<int64_t>(col) * p.n + row, p.n, cnt, v);
+              emit<16>(sink, p.s, static_cast<int64_t>(col + 16) * p.n + row, p.n, cnt - 16, v + 16);
             } else {
 #pragma unroll
               for (int i = 0; i < 32; ++i) tile[lane * 33 + i] = v[i] * xo;
               __syncwarp();
               const int r0 = it.ti * 128 + q * 32;
-              if (col + lane < p.m && lane < left) {
-                for (int rr = 0; rr < 32 && r0 + rr < p.n; ++rr)
-                  emit(sink, p.s, static_cast<int64_t>(r0 + rr) * p.m + col + lane, tile[rr * 33 + lane]);
-              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = tile[i * 33 + lane];
               __syncwarp();
+              const int cnt = col + lane < p.m && lane < left ? p.n - r0 : 0;
+              emit<16>(sink, p.s, static_cast<int64_t>(r0) * p.m + col + lane, p.m, cnt, v);
+              emit<16>(sink, p.s, static_cast<int64_t>(r0 + 16) * p.m + col + lane, p.m, cnt - 16, v + 16);
             }
           }
         }
@@ -662,31 +706,17 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   const uint32_t tlane = tmem + (static_cast<uint32_t>(q * 32) << 16);
 
   // the update's input, tall, raw, into tensor memory; its sum of squares
-  auto fetch = [&](int64_t e) -> float {
-    if constexpr (SRC == kSrcMuon) {
-      const float gi = p.s.grad[base + e] * clip;
-      const float mo = p.s.momentum * p.s.mom[mbase + e] + gi;
-      p.s.mom[mbase + e] = mo;
-      return p.s.nesterov ? gi + p.s.momentum * mo : mo;
-    } else {
-      return load_src<SRC>(g, base + e);
-    }
-  };
   double acc = 0.0;
   for (int u = grp; u < tiles * chunks; u += 4) {
     const int t = u / chunks, c0 = u % chunks * 16, r0 = t * 128 + q * 32;
     float v[16];
+    const int cl = lane & 15, rl = lane >> 4;
     if (wide) {  // consecutive lanes are consecutive columns of G
-      const int r = r0 + lane;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = (r < n && c0 + i < m) ? fetch(static_cast<int64_t>(c0 + i) * n + r) : 0.f;
+      fetch<SRC, 16>(g, p.s, base, mbase, clip, static_cast<int64_t>(c0) * n + r0 + lane, n,
+                     r0 + lane < n ? m - c0 : 0, v);
     } else {     // two rows at a time, turned in shared memory
-      const int cl = lane & 15;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int rl = 2 * i + (lane >> 4);
-        v[i] = (r0 + rl < n && c0 + cl < m) ? fetch(static_cast<int64_t>(r0 + rl) * m + c0 + cl) : 0.f;
-      }
+      fetch<SRC, 16>(g, p.s, base, mbase, clip, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
+                     c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) stage[(2 * i + (lane >> 4)) * 17 + cl] = v[i];
       __syncwarp();
@@ -845,24 +875,20 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
         continue;
       }
       const float xo = xi * p.a;
+      const int cl = lane & 15, rl = lane >> 4;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= xo;
       if (wide) {
-        if (r0 + lane < n) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c0 + i < m) emit(sink, p.s, static_cast<int64_t>(c0 + i) * n + r0 + lane, v[i] * xo);
-        }
+        emit<16>(sink, p.s, static_cast<int64_t>(c0) * n + r0 + lane, n, r0 + lane < n ? m - c0 : 0, v);
       } else {
-        const int cl = lane & 15;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) stage[lane * 17 + i] = v[i] * xo;
+        for (int i = 0; i < 16; ++i) stage[lane * 17 + i] = v[i];
         __syncwarp();
-#pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-          const int rl = 2 * i + (lane >> 4);
-          if (r0 + rl < n && c0 + cl < m)
-            emit(sink, p.s, static_cast<int64_t>(r0 + rl) * m + c0 + cl, stage[rl * 17 + cl]);
-        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = stage[(2 * i + rl) * 17 + cl];
         __syncwarp();
+        emit<16>(sink, p.s, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
+                 c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
       }
     }
     xi *= p.a;
