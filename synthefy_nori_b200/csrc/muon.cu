@@ -54,6 +54,11 @@ struct Mat {
   int64_t rows, cols;
 };
 
+struct Coeffs {
+  int steps;
+  float eps, a, ba, ca;  // the coefficients a, b / a, c / a
+};
+
 struct StepArgs {
   float* data;
   const float* grad;
@@ -164,15 +169,22 @@ __device__ __forceinline__ void fetch(const void* g, const StepArgs& s, int64_t 
   }
 }
 
-// 2^8 / norm as a product of two floats (it may lie outside fp32's range), and
-// f = norm / (norm + eps); all zero for a zero matrix.
-__device__ __forceinline__ void z_scale(double norm, double eps, float& s0, float& s1, float& f) {
-  int e = 0;
-  const double inv = norm > 0.0 ? frexp(static_cast<double>(kZScale) / norm, &e) : 0.0;
-  e = max(-250, min(250, e));
-  s0 = exp2f(static_cast<float>(e / 2));
-  s1 = static_cast<float>(inv * exp2(static_cast<double>(e - e / 2)));
-  f = static_cast<float>(norm > 0.0 ? norm / (norm + eps) : norm);
+// From a matrix's sum of squares v: 2^8 / norm as a product of two floats (it may lie outside
+// fp32's range; powers of two from the exponent, the rest is in [2^7, 2^8]), and
+// f = norm / (norm + eps).  All zero for a zero matrix; f is NaN where the sum is not finite.
+__device__ __forceinline__ void z_scale(double v, float eps, float& s0, float& s1, float& f) {
+  if (!(v > 0.0) || !(v < INFINITY)) {
+    s0 = s1 = 0.f;
+    f = v == 0.0 ? 0.f : NAN;
+    return;
+  }
+  const int k = (((__double2hiint(v) >> 20) & 0x7ff) - 1023) >> 1;  // norm is in [2^k, 2^(k+1))
+  const float r = rsqrtf(static_cast<float>(v * __hiloint2double((1023 - 2 * k) << 20, 0)));  // 2^k / norm
+  const int k0 = k / 2, k1 = k - k0;
+  s0 = __int_as_float((127 - k0) << 23);
+  const float t = __int_as_float((127 - k1) << 23) * r;
+  s1 = kZScale * t;
+  f = 1.f / (1.f + eps * s0 * t);
 }
 
 // ------------------------------------------------------------------ norm (and momentum)
@@ -223,7 +235,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const void* __restrict__ g, S
 template <int SRC>
 __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, StepArgs s, int first, int rows,
                                                     int cols, int slices, const double* __restrict__ partial,
-                                                    double eps, __half* __restrict__ zh, __half* __restrict__ zl,
+                                                    float eps, __half* __restrict__ zh, __half* __restrict__ zl,
                                                     int ldz, float* __restrict__ f) {
   if constexpr (SRC == kSrcMuon) {
     if (step_rejected(s)) return;
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
     double v = 0.0;
     for (int i = 0; i < slices; ++i) v += partial[static_cast<int64_t>(mat) * slices + i];
     float fm;
-    z_scale(sqrt(v), eps, scale[0], scale[1], fm);
+    z_scale(v, eps, scale[0], scale[1], fm);
     if (blockIdx.x == 0) f[mat] = fm;
   }
   __syncthreads();
@@ -289,7 +301,7 @@ struct NsParams {
   int n, m, ldz, batch;
   int bn;             // column tile of the update
   int phase, it, steps;
-  float a, b, c;
+  float a, ba, ca;    // the coefficients a, b / a, c / a
   __half* zh_out;     // the other Z (high) buffer
   const __half* zh;   // this step's
   __half* zl;         // updated in place
@@ -529,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float s[8];
                 unpack8(*reinterpret_cast<const uint4*>(p.A + at + 8 * j), s);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[8 * j + i] = (p.b * s[i] + p.c * v[8 * j + i]) / p.a;
+                for (int i = 0; i < 8; ++i) v[8 * j + i] = p.ba * s[i] + p.ca * v[8 * j + i];
               }
             }
           }
@@ -651,9 +663,8 @@ __host__ __device__ inline Fit single_fit(int rows, int cols) {
 }
 
 struct SingleParams {
-  int first, rows, cols, steps;
-  double eps;
-  float a, b, c;
+  int first, rows, cols;
+  Coeffs k;
   int out_type;
   void* out;
   StepArgs s;
@@ -665,7 +676,6 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ uint64_t bar[1 + kSingleMaxTiles];
   __shared__ double red[16];
-  __shared__ float sc[3];
   __shared__ uint32_t tmem_slot;
   if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
   int rows = p.rows, cols = p.cols;
@@ -704,21 +714,38 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const uint32_t tlane = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  const int cl = lane & 15, rl = lane >> 4;  // a 16-column chunk in memory: two rows per warp access
+  // this group's first (tile, chunk), and the one after
+  auto first = [&](int& t, int& c) {
+    t = 0;
+    c = grp;
+    while (c >= chunks) {
+      c -= chunks;
+      ++t;
+    }
+  };
+  auto next = [&](int& t, int& c) {
+    c += 4;
+    while (c >= chunks) {
+      c -= chunks;
+      ++t;
+    }
+  };
 
   // the update's input, tall, raw, into tensor memory; its sum of squares
   double acc = 0.0;
-  for (int u = grp; u < tiles * chunks; u += 4) {
-    const int t = u / chunks, c0 = u % chunks * 16, r0 = t * 128 + q * 32;
+  int t, c;
+  for (first(t, c); t < tiles; next(t, c)) {
+    const int c0 = c * 16, r0 = t * 128 + q * 32;
     float v[16];
-    const int cl = lane & 15, rl = lane >> 4;
     if (wide) {  // consecutive lanes are consecutive columns of G
       fetch<SRC, 16>(g, p.s, base, mbase, clip, static_cast<int64_t>(c0) * n + r0 + lane, n,
                      r0 + lane < n ? m - c0 : 0, v);
-    } else {     // two rows at a time, turned in shared memory
+    } else {     // turned in shared memory
       fetch<SRC, 16>(g, p.s, base, mbase, clip, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
                      c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) stage[(2 * i + (lane >> 4)) * 17 + cl] = v[i];
+      for (int i = 0; i < 16; ++i) stage[(2 * i + rl) * 17 + cl] = v[i];
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = stage[lane * 17 + i];
@@ -737,14 +764,14 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
   if (lane == 0) red[warp] = acc;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double v = 0.0;
-    for (int i = 0; i < 16; ++i) v += red[i];
-    z_scale(sqrt(v), p.eps, sc[0], sc[1], sc[2]);
-  }
-  __syncthreads();
+  acc = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc += red[i];
+  float s0, s1, xi;
+  z_scale(acc, p.k.eps, s0, s1, xi);
+  xi *= 1.f / kZScale;
 
-  // 16 columns of row r as fp16 into the swizzled rows at `panel0`
+  // 16 columns of row r as fp16 in the swizzled rows at `panel0`
   auto put16 = [&](uint8_t* panel0, int pstride, int r, int c0, const float* v) {
     uint8_t* d = panel0 + (c0 >> 6) * pstride + r * 128;
     const int k = (c0 & 63) >> 3, x = r & 7;
@@ -764,21 +791,6 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
   };
-  for (int u = grp; u < tiles * chunks; u += 4) {
-    const int t = u / chunks, c0 = u % chunks * 16;
-    float v[16];
-    ld16(tlane + t * mp + c0, v);
-    uint32_t r[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      v[i] = v[i] * sc[0] * sc[1];
-      r[i] = __float_as_uint(v[i]);
-    }
-    tmem_st16(tlane + t * mp + c0, r);
-    put16(zh, zpanel, t * 128 + q * 32 + lane, c0, v);
-  }
-  tmem_wait_st();
-  float xi = sc[2] * (1.f / kZScale);
 
   const uint32_t zs = smem_u32(zh), as = smem_u32(ac);
   const uint32_t d_a = tmem + tiles * mp;  // A's (and A^2's) accumulator
@@ -787,111 +799,132 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   const uint32_t lbo = fit.panels == 2 ? zpanel : 1024;
   const int row = q * 32 + lane;
   const Sink sink = {p.out_type, p.out, base, p.s.lr * lr_factor(p.s.adjust, rows, cols)};
-  uint32_t ph = 0;
   bool ok = true;
-  for (int it = 0; it < p.steps; ++it) {
-    const bool last = it == p.steps - 1;
-    // A = xi^2 Z^T Z
+  // All that the threads wrote to shared memory is there for the MMAs that one thread issues
+  // next; false once a wait of any thread has run out.
+  auto publish = [&]() -> bool {
     tc_fence_before();
     fence_proxy_async_smem();
-    if (__syncthreads_or(!ok)) break;
+    ok = !__syncthreads_or(!ok);
+    tc_fence_after();
+    return ok;
+  };
+  // A += Z^T Z over the rows of tile t
+  auto gram = [&](int t) {
     if (warp == 0 && elect_one()) {
-      tc_fence_after();
-      for (int k = 0; k < (n + 15) / 16; ++k) {
-        const uint64_t d = umma_smem_desc(zs + k * 2048, lbo, 1024, 2);
-        umma_bf16_ss(d_a, d, d, idesc_mn, k > 0 ? 1u : 0u);
+      const int k1 = min(8, (n - t * 128 + 15) / 16);
+      for (int k = 0; k < k1; ++k) {
+        const uint64_t d = umma_smem_desc(zs + (t * 8 + k) * 2048, lbo, 1024, 2);
+        umma_bf16_ss(d_a, d, d, idesc_mn, t > 0 || k > 0 ? 1u : 0u);
       }
-      umma_commit(&bar[0]);
+      if (t == tiles - 1) umma_commit(&bar[0]);
     }
     __syncwarp();
-    ok = mbar_wait_warp(&bar[0], ph, p.status, kTimeoutEpilogue, nullptr);
-    ph ^= 1;
-    tc_fence_after();
-    for (int c = grp; c < chunks; c += 4) {
-      float v[16];
-      ld16(tlane + tiles * mp + c * 16, v);
+  };
+
+  // the fp16 copy of Z_0 (and Z_0 itself, scaled in place)
+  for (first(t, c); t < tiles; next(t, c)) {
+    float v[16];
+    uint32_t r[16];
+    ld16(tlane + t * mp + c * 16, v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = v[i] * s0 * s1;
+      r[i] = __float_as_uint(v[i]);
+    }
+    tmem_st16(tlane + t * mp + c * 16, r);
+    put16(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
+  }
+  tmem_wait_st();
+  if (publish()) {
+    for (int i = 0; i < tiles; ++i) gram(i);
+    for (int it = 0; it < p.k.steps; ++it) {
+      // A = xi^2 Z^T Z
+      ok = mbar_wait_warp(&bar[0], 0, p.status, kTimeoutEpilogue, nullptr);
+      tc_fence_after();
       const float x2 = xi * xi;
+      for (int j = grp; j < chunks; j += 4) {
+        float v[16];
+        ld16(tlane + tiles * mp + j * 16, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = (row < m && c * 16 + i < m) ? v[i] * x2 : 0.f;
-      put16(ac, 16384, row, c * 16, v);
-    }
-    // C = (b A + c A^2) / a
-    tc_fence_before();
-    fence_proxy_async_smem();
-    if (__syncthreads_or(!ok)) break;
-    if (warp == 0 && elect_one()) {
-      tc_fence_after();
-      for (int k = 0; k < chunks; ++k) {
-        const uint64_t d = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
-        umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
+        for (int i = 0; i < 16; ++i) v[i] = (row < m && j * 16 + i < m) ? v[i] * x2 : 0.f;
+        put16(ac, 16384, row, j * 16, v);
       }
-      umma_commit(&bar[0]);
-    }
-    __syncwarp();
-    ok = mbar_wait_warp(&bar[0], ph, p.status, kTimeoutEpilogue, nullptr);
-    ph ^= 1;
-    tc_fence_after();
-    for (int c = grp; c < chunks; c += 4) {
-      float v[16], s[16];
-      ld16(tlane + tiles * mp + c * 16, v);
-      get16(ac, 16384, row, c * 16, s);
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        v[i] = (row < m && c * 16 + i < m) ? (p.b * s[i] + p.c * v[i]) / p.a : 0.f;
-      put16(ac, 16384, row, c * 16, v);
-    }
-    // Z += Z C, tile by tile
-    tc_fence_before();
-    fence_proxy_async_smem();
-    if (__syncthreads_or(!ok)) break;
-    if (warp == 0 && elect_one()) {
-      tc_fence_after();
-      for (int t = 0; t < tiles; ++t) {
+      if (!publish()) break;
+      if (warp == 0 && elect_one()) {
         for (int k = 0; k < chunks; ++k) {
-          const uint64_t da = umma_desc_kmajor_sw128(zs + (k >> 2) * zpanel + t * 16384 + (k & 3) * 32);
-          const uint64_t db = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
-          umma_bf16_ss(tmem + t * mp, da, db, idesc_k, 1u);
+          const uint64_t d = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
+          umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
         }
-        umma_commit(&bar[1 + t]);
+        umma_commit(&bar[0]);
       }
-    }
-    __syncwarp();
-    if (last) {  // the operands' place is free once the last tile is done
-      ok = mbar_wait_warp(&bar[tiles], it & 1, p.status, kTimeoutEpilogue, nullptr);
-      if (!ok) break;
+      __syncwarp();
+      // C = (b A + c A^2) / a
+      ok = mbar_wait_warp(&bar[0], 1, p.status, kTimeoutEpilogue, nullptr);
       tc_fence_after();
-    }
-    for (int u = grp, seen = -1; u < tiles * chunks; u += 4) {
-      const int t = u / chunks, c0 = u % chunks * 16, r0 = t * 128 + q * 32;
-      if (!last && t > seen) {
-        ok = ok && mbar_wait_warp(&bar[1 + t], it & 1, p.status, kTimeoutEpilogue, nullptr);
-        seen = t;
+      for (int j = grp; j < chunks; j += 4) {
+        float v[16], s[16];
+        ld16(tlane + tiles * mp + j * 16, v);
+        get16(ac, 16384, row, j * 16, s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          v[i] = (row < m && j * 16 + i < m) ? p.k.ba * s[i] + p.k.ca * v[i] : 0.f;
+        put16(ac, 16384, row, j * 16, v);
+      }
+      if (!publish()) break;
+      // Z += Z C, tile by tile
+      if (warp == 0 && elect_one()) {
+        for (int i = 0; i < tiles; ++i) {
+          for (int k = 0; k < chunks; ++k) {
+            const uint64_t da = umma_desc_kmajor_sw128(zs + (k >> 2) * zpanel + i * 16384 + (k & 3) * 32);
+            const uint64_t db = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
+            umma_bf16_ss(tmem + i * mp, da, db, idesc_k, 1u);
+          }
+          umma_commit(&bar[1 + i]);
+        }
+      }
+      __syncwarp();
+      xi *= p.k.a;
+      if (it == p.k.steps - 1) break;
+      // the fp16 copy of each finished tile, and its share of the next A behind it
+      first(t, c);
+      for (int i = 0; i < tiles; ++i) {
+        ok = ok && mbar_wait_warp(&bar[1 + i], it & 1, p.status, kTimeoutEpilogue, nullptr);
         tc_fence_after();
+        for (; t == i; next(t, c)) {
+          float v[16];
+          ld16(tlane + t * mp + c * 16, v);
+          put16(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
+        }
+        if (!publish()) break;  // every warp's part of the tile
+        gram(i);
       }
-      float v[16];
-      ld16(tlane + t * mp + c0, v);
-      if (!last) {
-        put16(zh, zpanel, r0 + lane, c0, v);
-        continue;
-      }
-      const float xo = xi * p.a;
-      const int cl = lane & 15, rl = lane >> 4;
+      if (!ok) break;
+    }
+    // the result: the operands' place is free once the last tile is done
+    ok = ok && mbar_wait_warp(&bar[tiles], (p.k.steps - 1) & 1, p.status, kTimeoutEpilogue, nullptr);
+    tc_fence_after();
+    if (ok) {
+      for (first(t, c); t < tiles; next(t, c)) {
+        const int c0 = c * 16, r0 = t * 128 + q * 32;
+        float v[16];
+        ld16(tlane + t * mp + c0, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] *= xo;
-      if (wide) {
-        emit<16>(sink, p.s, static_cast<int64_t>(c0) * n + r0 + lane, n, r0 + lane < n ? m - c0 : 0, v);
-      } else {
+        for (int i = 0; i < 16; ++i) v[i] *= xi;
+        if (wide) {
+          emit<16>(sink, p.s, static_cast<int64_t>(c0) * n + r0 + lane, n, r0 + lane < n ? m - c0 : 0, v);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) stage[lane * 17 + i] = v[i];
-        __syncwarp();
+          for (int i = 0; i < 16; ++i) stage[lane * 17 + i] = v[i];
+          __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = stage[(2 * i + rl) * 17 + cl];
-        __syncwarp();
-        emit<16>(sink, p.s, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
-                 c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
+          for (int i = 0; i < 16; ++i) v[i] = stage[(2 * i + rl) * 17 + cl];
+          __syncwarp();
+          emit<16>(sink, p.s, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
+                   c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
+        }
       }
     }
-    xi *= p.a;
   }
   // every product was waited for (or a wait has run out)
   tc_fence_before();
@@ -913,11 +946,6 @@ static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int b
 
 static int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-struct Coeffs {
-  int steps;
-  double eps;
-  float a, b, c;
-};
 
 // Orthogonalise `batch` matrices of one shape: Newton-Schulz output into `out`, or with
 // kSrcMuon / kOutMuon the whole step.  Work buffers come from PyTorch's allocator (per call
@@ -968,8 +996,8 @@ static void run_group(int src, const void* g, int out_type, void* out, const Ste
   p.bn = static_cast<int>(align_up((m + nb - 1) / nb, 16));
   p.steps = k.steps;
   p.a = k.a;
-  p.b = k.b;
-  p.c = k.c;
+  p.ba = k.ba;
+  p.ca = k.ca;
   p.zl = zl;
   p.A = A;
   p.C = C;
@@ -1007,11 +1035,7 @@ static void run_single(int src, const void* g, int out_type, void* out, const St
   p.first = static_cast<int>(first);
   p.rows = rows;
   p.cols = cols;
-  p.steps = k.steps;
-  p.eps = k.eps;
-  p.a = k.a;
-  p.b = k.b;
-  p.c = k.c;
+  p.k = k;
   p.out_type = out_type;
   p.out = out;
   p.s = s;
@@ -1032,7 +1056,8 @@ static Coeffs make_coeffs(int64_t steps, double eps, const std::vector<double>& 
   TORCH_CHECK(steps >= 1 && steps <= 64, who, ": steps must be in 1..64");
   TORCH_CHECK(eps >= 0.0, who, ": eps must not be negative");
   TORCH_CHECK(c.size() == 3 && c[0] > 0.0, who, ": three coefficients with a positive first one expected");
-  return {static_cast<int>(steps), eps, static_cast<float>(c[0]), static_cast<float>(c[1]), static_cast<float>(c[2])};
+  return {static_cast<int>(steps), static_cast<float>(eps), static_cast<float>(c[0]), static_cast<float>(c[1] / c[0]),
+          static_cast<float>(c[2] / c[0])};
 }
 
 static const float* opt_scalar(const c10::optional<torch::Tensor>& t, const torch::Device& dev, const char* what) {
