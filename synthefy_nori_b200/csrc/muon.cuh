@@ -1,0 +1,246 @@
+// Muon on sm_100a: momentum, orthogonalisation by Newton-Schulz products and the weight
+// update for a ragged set of matrices, and the orthogonalisation alone.
+//
+// For one matrix G (rows x cols; n = max, m = min of the two, taken tall, i.e. n x m):
+//   X_0 = G / (|G|_F + eps)
+//   A = X^T X,   C = (b A + c A^2) / a,   X <- a (X + X C)          (repeated `steps` times)
+//
+// Numerics.  The kernels carry Z_k = 2^8 X_k / (f a^k) with f = |G|_F / (|G|_F + eps), so
+// that one step is Z <- Z + Z C and the leading term needs no multiplication: X_k = xi_k Z_k
+// with xi_0 = f 2^-8 and xi_{k+1} = a xi_k.  Z is held as a pair of fp16 (high, low: 22
+// significant bits); the three products read fp16 operands (the high parts, A and C: 11
+// bits) and accumulate in fp32.  A small singular value of G lives in the pair and is only
+// multiplied by 1 + C, so it keeps its 22 bits, while the rounding of the products' operands
+// (2^-12 relative) perturbs the dominant directions only and is not amplified: the result is
+// 2e-4 .. 2e-3 (2-norm) from the exact iteration for flat, power-law, exponential and
+// rank-deficient spectra alike, about the rounding of a bf16 result.  With iterates rounded
+// to bf16 the noise 2^-9 |G|_F is amplified by up to a^5 = 485 in the small directions: 1e-2
+// for a flat spectrum and 0.1 .. 1 for steep ones.  Products of fp16 pairs (three MMAs each)
+// would give 1e-6 for three times the tensor work.
+//
+// Reference counterpart: training/optim.py:60-85 (Newton-Schulz), 180-319 (Muon step).
+#pragma once
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <climits>
+#include <vector>
+
+#include "sm100.cuh"
+#include "tma_host.h"
+
+namespace nori {
+namespace muon {
+
+constexpr float kZScale = 256.f;
+
+enum OutType : int { kOutF32 = 0, kOutBF16 = 1, kOutF16 = 2, kOutMuon = 3 };
+enum SrcType : int { kSrcF32 = 0, kSrcBF16 = 1, kSrcF16 = 2, kSrcMuon = 3 };
+
+// Learning-rate factor of the orthogonalised update, by shape.
+enum Adjust : int { kMatchRms = 0, kOriginal = 1, kNd = 2 };
+
+// One row of the plan's device table.
+struct Mat {
+  int64_t off;   // first element in the flat parameter / gradient / average buffers
+  int64_t moff;  // first element in the momentum buffer
+  int64_t rows, cols;
+};
+
+struct Coeffs {
+  int steps;
+  float eps, a, ba, ca;  // the coefficients a, b / a, c / a
+};
+
+struct StepArgs {
+  float* data;
+  const float* grad;
+  float* mom;
+  float* ema;  // or null
+  const Mat* table;
+  const float* norm_sq;  // or null
+  const float* skip;     // or null
+  float lr, wd, momentum, max_norm, ema_w;
+  int nesterov, adjust;
+};
+
+// A step that the trainer rejected on the device, or one whose gradient norm is not finite,
+// leaves weights, momentum and average as they are (as adamw_ema_kernel does).
+__device__ __forceinline__ bool step_rejected(const StepArgs& s) {
+  if (s.skip != nullptr && *s.skip > 0.f) return true;
+  return s.norm_sq != nullptr && !(*s.norm_sq < INFINITY);
+}
+
+__device__ __forceinline__ float clip_factor(const StepArgs& s) {
+  if (s.norm_sq == nullptr) return 1.f;
+  return fminf(1.f, s.max_norm / (sqrtf(*s.norm_sq) + 1e-6f));
+}
+
+__device__ __forceinline__ float lr_factor(int adjust, int rows, int cols) {
+  const float r = static_cast<float>(rows), c = static_cast<float>(cols);
+  if (adjust == kMatchRms) return 0.2f * sqrtf(fmaxf(r, c));
+  if (adjust == kOriginal) return sqrtf(fmaxf(1.f, r / c));
+  return sqrtf(fmaxf(r, c) / fminf(r, c));
+}
+
+template <int SRC>
+__device__ __forceinline__ float load_src(const void* g, int64_t i) {
+  if constexpr (SRC == kSrcF32) return static_cast<const float*>(g)[i];
+  if constexpr (SRC == kSrcBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]);
+  if constexpr (SRC == kSrcF16) return __half2float(static_cast<const __half*>(g)[i]);
+  return 0.f;
+}
+
+// Where one element of the result goes: a plain output tensor, or the weights.
+struct Sink {
+  int type;      // OutType
+  void* out;     // plain output of this matrix's batch, or null
+  int64_t base;  // first element of the matrix
+  float lr_o;    // kOutMuon: lr times the shape's factor
+};
+// Values o[0 .. cnt) go to elements e0, e0 + stride, ...: every load of the weights is issued
+// before the first store (the compiler may not move one past the other), so a thread waits
+// for memory once, not once per element.
+template <int N>
+__device__ __forceinline__ void emit(const Sink& k, const StepArgs& s, int64_t e0, int64_t stride, int cnt,
+                                     const float* o) {
+  e0 += k.base;
+  if (k.type == kOutMuon) {
+    float p[N], e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = i < cnt ? s.data[e0 + i * stride] : 0.f;
+    if (s.ema != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = i < cnt ? s.ema[e0 + i * stride] : 0.f;
+    }
+    const float keep = 1.f - s.lr * s.wd;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      p[i] = p[i] * keep - k.lr_o * o[i];
+      if (i < cnt) s.data[e0 + i * stride] = p[i];
+    }
+    if (s.ema != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < cnt) s.ema[e0 + i * stride] = e[i] + s.ema_w * (p[i] - e[i]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i < cnt) {
+      if (k.type == kOutF32)
+        static_cast<float*>(k.out)[e0 + i * stride] = o[i];
+      else if (k.type == kOutBF16)
+        static_cast<__nv_bfloat16*>(k.out)[e0 + i * stride] = __float2bfloat16(o[i]);
+      else
+        static_cast<__half*>(k.out)[e0 + i * stride] = __float2half_rn(o[i]);
+    }
+  }
+}
+
+// The update's input at elements e0, e0 + stride, ... (the momentum brought up to date on the
+// way), loads before stores as in emit.
+template <int SRC, int N>
+__device__ __forceinline__ void fetch(const void* g, const StepArgs& s, int64_t base, int64_t mbase, float clip,
+                                      int64_t e0, int64_t stride, int cnt, float* v) {
+  if constexpr (SRC == kSrcMuon) {
+    float m[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < cnt ? s.grad[base + e0 + i * stride] * clip : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m[i] = i < cnt ? s.mom[mbase + e0 + i * stride] : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      m[i] = s.momentum * m[i] + v[i];
+      if (i < cnt) s.mom[mbase + e0 + i * stride] = m[i];
+      v[i] = s.nesterov ? v[i] + s.momentum * m[i] : m[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < cnt ? load_src<SRC>(g, base + e0 + i * stride) : 0.f;
+  }
+}
+
+// From a matrix's sum of squares v: 2^8 / norm as a product of two floats (it may lie outside
+// fp32's range; powers of two from the exponent, the rest is in [2^7, 2^8]), and
+// f = norm / (norm + eps).  All zero for a zero matrix; f is NaN where the sum is not finite.
+__device__ __forceinline__ void z_scale(double v, float eps, float& s0, float& s1, float& f) {
+  if (!(v > 0.0) || !(v < INFINITY)) {
+    s0 = s1 = 0.f;
+    f = v == 0.0 ? 0.f : NAN;
+    return;
+  }
+  const int k = (((__double2hiint(v) >> 20) & 0x7ff) - 1023) >> 1;  // norm is in [2^k, 2^(k+1))
+  const float r = rsqrtf(static_cast<float>(v * __hiloint2double((1023 - 2 * k) << 20, 0)));  // 2^k / norm
+  const int k0 = k / 2, k1 = k - k0;
+  s0 = __int_as_float((127 - k0) << 23);
+  const float t = __int_as_float((127 - k1) << 23) * r;
+  s1 = kZScale * t;
+  f = 1.f / (1.f + eps * s0 * t);
+}
+
+// kind::f16 with fp16 operands, fp32 accumulators, M = 128.
+__device__ __forceinline__ uint32_t idesc_f16(int N, bool mn_major) {
+  return (1u << 4) | (mn_major ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  uint4 u;
+  __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  return u;
+}
+__device__ __forceinline__ void unpack8(uint4 u, float* v) {
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// ------------------------------------------------------------------ one matrix per CTA
+constexpr int kSingleThreads = 512;
+constexpr int kSingleMaxTiles = 12;
+constexpr int kSingleStage = 16 * 32 * 17 * 4;  // one [32][17] tile per warp, in the operands' place
+
+struct Fit {
+  int n, m, mp, tiles, panels;
+  int smem, tmem;
+  bool ok;
+};
+__host__ __device__ inline Fit single_fit(int rows, int cols) {
+  Fit f;
+  f.n = rows > cols ? rows : cols;
+  f.m = rows > cols ? cols : rows;
+  f.mp = (f.m + 15) / 16 * 16;
+  f.tiles = (f.n + 127) / 128;
+  f.panels = (f.mp + 63) / 64;
+  f.smem = (f.tiles + 1) * f.panels * 16384;
+  if (f.smem < kSingleStage) f.smem = kSingleStage;
+  f.tmem = (f.tiles + 1) * f.mp;
+  f.ok = f.m <= 128 && f.tiles <= kSingleMaxTiles && f.smem <= 220 * 1024 && f.tmem <= 512;
+  return f;
+}
+
+// Matrices first .. first + count of a set that all fit one CTA; `smem` is the largest need.
+void run_single(int src, const void* g, int out_type, void* out, const StepArgs& s, int64_t first, int64_t count,
+                int rows, int cols, int smem, const Coeffs& k, const torch::Tensor& status);
+
+// ------------------------------------------------------------------ matrices over the whole GPU
+struct Shape {
+  int64_t first, count;  // matrices of the plan's table (or of the batch)
+  int rows, cols;
+};
+void run_large(int src, const void* g, int out_type, void* out, const StepArgs& s, const std::vector<Shape>& shapes,
+               const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev);
+
+}  // namespace muon
+}  // namespace nori
