@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 #include <vector>
 
 #include "sm100.cuh"
@@ -105,41 +106,116 @@ struct Sink {
 // Values o[0 .. cnt) go to elements e0, e0 + stride, ...: every load of the weights is issued
 // before the first store (the compiler may not move one past the other), so a thread waits
 // for memory once, not once per element.
+template <typename T, int N>
+__device__ __forceinline__ void store_strided(T* p, int64_t stride, int cnt, const float* o) {
+#pragma unroll
+  for (int i = 0; i < N; ++i, p += stride)
+    if (i < cnt) {
+      if constexpr (sizeof(T) == 4)
+        *p = o[i];
+      else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        *p = __float2bfloat16(o[i]);
+      else
+        *p = __float2half_rn(o[i]);
+    }
+}
 template <int N>
 __device__ __forceinline__ void emit(const Sink& k, const StepArgs& s, int64_t e0, int64_t stride, int cnt,
                                      const float* o) {
   e0 += k.base;
   if (k.type == kOutMuon) {
     float p[N], e[N];
+    float* w = s.data + e0;
+    float* av = s.ema + e0;  // used where there is one
 #pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = i < cnt ? s.data[e0 + i * stride] : 0.f;
+    for (int i = 0; i < N; ++i) p[i] = i < cnt ? w[i * stride] : 0.f;
     if (s.ema != nullptr) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = i < cnt ? s.ema[e0 + i * stride] : 0.f;
+      for (int i = 0; i < N; ++i) e[i] = i < cnt ? av[i * stride] : 0.f;
     }
     const float keep = 1.f - s.lr * s.wd;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      p[i] = p[i] * keep - k.lr_o * o[i];
-      if (i < cnt) s.data[e0 + i * stride] = p[i];
+    for (int i = 0; i < N; ++i) p[i] = p[i] * keep - k.lr_o * o[i];
+    store_strided<float, N>(w, stride, cnt, p);
+    if (s.ema != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] += s.ema_w * (p[i] - e[i]);
+      store_strided<float, N>(av, stride, cnt, e);
     }
+  } else if (k.type == kOutF32) {
+    store_strided<float, N>(static_cast<float*>(k.out) + e0, stride, cnt, o);
+  } else if (k.type == kOutBF16) {
+    store_strided<__nv_bfloat16, N>(static_cast<__nv_bfloat16*>(k.out) + e0, stride, cnt, o);
+  } else {
+    store_strided<__half, N>(static_cast<__half*>(k.out) + e0, stride, cnt, o);
+  }
+}
+
+// The same for N groups of 4 consecutive values, `stride` apart, where sink4() allows it.
+__device__ __forceinline__ bool sink4(const Sink& k, const StepArgs& s) {
+  if (k.type == kOutMuon)
+    return ((reinterpret_cast<uintptr_t>(s.data + k.base) |
+             (s.ema != nullptr ? reinterpret_cast<uintptr_t>(s.ema + k.base) : 0)) & 15) == 0;
+  if (k.type == kOutF32) return (reinterpret_cast<uintptr_t>(static_cast<float*>(k.out) + k.base) & 15) == 0;
+  return (reinterpret_cast<uintptr_t>(static_cast<__half*>(k.out) + k.base) & 7) == 0;
+}
+template <int N>
+__device__ __forceinline__ void emit4(const Sink& k, const StepArgs& s, int64_t e0, int64_t stride, int cnt,
+                                      const float4* o) {
+  e0 += k.base;
+  if (k.type == kOutMuon) {
+    float4 p[N], e[N];
+    float* w = s.data + e0;
+    float* av = s.ema + e0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) p[i] = *reinterpret_cast<const float4*>(w + i * stride);
     if (s.ema != nullptr) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (i < cnt) s.ema[e0 + i * stride] = e[i] + s.ema_w * (p[i] - e[i]);
+        if (i < cnt) e[i] = *reinterpret_cast<const float4*>(av + i * stride);
     }
-    return;
-  }
+    const float keep = 1.f - s.lr * s.wd;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (i < cnt) {
-      if (k.type == kOutF32)
-        static_cast<float*>(k.out)[e0 + i * stride] = o[i];
-      else if (k.type == kOutBF16)
-        static_cast<__nv_bfloat16*>(k.out)[e0 + i * stride] = __float2bfloat16(o[i]);
-      else
-        static_cast<__half*>(k.out)[e0 + i * stride] = __float2half_rn(o[i]);
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) {
+        p[i].x = p[i].x * keep - k.lr_o * o[i].x;
+        p[i].y = p[i].y * keep - k.lr_o * o[i].y;
+        p[i].z = p[i].z * keep - k.lr_o * o[i].z;
+        p[i].w = p[i].w * keep - k.lr_o * o[i].w;
+        *reinterpret_cast<float4*>(w + i * stride) = p[i];
+      }
+    if (s.ema != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < cnt) {
+          e[i].x += s.ema_w * (p[i].x - e[i].x);
+          e[i].y += s.ema_w * (p[i].y - e[i].y);
+          e[i].z += s.ema_w * (p[i].z - e[i].z);
+          e[i].w += s.ema_w * (p[i].w - e[i].w);
+          *reinterpret_cast<float4*>(av + i * stride) = e[i];
+        }
     }
+  } else if (k.type == kOutF32) {
+    float* d = static_cast<float*>(k.out) + e0;
+#pragma unroll
+    for (int i = 0; i < N; ++i, d += stride)
+      if (i < cnt) *reinterpret_cast<float4*>(d) = o[i];
+  } else if (k.type == kOutBF16) {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(k.out) + e0;
+#pragma unroll
+    for (int i = 0; i < N; ++i, d += stride)
+      if (i < cnt) *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(o[i].x, o[i].y), pack_bf16x2(o[i].z, o[i].w));
+  } else {
+    __half* d = static_cast<__half*>(k.out) + e0;
+#pragma unroll
+    for (int i = 0; i < N; ++i, d += stride)
+      if (i < cnt) {
+        uint2 u;
+        *reinterpret_cast<__half2*>(&u.x) = __floats2half2_rn(o[i].x, o[i].y);
+        *reinterpret_cast<__half2*>(&u.y) = __floats2half2_rn(o[i].z, o[i].w);
+        *reinterpret_cast<uint2*>(d) = u;
+      }
   }
 }
 
@@ -150,19 +226,78 @@ __device__ __forceinline__ void fetch(const void* g, const StepArgs& s, int64_t 
                                       int64_t e0, int64_t stride, int cnt, float* v) {
   if constexpr (SRC == kSrcMuon) {
     float m[N];
+    const float* gr = s.grad + base + e0;
+    float* mo = s.mom + mbase + e0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i < cnt ? s.grad[base + e0 + i * stride] * clip : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = i < cnt ? gr[i * stride] * clip : 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m[i] = i < cnt ? s.mom[mbase + e0 + i * stride] : 0.f;
+    for (int i = 0; i < N; ++i) m[i] = i < cnt ? mo[i * stride] : 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       m[i] = s.momentum * m[i] + v[i];
-      if (i < cnt) s.mom[mbase + e0 + i * stride] = m[i];
       v[i] = s.nesterov ? v[i] + s.momentum * m[i] : m[i];
     }
+    store_strided<float, N>(mo, stride, cnt, m);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = i < cnt ? load_src<SRC>(g, base + e0 + i * stride) : 0.f;
+  }
+}
+
+// 4 consecutive values of the update's input, where aligned4() allows it.
+template <int SRC>
+__device__ __forceinline__ void load4(const void* g, int64_t i, float* v) {
+  if constexpr (SRC == kSrcF32) {
+    const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(g) + i);
+    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+  } else if constexpr (SRC == kSrcBF16) {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(g) + i);
+    v[0] = bf16lo(u.x), v[1] = bf16hi(u.x), v[2] = bf16lo(u.y), v[3] = bf16hi(u.y);
+  } else if constexpr (SRC == kSrcF16) {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(g) + i);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  }
+}
+template <int SRC>
+__device__ __forceinline__ bool aligned4(const void* g, const StepArgs& s, int64_t base, int64_t mbase) {
+  if constexpr (SRC == kSrcMuon)
+    return ((reinterpret_cast<uintptr_t>(s.grad + base) | reinterpret_cast<uintptr_t>(s.mom + mbase)) & 15) == 0;
+  if constexpr (SRC == kSrcF32) return (reinterpret_cast<uintptr_t>(static_cast<const float*>(g) + base) & 15) == 0;
+  return (reinterpret_cast<uintptr_t>(static_cast<const __half*>(g) + base) & 7) == 0;
+}
+// N groups of 4 consecutive values, `stride` apart.
+template <int SRC, int N>
+__device__ __forceinline__ void fetch4(const void* g, const StepArgs& s, int64_t base, int64_t mbase, float clip,
+                                       int64_t e0, int64_t stride, int cnt, float* v) {
+  if constexpr (SRC == kSrcMuon) {
+    float m[4 * N];
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) v[i] = m[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) load4<kSrcF32>(s.grad, base + e0 + i * stride, v + 4 * i);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) load4<kSrcF32>(s.mom, mbase + e0 + i * stride, m + 4 * i);
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+      v[i] *= clip;
+      m[i] = s.momentum * m[i] + v[i];
+      v[i] = s.nesterov ? v[i] + s.momentum * m[i] : m[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < cnt)
+        *reinterpret_cast<float4*>(s.mom + mbase + e0 + i * stride) =
+            make_float4(m[4 * i], m[4 * i + 1], m[4 * i + 2], m[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) v[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) load4<SRC>(g, base + e0 + i * stride, v + 4 * i);
   }
 }
 

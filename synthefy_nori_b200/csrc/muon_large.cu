@@ -32,31 +32,6 @@ __device__ __forceinline__ const double* partials(const Pre& p, int gi, int mat)
   return p.partial + at + static_cast<int64_t>(mat) * p.g[gi].slices;
 }
 
-// The update's input, 4 values at a time where every buffer allows 16-byte accesses.
-template <int SRC>
-__device__ __forceinline__ void load4(const void* g, int64_t i, float* v) {
-  if constexpr (SRC == kSrcF32) {
-    const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(g) + i);
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-  } else if constexpr (SRC == kSrcBF16) {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(g) + i);
-    v[0] = bf16lo(u.x), v[1] = bf16hi(u.x), v[2] = bf16lo(u.y), v[3] = bf16hi(u.y);
-  } else if constexpr (SRC == kSrcF16) {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(g) + i);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-  }
-}
-
-template <int SRC>
-__device__ __forceinline__ bool aligned4(const void* g, const StepArgs& s, int64_t base, int64_t mbase) {
-  if constexpr (SRC == kSrcMuon)
-    return ((reinterpret_cast<uintptr_t>(s.grad + base) | reinterpret_cast<uintptr_t>(s.mom + mbase)) & 15) == 0;
-  if constexpr (SRC == kSrcF32) return (reinterpret_cast<uintptr_t>(static_cast<const float*>(g) + base) & 15) == 0;
-  return (reinterpret_cast<uintptr_t>(static_cast<const __half*>(g) + base) & 7) == 0;
-}
-
 // ------------------------------------------------------------------ norm (and momentum)
 // Partial sums of squares of the update's input, one CTA per 8192 values of a matrix, in
 // double: no fp32 gradient overflows or vanishes in its own norm.  With kSrcMuon the momentum
@@ -606,25 +581,40 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             if (q.rows < q.cols) {
               const int64_t e0 = static_cast<int64_t>(col) * q.n + r0 + lane;
               const int cnt = r0 + lane < q.n ? q.m - col : 0;
-              emit<16>(sink, a.s, e0, q.n, cnt, v);
-              emit<16>(sink, a.s, e0 + 16ll * q.n, q.n, cnt - 16, v + 16);
+#pragma unroll
+              for (int k = 0; k < 32; k += 8) emit<8>(sink, a.s, e0 + static_cast<int64_t>(k) * q.n, q.n, cnt - k, v + k);
             } else {
-              auto cell = [&](int rr, int cc) -> float* {
+              // 16-byte cell j of row rr among the ones that this warp alone uses
+              auto cell = [&](int rr, int j) -> float4* {
                 const int rl = q4 * 32 + rr;
-                return reinterpret_cast<float*>((cc < 16 ? s0 : s1) + rl * 128 +
-                                                (((half * 4 + ((cc & 15) >> 2)) ^ (rl & 7)) << 4)) +
-                       ((cc ^ (rr >> 3)) & 3);
+                return reinterpret_cast<float4*>((j < 4 ? s0 : s1) + rl * 128 + (((half * 4 + (j & 3)) ^ (rl & 7)) << 4));
               };
               __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) *cell(lane, i) = v[i];
+              for (int j = 0; j < 8; ++j) *cell(lane, j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
               __syncwarp();
+              if (q.m % 4 == 0 && sink4(sink, a.s)) {  // 8 lanes of 4 columns a row, 4 rows at a time
+                const int rr = lane >> 3, cc = col + (lane & 7) * 4;
+                const int cnt = cc < q.m ? (q.n - r0 - rr + 3) / 4 : 0;
+                const int64_t e0 = static_cast<int64_t>(r0 + rr) * q.m + cc;
+#pragma unroll 1
+                for (int k = 0; k < 8; k += 4) {
+                  float4 o[4];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = *cell(i, lane);
-              const int64_t e0 = static_cast<int64_t>(r0) * q.m + col + lane;
-              const int cnt = col + lane < q.m ? q.n - r0 : 0;
-              emit<16>(sink, a.s, e0, q.m, cnt, v);
-              emit<16>(sink, a.s, e0 + 16ll * q.m, q.m, cnt - 16, v + 16);
+                  for (int i = 0; i < 4; ++i) o[i] = *cell(4 * (k + i) + rr, lane & 7);
+                  emit4<4>(sink, a.s, e0 + 4ll * k * q.m, 4ll * q.m, cnt - k, o);
+                }
+              } else {
+                const int cnt = col + lane < q.m ? q.n - r0 : 0;
+                const int64_t e0 = static_cast<int64_t>(r0) * q.m + col + lane;
+#pragma unroll 1
+                for (int k = 0; k < 32; k += 8) {
+                  float o[8];
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) o[i] = reinterpret_cast<const float*>(cell(k + i, lane >> 2))[lane & 3];
+                  emit<8>(sink, a.s, e0 + static_cast<int64_t>(k) * q.m, q.m, cnt - k, o);
+                }
+              }
             }
           }
         }
@@ -748,8 +738,8 @@ static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int b
 
 static int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-// Work of all matrices of a block should stay in L2 from one product to the next.
-constexpr int64_t kBlockBytes = 64ll << 20;
+// Work buffers of the matrices of a block.
+constexpr int64_t kBlockBytes = 400ll << 20;
 
 static void run_shapes(int src, const void* g, int out_type, void* out, const StepArgs& s, const Shape* shapes, int ns,
                        const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev) {

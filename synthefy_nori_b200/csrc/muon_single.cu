@@ -64,7 +64,9 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const uint32_t tlane = tmem + (static_cast<uint32_t>(q * 32) << 16);
-  const int cl = lane & 15, rl = lane >> 4;  // a 16-column chunk in memory: two rows per warp access
+  // a 16-column chunk in memory: 2 rows of single values, or 8 rows of groups of 4, per access
+  const int cl = lane & 15, rl = lane >> 4, c4 = (lane & 3) * 4, r8 = lane >> 2;
+  const bool in4 = m % 4 == 0 && aligned4<SRC>(g, p.s, base, mbase);
   // this group's first (tile, chunk), and the one after
   auto first = [&](int& t, int& c) {
     t = 0;
@@ -89,13 +91,25 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     const int c0 = c * 16, r0 = t * 128 + q * 32;
     float v[16];
     if (wide) {  // consecutive lanes are consecutive columns of G
-      fetch<SRC, 16>(g, p.s, base, mbase, clip, static_cast<int64_t>(c0) * n + r0 + lane, n,
-                     r0 + lane < n ? m - c0 : 0, v);
-    } else {     // turned in shared memory
-      fetch<SRC, 16>(g, p.s, base, mbase, clip, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
-                     c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
+      const int cnt = r0 + lane < n ? m - c0 : 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) stage[(2 * i + rl) * 17 + cl] = v[i];
+      for (int k = 0; k < 16; k += 8)
+        fetch<SRC, 8>(g, p.s, base, mbase, clip, static_cast<int64_t>(c0 + k) * n + r0 + lane, n, cnt - k, v + k);
+    } else {     // turned in shared memory
+      if (in4) {  // 4 lanes of 4 columns a row, 8 rows at a time
+        fetch4<SRC, 4>(g, p.s, base, mbase, clip, static_cast<int64_t>(r0 + r8) * m + c0 + c4, 8 * m,
+                       c0 + c4 < m ? (n - r0 - r8 + 7) / 8 : 0, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) stage[((i & ~3) * 2 + r8) * 17 + c4 + (i & 3)] = v[i];
+      } else {    // 16 lanes a row, 2 rows at a time
+        const int cnt = c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0;
+#pragma unroll
+        for (int k = 0; k < 16; k += 8)
+          fetch<SRC, 8>(g, p.s, base, mbase, clip, static_cast<int64_t>(r0 + rl + 2 * k) * m + c0 + cl, 2 * m, cnt - k,
+                        v + k);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) stage[(2 * i + rl) * 17 + cl] = v[i];
+      }
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = stage[lane * 17 + i];
@@ -149,6 +163,7 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   const uint32_t lbo = fit.panels == 2 ? zpanel : 1024;
   const int row = q * 32 + lane;
   const Sink sink = {p.out_type, p.out, base, p.s.lr * lr_factor(p.s.adjust, rows, cols)};
+  const bool out4 = m % 4 == 0 && sink4(sink, p.s);
   bool ok = true;
   // All that the threads wrote to shared memory is there for the MMAs that one thread issues
   // next; false once a wait of any thread has run out.
@@ -262,16 +277,34 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] *= xi;
         if (wide) {
-          emit<16>(sink, p.s, static_cast<int64_t>(c0) * n + r0 + lane, n, r0 + lane < n ? m - c0 : 0, v);
+          const int cnt = r0 + lane < n ? m - c0 : 0;
+#pragma unroll
+          for (int k = 0; k < 16; k += 8)
+            emit<8>(sink, p.s, static_cast<int64_t>(c0 + k) * n + r0 + lane, n, cnt - k, v + k);
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) stage[lane * 17 + i] = v[i];
           __syncwarp();
+          if (out4) {
+            float4 o[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = stage[(2 * i + rl) * 17 + cl];
+            for (int i = 0; i < 4; ++i) {
+              const float* at = stage + (8 * i + r8) * 17 + c4;
+              o[i] = make_float4(at[0], at[1], at[2], at[3]);
+            }
+            emit4<4>(sink, p.s, static_cast<int64_t>(r0 + r8) * m + c0 + c4, 8 * m,
+                     c0 + c4 < m ? (n - r0 - r8 + 7) / 8 : 0, o);
+          } else {
+            const int cnt = c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0;
+#pragma unroll
+            for (int k = 0; k < 16; k += 8) {
+              float o[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] = stage[(2 * (k + i) + rl) * 17 + cl];
+              emit<8>(sink, p.s, static_cast<int64_t>(r0 + rl + 2 * k) * m + c0 + cl, 2 * m, cnt - k, o);
+            }
+          }
           __syncwarp();
-          emit<16>(sink, p.s, static_cast<int64_t>(r0 + rl) * m + c0 + cl, 2 * m,
-                   c0 + cl < m ? (n - r0 - rl + 1) / 2 : 0, v);
         }
       }
     }
