@@ -3,8 +3,10 @@
 //   y = (x - mean) rstd w + b,  mean and variance over a row's C values (two passes over
 //   registers: the variance sums squares of differences, never a difference of sums)
 //
-// A row belongs to TPR threads (8, a warp, or a CTA of 256), each holding VPL values in
-// chunks of VEC consecutive columns, so a row is read from memory once in each direction.
+// A row belongs to TPR threads (8, a warp, 128 or 512), each holding up to 16 values in chunks
+// of VEC consecutive columns, so a row is read from memory once in each direction.  The threads
+// work on two rows at a time: both rows' loads are in flight together, their reductions overlap
+// and the weight is read (from L1) once for both.
 #pragma once
 
 #include <ATen/cuda/CUDAContext.h>
@@ -20,8 +22,10 @@
 namespace nori {
 namespace ln {
 
-constexpr int kThreads = 256;
-constexpr int kMaxRegCols = 8192;  // 256 threads x 32 values
+constexpr int kValues = 16;         // of one row in a thread
+constexpr int kMaxRegCols = 8192;   // 512 threads x 16 values
+template <int TPR>
+constexpr int kCta = TPR > 256 ? TPR : 256;
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -71,20 +75,68 @@ __device__ __forceinline__ void store_vec(T* p, const float* v) {
   *reinterpret_cast<Pack<T, VEC>*>(p) = u;
 }
 
-// Sum over the TPR threads of a row; every one of them gets it. `sh` holds 8 floats per
-// reduction of a CTA-wide row (a fresh slot for each, so one barrier is enough).
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* sh) {
+// A thread's chunks of one row; zero beyond the last row or column.
+template <typename T, int VEC, int TPR>
+struct Row {
+  static constexpr int CH = kValues / VEC;
+  Pack<T, VEC> p[CH];
+  __device__ __forceinline__ void load(const T* x, int64_t ld, int64_t row, int64_t R, int C, int t) {
+    const T* xr = x + row * ld;
 #pragma unroll
-  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (TPR > 32) {
-    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = 0.f;
+    for (int j = 0; j < CH; ++j) {
+      const int c = VEC * (t + TPR * j);
+      if (row < R && c < C) {
+        p[j] = *reinterpret_cast<const Pack<T, VEC>*>(xr + c);
+      } else {
 #pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) v += sh[i];
+        for (int i = 0; i < VEC; ++i) p[j].v[i] = from_f32<T>(0.f);
+      }
+    }
   }
-  return v;
+  __device__ __forceinline__ void values(float* v) const {
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[VEC * j + i] = to_f32<T>(p[j].v[i]);
+  }
+};
+// VEC columns of a weight vector (`fill` where there is none).
+template <int VEC>
+__device__ __forceinline__ void load_columns(const float* w, int c, float fill, float* v) {
+#pragma unroll
+  for (int i = 0; i < VEC; i += VEC < 4 ? 1 : 4) {
+    if (w == nullptr) {
+#pragma unroll
+      for (int k = 0; k < (VEC < 4 ? 1 : 4); ++k) v[i + k] = fill;
+    } else {
+      load_vec<float, VEC < 4 ? 1 : 4>(w + c + i, v + i);
+    }
+  }
+}
+
+// Sums of N values over the TPR threads of a row; every one of them gets them.  Rows wider
+// than a warp add their warps' sums through `sh`, which alternates between two places from one
+// use to the next, so one barrier is enough.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (&sh)[2][N][16], int& flip) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (TPR > 32) {
+    const int warp = threadIdx.x / 32, w0 = warp / (TPR / 32) * (TPR / 32);
+    if (threadIdx.x % 32 == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) sh[flip][k][warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) v[k] += sh[flip][k][w0 + i];
+    }
+    flip ^= 1;
+  }
 }
 
 // 16-byte accesses need rows that start on 16 bytes and a width that is a whole number of them.

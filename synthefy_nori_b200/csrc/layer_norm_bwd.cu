@@ -5,8 +5,9 @@
 //
 // One pass over x and dy: each thread keeps the sums of its own columns over all rows that it
 // visits in fp32 registers; a CTA adds its row groups in a fixed order and writes one partial
-// row, and a second kernel adds the partial rows in a fixed order.  No atomics: the same
-// inputs give the same bits.
+// row, and a second kernel adds the partial rows in a fixed order.  Where the partial rows
+// would be more traffic than reading x and dy (from L2) once more, the columns are summed by a
+// pass of their own.  No atomics: the same inputs give the same bits.
 //
 // Reference counterpart: torch LayerNorm's autograd (model/layer.py:219-230).
 #include "layer_norm.cuh"
@@ -14,115 +15,128 @@
 namespace nori {
 namespace ln {
 
-template <typename T, typename U, int VEC, int TPR, int VPL>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, typename U, int VEC, int TPR, bool GRADS>
+__global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
     bwd_kernel(const U* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx, int64_t R, int C,
                const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const float* __restrict__ w,
                T* __restrict__ dx, float* __restrict__ part_w, float* __restrict__ part_b) {
-  constexpr int CH = VPL / VEC, RPB = kThreads / TPR;
-  extern __shared__ float acc_sh[];  // [RPB][C] when a CTA holds several row groups
-  __shared__ float sh[32];
+  constexpr int CH = kValues / VEC, RPB = kCta<TPR> / TPR;
+  extern __shared__ float acc_sh[];  // [RPB][C] where a CTA holds several row groups
+  __shared__ float sh[2][4][16];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv_c = 1.f / static_cast<float>(C);
-  float gw[VPL], gb[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) gw[i] = gb[i] = 0.f;
   int flip = 0;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * RPB; base < R; base += static_cast<int64_t>(gridDim.x) * RPB) {
+  float gw[kValues], gb[kValues];
+#pragma unroll
+  for (int i = 0; i < kValues; ++i) gw[i] = gb[i] = 0.f;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (2 * RPB); base < R;
+       base += static_cast<int64_t>(gridDim.x) * (2 * RPB)) {
     const int64_t row = base + g;
-    const bool ok = row < R;
-    const float mean = ok ? mean_in[row] : 0.f, rstd = ok ? rstd_in[row] : 0.f;
-    float h[VPL], q[VPL];
-    float s1 = 0.f, s2 = 0.f;
+    float h[2][kValues], q[2][kValues], s[4] = {0.f, 0.f, 0.f, 0.f}, rstd[2];
+    {
+      Row<T, VEC, TPR> rx[2];
+      Row<U, VEC, TPR> ry[2];
+      float mean[2];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int c = VEC * (t + TPR * j);
-      if (ok && c < C) {
-        load_vec<T, VEC>(x + row * ldx + c, h + VEC * j);
-        load_vec<U, VEC>(dy + row * ldy + c, q + VEC * j);
-        float wv[VEC];
-        if (w != nullptr) load_vec<float, VEC>(w + c, wv);
+      for (int k = 0; k < 2; ++k) {
+        rx[k].load(x, ldx, row + k * RPB, R, C, t);
+        ry[k].load(dy, ldy, row + k * RPB, R, C, t);
+        mean[k] = row + k * RPB < R ? mean_in[row + k * RPB] : 0.f;
+        rstd[k] = row + k * RPB < R ? rstd_in[row + k * RPB] : 0.f;
+      }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int k = VEC * j + i;
-          h[k] = (h[k] - mean) * rstd;
-          gw[k] += q[k] * h[k];
-          gb[k] += q[k];
-          if (w != nullptr) q[k] *= wv[i];
-          s1 += q[k];
-          s2 += q[k] * h[k];
-        }
-      } else {
+      for (int k = 0; k < 2; ++k) {
+        rx[k].values(h[k]);
+        ry[k].values(q[k]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) h[VEC * j + i] = q[VEC * j + i] = 0.f;
+        for (int i = 0; i < kValues; ++i) h[k][i] = (h[k][i] - mean[k]) * rstd[k];
       }
     }
-    s1 = row_sum<TPR>(s1, sh + flip * 16) * inv_c;
-    s2 = row_sum<TPR>(s2, sh + flip * 16 + 8) * inv_c;
-    flip ^= 1;
-    if (!ok) continue;
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
+    for (int j = 0; j < CH; ++j) {  // q is 0 beyond the last row and column
       const int c = VEC * (t + TPR * j);
       if (c < C) {
-        float o[VEC];
+        float wv[VEC];
+        load_columns<VEC>(w, c, 1.f, wv);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = rstd * (q[VEC * j + i] - s1 - h[VEC * j + i] * s2);
-        store_vec<T, VEC>(dx + row * static_cast<int64_t>(C) + c, o);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int e = VEC * j + i;
+            if constexpr (GRADS) {
+              gw[e] += q[k][e] * h[k][e];
+              gb[e] += q[k][e];
+            }
+            q[k][e] *= wv[i];
+            s[2 * k] += q[k][e];
+            s[2 * k + 1] += q[k][e] * h[k][e];
+          }
+      }
+    }
+    row_sum<TPR, 4>(s, sh, flip);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (row + k * RPB < R) {
+        const float s1 = s[2 * k] * inv_c, s2 = s[2 * k + 1] * inv_c;
+        T* dxr = dx + (row + k * RPB) * static_cast<int64_t>(C);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          const int c = VEC * (t + TPR * j);
+          if (c < C) {
+            float o[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] = rstd[k] * (q[k][VEC * j + i] - s1 - h[k][VEC * j + i] * s2);
+            store_vec<T, VEC>(dxr + c, o);
+          }
+        }
       }
     }
   }
-  // this CTA's partial rows
-  for (int pass = 0; pass < 2; ++pass) {
-    float* out = pass == 0 ? part_w : part_b;
-    if (out == nullptr) continue;
-    out += static_cast<int64_t>(blockIdx.x) * C;
-    if constexpr (RPB == 1) {
+  if constexpr (GRADS) {  // this CTA's partial rows
+    for (int pass = 0; pass < 2; ++pass) {
+      float* out = pass == 0 ? part_w : part_b;
+      if (out == nullptr) continue;
+      out += static_cast<int64_t>(blockIdx.x) * C;
+      if constexpr (RPB > 1) __syncthreads();
 #pragma unroll
-      for (int k = 0; k < VPL; ++k) {
+      for (int k = 0; k < kValues; ++k) {
         const int c = VEC * (t + TPR * (k / VEC)) + k % VEC;
-        if (c < C) out[c] = pass == 0 ? gw[k] : gb[k];
+        if (c < C) (RPB > 1 ? acc_sh + g * C : out)[c] = pass == 0 ? gw[k] : gb[k];
       }
-    } else {
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < VPL; ++k) {
-        const int c = VEC * (t + TPR * (k / VEC)) + k % VEC;
-        if (c < C) acc_sh[g * C + c] = pass == 0 ? gw[k] : gb[k];
-      }
-      __syncthreads();
-      for (int c = threadIdx.x; c < C; c += kThreads) {
-        float s = 0.f;
-        for (int i = 0; i < RPB; ++i) s += acc_sh[i * C + c];
-        out[c] = s;
+      if constexpr (RPB > 1) {
+        __syncthreads();
+        for (int c = threadIdx.x; c < C; c += kCta<TPR>) {
+          float v = 0.f;
+          for (int i = 0; i < RPB; ++i) v += acc_sh[i * C + c];
+          out[c] = v;
+        }
       }
     }
   }
 }
 
-// Rows wider than the registers of a CTA: dx in two passes over the row ...
+// Rows wider than the registers of a CTA: dx in two passes over the row.
 template <typename T, typename U>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(512)
     bwd_wide_kernel(const U* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx, int64_t R, int C,
                     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const float* __restrict__ w,
                     T* __restrict__ dx) {
-  __shared__ float sh[32];
+  __shared__ float sh[2][2][16];
   const float inv_c = 1.f / static_cast<float>(C);
   int flip = 0;
   for (int64_t row = blockIdx.x; row < R; row += gridDim.x) {
     const float mean = mean_in[row], rstd = rstd_in[row];
     const T* xr = x + row * ldx;
     const U* dyr = dy + row * ldy;
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = threadIdx.x; c < C; c += kThreads) {
+    float s[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < C; c += 512) {
       const float q = to_f32<U>(dyr[c]) * (w != nullptr ? w[c] : 1.f);
-      s1 += q;
-      s2 += q * ((to_f32<T>(xr[c]) - mean) * rstd);
+      s[0] += q;
+      s[1] += q * ((to_f32<T>(xr[c]) - mean) * rstd);
     }
-    s1 = row_sum<kThreads>(s1, sh + flip * 16) * inv_c;
-    s2 = row_sum<kThreads>(s2, sh + flip * 16 + 8) * inv_c;
-    flip ^= 1;
-    for (int c = threadIdx.x; c < C; c += kThreads) {
+    row_sum<512, 2>(s, sh, flip);
+    const float s1 = s[0] * inv_c, s2 = s[1] * inv_c;
+    for (int c = threadIdx.x; c < C; c += 512) {
       const float q = to_f32<U>(dyr[c]) * (w != nullptr ? w[c] : 1.f);
       const float h = (to_f32<T>(xr[c]) - mean) * rstd;
       dx[row * static_cast<int64_t>(C) + c] = from_f32<T>(rstd * (q - s1 - h * s2));
@@ -130,61 +144,72 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// ... and the column sums by a pass down the columns: 32 columns x 8 row lanes per CTA, one
-// partial row per blockIdx.y.
+// The column sums by a pass down the columns: 64 columns (2 a lane) x 16 row lanes per CTA,
+// one partial row per blockIdx.y (the result itself where there is only one).
 template <typename T, typename U>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(512)
     colgrad_kernel(const U* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx, int64_t R, int C,
                    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, float* __restrict__ part_w,
                    float* __restrict__ part_b) {
-  __shared__ float sw[8][33], sb[8][33];
+  __shared__ float sw[16][65], sb[16][65];
   const int lane = threadIdx.x % 32, ry = threadIdx.x / 32;
-  const int c = blockIdx.x * 32 + lane;
+  const int c = blockIdx.x * 64 + lane;  // and c + 32
   const int64_t per = (R + gridDim.y - 1) / gridDim.y;
   const int64_t r0 = blockIdx.y * per, r1 = min(R, r0 + per);
-  float gw = 0.f, gb = 0.f;
-  if (c < C) {
-    for (int64_t r = r0 + ry; r < r1; r += 8) {
-      const float d = to_f32<U>(dy[r * ldy + c]);
-      gw += d * ((to_f32<T>(x[r * ldx + c]) - mean_in[r]) * rstd_in[r]);
-      gb += d;
+  float gw[2] = {0.f, 0.f}, gb[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int64_t r = r0 + ry; r < r1; r += 16) {
+    const float mean = mean_in[r], rstd = rstd_in[r];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (c + 32 * k < C) {
+        const float d = to_f32<U>(dy[r * ldy + c + 32 * k]);
+        gw[k] += d * ((to_f32<T>(x[r * ldx + c + 32 * k]) - mean) * rstd);
+        gb[k] += d;
+      }
     }
   }
-  sw[ry][lane] = gw;
-  sb[ry][lane] = gb;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    sw[ry][lane + 32 * k] = gw[k];
+    sb[ry][lane + 32 * k] = gb[k];
+  }
   __syncthreads();
-  if (ry == 0 && c < C) {
+  const int col = threadIdx.x;
+  if (col < 64 && blockIdx.x * 64 + col < C) {
     float a = 0.f, e = 0.f;
-    for (int i = 0; i < 8; ++i) {
-      a += sw[i][lane];
-      e += sb[i][lane];
+    for (int i = 0; i < 16; ++i) {
+      a += sw[i][col];
+      e += sb[i][col];
     }
-    if (part_w != nullptr) part_w[static_cast<int64_t>(blockIdx.y) * C + c] = a;
-    if (part_b != nullptr) part_b[static_cast<int64_t>(blockIdx.y) * C + c] = e;
+    const int64_t at = static_cast<int64_t>(blockIdx.y) * C + blockIdx.x * 64 + col;
+    if (part_w != nullptr) part_w[at] = a;
+    if (part_b != nullptr) part_b[at] = e;
   }
 }
 
-// out[c] = sum_p part[p][c], in a fixed order: 32 columns x 8 partial lanes per CTA; blockIdx.y
-// picks the weight's or the bias's sums.
-__global__ void __launch_bounds__(kThreads) reduce_kernel(const float* __restrict__ part_w,
-                                                          const float* __restrict__ part_b, int P, int C,
-                                                          float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float sh[8][33];
+// out[c] = sum_p part[p][c], in a fixed order: 32 columns x 32 partial lanes per CTA;
+// blockIdx.y picks the weight's or the bias's sums.
+__global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ part_w,
+                                                      const float* __restrict__ part_b, int P, int C,
+                                                      float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float sh[32][33];
   const float* part = blockIdx.y == 0 ? part_w : part_b;
   float* out = blockIdx.y == 0 ? dw : db;
   if (out == nullptr) return;
   const int lane = threadIdx.x % 32, py = threadIdx.x / 32;
   const int c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < C)
-    for (int p = py; p < P; p += 8) s += part[static_cast<int64_t>(p) * C + c];
+  if (c < C) {
+#pragma unroll 4
+    for (int p = py; p < P; p += 32) s += part[static_cast<int64_t>(p) * C + c];
+  }
   sh[py][lane] = s;
   __syncthreads();
-  if (py == 0 && c < C) {
-    float a = 0.f;
-    for (int i = 0; i < 8; ++i) a += sh[i][lane];
-    out[c] = a;
-  }
+  s = sh[lane][py];  // column py of this CTA
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0 && blockIdx.x * 32 + py < C) out[blockIdx.x * 32 + py] = s;
 }
 
 struct BwdArgs {
@@ -194,48 +219,58 @@ struct BwdArgs {
   bool want_w, want_b;
 };
 
+template <typename T, typename U, int VEC, int TPR>
+static void launch_rows(const U* dy, const T* x, T* dx, const BwdArgs& a, int P, float* pw, float* pb) {
+  auto stream = at::cuda::getCurrentCUDAStream();
+  constexpr int RPB = kCta<TPR> / TPR;
+  const size_t smem = RPB > 1 ? static_cast<size_t>(RPB) * a.C * sizeof(float) : 0;
+  if (pw != nullptr || pb != nullptr)
+    bwd_kernel<T, U, VEC, TPR, true><<<P, kCta<TPR>, smem, stream>>>(dy, a.ldy, x, a.ldx, a.R, a.C, a.mean, a.rstd,
+                                                                     a.w, dx, pw, pb);
+  else
+    bwd_kernel<T, U, VEC, TPR, false><<<P, kCta<TPR>, 0, stream>>>(dy, a.ldy, x, a.ldx, a.R, a.C, a.mean, a.rstd, a.w,
+                                                                   dx, nullptr, nullptr);
+}
+
 template <typename T, typename U, int VEC>
 static void launch(const U* dy, const T* x, T* dx, const BwdArgs& a, torch::Tensor& dw, torch::Tensor& db) {
   auto stream = at::cuda::getCurrentCUDAStream();
   const int C = a.C;
-  const int tpr = C <= 64 ? 8 : C <= 1024 ? 32 : 256, rpb = kThreads / tpr;
-  const bool wide = C > kMaxRegCols;
-  const int64_t cap = 148 * 2;
-  const int P = static_cast<int>(wide ? std::min<int64_t>(16, (a.R + 63) / 64)
-                                      : std::min<int64_t>(cap, (a.R + rpb - 1) / rpb));
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int tpr = C <= 128 ? 8 : C <= 512 ? 32 : C <= 2048 ? 128 : 512, cta = tpr > 256 ? tpr : 256;
+  const int64_t ctas = std::min<int64_t>(sms * (512 / cta), (a.R + 2 * cta / tpr - 1) / (2 * cta / tpr));
   const bool grads = a.want_w || a.want_b;
+  // partial rows are written and read in fp32 (16 bytes a column and CTA); a second pass over
+  // x and dy reads them again
+  const bool columns =
+      grads && (C > kMaxRegCols || ctas * 16 > a.R * static_cast<int64_t>(sizeof(T) + sizeof(U)));
+  const int P = static_cast<int>(
+      !columns ? ctas : std::max<int64_t>(1, std::min<int64_t>(a.R / 128, 4 * sms / ((C + 63) / 64))));
+  float *w_out = a.want_w ? dw.data_ptr<float>() : nullptr, *b_out = a.want_b ? db.data_ptr<float>() : nullptr;
+  float *pw = w_out, *pb = b_out;  // where the sums (or the partial rows) go
   torch::Tensor part;
-  float *pw = nullptr, *pb = nullptr;
-  if (grads) {
+  if (grads && P > 1) {
     part = torch::empty({2, P, C}, dw.options());
     pw = a.want_w ? part.data_ptr<float>() : nullptr;
     pb = a.want_b ? part.data_ptr<float>() + static_cast<int64_t>(P) * C : nullptr;
   }
-  const size_t smem = rpb > 1 && grads ? static_cast<size_t>(rpb) * C * sizeof(float) : 0;
-#define NORI_LN_BWD(TPR, VPL)                                                                                  \
-  bwd_kernel<T, U, VEC, TPR, VPL>                                                                              \
-      <<<P, kThreads, smem, stream>>>(dy, a.ldy, x, a.ldx, a.R, C, a.mean, a.rstd, a.w, dx, pw, pb)
-  if (C <= 64) NORI_LN_BWD(8, 8);
-  else if (C <= 256) NORI_LN_BWD(32, 8);
-  else if (C <= 512) NORI_LN_BWD(32, 16);
-  else if (C <= 1024) NORI_LN_BWD(32, 32);
-  else if (C <= 2048) NORI_LN_BWD(256, 8);
-  else if (C <= 4096) NORI_LN_BWD(256, 16);
-  else if (C <= kMaxRegCols) NORI_LN_BWD(256, 32);
-  else {
-    bwd_wide_kernel<T, U><<<static_cast<unsigned>(std::min<int64_t>(a.R, 148 * 8)), kThreads, 0, stream>>>(
+  float *rw = columns ? nullptr : pw, *rb = columns ? nullptr : pb;
+  const int n = static_cast<int>(ctas);
+  if (C <= 128) launch_rows<T, U, VEC, 8>(dy, x, dx, a, n, rw, rb);
+  else if (C <= 512) launch_rows<T, U, VEC, 32>(dy, x, dx, a, n, rw, rb);
+  else if (C <= 2048) launch_rows<T, U, VEC, 128>(dy, x, dx, a, n, rw, rb);
+  else if (C <= kMaxRegCols) launch_rows<T, U, VEC, 512>(dy, x, dx, a, n, rw, rb);
+  else
+    bwd_wide_kernel<T, U><<<static_cast<unsigned>(std::min<int64_t>(a.R, sms * 4)), 512, 0, stream>>>(
         dy, a.ldy, x, a.ldx, a.R, C, a.mean, a.rstd, a.w, dx);
-    if (grads) {
-      C10_CUDA_KERNEL_LAUNCH_CHECK();
-      colgrad_kernel<T, U><<<dim3((C + 31) / 32, P), kThreads, 0, stream>>>(dy, a.ldy, x, a.ldx, a.R, C, a.mean,
-                                                                            a.rstd, pw, pb);
-    }
-  }
-#undef NORI_LN_BWD
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (grads) {
-    reduce_kernel<<<dim3((C + 31) / 32, 2), kThreads, 0, stream>>>(pw, pb, P, C, a.want_w ? dw.data_ptr<float>() : nullptr,
-                                                                   a.want_b ? db.data_ptr<float>() : nullptr);
+  if (columns) {
+    colgrad_kernel<T, U><<<dim3((C + 63) / 64, P), 512, 0, stream>>>(dy, a.ldy, x, a.ldx, a.R, C, a.mean, a.rstd, pw,
+                                                                     pb);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  if (grads && P > 1) {
+    reduce_kernel<<<dim3((C + 31) / 32, 2), 1024, 0, stream>>>(pw, pb, P, C, w_out, b_out);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
 }
@@ -248,7 +283,7 @@ static void run(const torch::Tensor& dy, const torch::Tensor& x, torch::Tensor& 
   const T* xp = reinterpret_cast<const T*>(x.data_ptr());
   T* dxp = reinterpret_cast<T*>(dx.data_ptr());
   const bool vec = vec_ok(dyp, a.ldy, a.C, sizeof(U), VEC) && vec_ok(xp, a.ldx, a.C, sizeof(T), VEC) &&
-                   vec_ok(dxp, a.C, a.C, sizeof(T), VEC) && vec_ok(a.w, 0, a.C, 4, VEC);
+                   vec_ok(dxp, a.C, a.C, sizeof(T), VEC) && vec_ok(a.w, 0, a.C, 4, 4);
   if (vec)
     launch<T, U, VEC>(dyp, xp, dxp, a, dw, db);
   else

@@ -8,67 +8,79 @@
 namespace nori {
 namespace ln {
 
-template <typename T, typename U, int VEC, int TPR, int VPL>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int C,
-                                                       const float* __restrict__ w, const float* __restrict__ b,
-                                                       float eps, U* __restrict__ y, float* __restrict__ mean_out,
-                                                       float* __restrict__ rstd_out) {
-  constexpr int CH = VPL / VEC, RPB = kThreads / TPR;
-  __shared__ float sh[32];
+template <typename T, typename U, int VEC, int TPR>
+__global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int C,
+                                                        const float* __restrict__ w, const float* __restrict__ b,
+                                                        float eps, U* __restrict__ y, float* __restrict__ mean_out,
+                                                        float* __restrict__ rstd_out) {
+  constexpr int CH = kValues / VEC, RPB = kCta<TPR> / TPR;
+  __shared__ float sh[2][2][16];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv_c = 1.f / static_cast<float>(C);
   int flip = 0;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * RPB; base < R; base += static_cast<int64_t>(gridDim.x) * RPB) {
+  // a CTA's rows: 2 RPB neighbours, RPB apart within a group
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (2 * RPB); base < R;
+       base += static_cast<int64_t>(gridDim.x) * (2 * RPB)) {
     const int64_t row = base + g;
-    const bool ok = row < R;
-    float v[VPL];
-    float s = 0.f;
+    float v[2][kValues], s[2] = {0.f, 0.f}, mean[2], rstd[2];
+    {
+      Row<T, VEC, TPR> r[2];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int c = VEC * (t + TPR * j);
-      if (ok && c < C) {
-        load_vec<T, VEC>(x + row * ldx + c, v + VEC * j);
-      } else {
+      for (int k = 0; k < 2; ++k) r[k].load(x, ldx, row + k * RPB, R, C, t);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[VEC * j + i] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s += v[VEC * j + i];
+      for (int k = 0; k < 2; ++k) r[k].values(v[k]);
     }
-    const float mean = row_sum<TPR>(s, sh + flip * 16) * inv_c;
-    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) s[k] += v[k][i];
+    row_sum<TPR, 2>(s, sh, flip);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      mean[k] = s[k] * inv_c;
+      s[k] = 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       if (VEC * (t + TPR * j) < C) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          v[VEC * j + i] -= mean;
-          ss += v[VEC * j + i] * v[VEC * j + i];
-        }
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = VEC * j; i < VEC * (j + 1); ++i) {
+            v[k][i] -= mean[k];
+            s[k] += v[k][i] * v[k][i];
+          }
       }
     }
-    const float rstd = rsqrtf(row_sum<TPR>(ss, sh + flip * 16 + 8) * inv_c + eps);
-    flip ^= 1;  // the other half of `sh`: this row's sums may still be read
-    if (!ok) continue;
+    row_sum<TPR, 2>(s, sh, flip);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) rstd[k] = rsqrtf(s[k] * inv_c + eps);
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const int c = VEC * (t + TPR * j);
       if (c < C) {
-        float o[VEC], wv[VEC], bv[VEC];
-        if (w != nullptr) load_vec<float, VEC>(w + c, wv);
-        if (b != nullptr) load_vec<float, VEC>(b + c, bv);
+        float wv[VEC], bv[VEC];
+        load_columns<VEC>(w, c, 1.f, wv);
+        load_columns<VEC>(b, c, 0.f, bv);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          o[i] = v[VEC * j + i] * rstd;
-          if (w != nullptr) o[i] *= wv[i];
-          if (b != nullptr) o[i] += bv[i];
+        for (int k = 0; k < 2; ++k) {
+          if (row + k * RPB < R) {
+            float o[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] = v[k][VEC * j + i] * rstd[k] * wv[i] + bv[i];
+            store_vec<U, VEC>(y + (row + k * RPB) * static_cast<int64_t>(C) + c, o);
+          }
         }
-        store_vec<U, VEC>(y + row * static_cast<int64_t>(C) + c, o);
       }
     }
     if (t == 0) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (row + k * RPB < R) {
+          mean_out[row + k * RPB] = mean[k];
+          rstd_out[row + k * RPB] = rstd[k];
+        }
+      }
     }
   }
 }
@@ -76,27 +88,27 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const T* __restrict__ x, 
 // Rows wider than the registers of a CTA: three passes over the row (the second and third
 // hit L2 for all but the widest).
 template <typename T, typename U>
-__global__ void __launch_bounds__(kThreads) fwd_wide_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int C,
-                                                            const float* __restrict__ w, const float* __restrict__ b,
-                                                            float eps, U* __restrict__ y,
-                                                            float* __restrict__ mean_out,
-                                                            float* __restrict__ rstd_out) {
-  __shared__ float sh[32];
+__global__ void __launch_bounds__(512) fwd_wide_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int C,
+                                                       const float* __restrict__ w, const float* __restrict__ b,
+                                                       float eps, U* __restrict__ y, float* __restrict__ mean_out,
+                                                       float* __restrict__ rstd_out) {
+  __shared__ float sh[2][1][16];
   const float inv_c = 1.f / static_cast<float>(C);
   int flip = 0;
   for (int64_t row = blockIdx.x; row < R; row += gridDim.x) {
     const T* xr = x + row * ldx;
-    float s = 0.f;
-    for (int c = threadIdx.x; c < C; c += kThreads) s += to_f32<T>(xr[c]);
-    const float mean = row_sum<kThreads>(s, sh + flip * 16) * inv_c;
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < C; c += kThreads) {
+    float s[1] = {0.f};
+    for (int c = threadIdx.x; c < C; c += 512) s[0] += to_f32<T>(xr[c]);
+    row_sum<512, 1>(s, sh, flip);
+    const float mean = s[0] * inv_c;
+    s[0] = 0.f;
+    for (int c = threadIdx.x; c < C; c += 512) {
       const float d = to_f32<T>(xr[c]) - mean;
-      ss += d * d;
+      s[0] += d * d;
     }
-    const float rstd = rsqrtf(row_sum<kThreads>(ss, sh + flip * 16 + 8) * inv_c + eps);
-    flip ^= 1;
-    for (int c = threadIdx.x; c < C; c += kThreads) {
+    row_sum<512, 1>(s, sh, flip);
+    const float rstd = rsqrtf(s[0] * inv_c + eps);
+    for (int c = threadIdx.x; c < C; c += 512) {
       float o = (to_f32<T>(xr[c]) - mean) * rstd;
       if (w != nullptr) o *= w[c];
       if (b != nullptr) o += b[c];
@@ -113,20 +125,18 @@ template <typename T, typename U, int VEC>
 static void launch(const T* x, int64_t ldx, int64_t R, int C, const float* w, const float* b, float eps, U* y,
                    float* mean, float* rstd) {
   auto stream = at::cuda::getCurrentCUDAStream();
-  const int64_t cap = 148 * 8;
-#define NORI_LN_FWD(TPR, VPL)                                                                                       \
-  fwd_kernel<T, U, VEC, TPR, VPL>                                                                                   \
-      <<<static_cast<unsigned>(std::min<int64_t>((R + kThreads / TPR - 1) / (kThreads / TPR), cap)), kThreads, 0,  \
-         stream>>>(x, ldx, R, C, w, b, eps, y, mean, rstd)
-  if (C <= 64) NORI_LN_FWD(8, 8);
-  else if (C <= 256) NORI_LN_FWD(32, 8);
-  else if (C <= 512) NORI_LN_FWD(32, 16);
-  else if (C <= 1024) NORI_LN_FWD(32, 32);
-  else if (C <= 2048) NORI_LN_FWD(256, 8);
-  else if (C <= 4096) NORI_LN_FWD(256, 16);
-  else if (C <= kMaxRegCols) NORI_LN_FWD(256, 32);
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+#define NORI_LN_FWD(TPR)                                                                                            \
+  fwd_kernel<T, U, VEC, TPR>                                                                                        \
+      <<<static_cast<unsigned>(std::min<int64_t>((R + 2 * kCta<TPR> / TPR - 1) / (2 * kCta<TPR> / TPR),            \
+                                                 sms * (768 / kCta<TPR>))),                                      \
+         kCta<TPR>, 0, stream>>>(x, ldx, R, C, w, b, eps, y, mean, rstd)
+  if (C <= 128) NORI_LN_FWD(8);
+  else if (C <= 512) NORI_LN_FWD(32);
+  else if (C <= 2048) NORI_LN_FWD(128);
+  else if (C <= kMaxRegCols) NORI_LN_FWD(512);
   else
-    fwd_wide_kernel<T, U><<<static_cast<unsigned>(std::min<int64_t>(R, cap)), kThreads, 0, stream>>>(
+    fwd_wide_kernel<T, U><<<static_cast<unsigned>(std::min<int64_t>(R, sms * 4)), 512, 0, stream>>>(
         x, ldx, R, C, w, b, eps, y, mean, rstd);
 #undef NORI_LN_FWD
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -139,9 +149,8 @@ static void run(const torch::Tensor& x, const float* w, const float* b, float ep
   const T* xp = reinterpret_cast<const T*>(x.data_ptr());
   U* yp = reinterpret_cast<U*>(y.data_ptr());
   const int64_t R = x.size(0), C = x.size(1), ldx = x.stride(0);
-  const bool vec = vec_ok(xp, ldx, C, sizeof(T), VEC) && vec_ok(yp, C, C, sizeof(U), VEC) &&
-                   vec_ok(w, 0, C, 4, 4) && vec_ok(b, 0, C, 4, 4) &&
-                   (VEC == 4 || (vec_ok(w, 0, C, 4, 8) && vec_ok(b, 0, C, 4, 8)));
+  const bool vec = vec_ok(xp, ldx, C, sizeof(T), VEC) && vec_ok(yp, C, C, sizeof(U), VEC) && vec_ok(w, 0, C, 4, 4) &&
+                   vec_ok(b, 0, C, 4, 4);
   if (vec)
     launch<T, U, VEC>(xp, ldx, R, static_cast<int>(C), w, b, eps, yp, mean.data_ptr<float>(), rstd.data_ptr<float>());
   else

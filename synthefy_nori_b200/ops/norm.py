@@ -19,6 +19,8 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t [..., C]`` as [R, C] with contiguous columns (a view where the strides allow it)."""
+    if t.dim() == 2 and t.stride(1) == 1 and t.shape[1] and t.stride(0) >= 0:
+        return t
     if t.dim() == 0:
         raise ValueError("layer_norm: at least one dimension expected")
     t = t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(0, 0)
@@ -37,7 +39,9 @@ def _check(x: torch.Tensor, out_dtype) -> bool:
 
 
 def _vec(v):
-    return None if v is None else v.detach().to(torch.float32).contiguous()
+    if v is None or (v.dtype == torch.float32 and v.is_contiguous()):
+        return v
+    return v.detach().to(torch.float32).contiguous()
 
 
 def layer_norm_fwd(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dtype=None):
@@ -45,7 +49,7 @@ def layer_norm_fwd(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, o
     ``out_dtype``, fp32); ``mean`` and ``rstd`` are fp32, one per row."""
     f32 = _check(x, out_dtype)
     y, mean, rstd = _lib().layer_norm_fwd(_rows(x.detach()), _vec(weight), _vec(bias), float(eps), f32)
-    return y.view(x.shape), mean, rstd
+    return y if x.dim() == 2 else y.view(x.shape), mean, rstd
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None, *,
@@ -56,7 +60,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     weight_grad = weight is not None if weight_grad is None else weight_grad
     dx, dw, db = _lib().layer_norm_bwd(_rows(dy.detach()), _rows(x.detach()), mean, rstd, _vec(weight),
                                        bool(weight_grad), bool(bias_grad))
-    return dx.view(x.shape), dw if weight_grad else None, db if bias_grad else None
+    return dx if x.dim() == 2 else dx.view(x.shape), dw if weight_grad else None, db if bias_grad else None
 
 
 class _LayerNorm(torch.autograd.Function):
