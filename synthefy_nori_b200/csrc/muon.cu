@@ -2,6 +2,10 @@
 // whole GPU, and the checks of the arguments.
 #include "muon.cuh"
 
+#include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <c10/cuda/CUDAStream.h>
+
 namespace nori {
 namespace muon {
 
@@ -116,8 +120,32 @@ void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mo
     run_count += groups[i + 1];
     run_smem = std::max(run_smem, fit.smem);
   }
-  if (!large.empty()) run_large(kSrcMuon, nullptr, kOutMuon, nullptr, s, large, k, status, data.options());
+  auto whole = [&]() { run_large(kSrcMuon, nullptr, kOutMuon, nullptr, s, large, k, status, data.options()); };
+  if (large.empty() || run_count == 0 ||
+      at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+    if (!large.empty()) whole();
+    flush();
+    return;
+  }
+  // The two sets touch different matrices: the large ones, a chain of dependent products that
+  // seldom fills the GPU, run on a stream of higher priority beside the single CTAs.  (Not
+  // under capture, where a stream of the pool could belong to someone else.)
+  auto main = at::cuda::getCurrentCUDAStream();
+  auto side = at::cuda::getStreamFromPool(true, data.get_device());
+  at::cuda::CUDAEvent fork, join;
+  fork.record(main);
+  fork.block(side);
+  try {
+    c10::cuda::CUDAStreamGuard on(side);
+    whole();
+  } catch (...) {  // what was launched is still ordered before the caller's next work
+    join.record(side);
+    join.block(main);
+    throw;
+  }
+  join.record(side);
   flush();
+  join.block(main);
 }
 
 // Whether a matrix of this shape runs its whole step in one CTA.

@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
 //   blocks of matrices (their buffers fit L2 together; every shape spread over all blocks)
 //     steps
 //       A = xi^2 Z^T Z        128 x 128 tiles on and above the diagonal, then mirrored
-//       C = (b A + c A^2)/a   the same tiles
-//       Z += Z C              128 x 256 tiles (the last step writes the result instead)
+//       I + C = I + (b A + c A^2) / a   the same tiles
+//       Z <- Z C + Z          128 x 256 tiles (the last step writes the result instead)
 //
 // A tile needs all tiles of its own matrix's previous product: a counter per matrix, raised
 // when a tile's stores are complete, tells (release / acquire at GPU scope).  Tiles of other
@@ -231,22 +231,34 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
 // fill in among the others.  The launch is cooperative (every CTA resident), and a tile only
 // waits for tiles before it in the shared order, so the oldest unfinished tile can always run.
 //
-// Roles (384 threads): warp 0 loads operands by TMA into a ring of 16 KB units (128 x 64,
-// 128B-swizzled; MN-major for the Gram product, K-major otherwise), one thread of warp 1
-// issues tcgen05.mma (M = 128, N <= 128 per unit of the second operand) into two TMEM
-// accumulators, warps 2..9 run the epilogue on 64-column boxes, warp 10 loads the boxes that
-// an epilogue reads (Z's pair, or A) and warp 11 stores what it leaves there (Z's pair, or
-// A / C and their mirror image), both by TMA: the epilogue itself only touches tensor and
-// shared memory.
+// Roles (384 threads): warp 0 loads operands by TMA (128B-swizzled) into a ring of 48 KB
+// stages: 96 rows of Z for the Gram product (both operands MN-major: the sum runs over rows),
+// 64 columns of the rows of A or Z and C otherwise (K-major); one thread of warp 1 issues
+// tcgen05.mma (M = 128, N <= 256, K = 16) into two TMEM accumulators; warps 2..9 run the
+// epilogue on 64-column boxes, warp 10 loads the boxes that an epilogue reads (Z's low half, or
+// A) and warp 11 stores what it leaves there (Z's pair, or A / C and their mirror image), both
+// by TMA: the epilogue itself only touches tensor and shared memory.
+//
+// What bounds the update is the SM's shared memory: per 128 x 256 tile at K = 448 the MMAs
+// read 336 KB, the loads write 336 + 64 KB, the epilogue reads 64 and writes 128 KB and the
+// stores read 128 KB, about 8,300 of its cycles against 3,600 of the tensor core.  Hence N = 256
+// (two MMAs of 128 read the first operand twice: 112 KB more), and the high half of Z is not
+// loaded for the epilogue at all: C is kept as I + C, so that Z's high half comes out of the
+// product itself and only the low half is added.  (Rounding the diagonal of I + C to fp16 scales
+// Z's columns by 1 + 2^-12 at most, which no direction amplifies.)
 constexpr int kThreads = 384;
-constexpr int kUnits = 8, kUnitBytes = 16384;
-constexpr int kSlots = 3, kSlotBytes = 32768;
-constexpr int kSmemBytes = kUnits * kUnitBytes + kSlots * kSlotBytes + 1024 + 512;
+constexpr int kStages = 3, kStageBytes = 49152;
+constexpr int kGramK = 96, kGramPanel = kGramK * 128;  // rows of a stage, bytes of 64 columns
+constexpr int kSlots = 2, kSlotBytes = 32768;
+constexpr int kSmemBytes = kStages * kStageBytes + kSlots * kSlotBytes + 1024 + 512;
 
 enum Phase : int { kGram = 0, kPoly = 1, kUpdate = 2 };
 
 struct alignas(64) Maps {
-  CUtensorMap z[2], zl, A, C;    // boxes of 64 columns x 64 rows
+  CUtensorMap z[2], zl, A, C;    // boxes of 64 columns x 64 rows: the epilogue's
+  CUtensorMap zg[2];             // of 96 rows: MN-major operands
+  CUtensorMap zk[2], Ak, Ck;     // of 128 rows: K-major operands
+  CUtensorMap Ck2;               // of 256 rows
 };
 struct Args {
   Maps maps[kMaxShapes];
@@ -367,11 +379,11 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
 
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* units = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* slots = units + kUnits * kUnitBytes;
+  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* slots = stages + kStages * kStageBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(slots + kSlots * kSlotBytes);
-  uint64_t* empty = full + kUnits;
-  uint64_t* tfull = empty + kUnits;
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* sfull = tempty + 2;     // a slot is the epilogue's (its loads have landed)
   uint64_t* sdone = sfull + kSlots; // the epilogue has left it
@@ -384,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   if (a.out_type == kOutMuon && step_rejected(a.s)) return;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kUnits; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -410,85 +422,84 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 
   if (warp == 0) {
     if (elect_one()) {
-      int u = 0;
+      int stage = 0;
       uint32_t phase = 0;
-      // 128 x 64 operand values: two boxes, at (x, y) and beside it or below it
-      auto load = [&](const CUtensorMap* map, int x, int y, int dx, int dy, int z) -> bool {
-        if (!mbar_wait(&empty[u], phase ^ 1, a.status, kTimeoutProducer, abort_flag)) return false;
-        uint8_t* d = units + u * kUnitBytes;
-        mbar_arrive_expect_tx(&full[u], kUnitBytes);
-        tma_load_3d(d, map, &full[u], x, y, z);
-        tma_load_3d(d + 8192, map, &full[u], x + dx, y + dy, z);
-        if (++u == kUnits) {
-          u = 0;
-          phase ^= 1;
-        }
-        return true;
-      };
       bool ok = true;
       for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x) {
         const Item x = item_of(a, cur, t);
         const Group& q = a.g[x.g];
         const Maps& mp = a.maps[x.g];
-        const CUtensorMap* mz = &mp.z[x.it & 1];
         if (!wait_done(a, x, abort_flag)) break;
-        const int kbs = ((x.ph == kGram ? q.n : q.m) + 63) / 64;
-        const int nu = (x.ncols + 127) / 128;
-        for (int kb = 0; kb < kbs && ok; ++kb) {
-          const int k0 = kb * 64;
-          if (x.ph == kGram) {
-            ok = load(mz, x.ti * 128, k0, 64, 0, x.mat);
-            if (!x.diag) ok = ok && load(mz, x.tj * 128, k0, 64, 0, x.mat);
-          } else if (x.ph == kPoly) {
-            ok = load(&mp.A, k0, x.ti * 128, 0, 64, x.mat);
-            if (!x.diag) ok = ok && load(&mp.A, k0, x.tj * 128, 0, 64, x.mat);
+        const bool gram = x.ph == kGram, two = x.ncols > 128;
+        const int K = gram ? q.n : q.m, row = x.ti * 128, kstep = gram ? kGramK : 64;
+        const CUtensorMap* ma = gram ? &mp.zg[x.it & 1] : x.ph == kPoly ? &mp.Ak : &mp.zk[x.it & 1];
+        const CUtensorMap* mb = x.ph == kPoly ? &mp.Ak : two ? &mp.Ck2 : &mp.Ck;
+        const uint32_t half = gram ? 2 * kGramPanel : 16384;  // bytes of the first operand
+        const uint32_t bytes = half + (x.diag ? 0 : gram ? 2 * kGramPanel : two ? 32768 : 16384);
+        for (int k0 = 0; k0 < K; k0 += kstep) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = stages + stage * kStageBytes;
+          uint64_t* bar = &full[stage];
+          mbar_arrive_expect_tx(bar, bytes);
+          if (gram) {
+            tma_load_3d(sa, ma, bar, row, k0, x.mat);
+            tma_load_3d(sa + kGramPanel, ma, bar, row + 64, k0, x.mat);
+            if (!x.diag) {
+              tma_load_3d(sa + 2 * kGramPanel, ma, bar, x.n0, k0, x.mat);
+              tma_load_3d(sa + 3 * kGramPanel, ma, bar, x.n0 + 64, k0, x.mat);
+            }
           } else {
-            ok = load(mz, k0, x.ti * 128, 0, 64, x.mat);
-            for (int j = 0; j < nu; ++j) ok = ok && load(&mp.C, k0, x.n0 + j * 128, 0, 64, x.mat);
+            tma_load_3d(sa, ma, bar, k0, row, x.mat);
+            if (!x.diag) tma_load_3d(sa + 16384, mb, bar, k0, x.n0, x.mat);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
           }
         }
       }
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      int u = 0, acc = 0;
+      int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
+      const uint32_t stages_lo = smem_u32(stages) >> 4;
       bool ok = true;
       for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x) {
         const Item x = item_of(a, cur, t);
         const Group& q = a.g[x.g];
-        const int K = x.ph == kGram ? q.n : q.m;
-        const int kbs = (K + 63) / 64, nu = (x.ncols + 127) / 128;
-        const bool mn = x.ph == kGram;
-        const uint32_t i0 = idesc_f16(min(128, (x.ncols + 15) / 16 * 16), mn);
-        const uint32_t i1 = idesc_f16(nu > 1 ? (x.ncols - 128 + 15) / 16 * 16 : 16, mn);
+        const bool gram = x.ph == kGram;
+        const int K = gram ? q.n : q.m, kstep = gram ? kGramK : 64;
+        const uint32_t idesc = idesc_f16((x.ncols + 15) / 16 * 16, gram);
+        // descriptors without the address (their low 14 bits, in 16-byte units), and the steps
+        // of 16 along K: 16 rows of an MN-major panel, 32 bytes of a K-major row; a tile on the
+        // diagonal multiplies its rows by themselves
+        const uint64_t dbase = gram ? umma_smem_desc(0, kGramPanel, 1024, 2) : umma_smem_desc(0, 16, 1024, 2);
+        const uint32_t inc = gram ? 2048 / 16 : 32 / 16;
+        const uint32_t second = x.diag ? 0 : (gram ? 2 * kGramPanel : 16384) / 16;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kTimeoutMma, abort_flag)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * 256;
-        for (int kb = 0; kb < kbs; ++kb) {
-          int unit[3];
-          const int cnt = x.diag ? 1 : 1 + nu;
-          for (int j = 0; j < cnt && ok; ++j) {
-            unit[j] = u;
-            ok = mbar_wait(&full[u], phase, a.status, kTimeoutMma, abort_flag);
-            if (++u == kUnits) {
-              u = 0;
-              phase ^= 1;
-            }
+        for (int k0 = 0; k0 < K; k0 += kstep) {
+          if (!mbar_wait(&full[stage], phase, a.status, kTimeoutMma, abort_flag)) {
+            ok = false;
+            break;
           }
-          if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(units + unit[0] * kUnitBytes);
-          const int k16 = min(4, (K - kb * 64 + 15) / 16);  // the rest of the boxes is zero fill
-          for (int j = 0; j < nu; ++j) {
-            const uint32_t sb = x.diag ? sa : smem_u32(units + unit[1 + j] * kUnitBytes);
-            for (int k = 0; k < k16; ++k) {
-              const uint64_t da = mn ? umma_smem_desc(sa + k * 2048, 8192, 1024, 2) : umma_desc_kmajor_sw128(sa + k * 32);
-              const uint64_t db = mn ? umma_smem_desc(sb + k * 2048, 8192, 1024, 2) : umma_desc_kmajor_sw128(sb + k * 32);
-              umma_bf16_ss(d + j * 128, da, db, j == 0 ? i0 : i1, (kb > 0 || k > 0) ? 1u : 0u);
-            }
+          const uint64_t da = dbase + (stages_lo + stage * (kStageBytes / 16)), db = da + second;
+          const uint32_t more = k0 > 0 ? 1u : 0u;
+          const int steps = (min(kstep, K - k0) + 15) / 16;  // the rest of the boxes is zero fill
+#pragma unroll
+          for (int k = 0; k < kGramK / 16; ++k)
+            if (k < steps) umma_bf16_ss(d, da + k * inc, db + k * inc, idesc, k > 0 ? 1u : more);
+          umma_commit(&empty[stage]);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
           }
-          for (int j = 0; j < cnt; ++j) umma_commit(&empty[unit[j]]);
         }
         if (!ok) break;
         umma_commit(&tfull[acc]);
@@ -537,6 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
               unpack8(*cell, s);
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[8 * j + i] = a.k.ba * s[i] + a.k.ca * v[8 * j + i];
+              if (x.diag) {  // I + C
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (c + half * 32 + 8 * j + i == rt) v[8 * j + i] += 1.f;
+              }
             }
             *cell = pack8(v + 8 * j);
           }
@@ -553,12 +569,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int off = ((half * 4 + j) ^ x7) << 4;
-            float h[8], l[8];
-            unpack8(*reinterpret_cast<const uint4*>(row0 + off), h);
+            float l[8];
             unpack8(*reinterpret_cast<const uint4*>(row1 + off), l);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[8 * j + i] += h[i] + l[i];
+            for (int i = 0; i < 8; ++i) v[8 * j + i] += l[i];
             if (!x.last) {
+              float h[8];
               const uint4 hi = pack8(v + 8 * j);
               unpack8(hi, h);
 #pragma unroll
@@ -640,7 +656,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x) {
         const Item x = item_of(a, cur, t);
         const Maps& mp = a.maps[x.g];
-        const CUtensorMap* mz = &mp.z[x.it & 1];
         if (x.ph != kGram && !wait_done(a, x, abort_flag)) break;
         for (int c = 0; c < x.ncols && ok; c += 64) {
           ok = mbar_wait(&sfree[slot], phase ^ 1, a.status, kTimeoutProducer, abort_flag);
@@ -655,9 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             tma_load_3d(s0, &mp.A, bar, col, row, x.mat);
             tma_load_3d(s0 + 8192, &mp.A, bar, col, row + 64, x.mat);
           } else {
-            mbar_arrive_expect_tx(bar, 32768);
-            tma_load_3d(s0, mz, bar, col, row, x.mat);
-            tma_load_3d(s0 + 8192, mz, bar, col, row + 64, x.mat);
+            mbar_arrive_expect_tx(bar, 16384);
             tma_load_3d(s0 + 16384, &mp.zl, bar, col, row, x.mat);
             tma_load_3d(s0 + 24576, &mp.zl, bar, col, row + 64, x.mat);
           }
@@ -728,10 +741,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------------ host
-static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int batch) {
+static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int batch, int box_rows) {
   const int64_t dims[3] = {cols, rows, batch};
   const int64_t strides[2] = {static_cast<int64_t>(ld) * 2, static_cast<int64_t>(ld) * rows * 2};
-  const int box[3] = {64, 64, 1};
+  const int box[3] = {64, box_rows, 1};
   return make_tmap_nd_bf16(const_cast<__half*>(base), 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
 }
@@ -791,10 +804,18 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
     q.zl = reinterpret_cast<__half*>(w + at[i][2]);
     q.A = reinterpret_cast<__half*>(w + at[i][3]);
     q.C = reinterpret_cast<__half*>(w + at[i][4]);
-    a.maps[i] = {{map_f16(q.z[0], q.m, q.n, q.ldz, q.count), map_f16(q.z[1], q.m, q.n, q.ldz, q.count)},
-                 map_f16(q.zl, q.m, q.n, q.ldz, q.count),
-                 map_f16(q.A, q.m, q.m, q.ldz, q.count),
-                 map_f16(q.C, q.m, q.m, q.ldz, q.count)};
+    Maps& mp = a.maps[i];
+    for (int j = 0; j < 2; ++j) {
+      mp.z[j] = map_f16(q.z[j], q.m, q.n, q.ldz, q.count, 64);
+      mp.zg[j] = map_f16(q.z[j], q.m, q.n, q.ldz, q.count, kGramK);
+      mp.zk[j] = map_f16(q.z[j], q.m, q.n, q.ldz, q.count, 128);
+    }
+    mp.zl = map_f16(q.zl, q.m, q.n, q.ldz, q.count, 64);
+    mp.A = map_f16(q.A, q.m, q.m, q.ldz, q.count, 64);
+    mp.Ak = map_f16(q.A, q.m, q.m, q.ldz, q.count, 128);
+    mp.C = map_f16(q.C, q.m, q.m, q.ldz, q.count, 64);
+    mp.Ck = map_f16(q.C, q.m, q.m, q.ldz, q.count, 128);
+    mp.Ck2 = map_f16(q.C, q.m, q.m, q.ldz, q.count, 256);
     a.g[i] = q;
   }
   p.groups = ns;
@@ -827,8 +848,18 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
   }
 #undef NORI_MUON_SRC
   C10_CUDA_CHECK(cudaFuncSetAttribute(product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  // no more CTAs than the widest product has tiles
+  int64_t widest = 1;
+  for (int ph = 0; ph < 2; ++ph) {
+    int64_t n = 0;
+    for (int i = 0; i < ns; ++i) {
+      const Group& q = p.g[i];
+      n += (q.count + a.blocks - 1) / a.blocks * static_cast<int64_t>(ph == 0 ? q.nt * (q.nt + 1) / 2 : q.tm * q.tn);
+    }
+    widest = std::max(widest, n);
+  }
   const int sms = persistent_sms(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, sms));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(widest, sms));
   void* argv[] = {&a};
   C10_CUDA_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(product_kernel), dim3(grid), dim3(kThreads),
                                              argv, kSmemBytes, stream));
