@@ -150,8 +150,9 @@ void adamw_ema(torch::Tensor& p, const torch::Tensor& g, torch::Tensor& m, torch
                double wd, int64_t step, double ema_decay, double max_norm, double grad_scale, const c10::optional<torch::Tensor>& skip);
 std::vector<torch::Tensor> quantize_int8(const torch::Tensor& x);
 void dequantize_int8(const torch::Tensor& q, const torch::Tensor& scale, torch::Tensor& out);
-void newton_schulz(const torch::Tensor& g, torch::Tensor& out, int64_t steps, double eps, std::vector<double> coeffs,
-                   const torch::Tensor& status);
+torch::Tensor newton_schulz(const torch::Tensor& g, const c10::optional<torch::Tensor>& out_opt,
+                            c10::optional<c10::ScalarType> out_type, int64_t steps, double eps,
+                            std::vector<double> coeffs, const torch::Tensor& status);
 void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mom,
                const c10::optional<torch::Tensor>& ema, const torch::Tensor& table, std::vector<int64_t> groups,
                double lr, double wd, double momentum, bool nesterov, int64_t steps, double eps,

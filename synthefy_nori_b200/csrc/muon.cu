@@ -28,33 +28,40 @@ static const float* opt_scalar(const c10::optional<torch::Tensor>& t, const torc
 
 }  // namespace muon
 
-// O = Newton-Schulz(G) for contiguous G [batch, rows, cols] (fp32, bf16 or fp16) into out.
-void newton_schulz(const torch::Tensor& g, torch::Tensor& out, int64_t steps, double eps, std::vector<double> coeffs,
-                   const torch::Tensor& status) {
+// Newton-Schulz of every matrix of contiguous g [.., rows, cols] (fp32, bf16 or fp16), into
+// `out` (contiguous, of g's shape) or a new tensor of `out_type`.
+torch::Tensor newton_schulz(const torch::Tensor& g, const c10::optional<torch::Tensor>& out_opt,
+                            c10::optional<c10::ScalarType> out_type, int64_t steps, double eps,
+                            std::vector<double> coeffs, const torch::Tensor& status) {
   using namespace muon;
-  TORCH_CHECK(g.is_cuda() && g.dim() == 3 && g.is_contiguous(), "newton_schulz: contiguous CUDA [batch, rows, cols]");
-  TORCH_CHECK(out.device() == g.device() && out.is_contiguous() && out.sizes() == g.sizes(),
-              "newton_schulz: out must be contiguous, of g's shape and device");
-  auto kind = [](const torch::Tensor& t, const char* what) {
-    const auto s = t.scalar_type();
+  TORCH_CHECK(g.is_cuda() && g.dim() >= 2 && g.is_contiguous(), "newton_schulz: contiguous CUDA [.., rows, cols]");
+  auto kind = [](c10::ScalarType s, const char* what) {
     TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, "newton_schulz: ", what,
                 " must be fp32, bf16 or fp16");
     return s == at::kFloat ? 0 : s == at::kBFloat16 ? 1 : 2;
   };
-  const int src = kind(g, "g"), dst = kind(out, "out");
   const Coeffs k = make_coeffs(steps, eps, coeffs, "newton_schulz");
-  TORCH_CHECK(g.size(1) < kMaxDim && g.size(2) < kMaxDim, "newton_schulz: at most 2^20 rows and columns");
-  if (g.numel() == 0) return;
+  const int src = kind(g.scalar_type(), "g");
+  const int64_t rows = g.size(-2), cols = g.size(-1);
+  TORCH_CHECK(rows < kMaxDim && cols < kMaxDim, "newton_schulz: at most 2^20 rows and columns");
   const at::cuda::CUDAGuard guard(g.device());
-  const Fit fit = single_fit(static_cast<int>(g.size(1)), static_cast<int>(g.size(2)));
-  if (fit.ok) {
-    TORCH_CHECK(g.size(0) <= INT_MAX, "newton_schulz: at most 2^31 - 1 matrices");
-    run_single(src, g.data_ptr(), dst, out.data_ptr(), StepArgs{}, 0, g.size(0), static_cast<int>(g.size(1)),
-               static_cast<int>(g.size(2)), fit.smem, k, status);
-    return;
-  }
-  run_large(src, g.data_ptr(), dst, out.data_ptr(), StepArgs{},
-            {Shape{0, g.size(0), static_cast<int>(g.size(1)), static_cast<int>(g.size(2))}}, k, status, g.options());
+  torch::Tensor out = out_opt.has_value() && out_opt->defined()
+                          ? *out_opt
+                          : torch::empty(g.sizes(), g.options().dtype(out_type.value_or(g.scalar_type())));
+  TORCH_CHECK(out.device() == g.device() && out.is_contiguous() && out.sizes() == g.sizes(),
+              "newton_schulz: out must be contiguous, of g's shape and device");
+  const int dst = kind(out.scalar_type(), "out");
+  if (g.numel() == 0) return out;
+  const int64_t batch = g.numel() / (rows * cols);
+  TORCH_CHECK(batch <= INT_MAX, "newton_schulz: at most 2^31 - 1 matrices");
+  const Fit fit = single_fit(static_cast<int>(rows), static_cast<int>(cols));
+  if (fit.ok)
+    run_single(src, g.data_ptr(), dst, out.data_ptr(), StepArgs{}, 0, batch, static_cast<int>(rows),
+               static_cast<int>(cols), fit.smem, k, status);
+  else
+    run_large(src, g.data_ptr(), dst, out.data_ptr(), StepArgs{},
+              {Shape{0, batch, static_cast<int>(rows), static_cast<int>(cols)}}, k, status, g.options());
+  return out;
 }
 
 // One Muon step on the matrices of a plan: `table` [count, 4] int64 on the device (offset in

@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           }
           if (x.last) {
             // the result in G's orientation: as it lies, consecutive lanes being consecutive
-            // columns of a wide G, or turned in the slot's cells that this warp alone reads
+            // columns of a wide G, or turned in the slot's cells that this warp alone uses
             const float xo = xi * a.k.a;
             const Sink sink = {a.out_type, a.out,
                                a.out_type == kOutMuon ? a.s.table[q.first + x.mat].off

@@ -84,6 +84,23 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     }
   };
 
+  // what this CTA reads now, and what it updates at the end, on its way to L2
+  auto prefetch = [&](const void* at, int64_t bytes) {
+    const char* line = reinterpret_cast<const char*>(at);
+    for (int64_t i = threadIdx.x * 128; i < bytes; i += kSingleThreads * 128)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(line + i));
+  };
+  const int64_t numel = static_cast<int64_t>(rows) * cols;
+  if constexpr (SRC == kSrcMuon) {
+    prefetch(p.s.grad + base, numel * 4);
+    prefetch(p.s.mom + mbase, numel * 4);
+    prefetch(p.s.data + base, numel * 4);
+    if (p.s.ema != nullptr) prefetch(p.s.ema + base, numel * 4);
+  } else {
+    constexpr int size = SRC == kSrcF32 ? 4 : 2;
+    prefetch(static_cast<const char*>(g) + base * size, numel * size);
+  }
+
   // the update's input, tall, raw, into tensor memory; its sum of squares
   double acc = 0.0;
   int t, c;
@@ -156,11 +173,14 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
   };
 
-  const uint32_t zs = smem_u32(zh), as = smem_u32(ac);
+  // operand descriptors (addresses in their low 14 bits, in 16-byte units): Z's rows along K,
+  // Z's columns along K, and A's (then C's) rows
+  const uint32_t z16 = smem_u32(zh) >> 4, a16 = smem_u32(ac) >> 4, zp16 = zpanel >> 4;
   const uint32_t d_a = tmem + tiles * mp;  // A's (and A^2's) accumulator
   const uint32_t idesc_mn = idesc_f16(mp, true), idesc_k = idesc_f16(mp, false);
   // with one panel the MMA's rows 64..127 are padding: let them read the next rows
-  const uint32_t lbo = fit.panels == 2 ? zpanel : 1024;
+  const uint64_t dz_mn = umma_smem_desc(0, fit.panels == 2 ? zpanel : 1024, 1024, 2) + z16;
+  const uint64_t dz_k = umma_smem_desc(0, 16, 1024, 2) + z16, da_k = umma_smem_desc(0, 16, 1024, 2) + a16;
   const int row = q * 32 + lane;
   const Sink sink = {p.out_type, p.out, base, p.s.lr * lr_factor(p.s.adjust, rows, cols)};
   const bool out4 = m % 4 == 0 && sink4(sink, p.s);
@@ -174,14 +194,23 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     tc_fence_after();
     return ok;
   };
+  // zeros in A and C beyond the matrix (chunk j of this thread's row)
+  auto clear = [&](float* v, int j) {
+    const int keep = row < m ? m - j * 16 : 0;
+    if (keep < 16) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i >= keep) v[i] = 0.f;
+    }
+  };
   // A += Z^T Z over the rows of tile t
   auto gram = [&](int t) {
     if (warp == 0 && elect_one()) {
-      const int k1 = min(8, (n - t * 128 + 15) / 16);
-      for (int k = 0; k < k1; ++k) {
-        const uint64_t d = umma_smem_desc(zs + (t * 8 + k) * 2048, lbo, 1024, 2);
-        umma_bf16_ss(d_a, d, d, idesc_mn, t > 0 || k > 0 ? 1u : 0u);
-      }
+      const int k1 = (n - t * 128 + 15) / 16;
+      const uint64_t d = dz_mn + t * 1024;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < k1) umma_bf16_ss(d_a, d + k * 128, d + k * 128, idesc_mn, t > 0 || k > 0 ? 1u : 0u);
       if (t == tiles - 1) umma_commit(&bar[0]);
     }
     __syncwarp();
@@ -212,14 +241,16 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
         float v[16];
         ld16(tlane + tiles * mp + j * 16, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = (row < m && j * 16 + i < m) ? v[i] * x2 : 0.f;
+        for (int i = 0; i < 16; ++i) v[i] *= x2;
+        clear(v, j);
         put16(ac, 16384, row, j * 16, v);
       }
       if (!publish()) break;
       if (warp == 0 && elect_one()) {
-        for (int k = 0; k < chunks; ++k) {
-          const uint64_t d = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
-          umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t d = da_k + (k >> 2) * 1024 + (k & 3) * 2;
+          if (k < chunks) umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
         }
         umma_commit(&bar[0]);
       }
@@ -232,19 +263,20 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
         ld16(tlane + tiles * mp + j * 16, v);
         get16(ac, 16384, row, j * 16, s);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          v[i] = (row < m && j * 16 + i < m) ? p.k.ba * s[i] + p.k.ca * v[i] : 0.f;
+        for (int i = 0; i < 16; ++i) v[i] = p.k.ba * s[i] + p.k.ca * v[i];
+        clear(v, j);
         put16(ac, 16384, row, j * 16, v);
       }
       if (!publish()) break;
       // Z += Z C, tile by tile
       if (warp == 0 && elect_one()) {
         for (int i = 0; i < tiles; ++i) {
-          for (int k = 0; k < chunks; ++k) {
-            const uint64_t da = umma_desc_kmajor_sw128(zs + (k >> 2) * zpanel + i * 16384 + (k & 3) * 32);
-            const uint64_t db = umma_desc_kmajor_sw128(as + (k >> 2) * 16384 + (k & 3) * 32);
-            umma_bf16_ss(tmem + i * mp, da, db, idesc_k, 1u);
-          }
+          const uint64_t d = dz_k + i * 1024;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < chunks)
+              umma_bf16_ss(tmem + i * mp, d + (k >> 2) * zp16 + (k & 3) * 2, da_k + (k >> 2) * 1024 + (k & 3) * 2, idesc_k,
+                           1u);
           umma_commit(&bar[1 + i]);
         }
       }
@@ -335,7 +367,8 @@ void run_single(int src, const void* g, int out_type, void* out, const StepArgs&
                 : src == kSrcF16  ? single_kernel<kSrcF16>
                                   : single_kernel<kSrcMuon>;
   smem += 1024;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 221 * 1024));
+  if (smem > 48 * 1024)
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 221 * 1024));
   kernel<<<static_cast<unsigned>(count), kSingleThreads, smem, at::cuda::getCurrentCUDAStream()>>>(g, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }

@@ -39,21 +39,15 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, eps: float = 1e-7, coeffs=NS_
         raise ValueError("newton_schulz: a matrix or a batch of matrices [..., rows, cols] expected")
     if g.dtype not in _FLOATS:
         raise ValueError(f"newton_schulz: fp32, bf16 or fp16 expected, got {g.dtype}")
-    if out is None:
-        out_dtype = g.dtype if out_dtype is None else out_dtype
-        if out_dtype not in _FLOATS:
-            raise ValueError(f"newton_schulz: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
-        out = torch.empty(g.shape, device=g.device, dtype=out_dtype)
-    elif out.shape != g.shape or out.device != g.device or not out.is_contiguous():
-        raise ValueError("newton_schulz: out must be contiguous, of g's shape and on its device")
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError(f"newton_schulz: out is {out.dtype}, out_dtype {out_dtype}")
-    rows, cols = g.shape[-2:]
-    if g.numel() == 0:
-        return out
-    _lib().newton_schulz(g.detach().reshape(-1, rows, cols).contiguous(), out.view(-1, rows, cols), int(steps),
-                         float(eps), [float(c) for c in coeffs], status_word(g.device))
-    return out
+    if out_dtype is not None and out_dtype not in _FLOATS:
+        raise ValueError(f"newton_schulz: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
+    if out is not None:
+        if out.shape != g.shape or out.device != g.device or not out.is_contiguous() or out.dtype not in _FLOATS:
+            raise ValueError("newton_schulz: out must be contiguous fp32, bf16 or fp16, of g's shape and on its device")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"newton_schulz: out is {out.dtype}, out_dtype {out_dtype}")
+    return _lib().newton_schulz(g if g.is_contiguous() else g.contiguous(), out, out_dtype, steps, eps, coeffs,
+                                status_word(g.device))
 
 
 class MuonPlan:

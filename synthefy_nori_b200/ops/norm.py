@@ -48,7 +48,7 @@ def layer_norm_fwd(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, o
     """``(y, mean, rstd)`` of ``x [..., C]`` (fp32, bf16 or fp16; ``y`` in x's type or, with
     ``out_dtype``, fp32); ``mean`` and ``rstd`` are fp32, one per row."""
     f32 = _check(x, out_dtype)
-    y, mean, rstd = _lib().layer_norm_fwd(_rows(x.detach()), _vec(weight), _vec(bias), float(eps), f32)
+    y, mean, rstd = _lib().layer_norm_fwd(_rows(x), _vec(weight), _vec(bias), eps, f32)
     return y if x.dim() == 2 else y.view(x.shape), mean, rstd
 
 
@@ -58,7 +58,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     is a weight) and ``db`` are fp32 ``[C]``, or None where unwanted."""
     _check(x, None)
     weight_grad = weight is not None if weight_grad is None else weight_grad
-    dx, dw, db = _lib().layer_norm_bwd(_rows(dy.detach()), _rows(x.detach()), mean, rstd, _vec(weight),
+    dx, dw, db = _lib().layer_norm_bwd(_rows(dy), _rows(x), mean, rstd, _vec(weight),
                                        bool(weight_grad), bool(bias_grad))
     return dx if x.dim() == 2 else dx.view(x.shape), dw if weight_grad else None, db if bias_grad else None
 
