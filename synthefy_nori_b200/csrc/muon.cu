@@ -2,7 +2,6 @@
 // whole GPU, and the checks of the arguments.
 #include "muon.cuh"
 
-#include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAStream.h>
 
@@ -60,7 +59,8 @@ torch::Tensor newton_schulz(const torch::Tensor& g, const c10::optional<torch::T
                static_cast<int>(cols), fit.smem, k, status);
   else
     run_large(src, g.data_ptr(), dst, out.data_ptr(), StepArgs{},
-              {Shape{0, batch, static_cast<int>(rows), static_cast<int>(cols)}}, k, status, g.options());
+              {Shape{0, batch, static_cast<int>(rows), static_cast<int>(cols)}}, k, status, g.options(),
+              nullptr);
   return out;
 }
 
@@ -127,31 +127,32 @@ void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mo
     run_count += groups[i + 1];
     run_smem = std::max(run_smem, fit.smem);
   }
-  auto whole = [&]() { run_large(kSrcMuon, nullptr, kOutMuon, nullptr, s, large, k, status, data.options()); };
-  if (large.empty() || run_count == 0 ||
-      at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
-    if (!large.empty()) whole();
+  if (large.empty()) {
     flush();
     return;
   }
-  // The two sets touch different matrices: the large ones, a chain of dependent products that
-  // seldom fills the GPU, run on a stream of higher priority beside the single CTAs.  (Not
-  // under capture, where a stream of the pool could belong to someone else.)
-  auto main = at::cuda::getCurrentCUDAStream();
-  auto side = at::cuda::getStreamFromPool(true, data.get_device());
-  at::cuda::CUDAEvent fork, join;
-  fork.record(main);
-  fork.block(side);
-  try {
+  auto whole = [&](at::cuda::CUDAEvent* ready) {
+    run_large(kSrcMuon, nullptr, kOutMuon, nullptr, s, large, k, status, data.options(), ready);
+  };
+  if (run_count == 0 || at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+    whole(nullptr);
+    flush();
+    return;
+  }
+  // The two sets touch different matrices, and the products of the large ones, a chain that
+  // seldom fills the GPU, need all their CTAs at once: they start first, the single CTAs beside
+  // them on another stream.  (Not under capture, where a stream of the pool could belong to
+  // someone else.)
+  const auto main = at::cuda::getCurrentCUDAStream();
+  const auto side = at::cuda::getStreamFromPool(false, data.get_device());
+  at::cuda::CUDAEvent ready, join;
+  whole(&ready);
+  ready.block(side);
+  {
     c10::cuda::CUDAStreamGuard on(side);
-    whole();
-  } catch (...) {  // what was launched is still ordered before the caller's next work
-    join.record(side);
-    join.block(main);
-    throw;
+    flush();
   }
   join.record(side);
-  flush();
   join.block(main);
 }
 

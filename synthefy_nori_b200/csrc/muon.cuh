@@ -22,6 +22,7 @@
 #pragma once
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
 #include <torch/extension.h>
@@ -374,8 +375,9 @@ struct Shape {
   int64_t first, count;  // matrices of the plan's table (or of the batch)
   int rows, cols;
 };
+// `ready`, if given, is recorded once the norms and Z_0 are under way and before the products.
 void run_large(int src, const void* g, int out_type, void* out, const StepArgs& s, const std::vector<Shape>& shapes,
-               const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev);
+               const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev, at::cuda::CUDAEvent* ready);
 
 }  // namespace muon
 }  // namespace nori

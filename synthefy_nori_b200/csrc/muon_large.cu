@@ -755,7 +755,8 @@ static int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 constexpr int64_t kBlockBytes = 400ll << 20;
 
 static void run_shapes(int src, const void* g, int out_type, void* out, const StepArgs& s, const Shape* shapes, int ns,
-                       const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev) {
+                       const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev,
+                       at::cuda::CUDAEvent* ready) {
   Args a{};
   Pre p{};
   int64_t bytes = 0, mats = 0, parts = 0, norm_ctas = 0, scale_ctas = 0, items = 0;
@@ -860,16 +861,18 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
   }
   const int sms = persistent_sms(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(widest, sms));
+  if (ready != nullptr) ready->record(stream);
   void* argv[] = {&a};
   C10_CUDA_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(product_kernel), dim3(grid), dim3(kThreads),
                                              argv, kSmemBytes, stream));
 }
 
 void run_large(int src, const void* g, int out_type, void* out, const StepArgs& s, const std::vector<Shape>& shapes,
-               const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev) {
+               const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev, at::cuda::CUDAEvent* ready) {
   for (size_t i = 0; i < shapes.size(); i += kMaxShapes)
     run_shapes(src, g, out_type, out, s, shapes.data() + i,
-               static_cast<int>(std::min<size_t>(kMaxShapes, shapes.size() - i)), k, status, dev);
+               static_cast<int>(std::min<size_t>(kMaxShapes, shapes.size() - i)), k, status, dev,
+               i == 0 ? ready : nullptr);
 }
 
 }  // namespace muon
