@@ -12,7 +12,7 @@ constexpr int kSlice = 8192;     // values of one partial sum of squares
 struct Group {
   int first, count;              // matrices of the plan's table
   int rows, cols, n, m, ldz;
-  int nt, tm, tn;                // tiles: a side of A, update rows, update columns
+  int nt, tm;                    // tiles of 128 along m and n
   int base;                      // first matrix's index among all of the call
   int slices, norm_cta, scale_cta;  // partial sums of a matrix; first CTA of the group in each pre-pass
   int scale_tiles;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
 //     steps
 //       A = xi^2 Z^T Z        128 x 128 tiles on and above the diagonal, then mirrored
 //       I + C = I + (b A + c A^2) / a   the same tiles
-//       Z <- Z C + Z          128 x 256 tiles (the last step writes the result instead)
+//       Z <- Z (I + C)        all 128 x 128 tiles (the last step writes the result instead)
 //
 // A tile needs all tiles of its own matrix's previous product: a counter per matrix, raised
 // when a tile's stores are complete, tells (release / acquire at GPU scope).  Tiles of other
@@ -231,34 +231,36 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
 // fill in among the others.  The launch is cooperative (every CTA resident), and a tile only
 // waits for tiles before it in the shared order, so the oldest unfinished tile can always run.
 //
-// Roles (384 threads): warp 0 loads operands by TMA (128B-swizzled) into a ring of 48 KB
-// stages: 96 rows of Z for the Gram product (both operands MN-major: the sum runs over rows),
-// 64 columns of the rows of A or Z and C otherwise (K-major); one thread of warp 1 issues
-// tcgen05.mma (M = 128, N <= 256, K = 16) into two TMEM accumulators; warps 2..9 run the
-// epilogue on 64-column boxes, warp 10 loads the boxes that an epilogue reads (Z's low half, or
-// A) and warp 11 stores what it leaves there (Z's pair, or A / C and their mirror image), both
-// by TMA: the epilogue itself only touches tensor and shared memory.
+// Roles (448 threads).  Warp 10 walks ahead and waits for tiles' inputs (an acquire at GPU
+// scope and a proxy fence: 1,300 cycles even when they are there).  Warp 0 loads operands by
+// TMA (128B-swizzled) into a ring of four 32 KB stages: 64 rows of Z for the Gram product
+// (both operands MN-major: the sum runs over rows), 64 columns of the rows of A, or of Z and C,
+// otherwise (K-major).  One thread of warp 1 issues tcgen05.mma (M = 128, N <= 128, K = 16) into
+// four TMEM accumulators.  Warps 2..9 run the epilogue on 64-column boxes and touch only tensor
+// and shared memory: warp 11 loads the boxes that it reads (Z's low half, or A), warps 12 and 13
+// store, for alternate tiles, what it leaves there (Z's pair, or A / C and their mirror image)
+// and count the tile once its stores are complete, all by TMA.
 //
-// What bounds the update is the SM's shared memory: per 128 x 256 tile at K = 448 the MMAs
-// read 336 KB, the loads write 336 + 64 KB, the epilogue reads 64 and writes 128 KB and the
-// stores read 128 KB, about 8,300 of its cycles against 3,600 of the tensor core.  Hence N = 256
-// (two MMAs of 128 read the first operand twice: 112 KB more), and the high half of Z is not
-// loaded for the epilogue at all: C is kept as I + C, so that Z's high half comes out of the
-// product itself and only the low half is added.  (Rounding the diagonal of I + C to fp16 scales
-// Z's columns by 1 + 2^-12 at most, which no direction amplifies.)
-constexpr int kThreads = 384;
-constexpr int kStages = 3, kStageBytes = 49152;
-constexpr int kGramK = 96, kGramPanel = kGramK * 128;  // rows of a stage, bytes of 64 columns
-constexpr int kSlots = 2, kSlotBytes = 32768;
+// What bounds a tile is latency at every hand-over rather than a rate (at 81 x 1344 x 448 the
+// tensor core, L2 and DRAM each run at 25 - 40% of their peaks), so the choices below keep many
+// small pieces in flight: 128 x 128 tiles (with 128 x 256 ones the epilogue's boxes queued behind
+// 144 KB of operands, and a lone matrix had half as many tiles), two storing warps (one would
+// wait 2,000 cycles a tile for its stores), three boxes.  C is kept as I + C, so that Z's high
+// half comes out of the product itself and only the low half is loaded and added.  (Rounding the
+// diagonal of I + C to fp16 scales Z's columns by 1 + 2^-12 at most, which no direction
+// amplifies.)
+constexpr int kThreads = 448;
+constexpr int kStages = 4, kStageBytes = 32768;
+constexpr int kAccs = 4;                        // TMEM accumulators of 128 columns
+constexpr int kReady = 4;                       // tiles whose inputs are known to be there
+constexpr int kSlots = 3, kSlotBytes = 32768;   // boxes of 128 x 64, two halves each
 constexpr int kSmemBytes = kStages * kStageBytes + kSlots * kSlotBytes + 1024 + 512;
 
 enum Phase : int { kGram = 0, kPoly = 1, kUpdate = 2 };
 
 struct alignas(64) Maps {
-  CUtensorMap z[2], zl, A, C;    // boxes of 64 columns x 64 rows: the epilogue's
-  CUtensorMap zg[2];             // of 96 rows: MN-major operands
+  CUtensorMap z[2], zl, A, C;    // boxes of 64 columns x 64 rows: MN-major operands, the epilogue's
   CUtensorMap zk[2], Ak, Ck;     // of 128 rows: K-major operands
-  CUtensorMap Ck2;               // of 256 rows
 };
 struct Args {
   Maps maps[kMaxShapes];
@@ -281,7 +283,7 @@ struct Cursor {
     const Group& q = a.g[g];
     c0 = static_cast<int>(static_cast<int64_t>(q.count) * b / a.blocks);
     const int c1 = static_cast<int>(static_cast<int64_t>(q.count) * (b + 1) / a.blocks);
-    per = ph == kUpdate ? q.tm * q.tn : q.nt * (q.nt + 1) / 2;
+    per = ph == kUpdate ? q.tm * q.nt : q.nt * (q.nt + 1) / 2;
     size = (c1 - c0) * per;
   }
   __device__ __forceinline__ void start(const Args& a) {
@@ -322,13 +324,11 @@ __device__ __forceinline__ Item item_of(const Args& a, const Cursor& c, int t) {
   x.mat = c.c0 + (t - c.base) / c.per;
   int r = (t - c.base) % c.per;
   const int tri = q.nt * (q.nt + 1) / 2;
-  x.need = c.it * (2 * tri + q.tm * q.tn) + c.ph * tri;
+  x.need = c.it * (2 * tri + q.tm * q.nt) + c.ph * tri;
   x.last = c.ph == kUpdate && c.it == a.k.steps - 1;
   if (c.ph == kUpdate) {
-    x.ti = r / q.tn;
-    x.tj = r % q.tn;
-    x.n0 = x.tj * 256;
-    x.ncols = min(256, q.m - x.n0);
+    x.ti = r / q.nt;
+    x.tj = r % q.nt;
     x.diag = false;
   } else {
     int i = 0;
@@ -338,10 +338,10 @@ __device__ __forceinline__ Item item_of(const Args& a, const Cursor& c, int t) {
     }
     x.ti = i;
     x.tj = i + r;
-    x.n0 = x.tj * 128;
-    x.ncols = min(128, q.m - x.n0);
     x.diag = x.ti == x.tj;
   }
+  x.n0 = x.tj * 128;
+  x.ncols = min(128, q.m - x.n0);
   return x;
 }
 
@@ -384,8 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   uint64_t* full = reinterpret_cast<uint64_t*>(slots + kSlots * kSlotBytes);
   uint64_t* empty = full + kStages;
   uint64_t* tfull = empty + kStages;
-  uint64_t* tempty = tfull + 2;
-  uint64_t* sfull = tempty + 2;     // a slot is the epilogue's (its loads have landed)
+  uint64_t* tempty = tfull + kAccs;
+  uint64_t* ready = tempty + kAccs; // a tile's inputs are there
+  uint64_t* rfree = ready + kReady; // both loading warps know
+  uint64_t* sfull = rfree + kReady; // a slot is the epilogue's (its loads have landed)
   uint64_t* sdone = sfull + kSlots; // the epilogue has left it
   uint64_t* sfree = sdone + kSlots; // its stores have read it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sfree + kSlots);
@@ -400,9 +402,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kAccs; ++i) {
       mbar_init(&tfull[i], 1);
       mbar_init(&tempty[i], 8);
+    }
+    for (int i = 0; i < kReady; ++i) {
+      mbar_init(&ready[i], 1);
+      mbar_init(&rfree[i], 2);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&sfull[i], 1);
@@ -419,6 +425,15 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   const uint32_t tmem = *tmem_slot;
   Cursor cur;
   cur.start(a);
+  // this role's place in a ring of `n` (stages, accumulators, ready tiles or slots)
+  auto advance = [](int& i, uint32_t& phase, int n) {
+    if (++i == n) {
+      i = 0;
+      phase ^= 1;
+    }
+  };
+  int re = 0;
+  uint32_t rp = 0;
 
   if (warp == 0) {
     if (elect_one()) {
@@ -429,36 +444,31 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const Item x = item_of(a, cur, t);
         const Group& q = a.g[x.g];
         const Maps& mp = a.maps[x.g];
-        if (!wait_done(a, x, abort_flag)) break;
-        const bool gram = x.ph == kGram, two = x.ncols > 128;
-        const int K = gram ? q.n : q.m, row = x.ti * 128, kstep = gram ? kGramK : 64;
-        const CUtensorMap* ma = gram ? &mp.zg[x.it & 1] : x.ph == kPoly ? &mp.Ak : &mp.zk[x.it & 1];
-        const CUtensorMap* mb = x.ph == kPoly ? &mp.Ak : two ? &mp.Ck2 : &mp.Ck;
-        const uint32_t half = gram ? 2 * kGramPanel : 16384;  // bytes of the first operand
-        const uint32_t bytes = half + (x.diag ? 0 : gram ? 2 * kGramPanel : two ? 32768 : 16384);
-        for (int k0 = 0; k0 < K; k0 += kstep) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer, abort_flag)) {
-            ok = false;
-            break;
-          }
+        if (!mbar_wait(&ready[re], rp, a.status, kTimeoutProducer, abort_flag)) break;
+        mbar_arrive(&rfree[re]);
+        advance(re, rp, kReady);
+        const bool gram = x.ph == kGram;
+        const int K = gram ? q.n : q.m, row = x.ti * 128;
+        const CUtensorMap* ma = gram ? &mp.z[x.it & 1] : x.ph == kPoly ? &mp.Ak : &mp.zk[x.it & 1];
+        const CUtensorMap* mb = x.ph == kPoly ? &mp.Ak : &mp.Ck;
+        for (int k0 = 0; k0 < K; k0 += 64) {
+          ok = mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer, abort_flag);
+          if (!ok) break;
           uint8_t* sa = stages + stage * kStageBytes;
           uint64_t* bar = &full[stage];
-          mbar_arrive_expect_tx(bar, bytes);
+          mbar_arrive_expect_tx(bar, x.diag ? 16384 : 32768);
           if (gram) {
             tma_load_3d(sa, ma, bar, row, k0, x.mat);
-            tma_load_3d(sa + kGramPanel, ma, bar, row + 64, k0, x.mat);
+            tma_load_3d(sa + 8192, ma, bar, row + 64, k0, x.mat);
             if (!x.diag) {
-              tma_load_3d(sa + 2 * kGramPanel, ma, bar, x.n0, k0, x.mat);
-              tma_load_3d(sa + 3 * kGramPanel, ma, bar, x.n0 + 64, k0, x.mat);
+              tma_load_3d(sa + 16384, ma, bar, x.n0, k0, x.mat);
+              tma_load_3d(sa + 24576, ma, bar, x.n0 + 64, k0, x.mat);
             }
           } else {
             tma_load_3d(sa, ma, bar, k0, row, x.mat);
             if (!x.diag) tma_load_3d(sa + 16384, mb, bar, k0, x.n0, x.mat);
           }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          advance(stage, phase, kStages);
         }
       }
     }
@@ -472,39 +482,43 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const Item x = item_of(a, cur, t);
         const Group& q = a.g[x.g];
         const bool gram = x.ph == kGram;
-        const int K = gram ? q.n : q.m, kstep = gram ? kGramK : 64;
+        const int K = gram ? q.n : q.m;
         const uint32_t idesc = idesc_f16((x.ncols + 15) / 16 * 16, gram);
         // descriptors without the address (their low 14 bits, in 16-byte units), and the steps
         // of 16 along K: 16 rows of an MN-major panel, 32 bytes of a K-major row; a tile on the
         // diagonal multiplies its rows by themselves
-        const uint64_t dbase = gram ? umma_smem_desc(0, kGramPanel, 1024, 2) : umma_smem_desc(0, 16, 1024, 2);
+        const uint64_t dbase = umma_smem_desc(0, gram ? 8192 : 16, 1024, 2);
         const uint32_t inc = gram ? 2048 / 16 : 32 / 16;
-        const uint32_t second = x.diag ? 0 : (gram ? 2 * kGramPanel : 16384) / 16;
+        const uint32_t second = x.diag ? 0 : 16384 / 16;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kTimeoutMma, abort_flag)) break;
         tc_fence_after();
-        const uint32_t d = tmem + acc * 256;
-        for (int k0 = 0; k0 < K; k0 += kstep) {
-          if (!mbar_wait(&full[stage], phase, a.status, kTimeoutMma, abort_flag)) {
-            ok = false;
-            break;
-          }
+        const uint32_t d = tmem + acc * 128;
+        for (int k0 = 0; k0 < K; k0 += 64) {
+          ok = mbar_wait(&full[stage], phase, a.status, kTimeoutMma, abort_flag);
+          if (!ok) break;
           tc_fence_after();
           const uint64_t da = dbase + (stages_lo + stage * (kStageBytes / 16)), db = da + second;
           const uint32_t more = k0 > 0 ? 1u : 0u;
-          const int steps = (min(kstep, K - k0) + 15) / 16;  // the rest of the boxes is zero fill
+          const int steps = (min(64, K - k0) + 15) / 16;  // the rest of the boxes is zero fill
 #pragma unroll
-          for (int k = 0; k < kGramK / 16; ++k)
+          for (int k = 0; k < 4; ++k)
             if (k < steps) umma_bf16_ss(d, da + k * inc, db + k * inc, idesc, k > 0 ? 1u : more);
           umma_commit(&empty[stage]);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          advance(stage, phase, kStages);
         }
         if (!ok) break;
         umma_commit(&tfull[acc]);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        advance(acc, acc_phase, kAccs);
+      }
+    }
+  } else if (warp == 10) {
+    if (elect_one()) {
+      for (int t = blockIdx.x; cur.seek(a, t); t += gridDim.x) {
+        const Item x = item_of(a, cur, t);
+        if (!mbar_wait(&rfree[re], rp ^ 1, a.status, kTimeoutProducer, abort_flag)) break;
+        if (!wait_done(a, x, abort_flag)) break;
+        mbar_arrive(&ready[re]);
+        advance(re, rp, kReady);
       }
     }
   } else if (warp < 10) {
@@ -521,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       for (int k = 0; k < x.it; ++k) xi *= a.k.a;
       if (!mbar_wait_warp(&tfull[acc], acc_phase, a.status, kTimeoutEpilogue, abort_flag)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + acc * 256 + half * 32;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + acc * 128 + half * 32;
       for (int c = 0; c < x.ncols; c += 64) {
         uint8_t* s0 = slots + slot * kSlotBytes;
         uint8_t* s1 = s0 + 16384;
@@ -637,18 +651,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sdone[slot]);
-        if (++slot == kSlots) {
-          slot = 0;
-          s_phase ^= 1;
-        }
+        advance(slot, s_phase, kSlots);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
+      advance(acc, acc_phase, kAccs);
     }
-  } else if (warp == 10) {
+  } else if (warp == 11) {
     if (elect_one()) {
       int slot = 0;
       uint32_t phase = 0;
@@ -656,8 +666,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x) {
         const Item x = item_of(a, cur, t);
         const Maps& mp = a.maps[x.g];
-        if (x.ph != kGram && !wait_done(a, x, abort_flag)) break;
-        for (int c = 0; c < x.ncols && ok; c += 64) {
+        if (!mbar_wait(&ready[re], rp, a.status, kTimeoutProducer, abort_flag)) break;
+        mbar_arrive(&rfree[re]);
+        advance(re, rp, kReady);
+        for (int c = 0; c < x.ncols; c += 64) {
           ok = mbar_wait(&sfree[slot], phase ^ 1, a.status, kTimeoutProducer, abort_flag);
           if (!ok) break;
           uint8_t* s0 = slots + slot * kSlotBytes;
@@ -665,19 +677,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           const int col = x.n0 + c, row = x.ti * 128;
           if (x.ph == kGram) {
             mbar_arrive(bar);
-          } else if (x.ph == kPoly) {
-            mbar_arrive_expect_tx(bar, 16384);
-            tma_load_3d(s0, &mp.A, bar, col, row, x.mat);
-            tma_load_3d(s0 + 8192, &mp.A, bar, col, row + 64, x.mat);
           } else {
+            const CUtensorMap* m = x.ph == kPoly ? &mp.A : &mp.zl;
+            uint8_t* d = x.ph == kPoly ? s0 : s0 + 16384;
             mbar_arrive_expect_tx(bar, 16384);
-            tma_load_3d(s0 + 16384, &mp.zl, bar, col, row, x.mat);
-            tma_load_3d(s0 + 24576, &mp.zl, bar, col, row + 64, x.mat);
+            tma_load_3d(d, m, bar, col, row, x.mat);
+            tma_load_3d(d + 8192, m, bar, col, row + 64, x.mat);
           }
-          if (++slot == kSlots) {
-            slot = 0;
-            phase ^= 1;
-          }
+          advance(slot, phase, kSlots);
         }
       }
     }
@@ -685,12 +692,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     if (elect_one()) {
       int slot = 0;
       uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x) {
+      bool ok = true, mine = warp == 12;
+      for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x, mine = !mine) {
         const Item x = item_of(a, cur, t);
         const Group& q = a.g[x.g];
         const Maps& mp = a.maps[x.g];
-        for (int c = 0; c < x.ncols; c += 64) {
+        int before = -1;  // the slot that the box before this one left
+        for (int c = 0; c < x.ncols; c += 64, advance(slot, phase, kSlots)) {
+          if (!mine) continue;
           ok = mbar_wait(&sdone[slot], phase, a.status, kTimeoutEpilogue, abort_flag);
           if (!ok) break;
           uint8_t* s0 = slots + slot * kSlotBytes;
@@ -713,14 +722,15 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             }
           }
           bulk_commit();
-          bulk_wait_read0();
-          mbar_arrive(&sfree[slot]);
-          if (++slot == kSlots) {
-            slot = 0;
-            phase ^= 1;
+          if (before >= 0) {
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            mbar_arrive(&sfree[before]);
           }
+          before = slot;
         }
-        if (!ok) break;
+        if (!ok || !mine) continue;
+        bulk_wait_read0();
+        mbar_arrive(&sfree[before]);
         if (!x.last) {  // the tile is in memory: count it
           bulk_wait0();
           asm volatile("fence.proxy.async;" ::: "memory");
@@ -778,7 +788,6 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
     q.ldz = static_cast<int>(align_up(q.m, 8));
     q.nt = (q.m + 127) / 128;
     q.tm = (q.n + 127) / 128;
-    q.tn = (q.m + 255) / 256;
     q.base = static_cast<int>(mats);
     q.slices = static_cast<int>((numel + kSlice - 1) / kSlice);
     q.scale_tiles = ((q.rows + 63) / 64) * ((q.cols + 63) / 64);
@@ -788,7 +797,7 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
     parts += count * q.slices;
     norm_ctas += count * q.slices;
     scale_ctas += count * q.scale_tiles;
-    items += count * k.steps * (static_cast<int64_t>(q.nt) * (q.nt + 1) + static_cast<int64_t>(q.tm) * q.tn);
+    items += count * k.steps * (static_cast<int64_t>(q.nt) * (q.nt + 1) + static_cast<int64_t>(q.tm) * q.nt);
     const int64_t zb = count * q.n * q.ldz * 2, ab = count * q.m * q.ldz * 2;
     at[i] = {take(zb), take(zb), take(zb), take(ab), take(ab)};
     TORCH_CHECK(mats < INT_MAX && norm_ctas < INT_MAX && scale_ctas < INT_MAX && items < INT_MAX - (1 << 20),
@@ -808,7 +817,6 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
     Maps& mp = a.maps[i];
     for (int j = 0; j < 2; ++j) {
       mp.z[j] = map_f16(q.z[j], q.m, q.n, q.ldz, q.count, 64);
-      mp.zg[j] = map_f16(q.z[j], q.m, q.n, q.ldz, q.count, kGramK);
       mp.zk[j] = map_f16(q.z[j], q.m, q.n, q.ldz, q.count, 128);
     }
     mp.zl = map_f16(q.zl, q.m, q.n, q.ldz, q.count, 64);
@@ -816,7 +824,6 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
     mp.Ak = map_f16(q.A, q.m, q.m, q.ldz, q.count, 128);
     mp.C = map_f16(q.C, q.m, q.m, q.ldz, q.count, 64);
     mp.Ck = map_f16(q.C, q.m, q.m, q.ldz, q.count, 128);
-    mp.Ck2 = map_f16(q.C, q.m, q.m, q.ldz, q.count, 256);
     a.g[i] = q;
   }
   p.groups = ns;
@@ -855,7 +862,7 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
     int64_t n = 0;
     for (int i = 0; i < ns; ++i) {
       const Group& q = p.g[i];
-      n += (q.count + a.blocks - 1) / a.blocks * static_cast<int64_t>(ph == 0 ? q.nt * (q.nt + 1) / 2 : q.tm * q.tn);
+      n += (q.count + a.blocks - 1) / a.blocks * static_cast<int64_t>(ph == 0 ? q.nt * (q.nt + 1) / 2 : q.tm * q.nt);
     }
     widest = std::max(widest, n);
   }
