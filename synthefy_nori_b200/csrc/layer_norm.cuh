@@ -100,6 +100,16 @@ struct Row {
       for (int i = 0; i < VEC; ++i) v[VEC * j + i] = to_f32<T>(p[j].v[i]);
   }
 };
+// Brings a row's whole 16-byte pieces to L2: one instruction, no registers held.  A CTA asks for
+// its next rows before it works on the ones at hand, so its loads wait for L2 and not for DRAM.
+template <typename T>
+__device__ __forceinline__ void prefetch_row(const T* row, int C) {
+  const uintptr_t a = (reinterpret_cast<uintptr_t>(row) + 15) & ~uintptr_t(15);
+  const uintptr_t e = reinterpret_cast<uintptr_t>(row + C) & ~uintptr_t(15);
+  if (e > a)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"(static_cast<uint32_t>(e - a)) : "memory");
+}
+
 // VEC columns of a weight vector (`fill` where there is none).
 template <int VEC>
 __device__ __forceinline__ void load_columns(const float* w, int c, float fill, float* v) {

@@ -31,7 +31,13 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
   for (int i = 0; i < kValues; ++i) gw[i] = gb[i] = 0.f;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * (2 * RPB); base < R;
        base += static_cast<int64_t>(gridDim.x) * (2 * RPB)) {
-    const int64_t row = base + g;
+    const int64_t row = base + g, ahead = row + static_cast<int64_t>(gridDim.x) * (2 * RPB) + t % 2 * RPB;
+    if (t < 4 && ahead < R) {
+      if (t < 2)
+        prefetch_row(x + ahead * ldx, C);
+      else
+        prefetch_row(dy + ahead * ldy, C);
+    }
     float h[2][kValues], q[2][kValues], s[4] = {0.f, 0.f, 0.f, 0.f}, rstd[2];
     {
       Row<T, VEC, TPR> rx[2];

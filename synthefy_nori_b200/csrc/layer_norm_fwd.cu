@@ -21,7 +21,8 @@ __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T
   // a CTA's rows: 2 RPB neighbours, RPB apart within a group
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * (2 * RPB); base < R;
        base += static_cast<int64_t>(gridDim.x) * (2 * RPB)) {
-    const int64_t row = base + g;
+    const int64_t row = base + g, ahead = row + static_cast<int64_t>(gridDim.x) * (2 * RPB) + t * RPB;
+    if (t < 2 && ahead < R) prefetch_row(x + ahead * ldx, C);
     float v[2][kValues], s[2] = {0.f, 0.f}, mean[2], rstd[2];
     {
       Row<T, VEC, TPR> r[2];

@@ -153,7 +153,7 @@ def _step64(shapes, offsets, p, g, m, e, *, lr, wd, momentum, nesterov, adjust, 
 
 
 RAGGED = [(64, 64), (192, 64), (64, 1), (1, 1), (10, 96), (2, 96), (333, 127), (448, 64), (64, 64), (300, 200),
-          (200, 301), (300, 200), (999, 96), (17, 1500)]
+          (200, 301), (300, 200), (999, 96), (17, 1500)]  # single-CTA and whole-GPU shapes mixed
 
 
 def _ragged(seed=0, gap=13, shapes=RAGGED):
@@ -252,6 +252,68 @@ def test_muon_step_graph_replay_and_two_graphs():
     torch.cuda.synchronize()
     for _, got, want, *_ in runs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_muon_step_with_many_large_shapes():
+    """More shapes over the whole GPU than one launch takes, between single-CTA ones."""
+    from synthefy_nori_b200 import ops
+
+    shapes = [(130 + 9 * i, 129 + 7 * ((i * 5) % 20)) for i in range(19)] + [(64, 64), (40, 3)]
+    shapes = shapes[::2] + shapes[1::2] + [shapes[3]]
+    shapes, off, p, g, m, e = _ragged(7, shapes=shapes)
+    hyper = dict(lr=0.02, wd=0.1, momentum=0.9, nesterov=True)
+    ref_p, _, _, upd = _step64(shapes, off, p, g, m, e, **hyper, adjust="original", clip=1.0, decay=0.9)
+    p0 = p.clone()
+    ops.muon_step(ops.MuonPlan(shapes, off, "cuda"), p, g, m, **hyper, adjust_lr="original", ema=e, ema_decay=0.9)
+    for (r, c), o in zip(shapes, off):
+        sl = slice(o, o + r * c)
+        tol = NS_TOL * float(upd[sl].norm()) + 4 * F32 * float(p0[sl].norm() + upd[sl].norm())
+        assert float((p[sl].double() - ref_p[sl]).norm()) <= tol, (r, c)
+
+
+def test_muon_step_is_ordered_on_its_stream():
+    """Large and single-CTA matrices run on two streams inside; the caller's stream sees one call:
+    inputs written right before it, results read right after, buffers freed and reused."""
+    from synthefy_nori_b200 import ops
+
+    shapes, off, p, g, m, _ = _ragged(8)
+    plan = ops.MuonPlan(shapes, off, "cuda")
+    want_p, want_m = p.clone(), m.clone()
+    for _ in range(6):
+        ops.muon_step(plan, want_p, g, want_m, lr=0.02)
+        torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        q, n = p.clone(), m.clone()
+        for _ in range(6):
+            big = torch.full((1 << 24,), 7.0, device="cuda")  # keeps the stream busy, then is freed
+            grad = g * 1.0
+            ops.muon_step(plan, q, grad, n, lr=0.02)
+            grad.fill_(float("nan"))
+            del grad, big
+            q, n = q.clone(), n.clone()
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(q, want_p) and torch.equal(n, want_m)
+
+
+def test_two_calls_over_the_whole_gpu_at_once():
+    from synthefy_nori_b200 import ops
+
+    torch.manual_seed(9)
+    gs = [torch.randn(3, 700, 500, device="cuda"), torch.randn(2, 450, 900, device="cuda")]
+    want = [ops.newton_schulz(g) for g in gs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(ops.newton_schulz(gs[k]))
+    torch.cuda.synchronize()
+    ops.check_status(gs[0].device)
+    for k in (0, 1):
+        assert all(torch.equal(o, want[k]) for o in got[k])
 
 
 def test_muon_on_a_side_stream_beside_the_default_one():
