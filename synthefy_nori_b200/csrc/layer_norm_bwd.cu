@@ -26,9 +26,10 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const float inv_c = 1.f / static_cast<float>(C);
   int flip = 0;
-  float gw[kValues], gb[kValues];
+  constexpr int H = kValues / 2;
+  F2 gw[H], gb[H];
 #pragma unroll
-  for (int i = 0; i < kValues; ++i) gw[i] = gb[i] = 0.f;
+  for (int i = 0; i < H; ++i) gw[i] = gb[i] = f2(0.f, 0.f);
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * (2 * RPB); base < R;
        base += static_cast<int64_t>(gridDim.x) * (2 * RPB)) {
     const int64_t row = base + g, ahead = row + static_cast<int64_t>(gridDim.x) * (2 * RPB) + t % 2 * RPB;
@@ -38,7 +39,8 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
       else
         prefetch_row(dy + ahead * ldy, C);
     }
-    float h[2][kValues], q[2][kValues], s[4] = {0.f, 0.f, 0.f, 0.f}, rstd[2];
+    F2 h[2][H], q[2][H];
+    float s[4], rstd[2];
     {
       Row<T, VEC, TPR> rx[2];
       Row<U, VEC, TPR> ry[2];
@@ -52,48 +54,62 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        rx[k].values(h[k]);
-        ry[k].values(q[k]);
+        const F2 m = f2(-mean[k], -mean[k]), r = f2(rstd[k], rstd[k]);
+        float vx[kValues], vy[kValues];
+        rx[k].values(vx);
+        ry[k].values(vy);
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) h[k][i] = (h[k][i] - mean[k]) * rstd[k];
+        for (int i = 0; i < H; ++i) {
+          h[k][i] = mul2(add2(f2(vx[2 * i], vx[2 * i + 1]), m), r);
+          q[k][i] = f2(vy[2 * i], vy[2 * i + 1]);
+        }
+      }
+    }
+    float wv[kValues];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int c = VEC * (t + TPR * j);
+      if (c < C) {
+        load_columns<VEC>(w, c, 1.f, wv + VEC * j);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) wv[VEC * j + i] = 0.f;
       }
     }
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {  // q is 0 beyond the last row and column
-      const int c = VEC * (t + TPR * j);
-      if (c < C) {
-        float wv[VEC];
-        load_columns<VEC>(w, c, 1.f, wv);
+    for (int k = 0; k < 2; ++k) {  // dy is 0 beyond the last row and column
+      F2 s1 = f2(0.f, 0.f), s2 = f2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const int e = VEC * j + i;
-            if constexpr (GRADS) {
-              gw[e] += q[k][e] * h[k][e];
-              gb[e] += q[k][e];
-            }
-            q[k][e] *= wv[i];
-            s[2 * k] += q[k][e];
-            s[2 * k + 1] += q[k][e] * h[k][e];
-          }
+      for (int i = 0; i < H; ++i) {
+        if constexpr (GRADS) {
+          gw[i] = fma2(q[k][i], h[k][i], gw[i]);
+          gb[i] = add2(gb[i], q[k][i]);
+        }
+        q[k][i] = mul2(q[k][i], f2(wv[2 * i], wv[2 * i + 1]));
+        s1 = add2(s1, q[k][i]);
+        s2 = fma2(q[k][i], h[k][i], s2);
       }
+      float lo, hi;
+      unpack(s1, lo, hi);
+      s[2 * k] = lo + hi;
+      unpack(s2, lo, hi);
+      s[2 * k + 1] = lo + hi;
     }
     row_sum<TPR, 4>(s, sh, flip);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (row + k * RPB < R) {
-        const float s1 = s[2 * k] * inv_c, s2 = s[2 * k + 1] * inv_c;
+        const float a1 = -s[2 * k] * inv_c, a2 = -s[2 * k + 1] * inv_c;
+        const F2 n1 = f2(a1, a1), n2 = f2(a2, a2), r = f2(rstd[k], rstd[k]);
+        float o[kValues];
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+          unpack(mul2(r, fma2(h[k][i], n2, add2(q[k][i], n1))), o[2 * i], o[2 * i + 1]);
         T* dxr = dx + (row + k * RPB) * static_cast<int64_t>(C);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
           const int c = VEC * (t + TPR * j);
-          if (c < C) {
-            float o[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = rstd[k] * (q[k][VEC * j + i] - s1 - h[k][VEC * j + i] * s2);
-            store_vec<T, VEC>(dxr + c, o);
-          }
+          if (c < C) store_vec<T, VEC>(dxr + c, o + VEC * j);
         }
       }
     }
@@ -107,7 +123,9 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
 #pragma unroll
       for (int k = 0; k < kValues; ++k) {
         const int c = VEC * (t + TPR * (k / VEC)) + k % VEC;
-        if (c < C) (RPB > 1 ? acc_sh + g * C : out)[c] = pass == 0 ? gw[k] : gb[k];
+        float lo, hi;
+        unpack(pass == 0 ? gw[k / 2] : gb[k / 2], lo, hi);
+        if (c < C) (RPB > 1 ? acc_sh + g * C : out)[c] = k % 2 == 0 ? lo : hi;
       }
       if constexpr (RPB > 1) {
         __syncthreads();

@@ -45,12 +45,24 @@ __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T
     for (int j = 0; j < CH; ++j) {
       if (VEC * (t + TPR * j) < C) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (VEC > 1) {
+            const F2 m = f2(-mean[k], -mean[k]);
+            F2 ss = f2(0.f, 0.f);
 #pragma unroll
-          for (int i = VEC * j; i < VEC * (j + 1); ++i) {
-            v[k][i] -= mean[k];
-            s[k] += v[k][i] * v[k][i];
+            for (int i = VEC * j; i < VEC * (j + 1); i += 2) {
+              const F2 d = add2(f2(v[k][i], v[k][i + 1]), m);
+              ss = fma2(d, d, ss);
+              unpack(d, v[k][i], v[k][i + 1]);
+            }
+            float lo, hi;
+            unpack(ss, lo, hi);
+            s[k] += lo + hi;
+          } else {
+            v[k][j] -= mean[k];
+            s[k] += v[k][j] * v[k][j];
           }
+        }
       }
     }
     row_sum<TPR, 2>(s, sh, flip);
@@ -67,8 +79,16 @@ __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T
         for (int k = 0; k < 2; ++k) {
           if (row + k * RPB < R) {
             float o[VEC];
+            if constexpr (VEC > 1) {
+              const F2 r = f2(rstd[k], rstd[k]);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = v[k][VEC * j + i] * rstd[k] * wv[i] + bv[i];
+              for (int i = 0; i < VEC; i += 2)
+                unpack(fma2(mul2(f2(v[k][VEC * j + i], v[k][VEC * j + i + 1]), r), f2(wv[i], wv[i + 1]),
+                            f2(bv[i], bv[i + 1])),
+                       o[i], o[i + 1]);
+            } else {
+              o[0] = v[k][j] * rstd[k] * wv[0] + bv[0];
+            }
             store_vec<U, VEC>(y + (row + k * RPB) * static_cast<int64_t>(C) + c, o);
           }
         }
