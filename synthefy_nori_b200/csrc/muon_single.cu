@@ -10,7 +10,10 @@ namespace muon {
 // place (Z <- Z + Z C); its fp16 copy lies in shared memory once, as 128B-swizzled rows of 64
 // columns, and serves the Gram product (read MN-major, the sum running over rows) and the
 // update (read K-major).  A and then C take one 128-row tile beside it.  Nothing but the
-// matrix itself and its result crosses memory.  The chain of 3 x steps dependent products
+// matrix itself and its result crosses memory.  Up to 32 columns, where few roundings average
+// out (fp16 operands leave up to 1e-2 of a 2 x 2 matrix), the other half of the 64-column rows
+// holds the low parts of Z, A and C, and every product is three (high high, high low, low high:
+// 22-bit operands, 1e-6).  The chain of 3 x steps dependent products
 // bounds it: each is issued by one thread, waited for by all, read back by tcgen05.ld.
 struct SingleParams {
   int first, rows, cols;
@@ -48,6 +51,7 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   uint8_t* zh = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ac = zh + tiles * fit.panels * 16384;
   const int zpanel = tiles * 16384;  // bytes between two 64-column panels of Z
+  const bool pair = mp <= 32;        // low parts in columns 32 ..
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int q = warp & 3, grp = warp >> 2;  // lane quarter; 16-column chunks are dealt to 4 groups
@@ -165,6 +169,15 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     unpack8(*reinterpret_cast<const uint4*>(d + ((k ^ x) << 4)), v);
     unpack8(*reinterpret_cast<const uint4*>(d + (((k + 1) ^ x) << 4)), v + 8);
   };
+  // v's high parts at c0 and, for pairs, its low parts beside them
+  auto put = [&](uint8_t* panel0, int pstride, int r, int c0, float* v) {
+    put16(panel0, pstride, r, c0, v);
+    if (pair) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] -= __half2float(__float2half_rn(v[i]));
+      put16(panel0, pstride, r, c0 + 32, v);
+    }
+  };
   auto ld16 = [&](uint32_t addr, float* v) {
     uint32_t r[16];
     tmem_ld16(addr, r);
@@ -194,6 +207,12 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     tc_fence_after();
     return ok;
   };
+  // D (+)= x y^T for one step along K of the operands at `x`, `y` (low parts 64 bytes on)
+  auto mma3 = [&](uint32_t d, uint64_t x, uint64_t y, uint32_t idesc, uint32_t more) {
+    umma_bf16_ss(d, x, y, idesc, more);
+    umma_bf16_ss(d, x, y + 4, idesc, 1u);
+    umma_bf16_ss(d, x + 4, y, idesc, 1u);
+  };
   // zeros in A and C beyond the matrix (chunk j of this thread's row)
   auto clear = [&](float* v, int j) {
     const int keep = row < m ? m - j * 16 : 0;
@@ -208,9 +227,14 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
     if (warp == 0 && elect_one()) {
       const int k1 = (n - t * 128 + 15) / 16;
       const uint64_t d = dz_mn + t * 1024;
+      if (pair) {
+        for (int k = 0; k < min(k1, 8); ++k)
+          mma3(d_a, d + k * 128, d + k * 128, idesc_mn, t > 0 || k > 0 ? 1u : 0u);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < k1) umma_bf16_ss(d_a, d + k * 128, d + k * 128, idesc_mn, t > 0 || k > 0 ? 1u : 0u);
+        for (int k = 0; k < 8; ++k)
+          if (k < k1) umma_bf16_ss(d_a, d + k * 128, d + k * 128, idesc_mn, t > 0 || k > 0 ? 1u : 0u);
+      }
       if (t == tiles - 1) umma_commit(&bar[0]);
     }
     __syncwarp();
@@ -227,7 +251,7 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
       r[i] = __float_as_uint(v[i]);
     }
     tmem_st16(tlane + t * mp + c * 16, r);
-    put16(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
+    put(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
   }
   tmem_wait_st();
   if (publish()) {
@@ -243,14 +267,18 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] *= x2;
         clear(v, j);
-        put16(ac, 16384, row, j * 16, v);
+        put(ac, 16384, row, j * 16, v);
       }
       if (!publish()) break;
       if (warp == 0 && elect_one()) {
+        if (pair) {
+          for (int k = 0; k < chunks; ++k) mma3(d_a, da_k + k * 2, da_k + k * 2, idesc_k, k > 0 ? 1u : 0u);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t d = da_k + (k >> 2) * 1024 + (k & 3) * 2;
-          if (k < chunks) umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t d = da_k + (k >> 2) * 1024 + (k & 3) * 2;
+            if (k < chunks) umma_bf16_ss(d_a, d, d, idesc_k, k > 0 ? 1u : 0u);
+          }
         }
         umma_commit(&bar[0]);
       }
@@ -262,21 +290,31 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
         float v[16], s[16];
         ld16(tlane + tiles * mp + j * 16, v);
         get16(ac, 16384, row, j * 16, s);
+        if (pair) {
+          float l[16];
+          get16(ac, 16384, row, j * 16 + 32, l);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] += l[i];
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = p.k.ba * s[i] + p.k.ca * v[i];
         clear(v, j);
-        put16(ac, 16384, row, j * 16, v);
+        put(ac, 16384, row, j * 16, v);
       }
       if (!publish()) break;
       // Z += Z C, tile by tile
       if (warp == 0 && elect_one()) {
         for (int i = 0; i < tiles; ++i) {
           const uint64_t d = dz_k + i * 1024;
+          if (pair) {
+            for (int k = 0; k < chunks; ++k) mma3(tmem + i * mp, d + k * 2, da_k + k * 2, idesc_k, 1u);
+          } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < chunks)
-              umma_bf16_ss(tmem + i * mp, d + (k >> 2) * zp16 + (k & 3) * 2, da_k + (k >> 2) * 1024 + (k & 3) * 2, idesc_k,
-                           1u);
+            for (int k = 0; k < 8; ++k)
+              if (k < chunks)
+                umma_bf16_ss(tmem + i * mp, d + (k >> 2) * zp16 + (k & 3) * 2, da_k + (k >> 2) * 1024 + (k & 3) * 2,
+                             idesc_k, 1u);
+          }
           umma_commit(&bar[1 + i]);
         }
       }
@@ -291,7 +329,7 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
         for (; t == i; next(t, c)) {
           float v[16];
           ld16(tlane + t * mp + c * 16, v);
-          put16(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
+          put(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
         }
         if (!publish()) break;  // every warp's part of the tile
         gram(i);

@@ -61,6 +61,21 @@ def test_newton_schulz_matches_formula(batch, rows, cols):
     assert torch.equal(o, ops.newton_schulz(g, out_dtype=torch.float32))  # the same bits again
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 1), (2, 2), (5, 1), (2, 300), (3, 3), (130, 5), (16, 16), (17, 9), (700, 20),
+                                       (32, 32), (31, 400)])
+def test_newton_schulz_narrow_matrices_keep_22_bits(rows, cols):
+    """Up to 32 columns the products read pairs of fp16: 25 roundings of 2^-22 and as many sums of
+    2^-20 at most; the first rounding of the iterate, 2^-22 |G|, is amplified by no more than
+    a^5 = 485 in any direction, against a result of norm 0.65 or more."""
+    from synthefy_nori_b200 import ops
+
+    torch.manual_seed(rows + 31 * cols)
+    g = torch.randn(40, rows, cols, device="cuda")
+    o, ref = ops.newton_schulz(g, out_dtype=torch.float32), ns64(g)
+    for i in range(40):
+        assert rel(o[i], ref[i]) < 25 * (2.0 ** -22 + 2.0 ** -20) + 485 * 2.0 ** -22 / 0.65
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("out_dtype", [None, torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,cols", [(96, 64), (64, 200), (200, 600)])
