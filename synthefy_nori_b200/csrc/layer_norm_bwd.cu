@@ -7,7 +7,9 @@
 // visits in fp32 registers; a CTA adds its row groups in a fixed order and writes one partial
 // row, and a second kernel adds the partial rows in a fixed order.  Where the partial rows
 // would be more traffic than reading x and dy (from L2) once more, the columns are summed by a
-// pass of their own.  No atomics: the same inputs give the same bits.
+// pass of their own (257 x 8192 fp16: 30 + 7 us with partial rows, 6 + 7 + 5 with the pass).
+// 403200 x 448 bf16 in 220 us against 167 at the copy rate: 16 warps an SM issue 2.3
+// instructions a cycle.  No atomics: the same inputs give the same bits.
 //
 // Reference counterpart: torch LayerNorm's autograd (model/layer.py:219-230).
 #include "layer_norm.cuh"

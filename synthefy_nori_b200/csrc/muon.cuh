@@ -7,8 +7,8 @@
 //
 // Numerics.  The kernels carry Z_k = 2^8 X_k / (f a^k) with f = |G|_F / (|G|_F + eps), so
 // that one step is Z <- Z + Z C and the leading term needs no multiplication: X_k = xi_k Z_k
-// with xi_0 = f 2^-8 and xi_{k+1} = a xi_k.  Z is held as a pair of fp16 (high, low: 22
-// significant bits); the three products read fp16 operands (the high parts, A and C: 11
+// with xi_0 = f 2^-8 and xi_{k+1} = a xi_k.  Z is held in fp32 (one CTA a matrix) or as a pair of
+// fp16 (high, low: 22 significant bits; over the whole GPU); the three products read fp16 operands (the high parts, A and C: 11
 // bits) and accumulate in fp32.  A small singular value of G lives in the pair and is only
 // multiplied by 1 + C, so it keeps its 22 bits, while the rounding of the products' operands
 // (2^-12 relative) perturbs the dominant directions only and is not amplified: the result is
@@ -16,7 +16,8 @@
 // rank-deficient spectra alike, about the rounding of a bf16 result.  With iterates rounded
 // to bf16 the noise 2^-9 |G|_F is amplified by up to a^5 = 485 in the small directions: 1e-2
 // for a flat spectrum and 0.1 .. 1 for steep ones.  Products of fp16 pairs (three MMAs each)
-// would give 1e-6 for three times the tensor work.
+// give 1e-6 for three times the tensor work; the single-CTA kernel takes them up to 32 columns,
+// where the work is nothing and few roundings average out.
 //
 // Reference counterpart: training/optim.py:60-85 (Newton-Schulz), 180-319 (Muon step).
 #pragma once

@@ -241,9 +241,10 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
 // store, for alternate tiles, what it leaves there (Z's pair, or A / C and their mirror image)
 // and count the tile once its stores are complete, all by TMA.
 //
-// What bounds a tile is latency at every hand-over rather than a rate (at 81 x 1344 x 448 the
-// tensor core, L2 and DRAM each run at 25 - 40% of their peaks), so the choices below keep many
-// small pieces in flight: 128 x 128 tiles (with 128 x 256 ones the epilogue's boxes queued behind
+// What bounds a tile is latency at every hand-over rather than a rate (at 81 x 1344 x 448, 838 us,
+// the tensor core runs at 24%, L2 at 36% and DRAM at 41% of their peaks; a 128 x 128 tile of the
+// update takes 5,000 - 6,000 cycles to load and 3,000 in its epilogue), so the choices below keep
+// many small pieces in flight: 128 x 128 tiles (with 128 x 256 ones the epilogue's boxes queued behind
 // 144 KB of operands, and a lone matrix had half as many tiles), two storing warps (one would
 // wait 2,000 cycles a tile for its stores), three boxes.  C is kept as I + C, so that Z's high
 // half comes out of the product itself and only the low half is loaded and added.  (Rounding the
@@ -761,7 +762,9 @@ static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int b
 
 static int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-// Work buffers of the matrices of a block.
+// Work buffers of the matrices of a block: wide blocks put more tiles between a product and the
+// one that needs it (81 x 1344 x 448: 1,440 us with blocks of 64 MB, which stay in L2, 1,100 with
+// 400 MB, when the epilogues were new); several blocks only bound the reach of that.
 constexpr int64_t kBlockBytes = 400ll << 20;
 
 static void run_shapes(int src, const void* g, int out_type, void* out, const StepArgs& s, const Shape* shapes, int ns,

@@ -5,7 +5,8 @@ optimizer step for a set of matrices in flat buffers.
 ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``, from ``X = G / (|G|_F + eps)``.  The
 products run on tcgen05 with fp16 operands and fp32 accumulation while the iterate keeps 22
 or more bits, so the result is within 2e-4 .. 3e-3 (2-norm) of the exact iteration whatever
-the spectrum of ``G``: a bf16 result carries all of it.
+the spectrum of ``G`` (1e-5 for up to 32 columns, or rows, and 1,536 of the other): a bf16
+result carries all of it.
 
 ``MuonPlan`` describes which ranges of a flat parameter buffer are matrices; ``muon_step``
 runs clipping, momentum, orthogonalisation, weight decay, update and parameter average on
@@ -32,7 +33,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, eps: float = 1e-7, coeffs=NS_
     or fp16; any strides), in ``out_dtype`` (default: g's; about 11 significant bits are
     right).  ``out``, if given, is contiguous, of g's shape, and sets the type; it may be
     ``g`` itself.  A matrix of zeros gives zeros; a NaN or an infinity makes its own matrix
-    NaN and no other.  ``steps`` is at least 1 and the first coefficient positive."""
+    NaN and no other.  ``steps`` is at least 1 and the first coefficient positive.  Not
+    differentiable: the result has no graph."""
     if not isinstance(g, torch.Tensor) or not g.is_cuda:
         raise ValueError("newton_schulz: a CUDA tensor expected")
     if g.dim() < 2:
@@ -80,7 +82,7 @@ class MuonPlan:
             self.groups += [len(rows), len(idx), r, c]
             rows += [[offsets[i], moff[i], r, c] for i in idx]
         self.count = len(rows)
-        self.table = torch.tensor(rows, dtype=torch.int64).reshape(-1, 4).to(self.device)
+        self.table = torch.tensor(rows, dtype=torch.int64).reshape(len(rows), 4).to(self.device)
 
     @staticmethod
     def _extent(shapes, offsets, what) -> int:
@@ -110,7 +112,8 @@ def muon_step(plan: MuonPlan, data: torch.Tensor, grad: torch.Tensor, momentum_b
     ``scale`` is ``0.2 sqrt(max(rows, cols))`` (``"match_rms_adamw"``), ``sqrt(max(1, rows /
     cols))`` (``"original"``) or ``sqrt(max / min)`` (``"nd"``).  ``skip`` (fp32 device value)
     above 0, or a ``norm_sq`` that is not finite, leaves every buffer as it is, decided on the
-    device.  Values between the matrices are not touched."""
+    device (``norm_sq`` only counts with ``max_norm`` > 0).  Values between the matrices are not
+    touched.  The buffers must not overlap one another."""
     if adjust_lr not in _ADJUST:
         raise ValueError(f"unknown adjust_lr {adjust_lr!r}")
     for t, name in ((data, "data"), (grad, "grad"), (momentum_buf, "momentum_buf")):

@@ -52,7 +52,8 @@ def newton_schulz(G: torch.Tensor, steps: int = 5, eps: float = 1e-7) -> torch.T
     kernel on CUDA tensors, otherwise bf16 products."""
     from synthefy_nori_b200 import ops
 
-    if G.is_cuda and ops.native_available() and steps >= 1 and G.dtype in (torch.float32, torch.bfloat16, torch.float16):
+    if (G.is_cuda and ops.native_available() and 1 <= steps <= 64 and max(G.shape[-2:]) < 1 << 20
+            and G.dtype in (torch.float32, torch.bfloat16, torch.float16)):
         return ops.newton_schulz(G, steps, eps, NS_COEFFS)
     a, b, c = NS_COEFFS
     X = G.to(torch.bfloat16)
@@ -115,7 +116,7 @@ class HybridMuonAdamW:
             places += [((m, n), self.flat.offsets[i], off + j * m * n) for j, i in enumerate(ix)]
             off += -(-size // 64) * 64
         self.plan = None
-        if self.flat.data.is_cuda and ns_steps >= 1 and places:
+        if self.flat.data.is_cuda and 1 <= ns_steps <= 64 and places and all(max(s) < 1 << 20 for s, _, _ in places):
             from synthefy_nori_b200 import ops
 
             if ops.native_available():

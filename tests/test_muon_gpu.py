@@ -286,6 +286,20 @@ def test_muon_step_with_many_large_shapes():
         assert float((p[sl].double() - ref_p[sl]).norm()) <= tol, (r, c)
 
 
+def test_empty_plan_and_a_plan_of_one():
+    from synthefy_nori_b200 import ops
+
+    flat = torch.ones(8, device="cuda")
+    ops.muon_step(ops.MuonPlan([], [], "cuda"), flat, flat.clone(), flat.clone(), lr=0.1)
+    assert (flat == 1).all()
+    ops.muon_step(ops.MuonPlan([(1, 1)], [7], "cuda"), flat, flat.clone(), flat.clone(), lr=0.1, adjust_lr="original")
+    # the iteration on the number 1, five times the quintic
+    x = 1.0
+    for _ in range(5):
+        x = A * x + B * x ** 3 + C * x ** 5
+    assert (flat[:7] == 1).all() and abs(float(flat[7]) - (1 - 0.1 * x)) < 1e-5
+
+
 def test_muon_step_is_ordered_on_its_stream():
     """Large and single-CTA matrices run on two streams inside; the caller's stream sees one call:
     inputs written right before it, results read right after, buffers freed and reused."""
