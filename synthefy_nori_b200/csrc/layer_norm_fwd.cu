@@ -1,7 +1,7 @@
 // LayerNorm forward for rows of any width: fp32, bf16 or fp16 in, the same type or fp32 out
 // (fp32 from 16-bit rows is what bf16 autocast asks of a norm: no cast pass before it),
 // optional weight and bias, strided rows.  Memory bound: a row is read once and written once.
-// 403200 x 448 bf16 to fp32 in 187 us, 89% of the device's copy rate.  24 warps an SM with two
+// 403200 x 448 bf16 to fp32 in 187 - 204 us, 82 - 89% of the device's copy rate.  24 warps an SM with two
 // rows each did better than 32 with spilled registers or 40 with one (143, 166, 149 us bf16 to
 // bf16) and than one row with the next one's loads held in registers (189).
 //

@@ -762,10 +762,10 @@ static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int b
 
 static int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-// Work buffers of the matrices of a block: wide blocks put more tiles between a product and the
-// one that needs it (81 x 1344 x 448: 1,440 us with blocks of 64 MB, which stay in L2, 1,100 with
-// 400 MB, when the epilogues were new); several blocks only bound the reach of that.
-constexpr int64_t kBlockBytes = 400ll << 20;
+// Work buffers of the matrices of a block.  Wide blocks put more tiles between a product and the
+// one that needs it, narrow ones stay in L2: 81 x 1344 x 448 takes 977 us with 100 MB, 922 with
+// 200, 940 with 400 or more; 52 x 896 x 448 450, 433 and 433.
+constexpr int64_t kBlockBytes = 200ll << 20;
 
 static void run_shapes(int src, const void* g, int out_type, void* out, const StepArgs& s, const Shape* shapes, int ns,
                        const Coeffs& k, const torch::Tensor& status, const at::TensorOptions& dev,
