@@ -5,6 +5,8 @@
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cmath>
+
 namespace nori {
 namespace muon {
 
@@ -13,7 +15,9 @@ constexpr int64_t kMaxDim = 1 << 20;
 static Coeffs make_coeffs(int64_t steps, double eps, const std::vector<double>& c, const char* who) {
   TORCH_CHECK(steps >= 1 && steps <= 64, who, ": steps must be in 1..64");
   TORCH_CHECK(eps >= 0.0, who, ": eps must not be negative");
-  TORCH_CHECK(c.size() == 3 && c[0] > 0.0, who, ": three coefficients with a positive first one expected");
+  // below 1 the small directions shrink from step to step and the iterate's scale has no bound
+  TORCH_CHECK(c.size() == 3 && c[0] >= 1.0 && c[0] <= 1024.0 && std::isfinite(c[1]) && std::isfinite(c[2]), who,
+              ": three finite coefficients, the first in 1..1024, expected");
   return {static_cast<int>(steps), static_cast<float>(eps), static_cast<float>(c[0]), static_cast<float>(c[1] / c[0]),
           static_cast<float>(c[2] / c[0])};
 }

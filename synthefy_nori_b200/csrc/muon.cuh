@@ -5,15 +5,19 @@
 //   X_0 = G / (|G|_F + eps)
 //   A = X^T X,   C = (b A + c A^2) / a,   X <- a (X + X C)          (repeated `steps` times)
 //
-// Numerics.  The kernels carry Z_k = 2^8 X_k / (f a^k) with f = |G|_F / (|G|_F + eps), so
-// that one step is Z <- Z + Z C and the leading term needs no multiplication: X_k = xi_k Z_k
-// with xi_0 = f 2^-8 and xi_{k+1} = a xi_k.  Z is held in fp32 (one CTA a matrix) or as a pair of
-// fp16 (high, low: 22 significant bits; over the whole GPU); the three products read fp16 operands (the high parts, A and C: 11
+// Numerics.  The kernels carry Z_k = X_k / xi_k with xi_0 = f 2^-8, f = |G|_F / (|G|_F + eps), so
+// that one step is Z <- Z + Z C, xi <- a xi, and the leading term needs no multiplication.  X
+// stays of size 1 while xi grows by a (3.4 with the usual coefficients) a step, so Z would shrink
+// to nothing in fp16: where xi has grown past a limit a power of two, exact in all that holds Z,
+// goes from xi to Z (`renorm`), and any number of steps keeps its digits.  As long as X itself
+// is still growing (|G| far below eps) xi is below the limit and Z stays as it is.
+// Z is held in fp32 (one CTA a matrix) or as a pair of fp16 (high, low: 22 significant bits;
+// over the whole GPU); the three products read fp16 operands (the high parts, A and C: 11
 // bits) and accumulate in fp32.  A small singular value of G lives in the pair and is only
 // multiplied by 1 + C, so it keeps its 22 bits, while the rounding of the products' operands
-// (2^-12 relative) perturbs the dominant directions only and is not amplified: the result is
-// 2e-4 .. 2e-3 (2-norm) from the exact iteration for flat, power-law, exponential and
-// rank-deficient spectra alike, about the rounding of a bf16 result.  With iterates rounded
+// (2^-12 relative) perturbs the dominant directions only and is not amplified: five steps are
+// 1e-3 .. 3e-3 (2-norm) from the exact iteration for flat, power-law, exponential and
+// rank-deficient spectra alike, about the rounding of a bf16 result, and 64 steps about 1e-2.  With iterates rounded
 // to bf16 the noise 2^-9 |G|_F is amplified by up to a^5 = 485 in the small directions: 1e-2
 // for a flat spectrum and 0.1 .. 1 for steep ones.  Products of fp16 pairs (three MMAs each)
 // give 1e-6 for three times the tensor work; the single-CTA kernel takes them up to 32 columns,
@@ -40,6 +44,15 @@ namespace nori {
 namespace muon {
 
 constexpr float kZScale = 256.f;
+
+// Takes a power of two out of xi once it is above `limit` (at least 2^-8), leaving it in [2^-9, 2^-8),
+// and returns that power for Z to be multiplied by (1 where there is nothing to do, or xi is NaN).
+__device__ __forceinline__ float renorm(float& xi, float limit) {
+  if (!(xi > limit)) return 1.f;
+  const int e = (__float_as_int(xi) >> 23) - (127 - 9);
+  xi *= __int_as_float((127 - e) << 23);
+  return __int_as_float((127 + e) << 23);
+}
 
 enum OutType : int { kOutF32 = 0, kOutBF16 = 1, kOutF16 = 2, kOutMuon = 3 };
 enum SrcType : int { kSrcF32 = 0, kSrcBF16 = 1, kSrcF16 = 2, kSrcMuon = 3 };

@@ -533,7 +533,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const Item x = item_of(a, cur, t);
       const Group& q = a.g[x.g];
       float xi = a.f[q.base + x.mat] * (1.f / kZScale);
-      for (int k = 0; k < x.it; ++k) xi *= a.k.a;
+      for (int k = 0; k < x.it; ++k) {
+        xi *= a.k.a;
+        renorm(xi, 1.f / kZScale);
+      }
+      float next = xi * a.k.a;  // and the power of two that an update moves to Z
+      const float up = renorm(next, 1.f / kZScale);
       if (!mbar_wait_warp(&tfull[acc], acc_phase, a.status, kTimeoutEpilogue, abort_flag)) break;
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + acc * 128 + half * 32;
@@ -590,6 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             for (int i = 0; i < 8; ++i) v[8 * j + i] += l[i];
             if (!x.last) {
               float h[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[8 * j + i] *= up;
               const uint4 hi = pack8(v + 8 * j);
               unpack8(hi, h);
 #pragma unroll

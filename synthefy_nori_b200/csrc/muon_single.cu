@@ -323,6 +323,9 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
       __syncwarp();
       xi *= p.k.a;
       if (it == p.k.steps - 1) break;
+      // Z is fp32, so only its copy needs |Z| >= |X|: five steps of the usual coefficients never
+      // come here with another factor than 1
+      const float up = renorm(xi, 1.f);
       // the fp16 copy of each finished tile, and its share of the next A behind it
       first(t, c);
       for (int i = 0; i < tiles; ++i) {
@@ -331,8 +334,18 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
         for (; t == i; next(t, c)) {
           float v[16];
           ld16(tlane + t * mp + c * 16, v);
+          if (up != 1.f) {
+            uint32_t r[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              v[k] *= up;
+              r[k] = __float_as_uint(v[k]);
+            }
+            tmem_st16(tlane + t * mp + c * 16, r);
+          }
           put(zh, zpanel, t * 128 + q * 32 + lane, c * 16, v);
         }
+        tmem_wait_st();
         if (!publish()) break;  // every warp's part of the tile
         gram(i);
       }
