@@ -51,8 +51,12 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, eps: float = 1e-7, coeffs=NS_
             raise ValueError("newton_schulz: out must be contiguous fp32, bf16 or fp16, of g's shape and on its device")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"newton_schulz: out is {out.dtype}, out_dtype {out_dtype}")
-    return _lib().newton_schulz(g if g.is_contiguous() else g.contiguous(), out, out_dtype, steps, eps, coeffs,
-                                status_word(g.device))
+    res = _lib().newton_schulz(g if g.is_contiguous() else g.contiguous(), out, out_dtype, steps, eps, coeffs,
+                               status_word(g.device))
+    if out is None:
+        return res
+    torch.autograd.graph.increment_version(out)
+    return out
 
 
 class MuonPlan:
@@ -130,3 +134,5 @@ def muon_step(plan: MuonPlan, data: torch.Tensor, grad: torch.Tensor, momentum_b
     _lib().muon_step(data, grad, momentum_buf, ema, plan.table, plan.groups, float(lr), float(wd), float(momentum),
                      bool(nesterov), int(steps), float(eps), [float(c) for c in coeffs], _ADJUST[adjust_lr], norm_sq,
                      float(max_norm), skip, float(ema_decay), status_word(data.device))
+    # written through raw pointers: what autograd saved of them is no longer valid
+    torch.autograd.graph.increment_version([data, momentum_buf] if ema is None else [data, momentum_buf, ema])

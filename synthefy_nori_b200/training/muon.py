@@ -190,6 +190,7 @@ class HybridMuonAdamW:
         if self.ema is not None and self.plan is None:
             w = 1.0 - self.ema_decay
             self.ema.lerp_(self.flat.data, w if keep is None else keep * w)
+        self.flat.mark_updated()
 
     def _adamw_torch(self, p, g):
         b1, b2 = self.betas

@@ -42,6 +42,12 @@ class FlatParams:
                 p.grad = self.grad[o : o + p.numel()].view(p.shape)
 
 
+    def mark_updated(self) -> None:
+        """After a step that wrote through the flat buffer: raises the parameters' own version
+        counters, which caches of derived weights and autograd's check of saved tensors read."""
+        torch.autograd.graph.increment_version(self.params)
+
+
 class FusedAdamWEMA:
     def __init__(self, flat: FlatParams, lr=1e-4, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.0, ema_decay=0.999,
                  max_grad_norm=1.0):
@@ -63,6 +69,7 @@ class FusedAdamWEMA:
         self.step_count += 1
         if not self.flat.data.is_cuda:
             self._step_torch(grad_scale, skip)
+            self.flat.mark_updated()
             return
         if self.max_grad_norm and self.max_grad_norm > 0:
             self.norm_sq.zero_()
@@ -73,6 +80,7 @@ class FusedAdamWEMA:
                            ema_decay=self.ema_decay if self.ema_decay is not None else 0.0,
                            max_norm=self.max_grad_norm or 0.0, grad_scale=grad_scale,
                            skip=None if skip is None else skip.reshape(1).float())
+        self.flat.mark_updated()
 
     @torch.no_grad()
     def _step_torch(self, grad_scale, skip) -> None:
