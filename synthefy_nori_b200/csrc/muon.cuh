@@ -8,9 +8,10 @@
 // Numerics.  The kernels carry Z_k = X_k / xi_k with xi_0 = f 2^-8, f = |G|_F / (|G|_F + eps), so
 // that one step is Z <- Z + Z C, xi <- a xi, and the leading term needs no multiplication.  X
 // stays of size 1 while xi grows by a (3.4 with the usual coefficients) a step, so Z would shrink
-// to nothing in fp16: where xi has grown past a limit a power of two, exact in all that holds Z,
-// goes from xi to Z (`renorm`), and any number of steps keeps its digits.  As long as X itself
-// is still growing (|G| far below eps) xi is below the limit and Z stays as it is.
+// to nothing in fp16: where xi has grown past 1 (|Z| < |X|) a power of two, exact in all that holds Z,
+// goes from xi to Z (`renorm`), and any number of steps keeps its digits; five steps with the usual
+// coefficients never get there.  As long as X itself is still growing (|G| far below eps) xi is
+// below 1 and Z stays as it is.
 // Z is held in fp32 (one CTA a matrix) or as a pair of fp16 (high, low: 22 significant bits;
 // over the whole GPU); the three products read fp16 operands (the high parts, A and C: 11
 // bits) and accumulate in fp32.  A small singular value of G lives in the pair and is only
@@ -45,10 +46,10 @@ namespace muon {
 
 constexpr float kZScale = 256.f;
 
-// Takes a power of two out of xi once it is above `limit` (at least 2^-8), leaving it in [2^-9, 2^-8),
-// and returns that power for Z to be multiplied by (1 where there is nothing to do, or xi is NaN).
-__device__ __forceinline__ float renorm(float& xi, float limit) {
-  if (!(xi > limit)) return 1.f;
+// Takes a power of two out of xi once it is above 1, leaving it in [2^-9, 2^-8), and returns that
+// power for Z to be multiplied by (1 where there is nothing to do, or xi is NaN).
+__device__ __forceinline__ float renorm(float& xi) {
+  if (!(xi > 1.f)) return 1.f;
   const int e = (__float_as_int(xi) >> 23) - (127 - 9);
   xi *= __int_as_float((127 - e) << 23);
   return __int_as_float((127 + e) << 23);

@@ -21,7 +21,7 @@ struct Group {
 struct Pre {
   int groups;
   double* partial;               // [matrix][slices], the groups one after the other
-  float* f;
+  float2* scale;                 // [matrix][step]: xi before the step, and the power of two after it
   int* done;
   Group g[kMaxShapes];
 };
@@ -116,9 +116,9 @@ __global__ void __launch_bounds__(256) norm_kernel(const void* __restrict__ g, S
 
 // ------------------------------------------------------------------ Z_0
 // Z_0 = 2^8 G / |G|_F as a pair of fp16 [n, ldz], tall (a wide G is turned in shared memory),
-// and f = |G|_F / (|G|_F + eps).  One CTA per 64 x 64 tile.
+// and its scales over the steps, from f = |G|_F / (|G|_F + eps).  One CTA per 64 x 64 tile.
 template <int SRC>
-__global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, StepArgs s, float eps,
+__global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, StepArgs s, Coeffs k,
                                                     const __grid_constant__ Pre p) {
   if constexpr (SRC == kSrcMuon) {
     if (step_rejected(s)) return;
@@ -185,8 +185,16 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
   }
   __syncthreads();
   float s0, s1, f;
-  z_scale(total, eps, s0, s1, f);
-  if (ti == 0 && threadIdx.x == 0) p.f[q.base + mat] = f;
+  z_scale(total, k.eps, s0, s1, f);
+  if (ti == 0 && threadIdx.x == 0) {
+    float2* d = p.scale + static_cast<int64_t>(q.base + mat) * k.steps;
+    float xi = f * (1.f / kZScale);
+    for (int it = 0; it < k.steps; ++it) {
+      float next = xi * k.a;
+      d[it] = make_float2(xi, renorm(next));
+      xi = next;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -268,7 +276,7 @@ struct Args {
   Group g[kMaxShapes];
   int groups, blocks;
   Coeffs k;
-  const float* f;
+  const float2* scale;
   int* done;
   int out_type;
   void* out;
@@ -532,13 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     for (int t = blockIdx.x; ok && cur.seek(a, t); t += gridDim.x) {
       const Item x = item_of(a, cur, t);
       const Group& q = a.g[x.g];
-      float xi = a.f[q.base + x.mat] * (1.f / kZScale);
-      for (int k = 0; k < x.it; ++k) {
-        xi *= a.k.a;
-        renorm(xi, 1.f / kZScale);
-      }
-      float next = xi * a.k.a;  // and the power of two that an update moves to Z
-      const float up = renorm(next, 1.f / kZScale);
+      const float2 sc = a.scale[static_cast<int64_t>(q.base + x.mat) * a.k.steps + x.it];
+      const float xi = sc.x, up = sc.y;
       if (!mbar_wait_warp(&tfull[acc], acc_phase, a.status, kTimeoutEpilogue, abort_flag)) break;
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + acc * 128 + half * 32;
@@ -595,8 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             for (int i = 0; i < 8; ++i) v[8 * j + i] += l[i];
             if (!x.last) {
               float h[8];
+              if (up != 1.f) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[8 * j + i] *= up;
+                for (int i = 0; i < 8; ++i) v[8 * j + i] *= up;
+              }
               const uint4 hi = pack8(v + 8 * j);
               unpack8(hi, h);
 #pragma unroll
@@ -814,7 +819,7 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
                 "muon: too many matrices for one call");
   }
   const int64_t work = bytes;
-  const int64_t p_at = take(parts * 8), f_at = take(mats * 4), d_at = take(mats * 4);
+  const int64_t p_at = take(parts * 8), s_at = take(mats * k.steps * 8), d_at = take(mats * 4);
   auto ws = torch::empty({bytes}, dev.dtype(at::kByte));
   uint8_t* w = ws.data_ptr<uint8_t>();
   for (int i = 0; i < ns; ++i) {
@@ -838,12 +843,12 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
   }
   p.groups = ns;
   p.partial = reinterpret_cast<double*>(w + p_at);
-  p.f = reinterpret_cast<float*>(w + f_at);
+  p.scale = reinterpret_cast<float2*>(w + s_at);
   p.done = reinterpret_cast<int*>(w + d_at);
   a.groups = ns;
   a.blocks = static_cast<int>(std::max<int64_t>(1, (work + kBlockBytes - 1) / kBlockBytes));
   a.k = k;
-  a.f = p.f;
+  a.scale = p.scale;
   a.done = p.done;
   a.out_type = out_type;
   a.out = out;
@@ -853,7 +858,7 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
 #define NORI_MUON_SRC(S)                                                                    \
   norm_kernel<S><<<static_cast<unsigned>(norm_ctas), 256, 0, stream>>>(g, s, p);           \
   C10_CUDA_KERNEL_LAUNCH_CHECK();                                                           \
-  scale_kernel<S><<<static_cast<unsigned>(scale_ctas), 256, 0, stream>>>(g, s, k.eps, p);  \
+  scale_kernel<S><<<static_cast<unsigned>(scale_ctas), 256, 0, stream>>>(g, s, k, p);      \
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (src == kSrcF32) {
     NORI_MUON_SRC(kSrcF32)

@@ -323,9 +323,7 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
       __syncwarp();
       xi *= p.k.a;
       if (it == p.k.steps - 1) break;
-      // Z is fp32, so only its copy needs |Z| >= |X|: five steps of the usual coefficients never
-      // come here with another factor than 1
-      const float up = renorm(xi, 1.f);
+      const float up = renorm(xi);
       // the fp16 copy of each finished tile, and its share of the next A behind it
       first(t, c);
       for (int i = 0; i < tiles; ++i) {
