@@ -85,6 +85,13 @@ struct StepArgs {
   int nesterov, adjust;
 };
 
+// Whether a wait of an earlier kernel has run out (nothing is read or written from then on, until the
+// host has seen it).  The word can change at any time, so the CTA's threads settle on one answer:
+// with some gone and some not, tensor memory would be used before it is there.
+__device__ __forceinline__ bool timed_out(const int* status) {
+  return __syncthreads_or(*reinterpret_cast<const volatile int*>(status) != 0) != 0;
+}
+
 // A step that the trainer rejected on the device, or one whose gradient norm is not finite,
 // leaves weights, momentum and average as they are (as adamw_ema_kernel does).
 __device__ __forceinline__ bool step_rejected(const StepArgs& s) {

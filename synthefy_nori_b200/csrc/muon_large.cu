@@ -23,6 +23,7 @@ struct Pre {
   double* partial;               // [matrix][slices], the groups one after the other
   float2* scale;                 // [matrix][step]: xi before the step, and the power of two after it
   int* done;
+  const int* status;
   Group g[kMaxShapes];
 };
 
@@ -39,8 +40,8 @@ __device__ __forceinline__ const double* partials(const Pre& p, int gi, int mat)
 template <int SRC>
 __global__ void __launch_bounds__(256) norm_kernel(const void* __restrict__ g, StepArgs s,
                                                    const __grid_constant__ Pre p) {
-  if constexpr (SRC == kSrcMuon) {
-    if (step_rejected(s)) return;
+  if constexpr (SRC == kSrcMuon) {  // the momentum stays where the weights will
+    if (timed_out(p.status) || step_rejected(s)) return;
   }
   int gi = 0;
   while (gi + 1 < p.groups && static_cast<int>(blockIdx.x) >= p.g[gi + 1].norm_cta) ++gi;
@@ -365,7 +366,11 @@ __device__ __forceinline__ bool wait_done(const Args& a, const Item& x, volatile
     if (v >= x.need) break;
     if (spins == 0) t0 = globaltimer_ns();
     if ((spins & 63u) == 63u) {
-      if (*abort || *reinterpret_cast<volatile int*>(a.status) != 0) return false;
+      if (*abort) return false;
+      if (*reinterpret_cast<volatile int*>(a.status) != 0) {  // another CTA has given up
+        *abort = 1;
+        return false;
+      }
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         record_status(a.status, kTimeoutProducer);
         *abort = 1;
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (*reinterpret_cast<volatile int*>(a.status) != 0) return;
+  if (timed_out(a.status)) return;
   if (a.out_type == kOutMuon && step_rejected(a.s)) return;
 
   if (threadIdx.x == 0) {
@@ -440,6 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       i = 0;
       phase ^= 1;
     }
+  };
+  // a role that has given up waits (again with a limit) until what it last started in each place of
+  // its ring is complete: no copy or product is under way when the CTA's memory goes to another
+  auto drain = [&](uint64_t* bars, int i, uint32_t phase, int n) {
+    for (int k = 0; k < n; ++k)
+      mbar_wait(&bars[k], k < i ? phase : phase ^ 1, a.status, kTimeoutProducer, nullptr);
   };
   int re = 0;
   uint32_t rp = 0;
@@ -480,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           advance(stage, phase, kStages);
         }
       }
+      drain(full, stage, phase, kStages);
     }
   } else if (warp == 1) {
     if (elect_one()) {
@@ -519,6 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         umma_commit(&tfull[acc]);
         advance(acc, acc_phase, kAccs);
       }
+      drain(empty, stage, phase, kStages);
     }
   } else if (warp == 10) {
     if (elect_one()) {
@@ -700,6 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           advance(slot, phase, kSlots);
         }
       }
+      drain(sfull, slot, phase, kSlots);
     }
   } else {
     if (elect_one()) {
@@ -845,6 +859,7 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
   p.partial = reinterpret_cast<double*>(w + p_at);
   p.scale = reinterpret_cast<float2*>(w + s_at);
   p.done = reinterpret_cast<int*>(w + d_at);
+  p.status = status.data_ptr<int>();
   a.groups = ns;
   a.blocks = static_cast<int>(std::max<int64_t>(1, (work + kBlockBytes - 1) / kBlockBytes));
   a.k = k;

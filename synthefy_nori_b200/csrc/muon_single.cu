@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(kSingleThreads, 1) single_kernel(const void* _
   __shared__ uint64_t bar[1 + kSingleMaxTiles];
   __shared__ double red[16];
   __shared__ uint32_t tmem_slot;
-  if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
+  if (timed_out(p.status)) return;
   int rows = p.rows, cols = p.cols;
   int64_t base, mbase = 0;
   float clip = 1.f;

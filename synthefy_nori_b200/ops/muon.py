@@ -11,6 +11,10 @@ alone: 1e-2 after 64 on most matrices with the coefficients below (one whose sin
 the iteration's repelling fixed point, 0.868, spreads roundings as any precision does), 1.5e-3
 after 64 of a convergent iteration.
 
+After a bounded wait of any native kernel on the device has run out (``ops.check_status``
+raises), ``muon_step`` leaves its buffers as they are and ``newton_schulz`` its output
+unwritten; a wait of their own that runs out leaves results incomplete.
+
 ``MuonPlan`` describes which ranges of a flat parameter buffer are matrices; ``muon_step``
 runs clipping, momentum, orthogonalisation, weight decay, update and parameter average on
 all of them.

@@ -266,7 +266,13 @@ class NoriTrainer:
         self._skips.fill_(float(n))
 
     def poll(self) -> dict:
-        """Host view of the device counters (one synchronisation)."""
+        """Host view of the device counters (one synchronisation); raises where a native
+        kernel has given up waiting (weights and optimizer state are then not of one step)."""
+        if self.device.type == "cuda":
+            from synthefy_nori_b200 import ops
+
+            if ops.native_available():
+                ops.check_status(self.device)
         out = {"skipped_steps": int(self._skips.item()), "nonfinite_steps": int(self._fatal.item())}
         if self.peer is not None:
             d = self.peer.diag.tolist()
