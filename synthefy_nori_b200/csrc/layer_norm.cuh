@@ -17,6 +17,7 @@
 
 #include <algorithm>
 
+#include "plain.h"
 #include "sm100.cuh"
 
 namespace nori {
@@ -186,6 +187,7 @@ inline bool vec_ok(const void* p, int64_t ld, int64_t C, int64_t elem, int vec) 
 inline const float* opt_vec(const c10::optional<torch::Tensor>& t, int64_t C, const torch::Device& dev,
                             const char* what) {
   if (!t.has_value() || !t->defined()) return nullptr;
+  check_plain(*t, what);
   TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == C, what,
               ": contiguous fp32 vector of the row width on x's device expected");
   return t->data_ptr<float>();
@@ -193,6 +195,7 @@ inline const float* opt_vec(const c10::optional<torch::Tensor>& t, int64_t C, co
 
 // rows of `t`: [R, C] with unit column stride, any row stride
 inline void check_rows(const torch::Tensor& t, const char* what) {
+  check_plain(t, what);
   TORCH_CHECK(t.is_cuda() && t.dim() == 2, what, ": a CUDA matrix [rows, cols] expected");
   const auto s = t.scalar_type();
   TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, what, ": fp32, bf16 or fp16 expected");

@@ -333,6 +333,8 @@ std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::
   for (const torch::Tensor* t : std::initializer_list<const torch::Tensor*>{&mean, &rstd})
     TORCH_CHECK(t->device() == x.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == R,
                 "layer_norm_bwd: mean and rstd must be the forward's fp32 rows");
+  check_plain(mean, "layer_norm_bwd: mean");
+  check_plain(rstd, "layer_norm_bwd: rstd");
   BwdArgs a;
   a.w = opt_vec(w, C, x.device(), "layer_norm_bwd: weight");
   const at::cuda::CUDAGuard guard(x.device());
@@ -340,6 +342,7 @@ std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::
   auto dx = torch::empty({R, C}, x.options());
   auto dw = weight_grad ? torch::empty({C}, f32) : torch::empty({0}, f32);
   auto db = bias_grad ? torch::empty({C}, f32) : torch::empty({0}, f32);
+  check_plain(dx, "layer_norm_bwd");
   if (R == 0) {
     dw.zero_();
     db.zero_();

@@ -37,6 +37,7 @@ torch::Tensor newton_schulz(const torch::Tensor& g, const c10::optional<torch::T
                             c10::optional<c10::ScalarType> out_type, int64_t steps, double eps,
                             std::vector<double> coeffs, const torch::Tensor& status) {
   using namespace muon;
+  check_plain(g, "newton_schulz");
   TORCH_CHECK(g.is_cuda() && g.dim() >= 2 && g.is_contiguous(), "newton_schulz: contiguous CUDA [.., rows, cols]");
   auto kind = [](c10::ScalarType s, const char* what) {
     TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, "newton_schulz: ", what,
@@ -51,6 +52,7 @@ torch::Tensor newton_schulz(const torch::Tensor& g, const c10::optional<torch::T
   torch::Tensor out = out_opt.has_value() && out_opt->defined()
                           ? *out_opt
                           : torch::empty(g.sizes(), g.options().dtype(out_type.value_or(g.scalar_type())));
+  check_plain(out, "newton_schulz: out");
   TORCH_CHECK(out.device() == g.device() && out.is_contiguous() && out.sizes() == g.sizes(),
               "newton_schulz: out must be contiguous, of g's shape and device");
   const int dst = kind(out.scalar_type(), "out");
@@ -78,6 +80,8 @@ void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mo
                double max_norm, const c10::optional<torch::Tensor>& skip, double ema_decay,
                const torch::Tensor& status) {
   using namespace muon;
+  for (const auto& t : {data, grad, mom, table, status}) check_plain(t, "muon_step");
+  for (const auto& t : {ema, norm_sq, skip}) check_plain(t, "muon_step");
   for (const torch::Tensor* t : std::initializer_list<const torch::Tensor*>{&data, &grad, &mom})
     TORCH_CHECK(t->is_cuda() && t->device() == data.device() && t->scalar_type() == at::kFloat && t->dim() == 1 &&
                     t->is_contiguous(),

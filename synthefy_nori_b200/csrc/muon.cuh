@@ -38,6 +38,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "plain.h"
 #include "sm100.cuh"
 #include "tma_host.h"
 

@@ -835,6 +835,7 @@ static void run_shapes(int src, const void* g, int out_type, void* out, const St
   const int64_t work = bytes;
   const int64_t p_at = take(parts * 8), s_at = take(mats * k.steps * 8), d_at = take(mats * 4);
   auto ws = torch::empty({bytes}, dev.dtype(at::kByte));
+  check_plain(ws, "muon");
   uint8_t* w = ws.data_ptr<uint8_t>();
   for (int i = 0; i < ns; ++i) {
     Group& q = p.g[i];

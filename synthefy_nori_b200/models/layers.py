@@ -34,13 +34,16 @@ ACTIVATIONS = {"gelu": nn.GELU, "relu": nn.ReLU, "silu": nn.SiLU}
 
 class LayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` that runs the native kernel on CUDA tensors (``ops.layer_norm``; under
-    autocast the result is fp32, as torch's is, without a cast of the input before it)."""
+    autocast the result is fp32, as torch's is, without a cast of the input before it).  Function
+    transforms, forward-mode derivatives, tracing and fake tensors take torch's path.  Rows and
+    weights may be of different floating types."""
 
     def forward(self, x):
         from synthefy_nori_b200 import ops
 
-        if (x.is_cuda and len(self.normalized_shape) == 1 and x.dim() and x.shape[-1] == self.normalized_shape[0]
-                and x.dtype in (torch.float32, torch.bfloat16, torch.float16) and ops.native_available()):
+        if (x.is_cuda and ops.is_plain(x) and ops.native_available() and len(self.normalized_shape) == 1 and x.dim()
+                and 0 < x.shape[-1] == self.normalized_shape[0]
+                and x.dtype in (torch.float32, torch.bfloat16, torch.float16)):
             out = torch.float32 if torch.is_autocast_enabled("cuda") else None
             return ops.layer_norm(x, self.weight, self.bias, self.eps, out)
         return super().forward(x)

@@ -35,6 +35,7 @@ __all__ = [
     "adamw_ema_step",
     "quantize_int8",
     "dequantize_int8",
+    "is_plain",
     "status_word",
     "check_status",
     "interleave_swiglu_weights",
@@ -52,11 +53,23 @@ def _lib():
     return lib()
 
 
+def is_plain(t: torch.Tensor) -> bool:
+    """Whether ``t`` is memory that a native kernel can work on here and now: no subclass (fake and
+    other wrapped tensors have no memory of their own), and no function transform, forward-mode
+    level, tracer or dispatch mode that has to see the operation itself."""
+    return (type(t) in (torch.Tensor, torch.nn.Parameter) and not torch._C._are_functorch_transforms_active()
+            and torch.autograd.forward_ad._current_level < 0 and not torch._C._len_torch_dispatch_stack()
+            and not torch.compiler.is_compiling() and not torch.jit.is_tracing())
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 word that kernels set on a bounded-wait timeout (0 = ok)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _STATUS.get(idx)
     if t is None:
+        if torch._C._len_torch_dispatch_stack():  # a fake word would stay for every later call
+            with torch.utils._python_dispatch._disable_current_modes():
+                return status_word(device)
         t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
         _STATUS[idx] = t
     return t
