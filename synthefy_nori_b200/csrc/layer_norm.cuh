@@ -154,6 +154,19 @@ __device__ __forceinline__ void load_columns(const float* w, int c, float fill, 
   }
 }
 
+// The sum of a thread's values.  Sums are pairwise throughout, so a row of 2^k equal values has them
+// for its mean, exactly, and gives the bias.
+__device__ __forceinline__ float pairwise_sum(const float (&v)[kValues]) {
+  float a[kValues / 2];
+#pragma unroll
+  for (int i = 0; i < kValues / 2; ++i) a[i] = v[2 * i] + v[2 * i + 1];
+#pragma unroll
+  for (int n = kValues / 4; n > 0; n >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) a[i] += a[i + n];
+  return a[0];
+}
+
 // Sums of N values over the TPR threads of a row; every one of them gets them.  Rows wider
 // than a warp add their warps' sums through `sh`, which alternates between two places from one
 // use to the next, so one barrier is enough.
@@ -171,9 +184,14 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (&sh)[2][N][16], in
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      v[k] = 0.f;
+      float a[TPR / 32];
 #pragma unroll
-      for (int i = 0; i < TPR / 32; ++i) v[k] += sh[flip][k][w0 + i];
+      for (int i = 0; i < TPR / 32; ++i) a[i] = sh[flip][k][w0 + i];
+#pragma unroll
+      for (int n = TPR / 64; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) a[i] += a[i + n];
+      v[k] = a[0];
     }
     flip ^= 1;
   }

@@ -35,9 +35,7 @@ __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T
       for (int k = 0; k < 2; ++k) r[k].values(v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) s[k] += v[k][i];
+    for (int k = 0; k < 2; ++k) s[k] = pairwise_sum(v[k]);
     row_sum<TPR, 2>(s, sh, flip);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
