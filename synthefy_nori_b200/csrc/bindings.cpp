@@ -164,7 +164,9 @@ std::vector<torch::Tensor> layer_norm_fwd(const torch::Tensor& x, const c10::opt
                                           const c10::optional<torch::Tensor>& b, double eps, bool out_f32);
 std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x, const torch::Tensor& mean,
                                           const torch::Tensor& rstd, const c10::optional<torch::Tensor>& w,
-                                          bool weight_grad, bool bias_grad);
+                                          bool weight_grad, bool bias_grad, c10::ScalarType grad_type);
+torch::Tensor layer_norm(const torch::Tensor& x, const c10::optional<torch::Tensor>& w,
+                         const c10::optional<torch::Tensor>& b, double eps, bool out_f32, bool dual);
 }  // namespace nori
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -235,5 +237,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("muon_step", &nori::muon_step);
   m.def("muon_single_cta", &nori::muon_single_cta);
   m.def("layer_norm_fwd", &nori::layer_norm_fwd);
-  m.def("layer_norm_bwd", &nori::layer_norm_bwd);
+  m.def("layer_norm_bwd", &nori::layer_norm_bwd, py::arg("dy"), py::arg("x"), py::arg("mean"), py::arg("rstd"),
+        py::arg("weight"), py::arg("weight_grad"), py::arg("bias_grad"), py::arg("grad_type") = at::kFloat);
+  m.def("layer_norm", &nori::layer_norm);
 }

@@ -141,15 +141,16 @@ __device__ __forceinline__ void prefetch_row(const T* row, int C) {
 }
 
 // VEC columns of a weight vector (`fill` where there is none).
-template <int VEC>
-__device__ __forceinline__ void load_columns(const float* w, int c, float fill, float* v) {
+template <int VEC, typename W>
+__device__ __forceinline__ void load_columns(const W* w, int c, float fill, float* v) {
+  constexpr int N = VEC * sizeof(W) > 16 ? 16 / sizeof(W) : VEC;  // of one access
 #pragma unroll
-  for (int i = 0; i < VEC; i += VEC < 4 ? 1 : 4) {
+  for (int i = 0; i < VEC; i += N) {
     if (w == nullptr) {
 #pragma unroll
-      for (int k = 0; k < (VEC < 4 ? 1 : 4); ++k) v[i + k] = fill;
+      for (int k = 0; k < N; ++k) v[i + k] = fill;
     } else {
-      load_vec<float, VEC < 4 ? 1 : 4>(w + c + i, v + i);
+      load_vec<W, N>(w + c + i, v + i);
     }
   }
 }
@@ -202,13 +203,35 @@ inline bool vec_ok(const void* p, int64_t ld, int64_t C, int64_t elem, int vec) 
   return C % vec == 0 && (ld * elem) % (vec * elem) == 0 && reinterpret_cast<uintptr_t>(p) % (vec * elem) == 0;
 }
 
-inline const float* opt_vec(const c10::optional<torch::Tensor>& t, int64_t C, const torch::Device& dev,
-                            const char* what) {
-  if (!t.has_value() || !t->defined()) return nullptr;
-  check_plain(*t, what);
-  TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == C, what,
-              ": contiguous fp32 vector of the row width on x's device expected");
-  return t->data_ptr<float>();
+// The weight and the bias as the kernels read them: in x's type where both have it, else in fp32.
+struct Affine {
+  torch::Tensor w, b;  // undefined where there is none
+  bool f32;
+  const void* wp() const { return w.defined() ? w.data_ptr() : nullptr; }
+  const void* bp() const { return b.defined() ? b.data_ptr() : nullptr; }
+};
+inline Affine affine_of(const torch::Tensor& x, const c10::optional<torch::Tensor>& w,
+                        const c10::optional<torch::Tensor>& b, const char* what) {
+  Affine a;
+  a.f32 = x.scalar_type() == at::kFloat;
+  for (const auto* t : {&w, &b}) {
+    if (!t->has_value() || !(*t)->defined()) continue;
+    check_plain(**t, what);
+    TORCH_CHECK((*t)->device() == x.device() && at::isFloatingType((*t)->scalar_type()) && (*t)->numel() == x.size(1), what,
+                ": weight and bias must be floating vectors of the row width on x's device");
+    if ((*t)->scalar_type() != x.scalar_type()) a.f32 = true;
+  }
+  const auto type = a.f32 ? at::kFloat : x.scalar_type();
+  auto plain = [&](const torch::Tensor& t) {
+    return t.scalar_type() == type && t.is_contiguous() ? t : t.detach().to(type).contiguous();
+  };
+  if (w.has_value() && w->defined()) a.w = plain(*w);
+  if (b.has_value() && b->defined()) a.b = plain(*b);
+  return a;
+}
+template <typename W>
+inline bool vec_ok_columns(const void* p, int64_t C, int vec) {
+  return vec_ok(p, 0, C, sizeof(W), std::min<int>(vec, 16 / sizeof(W)));
 }
 
 // rows of `t`: [R, C] with unit column stride, any row stride

@@ -17,10 +17,10 @@
 namespace nori {
 namespace ln {
 
-template <typename T, typename U, int VEC, int TPR, bool GRADS>
+template <typename T, typename U, typename W, int VEC, int TPR, bool GRADS>
 __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
     bwd_kernel(const U* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx, int64_t R, int C,
-               const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const float* __restrict__ w,
+               const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const W* __restrict__ w,
                T* __restrict__ dx, float* __restrict__ part_w, float* __restrict__ part_b) {
   constexpr int CH = kValues / VEC, RPB = kCta<TPR> / TPR;
   extern __shared__ float acc_sh[];  // [RPB][C] where a CTA holds several row groups
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
     for (int j = 0; j < CH; ++j) {
       const int c = VEC * (t + TPR * j);
       if (c < C) {
-        load_columns<VEC>(w, c, 1.f, wv + VEC * j);
+        load_columns<VEC, W>(w, c, 1.f, wv + VEC * j);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) wv[VEC * j + i] = 0.f;
@@ -142,10 +142,10 @@ __global__ void __launch_bounds__(kCta<TPR>, 512 / kCta<TPR>)
 }
 
 // Rows wider than the registers of a CTA: dx in two passes over the row.
-template <typename T, typename U>
+template <typename T, typename U, typename W>
 __global__ void __launch_bounds__(512)
     bwd_wide_kernel(const U* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx, int64_t R, int C,
-                    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const float* __restrict__ w,
+                    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const W* __restrict__ w,
                     T* __restrict__ dx) {
   __shared__ float sh[2][2][16];
   const float inv_c = 1.f / static_cast<float>(C);
@@ -156,14 +156,14 @@ __global__ void __launch_bounds__(512)
     const U* dyr = dy + row * ldy;
     float s[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < C; c += 512) {
-      const float q = to_f32<U>(dyr[c]) * (w != nullptr ? w[c] : 1.f);
+      const float q = to_f32<U>(dyr[c]) * (w != nullptr ? to_f32<W>(w[c]) : 1.f);
       s[0] += q;
       s[1] += q * ((to_f32<T>(xr[c]) - mean) * rstd);
     }
     row_sum<512, 2>(s, sh, flip);
     const float s1 = s[0] * inv_c, s2 = s[1] * inv_c;
     for (int c = threadIdx.x; c < C; c += 512) {
-      const float q = to_f32<U>(dyr[c]) * (w != nullptr ? w[c] : 1.f);
+      const float q = to_f32<U>(dyr[c]) * (w != nullptr ? to_f32<W>(w[c]) : 1.f);
       const float h = (to_f32<T>(xr[c]) - mean) * rstd;
       dx[row * static_cast<int64_t>(C) + c] = from_f32<T>(rstd * (q - s1 - h * s2));
     }
@@ -216,12 +216,13 @@ __global__ void __launch_bounds__(512)
 
 // out[c] = sum_p part[p][c], in a fixed order: 32 columns x 32 partial lanes per CTA;
 // blockIdx.y picks the weight's or the bias's sums.
+template <typename O>
 __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ part_w,
                                                       const float* __restrict__ part_b, int P, int C,
-                                                      float* __restrict__ dw, float* __restrict__ db) {
+                                                      O* __restrict__ dw, O* __restrict__ db) {
   __shared__ float sh[32][33];
   const float* part = blockIdx.y == 0 ? part_w : part_b;
-  float* out = blockIdx.y == 0 ? dw : db;
+  O* out = blockIdx.y == 0 ? dw : db;
   if (out == nullptr) return;
   const int lane = threadIdx.x % 32, py = threadIdx.x / 32;
   const int c = blockIdx.x * 32 + lane;
@@ -235,30 +236,32 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ 
   s = sh[lane][py];  // column py of this CTA
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0 && blockIdx.x * 32 + py < C) out[blockIdx.x * 32 + py] = s;
+  if (lane == 0 && blockIdx.x * 32 + py < C) out[blockIdx.x * 32 + py] = from_f32<O>(s);
 }
 
 struct BwdArgs {
   int64_t ldy, ldx, R;
   int C;
-  const float *mean, *rstd, *w;
+  const float *mean, *rstd;
+  const void* w;
   bool want_w, want_b;
 };
 
-template <typename T, typename U, int VEC, int TPR>
+template <typename T, typename U, typename W, int VEC, int TPR>
 static void launch_rows(const U* dy, const T* x, T* dx, const BwdArgs& a, int P, float* pw, float* pb) {
   auto stream = at::cuda::getCurrentCUDAStream();
   constexpr int RPB = kCta<TPR> / TPR;
+  const W* w = static_cast<const W*>(a.w);
   const size_t smem = RPB > 1 ? static_cast<size_t>(RPB) * a.C * sizeof(float) : 0;
   if (pw != nullptr || pb != nullptr)
-    bwd_kernel<T, U, VEC, TPR, true><<<P, kCta<TPR>, smem, stream>>>(dy, a.ldy, x, a.ldx, a.R, a.C, a.mean, a.rstd,
-                                                                     a.w, dx, pw, pb);
+    bwd_kernel<T, U, W, VEC, TPR, true><<<P, kCta<TPR>, smem, stream>>>(dy, a.ldy, x, a.ldx, a.R, a.C, a.mean, a.rstd,
+                                                                        w, dx, pw, pb);
   else
-    bwd_kernel<T, U, VEC, TPR, false><<<P, kCta<TPR>, 0, stream>>>(dy, a.ldy, x, a.ldx, a.R, a.C, a.mean, a.rstd, a.w,
-                                                                   dx, nullptr, nullptr);
+    bwd_kernel<T, U, W, VEC, TPR, false><<<P, kCta<TPR>, 0, stream>>>(dy, a.ldy, x, a.ldx, a.R, a.C, a.mean, a.rstd, w,
+                                                                      dx, nullptr, nullptr);
 }
 
-template <typename T, typename U, int VEC>
+template <typename T, typename U, typename W, int VEC>
 static void launch(const U* dy, const T* x, T* dx, const BwdArgs& a, torch::Tensor& dw, torch::Tensor& db) {
   auto stream = at::cuda::getCurrentCUDAStream();
   const int C = a.C;
@@ -272,36 +275,48 @@ static void launch(const U* dy, const T* x, T* dx, const BwdArgs& a, torch::Tens
       grads && (C > kMaxRegCols || ctas * 16 > a.R * static_cast<int64_t>(sizeof(T) + sizeof(U)));
   const int P = static_cast<int>(
       !columns ? ctas : std::max<int64_t>(1, std::min<int64_t>(a.R / 256, 4 * sms / ((C + 63) / 64))));
-  float *w_out = a.want_w ? dw.data_ptr<float>() : nullptr, *b_out = a.want_b ? db.data_ptr<float>() : nullptr;
-  float *pw = w_out, *pb = b_out;  // where the sums (or the partial rows) go
+  // where the sums (or the partial rows) go
+  const bool direct = P == 1 && dw.scalar_type() == at::kFloat;
+  float *pw = direct && a.want_w ? dw.data_ptr<float>() : nullptr, *pb = direct && a.want_b ? db.data_ptr<float>() : nullptr;
   torch::Tensor part;
-  if (grads && P > 1) {
-    part = torch::empty({2, P, C}, dw.options());
+  if (grads && !direct) {
+    part = torch::empty({2, P, C}, dw.options().dtype(at::kFloat));
     pw = a.want_w ? part.data_ptr<float>() : nullptr;
     pb = a.want_b ? part.data_ptr<float>() + static_cast<int64_t>(P) * C : nullptr;
   }
   float *rw = columns ? nullptr : pw, *rb = columns ? nullptr : pb;
   const int n = static_cast<int>(ctas);
-  if (C <= 128) launch_rows<T, U, VEC, 8>(dy, x, dx, a, n, rw, rb);
-  else if (C <= 512) launch_rows<T, U, VEC, 32>(dy, x, dx, a, n, rw, rb);
-  else if (C <= 2048) launch_rows<T, U, VEC, 128>(dy, x, dx, a, n, rw, rb);
-  else if (C <= kMaxRegCols) launch_rows<T, U, VEC, 512>(dy, x, dx, a, n, rw, rb);
+  if (C <= 128) launch_rows<T, U, W, VEC, 8>(dy, x, dx, a, n, rw, rb);
+  else if (C <= 512) launch_rows<T, U, W, VEC, 32>(dy, x, dx, a, n, rw, rb);
+  else if (C <= 2048) launch_rows<T, U, W, VEC, 128>(dy, x, dx, a, n, rw, rb);
+  else if (C <= kMaxRegCols) launch_rows<T, U, W, VEC, 512>(dy, x, dx, a, n, rw, rb);
   else
-    bwd_wide_kernel<T, U><<<static_cast<unsigned>(std::min<int64_t>(a.R, sms * 4)), 512, 0, stream>>>(
-        dy, a.ldy, x, a.ldx, a.R, C, a.mean, a.rstd, a.w, dx);
+    bwd_wide_kernel<T, U, W><<<static_cast<unsigned>(std::min<int64_t>(a.R, sms * 4)), 512, 0, stream>>>(
+        dy, a.ldy, x, a.ldx, a.R, C, a.mean, a.rstd, static_cast<const W*>(a.w), dx);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (columns) {
     colgrad_kernel<T, U><<<dim3((C + 63) / 64, P), 512, 0, stream>>>(dy, a.ldy, x, a.ldx, a.R, C, a.mean, a.rstd, pw,
                                                                      pb);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
-  if (grads && P > 1) {
-    reduce_kernel<<<dim3((C + 31) / 32, 2), 1024, 0, stream>>>(pw, pb, P, C, w_out, b_out);
+  if (grads && !direct) {
+    const dim3 grid((C + 31) / 32, 2);
+    auto reduce = [&](auto kind) {
+      using O = decltype(kind);
+      reduce_kernel<O><<<grid, 1024, 0, stream>>>(pw, pb, P, C, a.want_w ? static_cast<O*>(dw.data_ptr()) : nullptr,
+                                                  a.want_b ? static_cast<O*>(db.data_ptr()) : nullptr);
+    };
+    if (dw.scalar_type() == at::kFloat)
+      reduce(float{});
+    else if (dw.scalar_type() == at::kBFloat16)
+      reduce(__nv_bfloat16{});
+    else
+      reduce(__half{});
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
 }
 
-template <typename T, typename U>
+template <typename T, typename U, typename W>
 static void run(const torch::Tensor& dy, const torch::Tensor& x, torch::Tensor& dx, const BwdArgs& a,
                 torch::Tensor& dw, torch::Tensor& db) {
   constexpr int VEC = sizeof(T) == 4 || sizeof(U) == 4 ? 4 : 8;
@@ -309,20 +324,28 @@ static void run(const torch::Tensor& dy, const torch::Tensor& x, torch::Tensor& 
   const T* xp = reinterpret_cast<const T*>(x.data_ptr());
   T* dxp = reinterpret_cast<T*>(dx.data_ptr());
   const bool vec = vec_ok(dyp, a.ldy, a.C, sizeof(U), VEC) && vec_ok(xp, a.ldx, a.C, sizeof(T), VEC) &&
-                   vec_ok(dxp, a.C, a.C, sizeof(T), VEC) && vec_ok(a.w, 0, a.C, 4, 4);
+                   vec_ok(dxp, a.C, a.C, sizeof(T), VEC) && vec_ok_columns<W>(a.w, a.C, VEC);
   if (vec)
-    launch<T, U, VEC>(dyp, xp, dxp, a, dw, db);
+    launch<T, U, W, VEC>(dyp, xp, dxp, a, dw, db);
   else
-    launch<T, U, 1>(dyp, xp, dxp, a, dw, db);
+    launch<T, U, W, 1>(dyp, xp, dxp, a, dw, db);
+}
+template <typename T>
+static void run_half(const torch::Tensor& dy, const torch::Tensor& x, torch::Tensor& dx, const BwdArgs& a, bool w_f32,
+                     torch::Tensor& dw, torch::Tensor& db) {
+  if (dy.scalar_type() == at::kFloat)
+    w_f32 ? run<T, float, float>(dy, x, dx, a, dw, db) : run<T, float, T>(dy, x, dx, a, dw, db);
+  else
+    w_f32 ? run<T, T, float>(dy, x, dx, a, dw, db) : run<T, T, T>(dy, x, dx, a, dw, db);
 }
 
 }  // namespace ln
 
-// (dx [R, C] of x's type, dw [C], db [C] fp32; an unwanted one is empty) from dy [R, C] (x's
-// type or fp32), x and the forward's mean and rstd.
+// (dx [R, C] of x's type, dw [C], db [C] of `grad_type`, fp32 or x's; an unwanted one is empty) from
+// dy [R, C] (x's type or fp32), x and the forward's mean and rstd.
 std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::Tensor& x, const torch::Tensor& mean,
                                           const torch::Tensor& rstd, const c10::optional<torch::Tensor>& w,
-                                          bool weight_grad, bool bias_grad) {
+                                          bool weight_grad, bool bias_grad, c10::ScalarType grad_type) {
   using namespace ln;
   check_rows(x, "layer_norm_bwd: x");
   check_rows(dy, "layer_norm_bwd: dy");
@@ -335,13 +358,16 @@ std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::
                 "layer_norm_bwd: mean and rstd must be the forward's fp32 rows");
   check_plain(mean, "layer_norm_bwd: mean");
   check_plain(rstd, "layer_norm_bwd: rstd");
+  TORCH_CHECK(grad_type == at::kFloat || grad_type == x.scalar_type(),
+              "layer_norm_bwd: the weight's gradients are fp32 or of x's type");
   BwdArgs a;
-  a.w = opt_vec(w, C, x.device(), "layer_norm_bwd: weight");
   const at::cuda::CUDAGuard guard(x.device());
-  auto f32 = x.options().dtype(at::kFloat);
+  const Affine affine = affine_of(x, w, c10::nullopt, "layer_norm_bwd");
+  a.w = affine.wp();
+  auto vec = x.options().dtype(grad_type);
   auto dx = torch::empty({R, C}, x.options());
-  auto dw = weight_grad ? torch::empty({C}, f32) : torch::empty({0}, f32);
-  auto db = bias_grad ? torch::empty({C}, f32) : torch::empty({0}, f32);
+  auto dw = weight_grad ? torch::empty({C}, vec) : torch::empty({0}, vec);
+  auto db = bias_grad ? torch::empty({C}, vec) : torch::empty({0}, vec);
   check_plain(dx, "layer_norm_bwd");
   if (R == 0) {
     dw.zero_();
@@ -356,13 +382,12 @@ std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::
   a.rstd = rstd.data_ptr<float>();
   a.want_w = weight_grad;
   a.want_b = bias_grad;
-  const bool f = dy.scalar_type() == at::kFloat;
   if (x.scalar_type() == at::kFloat)
-    run<float, float>(dy, x, dx, a, dw, db);
+    run<float, float, float>(dy, x, dx, a, dw, db);
   else if (x.scalar_type() == at::kBFloat16)
-    f ? run<__nv_bfloat16, float>(dy, x, dx, a, dw, db) : run<__nv_bfloat16, __nv_bfloat16>(dy, x, dx, a, dw, db);
+    run_half<__nv_bfloat16>(dy, x, dx, a, affine.f32, dw, db);
   else
-    f ? run<__half, float>(dy, x, dx, a, dw, db) : run<__half, __half>(dy, x, dx, a, dw, db);
+    run_half<__half>(dy, x, dx, a, affine.f32, dw, db);
   return {dx, dw, db};
 }
 

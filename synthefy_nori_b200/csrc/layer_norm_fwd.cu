@@ -11,9 +11,9 @@
 namespace nori {
 namespace ln {
 
-template <typename T, typename U, int VEC, int TPR>
+template <typename T, typename U, typename W, int VEC, int TPR>
 __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int C,
-                                                        const float* __restrict__ w, const float* __restrict__ b,
+                                                        const W* __restrict__ w, const W* __restrict__ b,
                                                         float eps, U* __restrict__ y, float* __restrict__ mean_out,
                                                         float* __restrict__ rstd_out) {
   constexpr int CH = kValues / VEC, RPB = kCta<TPR> / TPR;
@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T
       const int c = VEC * (t + TPR * j);
       if (c < C) {
         float wv[VEC], bv[VEC];
-        load_columns<VEC>(w, c, 1.f, wv);
-        load_columns<VEC>(b, c, 0.f, bv);
+        load_columns<VEC, W>(w, c, 1.f, wv);
+        load_columns<VEC, W>(b, c, 0.f, bv);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (row + k * RPB < R) {
@@ -109,9 +109,9 @@ __global__ void __launch_bounds__(kCta<TPR>, 768 / kCta<TPR>) fwd_kernel(const T
 
 // Rows wider than the registers of a CTA: three passes over the row (the second and third
 // hit L2 for all but the widest).
-template <typename T, typename U>
+template <typename T, typename U, typename W>
 __global__ void __launch_bounds__(512) fwd_wide_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int C,
-                                                       const float* __restrict__ w, const float* __restrict__ b,
+                                                       const W* __restrict__ w, const W* __restrict__ b,
                                                        float eps, U* __restrict__ y, float* __restrict__ mean_out,
                                                        float* __restrict__ rstd_out) {
   __shared__ float sh[2][1][16];
@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(512) fwd_wide_kernel(const T* __restrict__ x, 
     const float rstd = rsqrtf(s[0] * inv_c + eps);
     for (int c = threadIdx.x; c < C; c += 512) {
       float o = (to_f32<T>(xr[c]) - mean) * rstd;
-      if (w != nullptr) o *= w[c];
-      if (b != nullptr) o += b[c];
+      if (w != nullptr) o *= to_f32<W>(w[c]);
+      if (b != nullptr) o += to_f32<W>(b[c]);
       y[row * static_cast<int64_t>(C) + c] = from_f32<U>(o);
     }
     if (threadIdx.x == 0) {
@@ -143,13 +143,13 @@ __global__ void __launch_bounds__(512) fwd_wide_kernel(const T* __restrict__ x, 
   }
 }
 
-template <typename T, typename U, int VEC>
-static void launch(const T* x, int64_t ldx, int64_t R, int C, const float* w, const float* b, float eps, U* y,
+template <typename T, typename U, typename W, int VEC>
+static void launch(const T* x, int64_t ldx, int64_t R, int C, const W* w, const W* b, float eps, U* y,
                    float* mean, float* rstd) {
   auto stream = at::cuda::getCurrentCUDAStream();
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
 #define NORI_LN_FWD(TPR)                                                                                            \
-  fwd_kernel<T, U, VEC, TPR>                                                                                        \
+  fwd_kernel<T, U, W, VEC, TPR>                                                                                        \
       <<<static_cast<unsigned>(std::min<int64_t>((R + 2 * kCta<TPR> / TPR - 1) / (2 * kCta<TPR> / TPR),            \
                                                  sms * (768 / kCta<TPR>))),                                      \
          kCta<TPR>, 0, stream>>>(x, ldx, R, C, w, b, eps, y, mean, rstd)
@@ -158,38 +158,47 @@ static void launch(const T* x, int64_t ldx, int64_t R, int C, const float* w, co
   else if (C <= 2048) NORI_LN_FWD(128);
   else if (C <= kMaxRegCols) NORI_LN_FWD(512);
   else
-    fwd_wide_kernel<T, U><<<static_cast<unsigned>(std::min<int64_t>(R, sms * 4)), 512, 0, stream>>>(
+    fwd_wide_kernel<T, U, W><<<static_cast<unsigned>(std::min<int64_t>(R, sms * 4)), 512, 0, stream>>>(
         x, ldx, R, C, w, b, eps, y, mean, rstd);
 #undef NORI_LN_FWD
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-template <typename T, typename U>
-static void run(const torch::Tensor& x, const float* w, const float* b, float eps, torch::Tensor& y,
-                torch::Tensor& mean, torch::Tensor& rstd) {
+template <typename T, typename U, typename W>
+static void run(const torch::Tensor& x, const Affine& a, float eps, torch::Tensor& y, torch::Tensor& mean,
+                torch::Tensor& rstd) {
   constexpr int VEC = sizeof(T) == 4 || sizeof(U) == 4 ? 4 : 8;  // 16-byte accesses of the wider type
   const T* xp = reinterpret_cast<const T*>(x.data_ptr());
   U* yp = reinterpret_cast<U*>(y.data_ptr());
+  const W *w = static_cast<const W*>(a.wp()), *b = static_cast<const W*>(a.bp());
   const int64_t R = x.size(0), C = x.size(1), ldx = x.stride(0);
-  const bool vec = vec_ok(xp, ldx, C, sizeof(T), VEC) && vec_ok(yp, C, C, sizeof(U), VEC) && vec_ok(w, 0, C, 4, 4) &&
-                   vec_ok(b, 0, C, 4, 4);
+  const bool vec = vec_ok(xp, ldx, C, sizeof(T), VEC) && vec_ok(yp, C, C, sizeof(U), VEC) &&
+                   vec_ok_columns<W>(w, C, VEC) && vec_ok_columns<W>(b, C, VEC);
   if (vec)
-    launch<T, U, VEC>(xp, ldx, R, static_cast<int>(C), w, b, eps, yp, mean.data_ptr<float>(), rstd.data_ptr<float>());
+    launch<T, U, W, VEC>(xp, ldx, R, static_cast<int>(C), w, b, eps, yp, mean.data_ptr<float>(), rstd.data_ptr<float>());
   else
-    launch<T, U, 1>(xp, ldx, R, static_cast<int>(C), w, b, eps, yp, mean.data_ptr<float>(), rstd.data_ptr<float>());
+    launch<T, U, W, 1>(xp, ldx, R, static_cast<int>(C), w, b, eps, yp, mean.data_ptr<float>(), rstd.data_ptr<float>());
+}
+template <typename T>
+static void run_half(const torch::Tensor& x, const Affine& a, float eps, bool out_f32, torch::Tensor& y,
+                     torch::Tensor& mean, torch::Tensor& rstd) {
+  if (out_f32)
+    a.f32 ? run<T, float, float>(x, a, eps, y, mean, rstd) : run<T, float, T>(x, a, eps, y, mean, rstd);
+  else
+    a.f32 ? run<T, T, float>(x, a, eps, y, mean, rstd) : run<T, T, T>(x, a, eps, y, mean, rstd);
 }
 
 }  // namespace ln
 
-// (y [R, C], mean [R], rstd [R]) of x [R, C]; y has x's type, or fp32 with out_f32.
+// (y [R, C], mean [R], rstd [R]) of x [R, C]; y has x's type, or fp32 with out_f32.  Weight and bias
+// are read as they are in fp32 or in x's type, and cast to fp32 otherwise.
 std::vector<torch::Tensor> layer_norm_fwd(const torch::Tensor& x, const c10::optional<torch::Tensor>& w,
                                           const c10::optional<torch::Tensor>& b, double eps, bool out_f32) {
   using namespace ln;
   check_rows(x, "layer_norm_fwd: x");
   TORCH_CHECK(eps >= 0.0, "layer_norm_fwd: eps must not be negative");
-  const float* wp = opt_vec(w, x.size(1), x.device(), "layer_norm_fwd: weight");
-  const float* bp = opt_vec(b, x.size(1), x.device(), "layer_norm_fwd: bias");
   const at::cuda::CUDAGuard guard(x.device());
+  const Affine a = affine_of(x, w, b, "layer_norm_fwd");
   auto y = torch::empty({x.size(0), x.size(1)}, x.options().dtype(out_f32 ? at::kFloat : x.scalar_type()));
   auto mean = torch::empty({x.size(0)}, x.options().dtype(at::kFloat));
   auto rstd = torch::empty({x.size(0)}, x.options().dtype(at::kFloat));
@@ -197,12 +206,11 @@ std::vector<torch::Tensor> layer_norm_fwd(const torch::Tensor& x, const c10::opt
   if (x.size(0) == 0) return {y, mean, rstd};
   const float e = static_cast<float>(eps);
   if (x.scalar_type() == at::kFloat)
-    run<float, float>(x, wp, bp, e, y, mean, rstd);
+    run<float, float, float>(x, a, e, y, mean, rstd);
   else if (x.scalar_type() == at::kBFloat16)
-    out_f32 ? run<__nv_bfloat16, float>(x, wp, bp, e, y, mean, rstd)
-            : run<__nv_bfloat16, __nv_bfloat16>(x, wp, bp, e, y, mean, rstd);
+    run_half<__nv_bfloat16>(x, a, e, out_f32, y, mean, rstd);
   else
-    out_f32 ? run<__half, float>(x, wp, bp, e, y, mean, rstd) : run<__half, __half>(x, wp, bp, e, y, mean, rstd);
+    run_half<__half>(x, a, e, out_f32, y, mean, rstd);
   return {y, mean, rstd};
 }
 

@@ -38,17 +38,11 @@ def _check(x: torch.Tensor, out_dtype) -> bool:
     return out_dtype == torch.float32
 
 
-def _vec(v):
-    if v is None or (v.dtype == torch.float32 and v.is_contiguous()):
-        return v
-    return v.detach().to(torch.float32).contiguous()
-
-
 def layer_norm_fwd(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dtype=None):
     """``(y, mean, rstd)`` of ``x [..., C]`` (fp32, bf16 or fp16; ``y`` in x's type or, with
     ``out_dtype``, fp32); ``mean`` and ``rstd`` are fp32, one per row."""
     f32 = _check(x, out_dtype)
-    y, mean, rstd = _lib().layer_norm_fwd(_rows(x), _vec(weight), _vec(bias), eps, f32)
+    y, mean, rstd = _lib().layer_norm_fwd(_rows(x), weight, bias, eps, f32)
     return y if x.dim() == 2 else y.view(x.shape), mean, rstd
 
 
@@ -58,47 +52,16 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     is a weight) and ``db`` are fp32 ``[C]``, or None where unwanted."""
     _check(x, None)
     weight_grad = weight is not None if weight_grad is None else weight_grad
-    dx, dw, db = _lib().layer_norm_bwd(_rows(dy), _rows(x), mean, rstd, _vec(weight),
-                                       bool(weight_grad), bool(bias_grad))
+    dx, dw, db = _lib().layer_norm_bwd(_rows(dy), _rows(x), mean, rstd, weight, bool(weight_grad), bool(bias_grad))
     return dx if x.dim() == 2 else dx.view(x.shape), dw if weight_grad else None, db if bias_grad else None
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, out_dtype):
-        y, mean, rstd = layer_norm_fwd(x, weight, bias, eps, out_dtype)
-        ctx.save_for_backward(x, mean, rstd, weight, bias)
-        ctx.eps = eps
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, mean, rstd, weight, bias = ctx.saved_tensors
-        if torch.is_grad_enabled():  # a second derivative is wanted: differentiable operations
-            return *_bwd_plain(dy, x, weight, bias, ctx.eps), None, None
-        if dy.dtype != x.dtype and dy.dtype != torch.float32:
-            dy = dy.float()
-        dx, dw, db = layer_norm_bwd(dy, x, mean, rstd, weight, weight_grad=ctx.needs_input_grad[1],
-                                    bias_grad=ctx.needs_input_grad[2])
-        return (dx if ctx.needs_input_grad[0] else None, None if dw is None else dw.to(weight.dtype),
-                None if db is None else db.to(bias.dtype), None, None)
-
-
-def _bwd_plain(dy, x, weight, bias, eps):
-    """The backward in differentiable tensor operations (for gradients of gradients)."""
-    xf, d = x.float(), dy.float()
-    xc = xf - xf.mean(-1, keepdim=True)
-    rstd = (xc.square().mean(-1, keepdim=True) + eps).rsqrt()
-    h = xc * rstd
-    q = d if weight is None else d * weight.float()
-    dx = rstd * (q - q.mean(-1, keepdim=True) - h * (q * h).mean(-1, keepdim=True))
-    dw = None if weight is None else (d * h).reshape(-1, x.shape[-1]).sum(0).to(weight.dtype)
-    db = None if bias is None else d.reshape(-1, x.shape[-1]).sum(0).to(bias.dtype)
-    return dx.to(x.dtype), dw, db
 
 
 def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dtype=None) -> torch.Tensor:
     """LayerNorm of ``x [..., C]`` over its last dimension, differentiable in ``x``, ``weight``
-    and ``bias`` (``[C]`` or None, any floating type on x's device).  The result has x's type,
+    and ``bias`` (``[C]`` or None, any floating type on x's device; fp32 and x's type are read as
+    they are, others cast).  The result has x's type,
     or fp32 with ``out_dtype=torch.float32``."""
-    return _LayerNorm.apply(x, weight, bias, float(eps), out_dtype)
+    f32 = _check(x, out_dtype)
+    if x.dim() == 0:
+        raise ValueError("layer_norm: at least one dimension expected")
+    return _lib().layer_norm(x, weight, bias, eps, f32, torch.autograd.forward_ad._current_level >= 0)
