@@ -127,7 +127,8 @@ class HybridMuonAdamW:
     def step(self, grad_scale: float = 1.0, skip: torch.Tensor | None = None) -> None:
         """``skip`` (device scalar, > 0 = reject the step): every update below is blended
         with ``keep = (skip <= 0)`` on the device, so a rejected step changes nothing and
-        no host synchronisation is needed."""
+        no host synchronisation is needed.  With clipping, a gradient norm that is not finite
+        rejects the step as well."""
         from synthefy_nori_b200 import ops
 
         self.step_count += 1
@@ -143,6 +144,13 @@ class HybridMuonAdamW:
             else:
                 self.norm_sq.copy_(grad.double().pow(2).sum().float().view(1))
             clip = (self.max_grad_norm / (self.norm_sq.sqrt() + 1e-6)).clamp(max=1.0)
+        if self.plan is None:  # (the kernels look for themselves)
+            finite = None if clip is None else torch.isfinite(self.norm_sq).reshape(())
+            if not grad.is_cuda:  # a host decision costs nothing
+                if (keep is not None and float(keep) == 0.0) or (finite is not None and not bool(finite)):
+                    return
+            elif finite is not None:
+                keep = finite.float() if keep is None else keep * finite
         lr_m = self.muon_lr if self.muon_lr is not None else self.lr
         native = grad.is_cuda and ops.native_available()
         skip1 = None if skip is None else skip.reshape(1).float()
@@ -157,6 +165,8 @@ class HybridMuonAdamW:
             g = torch.stack([p.grad.reshape(m, n) for p in ps])
             if clip is not None:
                 g.mul_(clip)
+            if keep is not None:
+                g = torch.where(keep > 0, g, 0.0)  # (nothing times NaN is NaN)
             if keep is None:
                 buf.mul_(self.momentum).add_(g)
             else:  # buf <- momentum buf + g when kept, unchanged when rejected
@@ -183,9 +193,7 @@ class HybridMuonAdamW:
                                    ema_decay=self.ema_decay if tail_ema is not None else 0.0,
                                    max_norm=self.max_grad_norm or 0.0, grad_scale=1.0, skip=skip1)
             else:
-                if keep is not None and float(keep) == 0.0:  # CPU path: a host decision costs nothing
-                    pass
-                else:
+                if keep is None or float(keep) > 0.0:
                     self._adamw_torch(data, g * (clip if clip is not None else 1.0))
         if self.ema is not None and self.plan is None:
             w = 1.0 - self.ema_decay

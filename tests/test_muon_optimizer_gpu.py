@@ -1,0 +1,38 @@
+"""HybridMuonAdamW on the GPU beside its kernels: rejected steps without a plan, matrices without
+values, and the kernels against the exact iteration with nothing else in their place."""
+
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("skip", [None, 0.0, 1.0])
+@pytest.mark.parametrize("ns_steps", [0, 5])
+def test_gradient_norm_that_is_not_finite(bad, skip, ns_steps):
+    """With the kernels and without (no iteration at all is not theirs)."""
+    from synthefy_nori_b200.training.muon import HybridMuonAdamW
+
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(6, 5), torch.nn.Linear(5, 300)).cuda()
+    opt = HybridMuonAdamW(net, "cuda", lr=0.1, max_grad_norm=1.0, ns_steps=ns_steps)
+    assert (opt.plan is None) == (ns_steps == 0)
+
+    def state():
+        sd = opt.state_dict()
+        return [opt.flat.data, sd["m"], sd["v"], sd["ema"], *sd["muon_momentum"]]
+
+    sk = None if skip is None else torch.tensor(skip, device="cuda")
+    opt.flat.grad.normal_()
+    opt.step()
+    before = copy.deepcopy(state())
+    opt.flat.grad[3] = bad
+    opt.step(skip=sk)
+    assert all(torch.equal(a, b) for a, b in zip(before, state()))
+    opt.flat.grad.normal_()
+    opt.step()
+    assert not any(torch.equal(a, b) for a, b in zip(before, state()))
+    assert all(t.isfinite().all() for t in state())
