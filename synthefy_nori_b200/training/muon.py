@@ -113,7 +113,8 @@ class HybridMuonAdamW:
             size = len(ix) * m * n
             stack = self.momentum_buf[off : off + size].view(len(ix), m, n)
             self.groups.append(((m, n), [self.flat.params[i] for i in ix], stack))
-            places += [((m, n), self.flat.offsets[i], off + j * m * n) for j, i in enumerate(ix)]
+            if m and n:
+                places += [((m, n), self.flat.offsets[i], off + j * m * n) for j, i in enumerate(ix)]
             off += -(-size // 64) * 64
         self.plan = None
         if self.flat.data.is_cuda and 1 <= ns_steps <= 64 and places and all(max(s) < 1 << 20 for s, _, _ in places):

@@ -36,3 +36,23 @@ def test_gradient_norm_that_is_not_finite(bad, skip, ns_steps):
     opt.step()
     assert not any(torch.equal(a, b) for a, b in zip(before, state()))
     assert all(t.isfinite().all() for t in state())
+
+
+def test_matrices_without_values():
+    from synthefy_nori_b200.training.muon import HybridMuonAdamW
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.b = torch.nn.Parameter(torch.randn(7, 6))
+            self.c = torch.nn.Parameter(torch.randn(0, 6))
+
+    torch.manual_seed(1)
+    net = Net().cuda()
+    opt = HybridMuonAdamW(net, "cuda", lr=0.1)
+    assert opt.plan is not None and opt.plan.count == 1
+    before = net.b.detach().clone()
+    opt.flat.grad.normal_()
+    opt.step()
+    assert not torch.equal(before, net.b) and net.b.isfinite().all()
+    assert [tuple(t.shape) for t in opt.state_dict()["muon_momentum"]] == [(1, 7, 6), (1, 0, 6)]
