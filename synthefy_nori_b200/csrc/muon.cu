@@ -56,6 +56,9 @@ torch::Tensor newton_schulz(const torch::Tensor& g, const c10::optional<torch::T
   TORCH_CHECK(out.device() == g.device() && out.is_contiguous() && out.sizes() == g.sizes(),
               "newton_schulz: out must be contiguous, of g's shape and device");
   const int dst = kind(out.scalar_type(), "out");
+  // matrix i is written while others are still read: in place, or apart
+  TORCH_CHECK((out.const_data_ptr() == g.const_data_ptr() && dst == src) || !overlap(out, g),
+              "newton_schulz: out must be g itself or share no memory with it");
   if (g.numel() == 0) return out;
   const int64_t batch = g.numel() / (rows * cols);
   TORCH_CHECK(batch <= INT_MAX, "newton_schulz: at most 2^31 - 1 matrices");
@@ -99,6 +102,13 @@ void muon_step(torch::Tensor& data, const torch::Tensor& grad, torch::Tensor& mo
                     ema->is_contiguous() && ema->numel() == data.numel(),
                 "muon_step: ema must be a flat fp32 buffer of data's length");
     s.ema = ema->data_ptr<float>();
+  }
+  const torch::Tensor* written[3] = {&data, &mom, s.ema != nullptr ? &*ema : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    if (written[i] == nullptr) continue;
+    bool shared = overlap(*written[i], grad);
+    for (int j = 0; j < i; ++j) shared = shared || overlap(*written[i], *written[j]);
+    TORCH_CHECK(!shared, "muon_step: data, grad, momentum and ema must not share memory");
   }
   s.table = reinterpret_cast<const Mat*>(table.data_ptr<int64_t>());
   s.norm_sq = opt_scalar(norm_sq, data.device(), "muon_step: norm_sq");

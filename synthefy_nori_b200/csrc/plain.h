@@ -16,4 +16,10 @@ inline void check_plain(const c10::optional<torch::Tensor>& t, const char* what)
   if (t.has_value() && t->defined()) check_plain(*t, what);
 }
 
+// Whether two contiguous tensors share memory.
+inline bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  const char *pa = static_cast<const char*>(a.const_data_ptr()), *pb = static_cast<const char*>(b.const_data_ptr());
+  return pa < pb + b.nbytes() && pb < pa + a.nbytes();
+}
+
 }  // namespace nori

@@ -39,7 +39,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, eps: float = 1e-7, coeffs=NS_
     """Newton-Schulz orthogonalisation of every matrix of ``g [..., rows, cols]`` (fp32, bf16
     or fp16; any strides), in ``out_dtype`` (default: g's; about 11 significant bits are
     right).  ``out``, if given, is contiguous, of g's shape, and sets the type; it may be
-    ``g`` itself.  A matrix of zeros gives zeros; a NaN or an infinity makes its own matrix
+    ``g`` itself, but share no other memory with it.  A matrix of zeros gives zeros; a NaN or an infinity makes its own matrix
     NaN and no other.  ``steps`` is 1 to 64, the first coefficient 1 to 1024; the coefficients
     are such that the iteration stays bounded (singular values of 100 leave fp16's range).  Not differentiable: the result has no graph."""
     if not isinstance(g, torch.Tensor) or not g.is_cuda:
