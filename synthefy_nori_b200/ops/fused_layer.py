@@ -109,9 +109,9 @@ def _unpad_heads(t: torch.Tensor, H: int, D: int, Dp: int) -> torch.Tensor:
     return t.view(-1, H, Dp, C)[:, :, :D].reshape(-1, C)
 
 
-# bf16 copies of the fused weight layouts, per layer, valid for one weight generation.
-# Anything that changes weights in place outside a training optimizer calls
-# ``bump_weight_generation()``.  During training the optimizer keeps persistent layouts
+# bf16 copies of the fused weight layouts, per layer, valid for one weight generation and one
+# version of every parameter.  Anything that changes weights behind their version counters calls
+# ``bump_weight_generation()`` (in-place operations and the optimizers raise the counters).  During training the optimizer keeps persistent layouts
 # (``ops.weight_layouts.WeightLayouts``, attached to the layer as ``_nori_layouts``)
 # up to date itself, so no per-step cast happens.
 _GENERATION = [0]
@@ -121,12 +121,17 @@ def bump_weight_generation() -> None:
     _GENERATION[0] += 1
 
 
+def weights_key(params) -> tuple:
+    """What a copy derived from ``params`` is valid for (inference tensors have no version)."""
+    return _GENERATION[0], tuple((p.data_ptr(), 0 if p.is_inference() else p._version) for p in params)
+
+
 def _cached_bf16(layer, w: dict) -> dict:
     ptrs = tuple(p.data_ptr() for p in layer.parameters())
     persistent = getattr(layer, "_nori_layouts", None)
     if persistent is not None and persistent[0] == ptrs:  # (a copied model has other storage)
         return persistent[1]
-    key = (_GENERATION[0], ptrs)
+    key = weights_key(layer.parameters())
     cache = getattr(layer, "_nori_bf16_cache", None)
     if cache is not None and cache[0] == key:
         return cache[1]

@@ -15,7 +15,7 @@ backward  dW2 (split-K weight-gradient GEMM), db2 (column sums), dG (GEMM with t
           backward - all on this library's kernels (no cuBLAS, no eager elementwise).
 
 The bf16 operand copies of the two weight matrices come from the trainer's persistent
-layouts (refreshed by the optimizer) or, outside training, from a per-generation cast.
+layouts (refreshed by the optimizer) or, outside training, from a cast per weight version.
 """
 
 from __future__ import annotations
@@ -68,9 +68,9 @@ def _head_bf16(model) -> dict:
     pers = getattr(model, "_nori_head_layouts", None)
     if pers is not None and pers[0] == ptrs:
         return pers[1]
-    from synthefy_nori_b200.ops.fused_layer import _GENERATION
+    from synthefy_nori_b200.ops.fused_layer import weights_key
 
-    key = (_GENERATION[0], ptrs)
+    key = weights_key(dec.parameters())
     hit = getattr(model, "_nori_head_cast", None)
     if hit is not None and hit[0] == key:
         return hit[1]

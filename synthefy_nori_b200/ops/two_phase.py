@@ -32,6 +32,7 @@ import math
 import torch
 
 from synthefy_nori_b200 import ops
+from synthefy_nori_b200.ops.fused_layer import weights_key
 
 BF16 = torch.bfloat16
 
@@ -76,7 +77,7 @@ def supported(enc) -> bool:
 # ---------------------------------------------------------------- weights (bf16, cached)
 def _weights(enc) -> dict:
     """bf16 operand copies of every weight, rebuilt when any parameter changes."""
-    key = tuple((p.data_ptr(), p._version) for p in enc.parameters())
+    key = weights_key(enc.parameters())
     hit = getattr(enc, "_nori_native_weights", None)
     if hit is not None and hit[0] == key:
         return hit[1]

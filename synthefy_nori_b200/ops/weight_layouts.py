@@ -17,7 +17,7 @@ all-gather: it reads each element from the rank that owns it (peer memory), writ
 into the local fp32 master buffer and into the bf16 layout in the same pass.
 
 Without a flat buffer (inference), ``fused_layer._cached_bf16`` casts the layouts once
-per weight generation instead.
+per weight version instead.
 """
 
 from __future__ import annotations
