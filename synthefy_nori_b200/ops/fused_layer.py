@@ -121,17 +121,21 @@ def bump_weight_generation() -> None:
     _GENERATION[0] += 1
 
 
-def weights_key(params) -> tuple:
-    """What a copy derived from ``params`` is valid for (inference tensors have no version)."""
-    return _GENERATION[0], tuple((p.data_ptr(), 0 if p.is_inference() else p._version) for p in params)
+def weights_key(params: list) -> tuple:
+    """What a copy derived from ``params`` is valid for: their addresses and versions in this weight
+    generation (inference tensors have no version)."""
+    try:
+        versions = tuple([p._version for p in params])
+    except RuntimeError:
+        versions = None
+    return tuple([p.data_ptr() for p in params]), versions, _GENERATION[0]
 
 
 def _cached_bf16(layer, w: dict) -> dict:
-    ptrs = tuple(p.data_ptr() for p in layer.parameters())
+    key = weights_key(list(layer.parameters()))
     persistent = getattr(layer, "_nori_layouts", None)
-    if persistent is not None and persistent[0] == ptrs:  # (a copied model has other storage)
+    if persistent is not None and persistent[0] == key[0]:  # (a copied model has other storage)
         return persistent[1]
-    key = weights_key(layer.parameters())
     cache = getattr(layer, "_nori_bf16_cache", None)
     if cache is not None and cache[0] == key:
         return cache[1]

@@ -64,13 +64,12 @@ def head_blocks(model):
 
 def _head_bf16(model) -> dict:
     dec = model.reg_y_decoder
-    ptrs = tuple(p.data_ptr() for p in dec.parameters())
-    pers = getattr(model, "_nori_head_layouts", None)
-    if pers is not None and pers[0] == ptrs:
-        return pers[1]
     from synthefy_nori_b200.ops.fused_layer import weights_key
 
-    key = weights_key(dec.parameters())
+    key = weights_key(list(dec.parameters()))
+    pers = getattr(model, "_nori_head_layouts", None)
+    if pers is not None and pers[0] == key[0]:
+        return pers[1]
     hit = getattr(model, "_nori_head_cast", None)
     if hit is not None and hit[0] == key:
         return hit[1]

@@ -77,7 +77,7 @@ def supported(enc) -> bool:
 # ---------------------------------------------------------------- weights (bf16, cached)
 def _weights(enc) -> dict:
     """bf16 operand copies of every weight, rebuilt when any parameter changes."""
-    key = weights_key(enc.parameters())
+    key = weights_key(list(enc.parameters()))
     hit = getattr(enc, "_nori_native_weights", None)
     if hit is not None and hit[0] == key:
         return hit[1]
