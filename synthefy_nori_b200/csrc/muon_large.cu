@@ -250,15 +250,15 @@ __global__ void __launch_bounds__(256) scale_kernel(const void* __restrict__ g, 
 // store, for alternate tiles, what it leaves there (Z's pair, or A / C and their mirror image)
 // and count the tile once its stores are complete, all by TMA.
 //
-// What bounds a tile is latency at every hand-over rather than a rate (at 81 x 1344 x 448, 838 us,
-// the tensor core runs at 24%, L2 at 36% and DRAM at 41% of their peaks; a 128 x 128 tile of the
+// What bounds a tile is latency at every hand-over rather than a rate (at 81 x 1344 x 448, 838 us
+// under ncu, the tensor core runs at 24%, L2 at 36% and DRAM at 41% of their peaks; a 128 x 128 tile of the
 // update takes 5,000 - 6,000 cycles to load and 3,000 in its epilogue), so the choices below keep
 // many small pieces in flight: 128 x 128 tiles (with 128 x 256 ones the epilogue's boxes queued behind
 // 144 KB of operands, and a lone matrix had half as many tiles), two storing warps (one would
 // wait 2,000 cycles a tile for its stores), three boxes.  C is kept as I + C, so that Z's high
 // half comes out of the product itself and only the low half is loaded and added.  (Rounding the
-// diagonal of I + C to fp16 scales Z's columns by 1 + 2^-12 at most, which no direction
-// amplifies.)
+// diagonal of I + C to fp16 scales Z's columns by 1 + 2^-11 at most: an error like the other
+// operands'.)
 constexpr int kThreads = 448;
 constexpr int kStages = 4, kStageBytes = 32768;
 constexpr int kAccs = 4;                        // TMEM accumulators of 128 columns
@@ -789,8 +789,8 @@ static CUtensorMap map_f16(const __half* base, int cols, int rows, int ld, int b
 static int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 // Work buffers of the matrices of a block.  Wide blocks put more tiles between a product and the
-// one that needs it, narrow ones stay in L2: 81 x 1344 x 448 takes 977 us with 100 MB, 922 with
-// 200, 940 with 400 or more; 52 x 896 x 448 450, 433 and 433.
+// one that needs it, narrow ones stay in L2: calls of 81 x 1344 x 448 in a loop take 977 us with 100 MB, 922
+// with 200, 940 with 400 or more; 52 x 896 x 448 450, 433 and 433.
 constexpr int64_t kBlockBytes = 200ll << 20;
 
 static void run_shapes(int src, const void* g, int out_type, void* out, const StepArgs& s, const Shape* shapes, int ns,
