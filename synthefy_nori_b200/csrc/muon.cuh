@@ -16,10 +16,10 @@
 // over the whole GPU); the three products read fp16 operands (the high parts, A and C: 11
 // bits) and accumulate in fp32.  A small singular value of G lives in the pair and is only
 // multiplied by 1 + C, so it keeps its 22 bits, while the rounding of the products' operands
-// (2^-12 relative) perturbs the dominant directions only and is not amplified: five steps are
+// (2^-11 relative at most) perturbs the dominant directions only and is not amplified: five steps are
 // 1e-3 .. 3e-3 (2-norm) from the exact iteration for flat, power-law, exponential and
 // rank-deficient spectra alike, about the rounding of a bf16 result, and 64 steps about 1e-2.  With iterates rounded
-// to bf16 the noise 2^-9 |G|_F is amplified by up to a^5 = 485 in the small directions: 1e-2
+// to bf16 the noise 2^-8 |G|_F is amplified by up to a^5 = 485 in the small directions: 1e-2
 // for a flat spectrum and 0.1 .. 1 for steep ones.  Products of fp16 pairs (three MMAs each)
 // give 1e-6 for three times the tensor work; the single-CTA kernel takes them up to 32 columns,
 // where the work is nothing and few roundings average out.
