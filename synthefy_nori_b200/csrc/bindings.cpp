@@ -167,6 +167,16 @@ std::vector<torch::Tensor> layer_norm_bwd(const torch::Tensor& dy, const torch::
                                           bool weight_grad, bool bias_grad, c10::ScalarType grad_type);
 torch::Tensor layer_norm(const torch::Tensor& x, const c10::optional<torch::Tensor>& w,
                          const c10::optional<torch::Tensor>& b, double eps, bool out_f32, bool dual);
+void block_cache_write(const torch::Tensor& ck, const torch::Tensor& cv, const torch::Tensor& cks, const torch::Tensor& cvs,
+                       int64_t width, const torch::Tensor& k, const torch::Tensor& v, int64_t start_all,
+                       const c10::optional<torch::Tensor>& start_dev, const c10::optional<torch::Tensor>& count_dev);
+std::vector<torch::Tensor> block_cache_read(const torch::Tensor& ck, const torch::Tensor& cv, const torch::Tensor& cks,
+                                            const torch::Tensor& cvs, int64_t width, int64_t start, int64_t n,
+                                            c10::ScalarType out_type);
+torch::Tensor block_cache_attention(const torch::Tensor& q, const torch::Tensor& ck, const torch::Tensor& cv,
+                                    const torch::Tensor& cks, const torch::Tensor& cvs, int64_t width, int64_t length_all,
+                                    const c10::optional<torch::Tensor>& length_dev, double scale, const torch::Tensor& o,
+                                    bool want_lse, const torch::Tensor& status);
 }  // namespace nori
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -240,4 +250,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_bwd", &nori::layer_norm_bwd, py::arg("dy"), py::arg("x"), py::arg("mean"), py::arg("rstd"),
         py::arg("weight"), py::arg("weight_grad"), py::arg("bias_grad"), py::arg("grad_type") = at::kFloat);
   m.def("layer_norm", &nori::layer_norm);
+  m.def("block_cache_write", &nori::block_cache_write);
+  m.def("block_cache_read", &nori::block_cache_read);
+  m.def("block_cache_attention", &nori::block_cache_attention);
 }

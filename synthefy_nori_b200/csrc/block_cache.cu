@@ -1,0 +1,376 @@
+// Context cache in 8 bits with a scale for each block of rows and head: rows quantised as they
+// are written, and read back.
+//
+// Write.  For one (sequence, head, block) of K or V, with Q = 127 (int8) or 448 (e4m3):
+//   s  = max(max(|x| of the block's new rows, 1e-12) / Q, s_old)   s_old where earlier rows stay
+//   q  = round(x * (1 / s)),   rows that stay: q' = round(q * (s_old * (1 / s)))
+// every operation in fp32 with one rounding, ties to even.  A block with an infinity or a NaN gets
+// a NaN scale: all of it reads as NaN, rather than as something finite.
+// One CTA of 128 threads takes one such block, its new rows in registers between the maximum and
+// the rounding: each new value is read once (2 bytes, or 4) and written once (1 byte).  K and V
+// and all heads of a row are neighbouring CTAs, so the pieces of a cache line that different heads
+// own are read together.
+//
+// Read.  x = q * s, rounded once to the result's type: 8 values a thread and step.
+//
+// Reference counterpart: per-vector int8 quantisation (kv_cache_scaling.py:29-41).
+#include "block_cache.cuh"
+
+namespace nori {
+namespace bc {
+namespace {
+
+constexpr int kWriteThreads = 128;
+
+template <int TYPE>
+struct Raw;  // eight values as they were loaded
+template <>
+struct Raw<kF32> {
+  uint32_t r[8];
+};
+template <>
+struct Raw<kBF16> {
+  uint32_t r[4];
+};
+template <>
+struct Raw<kF16> {
+  uint32_t r[4];
+};
+
+// Eight values from p, the first `have` of them there (the rest 0), in pieces of ALIGN values.
+template <int TYPE, int ALIGN>
+__device__ __forceinline__ Raw<TYPE> load8(const void* base, int64_t at, int have) {
+  Raw<TYPE> x;
+  if constexpr (TYPE == kF32) {
+    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
+    if constexpr (ALIGN >= 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 v = 4 * i < have ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        x.r[4 * i] = v.x, x.r[4 * i + 1] = v.y, x.r[4 * i + 2] = v.z, x.r[4 * i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.r[i] = i < have ? __ldg(p + i) : 0u;
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if constexpr (ALIGN == 8) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      x.r[0] = v.x, x.r[1] = v.y, x.r[2] = v.z, x.r[3] = v.w;
+    } else if constexpr (ALIGN == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint2 v = 4 * i < have ? __ldg(reinterpret_cast<const uint2*>(p) + i) : make_uint2(0, 0);
+        x.r[2 * i] = v.x, x.r[2 * i + 1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = 2 * i < have ? __ldg(p + 2 * i) : 0u, b = 2 * i + 1 < have ? __ldg(p + 2 * i + 1) : 0u;
+        x.r[i] = a | b << 16;
+      }
+    }
+  }
+  return x;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float value(const Raw<TYPE>& x, int i) {
+  if constexpr (TYPE == kF32) return __uint_as_float(x.r[i]);
+  const uint32_t w = x.r[i / 2];
+  if constexpr (TYPE == kBF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+  return __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? w >> 16 : w)));
+}
+
+// The largest magnitude so far as bits (ordered like the magnitudes, infinities and NaN on top):
+// 16-bit types in both halves of a word.
+template <int TYPE>
+__device__ __forceinline__ uint32_t top_bits(const Raw<TYPE>& x, uint32_t m) {
+  if constexpr (TYPE == kF32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, x.r[i] & 0x7fffffffu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, x.r[i] & 0x7fff7fffu);
+  }
+  return m;
+}
+template <int TYPE>
+__device__ __forceinline__ float top_value(uint32_t m) {
+  if constexpr (TYPE == kF32) return __uint_as_float(m);
+  const uint32_t h = max(m & 0xffffu, m >> 16);
+  if constexpr (TYPE == kBF16) return __uint_as_float(h << 16);
+  return __half2float(__ushort_as_half(static_cast<uint16_t>(h)));
+}
+
+// Four values as codes: round to nearest even.  |y| <= Q (1 + 2^-22), so int8 needs no clamp.
+template <bool FP8>
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  if (FP8) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  }
+  // adding 1.5 * 2^23 leaves the rounded integer in the low bits (two's complement)
+  constexpr float kRound = 12582912.f;
+  const uint32_t x = __float_as_uint(__fadd_rn(a, kRound)), y = __float_as_uint(__fadd_rn(b, kRound));
+  const uint32_t z = __float_as_uint(__fadd_rn(c, kRound)), w = __float_as_uint(__fadd_rn(d, kRound));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+
+template <bool FP8>
+__device__ __forceinline__ float code_value(uint32_t byte) {
+  if (FP8) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
+    return __half2float(*reinterpret_cast<const __half*>(&h));
+  }
+  return static_cast<float>(static_cast<int8_t>(byte));
+}
+
+// Row and eight-column unit of the i-th piece of a block (i < 1024, up to 8 units a row).
+struct Pieces {
+  int units;
+  uint32_t inverse;  // 65536 / units + 1
+  __device__ __forceinline__ void at(int i, int& row, int& unit) const {
+    row = static_cast<int>(static_cast<uint32_t>(i) * inverse >> 16);
+    unit = i - row * units;
+  }
+};
+
+template <int TYPE, bool FP8, int ALIGN, int BLOCK>
+__global__ void __launch_bounds__(kWriteThreads)
+    write_kernel(View c, Rows rk, Rows rv, PerSequence start, PerSequence count, int64_t n, int64_t per_seq,
+                 Pieces pieces) {
+  constexpr int kEach = BLOCK * (kMaxWidth / 8) / kWriteThreads;
+  constexpr float kTop = FP8 ? 448.f : 127.f;
+  int64_t unit = blockIdx.x;
+  const int h = static_cast<int>(unit % c.heads);
+  unit /= c.heads;
+  const int which = static_cast<int>(unit & 1);
+  unit >>= 1;
+  const int64_t j = unit % per_seq;
+  const int b = static_cast<int>(unit / per_seq);
+  const int64_t first = start.at(b), m = min(max(count.at(b), int64_t{0}), n);
+  const int64_t lo = max(first, int64_t{0}), hi = min(first + m, c.cap);  // rows of the cache that get values
+  const int64_t blk = lo / BLOCK + j, row0 = blk * BLOCK;
+  if (lo >= hi || row0 >= hi) return;
+  const int r0 = static_cast<int>(max(lo - row0, int64_t{0})), r1 = static_cast<int>(min(hi - row0, int64_t{BLOCK}));
+  const int64_t bh = static_cast<int64_t>(b) * c.heads + h;
+  uint8_t* dst = c.data(which) + (bh * c.cap + row0) * c.stored;
+  float* scale = c.scale(which) + bh * c.blocks() + blk;
+  const int64_t from = which ? rv.offset(b, row0 - first, h) : rk.offset(b, row0 - first, h);
+  const int64_t stride = which ? rv.sn : rk.sn;
+  const void* src = which ? rv.p : rk.p;
+
+  Raw<TYPE> x[kEach];
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    int row, u;
+    pieces.at(threadIdx.x + e * kWriteThreads, row, u);
+    if (row >= r0 && row < r1) {
+      x[e] = load8<TYPE, ALIGN>(src, from + row * stride + u * 8, c.width - u * 8);
+      top = top_bits<TYPE>(x[e], top);
+    }
+  }
+  float amax = top_value<TYPE>(top);
+  // over the CTA: magnitudes order like their bits
+  __shared__ uint32_t tops[kWriteThreads / 32];
+  const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+  if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = w;
+  const float old = r0 > 0 ? *scale : 0.f;  // rows before r0 stay
+  __syncthreads();
+  amax = __uint_as_float(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+  float s = __fdiv_rn(fmaxf(amax, 1e-12f), kTop);
+  s = old > s ? old : s;
+  if (!(amax < INFINITY) || old != old) s = __uint_as_float(0x7fc00000u);
+  const float inv = __frcp_rn(s);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    int row, u;
+    pieces.at(threadIdx.x + e * kWriteThreads, row, u);
+    if (row >= r0 && row < r1) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(value<TYPE>(x[e], i), inv);
+      *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(row) * c.stored + u * 8) =
+          make_uint2(codes4<FP8>(y[0], y[1], y[2], y[3]), codes4<FP8>(y[4], y[5], y[6], y[7]));
+    }
+  }
+  if (r0 > 0 && s != old) {  // the rows that stay, under the new scale
+    const float ratio = __fmul_rn(old, inv);
+    for (int i = threadIdx.x; i < r0 * pieces.units; i += kWriteThreads) {
+      uint2* p = reinterpret_cast<uint2*>(dst) + i;  // W = 8 units: pieces are contiguous
+      const uint2 q = *p;
+      float y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        y[k] = __fmul_rn(code_value<FP8>(((k < 4 ? q.x : q.y) >> 8 * (k & 3)) & 0xffu), ratio);
+      *p = make_uint2(codes4<FP8>(y[0], y[1], y[2], y[3]), codes4<FP8>(y[4], y[5], y[6], y[7]));
+    }
+  }
+  if (threadIdx.x == 0) *scale = s;
+}
+
+// ------------------------------------------------------------------ read back
+constexpr int kReadThreads = 256, kReadEach = 4;
+
+template <int TYPE, int ALIGN>
+__device__ __forceinline__ void store8(void* base, int64_t at, const float (&y)[8], int have) {
+  if constexpr (TYPE == kF32) {
+    float* p = static_cast<float*>(base) + at;
+    if constexpr (ALIGN >= 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+      if (have > 4) *reinterpret_cast<float4*>(p + 4) = make_float4(y[4], y[5], y[6], y[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < have) p[i] = y[i];
+    }
+  } else {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (TYPE == kBF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        const __half2 v = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    if constexpr (ALIGN == 8) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
+    } else if constexpr (ALIGN == 4) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(r[0], r[1]);
+      if (have > 4) *reinterpret_cast<uint2*>(p + 4) = make_uint2(r[2], r[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < have) p[i] = static_cast<uint16_t>(r[i / 2] >> 16 * (i & 1));
+    }
+  }
+}
+
+// k, v [batch, heads, n, D]; one CTA: kReadThreads * kReadEach pieces of one (sequence, head)
+template <int TYPE, bool FP8, int ALIGN>
+__global__ void __launch_bounds__(kReadThreads)
+    read_kernel(View c, void* k, void* v, int64_t start, int64_t n, int64_t chunks) {
+  int64_t unit = blockIdx.x;
+  const int64_t chunk = unit % chunks;
+  unit /= chunks;
+  const int which = static_cast<int>(unit & 1);
+  const int64_t bh = unit >> 1;
+  const int units = c.stored / 8;
+  const int64_t total = n * units;
+  const int64_t i0 = chunk * (kReadThreads * kReadEach) + threadIdx.x;
+  const uint2* src = reinterpret_cast<const uint2*>(c.data(which) + (bh * c.cap + start) * c.stored);
+  const float* scale = c.scale(which) + bh * c.blocks();
+  void* out = which ? v : k;
+  uint2 q[kReadEach];
+  float s[kReadEach];
+#pragma unroll
+  for (int e = 0; e < kReadEach; ++e) {
+    const int64_t i = i0 + e * kReadThreads;
+    if (i < total) {
+      q[e] = __ldg(src + i);
+      s[e] = __ldg(scale + ((start + i / units) >> c.block_log2));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kReadEach; ++e) {
+    const int64_t i = i0 + e * kReadThreads;
+    if (i < total) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        y[j] = __fmul_rn(code_value<FP8>(((j < 4 ? q[e].x : q[e].y) >> 8 * (j & 3)) & 0xffu), s[e]);
+      const int64_t row = i / units;
+      const int u = static_cast<int>(i - row * units);
+      store8<TYPE, ALIGN>(out, (bh * n + row) * c.width + u * 8, y, c.width - u * 8);
+    }
+  }
+}
+
+// How many values each access may take: rows, heads and the base all on that boundary.
+int alignment(int type, int width, const Rows& r) {
+  const int size = type == kF32 ? 4 : 2;
+  for (int a : {8, 4}) {
+    const int64_t bytes = a * size > 16 ? 16 : a * size;
+    const int64_t values = bytes / size;
+    if (width % a == 0 && reinterpret_cast<uintptr_t>(r.p) % bytes == 0 && r.s0 % values == 0 && r.s1 % values == 0 &&
+        r.sn % values == 0 && r.sh % values == 0)
+      return a;
+  }
+  return 1;
+}
+
+template <int TYPE, bool FP8, int ALIGN>
+cudaError_t write_typed(const View& c, const Rows& k, const Rows& v, const PerSequence& start, const PerSequence& count,
+                        int64_t n, cudaStream_t stream) {
+  const int block = 1 << c.block_log2;
+  // blocks that n rows can touch: one more where they need not begin on a block's first row
+  const bool at_edge = start.dev == nullptr && start.all % block == 0;
+  const int64_t most = c.cap / block, span = (n + block - 1) / block + (at_edge ? 0 : 1);
+  const int64_t per_seq = span < most ? span : most;
+  const int64_t grid = static_cast<int64_t>(c.batch) * per_seq * 2 * c.heads;
+  if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const int units = c.stored / 8;
+  const Pieces pieces{units, 65536u / units + 1};
+  auto go = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(grid), kWriteThreads, 0, stream>>>(c, k, v, start, count, n, per_seq, pieces);
+  };
+  if (block == 32)
+    go(write_kernel<TYPE, FP8, ALIGN, 32>);
+  else if (block == 64)
+    go(write_kernel<TYPE, FP8, ALIGN, 64>);
+  else
+    go(write_kernel<TYPE, FP8, ALIGN, 128>);
+  return cudaGetLastError();
+}
+
+template <int TYPE, bool FP8, int ALIGN>
+cudaError_t read_typed(const View& c, void* k, void* v, int64_t start, int64_t n, cudaStream_t stream) {
+  const int64_t pieces = n * (c.stored / 8), chunks = (pieces + kReadThreads * kReadEach - 1) / (kReadThreads * kReadEach);
+  const int64_t grid = chunks * 2 * c.batch * c.heads;
+  if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+  read_kernel<TYPE, FP8, ALIGN><<<static_cast<unsigned>(grid), kReadThreads, 0, stream>>>(c, k, v, start, n, chunks);
+  return cudaGetLastError();
+}
+
+// calls f<TYPE, FP8, ALIGN> for values known at run time
+template <typename F>
+cudaError_t dispatch(int type, bool fp8, int align, F&& f) {
+  auto by_align = [&](auto t, auto q) {
+    if (align == 8) return f(t, q, std::integral_constant<int, 8>());
+    if (align == 4) return f(t, q, std::integral_constant<int, 4>());
+    return f(t, q, std::integral_constant<int, 1>());
+  };
+  auto by_code = [&](auto t) { return fp8 ? by_align(t, std::true_type()) : by_align(t, std::false_type()); };
+  if (type == kF32) return by_code(std::integral_constant<int, kF32>());
+  if (type == kBF16) return by_code(std::integral_constant<int, kBF16>());
+  return by_code(std::integral_constant<int, kF16>());
+}
+
+}  // namespace
+
+cudaError_t launch_write(const View& c, const Rows& k, const Rows& v, int type, const PerSequence& start,
+                         const PerSequence& count, int64_t n, cudaStream_t stream) {
+  const int ak = alignment(type, c.width, k), av = alignment(type, c.width, v);
+  return dispatch(type, c.fp8, ak < av ? ak : av, [&](auto t, auto q, auto a) {
+    return write_typed<t.value, q.value, a.value>(c, k, v, start, count, n, stream);
+  });
+}
+
+cudaError_t launch_read(const View& c, void* k, void* v, int type, int64_t start, int64_t n, cudaStream_t stream) {
+  // rows of the result follow one another, so the width alone decides (the base is an allocation's)
+  const int align = c.width % 8 == 0 ? 8 : c.width % 4 == 0 ? 4 : 1;
+  return dispatch(type, c.fp8, align, [&](auto t, auto q, auto a) {
+    return read_typed<t.value, q.value, a.value>(c, k, v, start, n, stream);
+  });
+}
+
+}  // namespace bc
+}  // namespace nori

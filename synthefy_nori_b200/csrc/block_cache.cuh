@@ -1,0 +1,134 @@
+// Shared by the kernels of the context cache in 8 bits with block scales: what they are given,
+// and the exact widening of stored values to fp16.
+//
+// Storage: rows of W = D up to a multiple of 8 bytes, [batch, heads, capacity, W], int8 or e4m3,
+// one fp32 scale per (sequence, head, block of rows); a value is q * scale.  The capacity is a
+// multiple of 128 rows and every row of 8 bytes' alignment, so a tile of 128 rows is one
+// contiguous, 16-byte aligned piece of memory for every width (no padding to TMA's strides).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace nori {
+namespace bc {
+
+constexpr int kMaxWidth = 64;  // head width, as in the framework's other attention kernels
+constexpr int kTile = 128;     // rows of a key tile; the capacity is a multiple
+
+enum Float : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+struct View {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;
+  int batch, heads;
+  int64_t cap;
+  int width, stored;  // D, W
+  int block_log2;
+  bool fp8;
+  __host__ __device__ __forceinline__ int64_t blocks() const { return cap >> block_log2; }
+  __device__ __forceinline__ uint8_t* data(int which) const { return which ? v : k; }
+  __device__ __forceinline__ float* scale(int which) const { return which ? v_scale : k_scale; }
+};
+
+// [b0, b1, n, h, d] with contiguous d; sequence b = b0 * n1 + b1
+struct Rows {
+  void* p;
+  int64_t s0, s1, sn, sh;
+  int n1;
+  __device__ __forceinline__ int64_t offset(int b, int64_t n, int h) const {
+    return (b / n1) * s0 + (b % n1) * s1 + n * sn + h * sh;
+  }
+};
+
+// One value for all sequences or one of each, on the device.
+struct PerSequence {
+  const int* dev;
+  int64_t all;
+  __device__ __forceinline__ int64_t at(int b) const { return dev != nullptr ? dev[b] : all; }
+};
+
+struct Attention {
+  Rows q, o;
+  int type;  // of q and o (kBF16, kF16)
+  View c;
+  PerSequence length;
+  int64_t n;        // query rows
+  int group;        // query heads of one K/V head
+  int64_t rows;     // n * group: the rows that read one K/V head
+  float scale_log2; // softmax scale * log2(e)
+  float* lse;       // [batch, query heads, n] or null
+  int splits;       // of the key range
+  float* part_o;    // [units, splits, tile rows, 64], unnormalised
+  float2* part_ml;  // [units, splits, tile rows] (maximum, sum)
+  int* status;
+};
+
+// Weights are 2^(t - m + kLift): fp16 keeps 11 bits of them down to 2^-25 of the largest, and a
+// maximum that lags by up to kLazy (no rescale of the sums) stays below fp16's largest value.
+constexpr float kLift = 11.f;
+constexpr float kLazy = 4.f;
+
+// e4m3 codes widen to fp16 by their bits alone, as value * 2^-8 (exponent biases 15 and 7; the
+// subnormals of both formats are linear, so they agree too).
+template <bool FP8>
+constexpr float kCodeScale = FP8 ? 256.f : 1.f;
+
+#ifdef __CUDACC__
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Four codes (bytes of x, int8 ones biased by 128) -> two fp16 pairs, exact.
+// int8: 0x64uu is the fp16 1024 + u, minus 1152.  e4m3: sign eeee mmm -> sign 0eeee mmm0000000.
+template <bool FP8>
+__device__ __forceinline__ void widen(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  if (FP8) {
+    const uint32_t a = __byte_perm(x, 0, 0x1404), b = __byte_perm(x, 0, 0x3424);
+    lo = ((a >> 1) & 0x3f803f80u) | (a & 0x80008000u);
+    hi = ((b >> 1) & 0x3f803f80u) | (b & 0x80008000u);
+  } else {
+    lo = hsub2(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
+    hi = hsub2(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
+  }
+}
+template <bool FP8>
+__device__ __forceinline__ uint32_t biased(uint32_t x) {
+  return FP8 ? x : x ^ 0x80808080u;
+}
+
+// A power of two that brings a row's largest magnitude near 2^14 and its inverse (both normal
+// numbers); a row with an infinity or a NaN gets a NaN inverse.
+__device__ __forceinline__ void row_scale(float top, float& up, float& down) {
+  if (!(top < INFINITY)) {
+    up = 1.f;
+    down = __uint_as_float(0x7fc00000u);
+    return;
+  }
+  int e = 14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127);
+  e = min(max(e, -120), 120);
+  up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+  down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+}
+
+// log2 of a V scale and its inverse: a block that was never written has scale 0 and holds zeros,
+// which any small scale says as well.
+__device__ __forceinline__ float safe_scale(float s) { return s < 7.9e-31f ? 7.9e-31f : s; }
+#endif
+
+cudaError_t launch_write(const View& c, const Rows& k, const Rows& v, int type, const PerSequence& start,
+                         const PerSequence& count, int64_t n, cudaStream_t stream);
+cudaError_t launch_read(const View& c, void* k, void* v, int type, int64_t start, int64_t n, cudaStream_t stream);
+// rows of a tile of the two attention kernels, and how many splits of the keys they would take
+int few_tile_rows(int64_t rows);
+cudaError_t launch_few(const Attention& a, cudaStream_t stream);
+cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream);
+
+}  // namespace bc
+}  // namespace nori

@@ -1,0 +1,187 @@
+// Entry points of the context cache in 8 bits with block scales: checks of the arguments, the
+// choice of kernel and of how far the keys are split.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+
+#include "block_cache.cuh"
+#include "plain.h"
+
+namespace nori {
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+bc::View view_of(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t width, const char* who) {
+  for (const Tensor* t : {&k, &v, &ks, &vs}) {
+    check_plain(*t, who);
+    TORCH_CHECK(t->is_contiguous(), who, ": contiguous cache tensors expected");
+  }
+  TORCH_CHECK(k.scalar_type() == v.scalar_type() &&
+                  (k.scalar_type() == at::kChar || k.scalar_type() == at::kFloat8_e4m3fn),
+              who, ": the cache's k and v must both be int8 or float8_e4m3fn");
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), who, ": k and v [batch, heads, capacity, width] expected");
+  TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.dim() == 3 &&
+                  ks.sizes() == vs.sizes() && ks.size(0) == k.size(0) && ks.size(1) == k.size(1),
+              who, ": fp32 scales [batch, heads, capacity / block] expected");
+  const int64_t cap = k.size(2), blocks = ks.size(2);
+  TORCH_CHECK(width >= 1 && width <= bc::kMaxWidth && k.size(3) == (width + 7) / 8 * 8, who,
+              ": head widths of 1 to 64 in rows of the next multiple of 8 expected");
+  TORCH_CHECK(cap >= bc::kTile && cap % bc::kTile == 0 && cap < (int64_t{1} << 31), who,
+              ": the capacity must be a multiple of 128 below 2^31");
+  int log2 = 0;
+  for (int l : {5, 6, 7})
+    if (blocks << l == cap) log2 = l;
+  TORCH_CHECK(log2 != 0, who, ": one scale for each 32, 64 or 128 rows expected");
+  TORCH_CHECK(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX, who, ": too many sequences or heads");
+  for (const Tensor* t : {&k, &v, &ks, &vs})
+    TORCH_CHECK(t->is_cuda() && t->device() == k.device(), who, ": cache tensors on one CUDA device expected");
+  for (const Tensor* t : {&k, &v})
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0, who, ": a cache 16-byte aligned expected");
+  bc::View c{};
+  c.k = static_cast<uint8_t*>(const_cast<void*>(k.const_data_ptr()));
+  c.v = static_cast<uint8_t*>(const_cast<void*>(v.const_data_ptr()));
+  c.k_scale = const_cast<float*>(ks.const_data_ptr<float>());
+  c.v_scale = const_cast<float*>(vs.const_data_ptr<float>());
+  c.batch = static_cast<int>(k.size(0));
+  c.heads = static_cast<int>(k.size(1));
+  c.cap = cap;
+  c.width = static_cast<int>(width);
+  c.stored = static_cast<int>(k.size(3));
+  c.block_log2 = log2;
+  c.fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
+  return c;
+}
+
+int float_type(const Tensor& t, bool fp32, const char* who, const char* what) {
+  const auto s = t.scalar_type();
+  TORCH_CHECK(s == at::kBFloat16 || s == at::kHalf || (fp32 && s == at::kFloat), who, ": ", what, " must be ",
+              fp32 ? "fp32, bf16 or fp16" : "bf16 or fp16", ", got ", s);
+  return s == at::kFloat ? bc::kF32 : s == at::kBFloat16 ? bc::kBF16 : bc::kF16;
+}
+
+// [batch, n, heads, width] or [b0, b1, n, heads, width] (b0 * b1 = batch), columns contiguous
+bc::Rows rows_of(const Tensor& t, const bc::View& c, int64_t n, int64_t heads, const torch::Device& dev, const char* who,
+                 const char* what) {
+  check_plain(t, who);
+  TORCH_CHECK(t.is_cuda() && t.device() == dev, who, ": ", what, " must be on the cache's device");
+  const int64_t d = t.dim();
+  TORCH_CHECK((d == 4 || d == 5) && t.size(d - 1) == c.width && t.size(d - 2) == heads && t.size(d - 3) == n &&
+                  (d == 4 ? t.size(0) : t.size(0) * t.size(1)) == c.batch,
+              who, ": ", what, " must be [batch, n, heads, width] (or two batch dimensions), batch ", c.batch, ", n ", n,
+              ", heads ", heads, ", width ", c.width);
+  TORCH_CHECK(c.width == 1 || t.stride(d - 1) == 1, who, ": the columns of ", what, " must be contiguous");
+  bc::Rows r{};
+  r.p = const_cast<void*>(t.const_data_ptr());
+  r.s0 = t.stride(0);
+  r.s1 = d == 5 ? t.stride(1) : 0;
+  r.n1 = d == 5 ? static_cast<int>(std::max<int64_t>(t.size(1), 1)) : 1;
+  r.sn = t.stride(d - 3);
+  r.sh = t.stride(d - 2);
+  return r;
+}
+
+bc::PerSequence per_sequence(const OptTensor& dev, int64_t all, const bc::View& c, const torch::Device& device,
+                             const char* who, const char* what) {
+  bc::PerSequence p{nullptr, all};
+  if (dev.has_value() && dev->defined()) {
+    check_plain(*dev, who);
+    TORCH_CHECK(dev->device() == device && dev->scalar_type() == at::kInt && dev->is_contiguous() && dev->numel() == c.batch,
+                who, ": ", what, " must be an int or int32 [batch] on the cache's device");
+    p.dev = dev->const_data_ptr<int>();
+  }
+  return p;
+}
+
+int sm_count(int dev) { return at::cuda::getDeviceProperties(dev)->multiProcessorCount; }
+
+}  // namespace
+
+void block_cache_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs, int64_t width,
+                       const Tensor& k, const Tensor& v, int64_t start_all, const OptTensor& start_dev,
+                       const OptTensor& count_dev) {
+  const char* who = "block_cache_write";
+  const bc::View c = view_of(ck, cv, cks, cvs, width, who);
+  TORCH_CHECK(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), who, ": k and v of one shape and type expected");
+  const int type = float_type(k, true, who, "k");
+  TORCH_CHECK(k.dim() >= 4, who, ": k [batch, n, heads, width] expected");
+  const int64_t n = k.size(-3);
+  const bc::Rows rk = rows_of(k, c, n, c.heads, ck.device(), who, "k"), rv = rows_of(v, c, n, c.heads, ck.device(), who, "v");
+  const bc::PerSequence start = per_sequence(start_dev, start_all, c, ck.device(), who, "start");
+  const bc::PerSequence count = per_sequence(count_dev, n, c, ck.device(), who, "counts");
+  if (start.dev == nullptr)
+    TORCH_CHECK(start_all >= 0 && start_all + n <= c.cap, who, ": rows ", start_all, " to ", start_all + n,
+                " of a cache of ", c.cap);
+  if (n == 0 || c.batch == 0 || c.heads == 0) return;
+  const at::cuda::CUDAGuard guard(ck.device());
+  C10_CUDA_CHECK(bc::launch_write(c, rk, rv, type, start, count, n, at::cuda::getCurrentCUDAStream()));
+}
+
+std::vector<Tensor> block_cache_read(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs,
+                                     int64_t width, int64_t start, int64_t n, c10::ScalarType out_type) {
+  const char* who = "block_cache_read";
+  const bc::View c = view_of(ck, cv, cks, cvs, width, who);
+  TORCH_CHECK(start >= 0 && n >= 0 && start <= c.cap && n <= c.cap - start, who, ": rows ", start, " to ", start + n,
+              " of a cache of ", c.cap);
+  const at::cuda::CUDAGuard guard(ck.device());
+  std::vector<Tensor> out;
+  for (int i = 0; i < 2; ++i)
+    out.push_back(torch::empty({c.batch, c.heads, n, width}, ck.options().dtype(out_type)));
+  const int type = float_type(out[0], true, who, "the result");
+  if (out[0].numel() > 0)
+    C10_CUDA_CHECK(bc::launch_read(c, out[0].data_ptr(), out[1].data_ptr(), type, start, n, at::cuda::getCurrentCUDAStream()));
+  for (auto& t : out) t = t.transpose(1, 2);
+  return out;
+}
+
+// Returns the log-sum-exp [batch, heads, n] (empty where it is not wanted); o is written.
+Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs,
+                             int64_t width, int64_t length_all, const OptTensor& length_dev, double scale, const Tensor& o,
+                             bool want_lse, const Tensor& status) {
+  const char* who = "block_cache_attention";
+  bc::Attention a{};
+  a.c = view_of(ck, cv, cks, cvs, width, who);
+  TORCH_CHECK(q.dim() >= 4, who, ": q [batch, n, heads, width] expected");
+  a.n = q.size(-3);
+  const int64_t heads = q.size(-2);
+  TORCH_CHECK(a.c.heads > 0 ? heads % a.c.heads == 0 : heads == 0, who, ": ", heads, " query heads do not share ",
+              a.c.heads, " K/V heads evenly");
+  a.type = float_type(q, false, who, "q");
+  a.q = rows_of(q, a.c, a.n, heads, ck.device(), who, "q");
+  TORCH_CHECK(o.scalar_type() == q.scalar_type() && o.sizes() == q.sizes(), who, ": out of q's shape and type expected");
+  a.o = rows_of(o, a.c, a.n, heads, ck.device(), who, "out");
+  a.length = per_sequence(length_dev, length_all, a.c, ck.device(), who, "lengths");
+  if (a.length.dev == nullptr)
+    TORCH_CHECK(length_all >= 0 && length_all <= a.c.cap, who, ": length ", length_all, " of a cache of ", a.c.cap);
+  TORCH_CHECK(scale > 0.0 && scale < 1e30, who, ": a positive finite scale expected");
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  const at::cuda::CUDAGuard guard(ck.device());
+  Tensor lse = torch::empty({want_lse ? a.c.batch : 0, heads, a.n}, ck.options().dtype(at::kFloat));
+  if (q.numel() == 0) return lse;
+  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  a.group = static_cast<int>(heads / a.c.heads);
+  a.rows = a.n * a.group;
+  a.status = status.data_ptr<int>();
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  const int tile = bc::few_tile_rows(a.rows);
+  const int64_t cells = (a.rows + tile - 1) / tile * a.c.batch * a.c.heads;
+  // the longest a sequence can be (lengths on the device are not read here)
+  const int64_t longest = a.length.dev != nullptr ? a.c.cap : length_all;
+  const int64_t fill = 4 * sm_count(ck.get_device());
+  a.splits = static_cast<int>(std::clamp<int64_t>(fill / cells, 1, std::max<int64_t>((longest + 255) / 256, 1)));
+  Tensor part_o, part_ml;
+  if (a.splits > 1) {
+    part_o = torch::empty({cells * a.splits * tile * bc::kMaxWidth}, lse.options());
+    part_ml = torch::empty({cells * a.splits * tile * 2}, lse.options());
+    a.part_o = part_o.data_ptr<float>();
+    a.part_ml = reinterpret_cast<float2*>(part_ml.data_ptr<float>());
+  }
+  C10_CUDA_CHECK(bc::launch_few(a, stream));
+  if (a.splits > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
+  return lse;
+}
+
+}  // namespace nori

@@ -36,3 +36,4 @@ def lib():
 from synthefy_nori_b200.ops.api import *  # noqa: E402,F401,F403
 from synthefy_nori_b200.ops.norm import *  # noqa: E402,F401,F403
 from synthefy_nori_b200.ops.muon import *  # noqa: E402,F401,F403
+from synthefy_nori_b200.ops.block_cache import *  # noqa: E402,F401,F403
