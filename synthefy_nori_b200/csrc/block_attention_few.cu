@@ -61,11 +61,6 @@ __device__ __forceinline__ float quad_sum(float x) {
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
 
-// out = o / l and the log-sum-exp of one row from maximum m, sum l (with kLift) and values o
-__device__ __forceinline__ float row_lse(float m, float l) {
-  return l != 0.f ? 0.6931471805599453f * (m + log2f(l) - kLift) : -INFINITY;
-}
-
 struct Row {  // where row r of a K/V head's query rows lies
   int64_t n;
   int head;
@@ -306,7 +301,8 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
   float sum = 0.f, a0 = 0.f, a1 = 0.f;
   for (int s = warp; s < a.splits; s += kJoinThreads / 32) {
     const float2 ml = a.part_ml[(cell0 + s) * tile_rows + tr];
-    const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - top);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no keys there (and perhaps no values written)
+    const float f = exp2f(ml.x - top);
     const float2 v = *reinterpret_cast<const float2*>(a.part_o + ((cell0 + s) * tile_rows + tr) * kMaxWidth + 2 * lane);
     sum = fmaf(ml.y, f, sum);
     a0 = fmaf(v.x, f, a0);

@@ -120,6 +120,11 @@ __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
 // log2 of a V scale and its inverse: a block that was never written has scale 0 and holds zeros,
 // which any small scale says as well.
 __device__ __forceinline__ float safe_scale(float s) { return s < 7.9e-31f ? 7.9e-31f : s; }
+
+// The natural log-sum-exp of a row from its maximum and its sum (which carries kLift).
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l != 0.f ? 0.6931471805599453f * (m + log2f(l) - kLift) : -INFINITY;
+}
 #endif
 
 cudaError_t launch_write(const View& c, const Rows& k, const Rows& v, int type, const PerSequence& start,
@@ -128,6 +133,9 @@ cudaError_t launch_read(const View& c, void* k, void* v, int type, int64_t start
 // rows of a tile of the two attention kernels, and how many splits of the keys they would take
 int few_tile_rows(int64_t rows);
 cudaError_t launch_few(const Attention& a, cudaStream_t stream);
+// rows of a tile pair of the kernel for many rows; one CTA per SM
+constexpr int kPairRows = 256;
+cudaError_t launch_tc(const Attention& a, int ctas, cudaStream_t stream);
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream);
 
 }  // namespace bc

@@ -8,6 +8,7 @@
 
 #include "block_cache.cuh"
 #include "plain.h"
+#include "tma_host.h"
 
 namespace nori {
 namespace {
@@ -98,6 +99,27 @@ bc::PerSequence per_sequence(const OptTensor& dev, int64_t all, const bc::View& 
 
 int sm_count(int dev) { return at::cuda::getDeviceProperties(dev)->multiProcessorCount; }
 
+// Up to this many rows of one K/V head run on the kernel that streams the cache through registers.
+constexpr int64_t kFewRows = 16;
+
+int few_splits(int64_t cells, int64_t longest, int sms) {
+  return static_cast<int>(std::clamp<int64_t>(4 * sms / cells, 1, std::max<int64_t>((longest + 255) / 256, 1)));
+}
+
+// Splits of the keys for the persistent kernel: the waves of items, each as long as its key tiles
+// and the start and end of an item; partial results cost a second kernel and their traffic.
+int tc_splits(int64_t cells, int64_t longest, int ctas) {
+  const int64_t tiles = std::max<int64_t>((longest + bc::kTile - 1) / bc::kTile, 1);
+  int best = 1;
+  double least = 0;
+  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
+    const double waves = static_cast<double>((cells * s + ctas - 1) / ctas);
+    const double cost = waves * (static_cast<double>((tiles + s - 1) / s) + 3.0) + (s > 1 ? 4.0 + 0.04 * cells * s : 0.0);
+    if (s == 1 || cost < least) least = cost, best = static_cast<int>(s);
+  }
+  return best;
+}
+
 }  // namespace
 
 void block_cache_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs, int64_t width,
@@ -165,13 +187,13 @@ Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv
   a.group = static_cast<int>(heads / a.c.heads);
   a.rows = a.n * a.group;
   a.status = status.data_ptr<int>();
-  const auto stream = at::cuda::getCurrentCUDAStream();
-  const int tile = bc::few_tile_rows(a.rows);
-  const int64_t cells = (a.rows + tile - 1) / tile * a.c.batch * a.c.heads;
   // the longest a sequence can be (lengths on the device are not read here)
   const int64_t longest = a.length.dev != nullptr ? a.c.cap : length_all;
-  const int64_t fill = 4 * sm_count(ck.get_device());
-  a.splits = static_cast<int>(std::clamp<int64_t>(fill / cells, 1, std::max<int64_t>((longest + 255) / 256, 1)));
+  const int sms = sm_count(ck.get_device());
+  const bool few = a.rows <= kFewRows;
+  const int tile = few ? bc::few_tile_rows(a.rows) : bc::kPairRows;
+  const int64_t cells = (a.rows + tile - 1) / tile * a.c.batch * a.c.heads;
+  a.splits = few ? few_splits(cells, longest, sms) : tc_splits(cells, longest, persistent_sms(sms));
   Tensor part_o, part_ml;
   if (a.splits > 1) {
     part_o = torch::empty({cells * a.splits * tile * bc::kMaxWidth}, lse.options());
@@ -179,7 +201,8 @@ Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv
     a.part_o = part_o.data_ptr<float>();
     a.part_ml = reinterpret_cast<float2*>(part_ml.data_ptr<float>());
   }
-  C10_CUDA_CHECK(bc::launch_few(a, stream));
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  C10_CUDA_CHECK(few ? bc::launch_few(a, stream) : bc::launch_tc(a, persistent_sms(sms), stream));
   if (a.splits > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
   return lse;
 }
