@@ -1,23 +1,28 @@
 // Attention of many query rows over a context cache in 8 bits with block scales, on the 5th-generation
 // tensor cores.
 //
-// Persistent, one CTA of 16 warps per SM; a work item is 256 query rows (two tiles of 128, one per
-// softmax group) against a range of the keys of one (sequence, K/V head).  Roles:
+// Persistent, one CTA of 28 warps per SM; a work item is 256 query rows (two tiles of 128) against a
+// range of the keys of one (sequence, K/V head).  Roles:
 //   warp 0        copies the codes of 128-key tiles of K and V, each one contiguous piece of the
 //                 cache, into two rings (untiled bulk copies: no stride rules, so any width);
-//   warps 12..15  widen the codes to fp16, exactly, into the swizzled tiles that the products read;
-//                 both groups use them, so a code is widened once for 256 query rows;
-//   warp 1        issues S_g = Q_g K^T (128 x 128 x 64) and O_g += P_g V (A = P_g from TMEM); S_g of
-//                 the next tile goes out as soon as group g has S_g in registers;
-//   warps 4..11   softmax: thread = query row (its TMEM lane), the whole score row in registers; P_g
-//                 (fp16 pairs) has TMEM columns of its own, so scores never wait for P . V.
+//   warps 4..7    widen the codes of K to fp16, exactly, into the swizzled tiles that the products
+//   warps 8..11   read, and those of V: once for 256 query rows;
+//   warps 1, 2    issue the products of one query tile each: S = Q K^T (128 x 64 x 64) and O += P V;
+//   warps 12..27  softmax, four groups: (query tile) x (half of the keys of every tile), each with its
+//                 own maximum, sum and accumulator; thread = query row (its TMEM lane), 64 score columns
+//                 in registers; P (fp16 pairs) goes over S in TMEM and is the A operand of P V.
+// A group's tile is a chain (scores, maximum, weights, two products) whose latency is several times its
+// arithmetic, so four of them share an SM: with one thread for all 128 columns of a row and two
+// groups the same arithmetic took 1.3 times as long, with row maxima exchanged between the
+// halves 1.2 times.  The two halves of a query tile are joined once per item.
 //
 // Scales cost nothing per value: with c = scale log2(e) s_k 2^-e (2^e brings the query row into
 // fp16's range, exactly) and t = c (q . k) + log2 s_v,
 //   w = 2^(t - max t),  O = sum w v_code,  l = sum over blocks of (sum of w) / s_v.
 // The maximum is lazy (O is rescaled when it grows by more than 2^4); w is kept at up to 2^15 so
-// that fp16 holds 11 bits down to 2^-25 of the largest weight.  Half of the exponentials run on the
-// MUFU, half as a polynomial on the FMA pipe.  Scores, sums and O are fp32.
+// that fp16 holds 11 bits down to 2^-25 of the largest weight.  Scores, sums and O are fp32.
+// All exponentials run on the MUFU: a polynomial on the FMA pipe for a quarter of them made a tile
+// slower (3634 cycles for 3180), since the warps' issue slots are as scarce as the MUFU.
 //
 // Every wait is bounded (sm100.cuh); on a timeout the CTA records it in the status word, waits for
 // its own copies and products, frees its TMEM and returns.
@@ -32,17 +37,18 @@ namespace {
 
 constexpr int kM = 128, kN = kTile, kD = kMaxWidth;
 static_assert(kPairRows == 2 * kM);
-constexpr int kThreads = 512;
+constexpr int kThreads = 896;
 constexpr int kRing = 3;                 // stages of each ring (codes and fp16 tiles, K and V)
 constexpr int kTile16 = kN * kD * 2;     // bytes of an fp16 tile of 128 x 64 (Q, K or V)
 constexpr int kTile8 = kN * kD;          // room for a tile of codes
 constexpr int kSmem = kTile16 * (2 + 2 * kRing) + kTile8 * 2 * kRing + 512 + 1024;
-// S 0..255 (128 a group), P 256..383 (64 a group), O 384..511 (64 a group)
-constexpr uint32_t kTmemCols = 512, kPcol = 256, kOcol = 384;
-constexpr int kConvertWarps = 4, kGroupWarps = 4;
-// registers of a thread: launch 128 (512 threads); the softmax warps take what the others give up
-constexpr uint32_t kRegsLow = 56, kRegsSoftmax = 200;
-static_assert(8 * 32 * (kRegsLow + kRegsSoftmax) <= kThreads * 128, "register split over the launch total");
+constexpr int kHalf = kN / 2;            // keys of a group's tile
+// S 0..255 (64 a group, P over its first 32), O 256..511 (64 a group)
+constexpr uint32_t kTmemCols = 512, kOcol = 256;
+constexpr int kConvertWarps = 4, kSoftmaxWarp0 = 12;
+// registers of a thread: launch 72 (896 threads); the softmax warps take what the others give up
+constexpr uint32_t kRegsLow = 40, kRegsSoftmax = 96;
+static_assert(12 * 32 * kRegsLow + 16 * 32 * kRegsSoftmax <= kThreads * 72, "register split over the launch total");
 
 constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {  // fp16 A and B, fp32 D
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
@@ -80,38 +86,10 @@ __device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t f2sub(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-
-// 2^x of a pair without the MUFU: x = n + f, n by adding 1.5 * 2^23, 2^f by a polynomial of degree 4
-// fitted for the smallest relative error on [-0.5, 0.5] (2.7e-6), n added to the exponent.  x is
-// held at -125 and above so that the result stays a normal number.
-__device__ __forceinline__ void exp2_poly2(uint64_t x2, float& e0, float& e1) {
-  constexpr float kRound = 12582912.0f;
-  float x0, x1;
-  f2unpack(x2, x0, x1);
-  x2 = f2pack(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
-  const uint64_t r2 = f2pack(kRound, kRound);
-  const uint64_t t2 = f2add(x2, r2);
-  const uint64_t f2 = f2sub(x2, f2sub(t2, r2));
-  uint64_t p = f2fma(f2, f2pack(0.009570102207362652f, 0.009570102207362652f),
-                     f2pack(0.05591785907745361f, 0.05591785907745361f));
-  p = f2fma(p, f2, f2pack(0.240247443318367f, 0.240247443318367f));
-  p = f2fma(p, f2, f2pack(0.6931217908859253f, 0.6931217908859253f));
-  p = f2fma(p, f2, f2pack(0.9999992847442627f, 0.9999992847442627f));
-  float p0, p1, t0, t1;
-  f2unpack(p, p0, p1);
-  f2unpack(t2, t0, t1);
-  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -119,85 +97,77 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ float max32(const uint32_t (&v)[32], int valid) {
-  if (valid >= 32) {
-    float m[8];
+__device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
+  float m[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      m[i] = max3(__uint_as_float(v[i]), __uint_as_float(v[i + 8]), __uint_as_float(v[i + 16]));
+  for (int i = 0; i < 8; ++i)
+    m[i] = max3(__uint_as_float(v[i]), __uint_as_float(v[i + 8]), __uint_as_float(v[i + 16]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], __uint_as_float(v[i + 24]));
-    return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (i < valid) m = fmaxf(m, __uint_as_float(v[i]));
-  return m;
+  for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], __uint_as_float(v[i + 24]));
+  return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
 }
 
-// w = 2^(s c + shift) for 32 columns as fp16 pairs; returns their sum in fp32.  Columns at or past
-// `valid` give 0.
-__device__ __forceinline__ float weights32(const uint32_t (&v)[32], int valid, float c, float shift, uint32_t (&pk)[16]) {
-  if (valid >= 32) {
-    const uint64_t c2 = f2pack(c, c), s2 = f2pack(shift, shift);
-    uint64_t ra = 0, rb = 0;
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// w = 2^(s c + shift) for 32 columns as fp16 pairs, to TMEM; returns their sum in fp32.
+__device__ __forceinline__ float weights32(const uint32_t (&v)[32], float c, float shift, uint32_t tP) {
+  const uint64_t c2 = f2pack(c, c), s2 = f2pack(shift, shift);
+  uint64_t ra = 0, rb = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t pk[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint64_t xa = f2fma(f2pack(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), c2, s2);
-      const uint64_t xb = f2fma(f2pack(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), c2, s2);
-      float x0, x1, e2, e3;
-      f2unpack(xa, x0, x1);
-      const float e0 = exp2_mufu(x0), e1 = exp2_mufu(x1);
-      exp2_poly2(xb, e2, e3);
-      pk[2 * i] = pack_half2(e0, e1);
-      pk[2 * i + 1] = pack_half2(e2, e3);
-      ra = f2add(ra, f2pack(e0, e1));
-      rb = f2add(rb, f2pack(e2, e3));
+      float e0, e1;
+      f2unpack(f2fma(f2pack(__uint_as_float(v[16 * h + 2 * i]), __uint_as_float(v[16 * h + 2 * i + 1])), c2, s2), e0, e1);
+      e0 = exp2_mufu(e0), e1 = exp2_mufu(e1);
+      pk[i] = pack_half2(e0, e1);
+      if (i % 2)
+        rb = f2add(rb, f2pack(e0, e1));
+      else
+        ra = f2add(ra, f2pack(e0, e1));
     }
-    float r0, r1;
-    f2unpack(f2add(ra, rb), r0, r1);
-    return r0 + r1;
+    tmem_st8(tP + 8 * h, pk);
   }
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float e0 = 2 * i < valid ? exp2_mufu(fmaf(__uint_as_float(v[2 * i]), c, shift)) : 0.f;
-    const float e1 = 2 * i + 1 < valid ? exp2_mufu(fmaf(__uint_as_float(v[2 * i + 1]), c, shift)) : 0.f;
-    pk[i] = pack_half2(e0, e1);
-    sum += e0 + e1;
-  }
-  return sum;
+  float r0, r1;
+  f2unpack(f2add(ra, rb), r0, r1);
+  return r0 + r1;
 }
 
+// (everything below 2^31, checked on the host: 64-bit divisions would take a microsecond an item)
 struct Item {
-  int b, h, split;
-  int64_t bh, row0, key0;  // first query row, first key
-  int64_t len;             // keys of the sequence
-  int tiles;               // key tiles of this item
-  int groups;              // query tiles with rows in them (1 or 2)
+  uint32_t b, h, split, bh;
+  uint32_t pair, row0;  // pair of query tiles, its first row
+  uint32_t tile0;       // first key tile
+  int len;              // keys of the sequence
+  int tiles;            // key tiles of this item
+  int groups;           // query tiles with rows in them (1 or 2)
 };
 
-__device__ __forceinline__ Item item_at(const Attention& a, int64_t w) {
+__device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
   Item it;
-  const int64_t pairs = (a.rows + kPairRows - 1) / kPairRows;
-  it.row0 = w % pairs * kPairRows;
+  const uint32_t pairs = (static_cast<uint32_t>(a.rows) + kPairRows - 1) / kPairRows;
+  it.pair = w % pairs;
+  it.row0 = it.pair * kPairRows;
   w /= pairs;
-  it.split = static_cast<int>(w % a.splits);
-  it.bh = w / a.splits;
-  it.b = static_cast<int>(it.bh / a.c.heads);
-  it.h = static_cast<int>(it.bh % a.c.heads);
-  it.len = min(max(a.length.at(it.b), int64_t{0}), a.c.cap);
-  const int64_t all = (it.len + kN - 1) / kN, each = (all + a.splits - 1) / a.splits;
-  const int64_t t0 = min(it.split * each, all);
-  it.key0 = t0 * kN;
-  it.tiles = static_cast<int>(min(t0 + each, all) - t0);
-  it.groups = it.row0 + kM < a.rows ? 2 : 1;
+  it.split = w % static_cast<uint32_t>(a.splits);
+  it.bh = w / static_cast<uint32_t>(a.splits);
+  it.b = it.bh / static_cast<uint32_t>(a.c.heads);
+  it.h = it.bh - it.b * static_cast<uint32_t>(a.c.heads);
+  it.len = static_cast<int>(min(max(a.length.at(it.b), int64_t{0}), a.c.cap));
+  const uint32_t all = (static_cast<uint32_t>(it.len) + kN - 1) / kN, each = (all + a.splits - 1) / static_cast<uint32_t>(a.splits);
+  it.tile0 = min(it.split * each, all);
+  it.tiles = static_cast<int>(min(it.tile0 + each, all) - it.tile0);
+  it.groups = it.row0 + kM < static_cast<uint32_t>(a.rows) ? 2 : 1;
   return it;
 }
 
 template <bool FP8>
-__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Attention a, int64_t items, bool q_vec,
+__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool q_vec,
                                                          bool o_vec) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -215,16 +185,16 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
   uint64_t* k_empty = k_full + kRing;     // the products that read it are done
   uint64_t* v_full = k_empty + kRing;
   uint64_t* v_empty = v_full + kRing;
-  uint64_t* q_full = v_empty + kRing;     // [group] per item
-  uint64_t* s_full = q_full + 2;          // [group] per tile
-  uint64_t* s_free = s_full + 2;          // [group] scores are in registers
-  uint64_t* p_full = s_free + 2;          // [group]
-  uint64_t* o_full = p_full + 2;          // [group] P . V of a tile is done
-  uint64_t* o_free = o_full + 2;          // [group] per item: O is in registers
-  uint64_t* done = o_free + 2;            // every product of this CTA
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* q_full = v_empty + kRing;     // [query tile] per item
+  uint64_t* o_free = q_full + 2;          // [query tile] per item: O is in registers
+  uint64_t* s_full = o_free + 2;          // [group] per tile: scores (and the last P V), and once more per item
+  uint64_t* p_full = s_full + 4;          // [group] per tile: P is in TMEM
+  uint64_t* pair = p_full + 4;            // [query tile][lane quarter] the two halves have exchanged
+  uint64_t* done = pair + 8;              // [query tile] every product of this CTA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((8 * kRing + 13) * 8 + 8 <= 512, "barriers fit their room");
+  __shared__ float2 swap[2][16][32];  // [parity of the exchange][softmax warp][row]
+  static_assert((8 * kRing + 22) * 8 + 8 <= 512, "barriers fit their room");
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (*reinterpret_cast<volatile int*>(a.status) != 0) return;  // another CTA or kernel timed out
@@ -237,18 +207,19 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
       mbar_init(&rv_empty[i], kConvertWarps);
       mbar_init(&k_full[i], kConvertWarps);
       mbar_init(&v_full[i], kConvertWarps);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
+      mbar_init(&v_empty[i], 2);
     }
-    for (int g = 0; g < 2; ++g) {
-      mbar_init(&q_full[g], kGroupWarps);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 8);
+      mbar_init(&o_free[t], 8);
+      mbar_init(&done[t], 1);
+    }
+    for (int g = 0; g < 4; ++g) {
       mbar_init(&s_full[g], 1);
-      mbar_init(&s_free[g], kGroupWarps);
-      mbar_init(&p_full[g], kGroupWarps);
-      mbar_init(&o_full[g], 1);
-      mbar_init(&o_free[g], kGroupWarps);
+      mbar_init(&p_full[g], 4);
     }
-    mbar_init(done, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&pair[i], 2);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -268,9 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
       const uint32_t bytes = static_cast<uint32_t>(kN * a.c.stored);
       uint32_t nk = 0, nv = 0;  // tiles asked for so far
       bool ok = true;
-      for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+      for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
         const Item it = item_at(a, w);
-        const int64_t at = (it.bh * a.c.cap + it.key0) * a.c.stored;
+        const int64_t at = (it.bh * a.c.cap + static_cast<int64_t>(it.tile0) * kN) * a.c.stored;
         auto load = [&](int j, const uint8_t* src, uint8_t* dst, uint64_t* full, uint64_t* empty, uint32_t& n) -> bool {
           const uint32_t st = n % kRing;
           if (!mbar_wait(&empty[st], (n / kRing & 1) ^ 1, a.status, kTimeoutProducer, abort_flag)) return false;
@@ -291,165 +262,194 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         if (nv > i) mbar_wait(&rv_full[(nv - 1 - i) % kRing], (nv - 1 - i) / kRing & 1, a.status, kTimeoutProducer, nullptr);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp <= 2) {
     setmaxnreg_dec<kRegsLow>();
     if (elect_one()) {
-      constexpr uint32_t idesc_s = idesc_f16(kM, kN, false), idesc_o = idesc_f16(kM, kD, true);
+      constexpr uint32_t idesc_s = idesc_f16(kM, kHalf, false), idesc_o = idesc_f16(kM, kD, true);
+      const int t = warp - 1;          // query tile
+      // operands: 32 bytes further for each 16 columns of Q and K, 2048 for each 16 keys of V
+      const uint64_t dq = umma_desc_kmajor_sw128(smem_u32(sQ + t * kTile16));
+      const uint64_t dk = umma_desc_kmajor_sw128(smem_u32(sK)), dv = umma_smem_desc(smem_u32(sV), 8192, 1024, 2);
+      constexpr uint32_t kStage = kTile16 >> 4, kHalfTile = kStage / 2;
       uint32_t nk = 0, nv = 0;         // ring positions
-      uint32_t cnt[2] = {0, 0};        // tiles of a group whose P . V was issued
-      uint32_t scnt[2] = {0, 0};       // tiles of a group whose scores were issued
-      uint32_t qcnt[2] = {0, 0};       // items of a group
+      uint32_t cnt = 0;                // tiles of this query tile so far
+      uint32_t qcnt = 0;               // items of this query tile so far
       bool ok = true;
-      for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+      auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+        return mbar_wait(b, parity & 1, a.status, kTimeoutMma, abort_flag);
+      };
+      for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
         const Item it = item_at(a, w);
         if (it.tiles == 0) continue;
-        // scores of the next tile for one group; its K tile is freed behind the last group
-        auto scores = [&](int g) -> bool {
-          const uint32_t st = nk % kRing;
-          if (!mbar_wait(&k_full[st], nk / kRing & 1, a.status, kTimeoutMma, abort_flag)) return false;
-          if (scnt[g] > 0 && !mbar_wait(&s_free[g], (scnt[g] - 1) & 1, a.status, kTimeoutMma, abort_flag)) return false;
-          tc_fence_after();
-          const uint32_t q = smem_u32(sQ + g * kTile16), k = smem_u32(sK + st * kTile16);
+        if (t >= it.groups) {  // no rows: the tiles of K and V are the other issuer's
+          for (int j = 0; ok && j < it.tiles; ++j) {
+            if (!(ok = wait(&k_full[nk % kRing], nk / kRing))) break;
+            mbar_arrive(&k_empty[nk++ % kRing]);
+            if (!(ok = wait(&v_full[nv % kRing], nv / kRing))) break;
+            mbar_arrive(&v_empty[nv++ % kRing]);
+          }
+          continue;
+        }
+        auto scores = [&](int p) {  // of K tile nk, for keys 64 p .. + 63
+          const uint64_t k = dk + nk % kRing * kStage + p * kHalfTile;
 #pragma unroll
           for (int i = 0; i < kD / 16; ++i)
-            umma_bf16_ss(tmem + g * kN, umma_desc_kmajor_sw128(q + i * 32), umma_desc_kmajor_sw128(k + i * 32), idesc_s,
-                         i > 0 ? 1u : 0u);
-          umma_commit(&s_full[g]);
-          ++scnt[g];
-          if (g == it.groups - 1) {
-            umma_commit(&k_empty[st]);
-            ++nk;
-          }
-          return true;
+            umma_bf16_ss(tmem + (2 * t + p) * kHalf, dq + 2 * i, k + 2 * i, idesc_s, i > 0 ? 1u : 0u);
         };
-        for (int g = 0; ok && g < it.groups; ++g) {
-          ok = mbar_wait(&q_full[g], qcnt[g] & 1, a.status, kTimeoutMma, abort_flag) && scores(g);
+        if (!(ok = wait(&q_full[t], qcnt) && wait(&k_full[nk % kRing], nk / kRing))) break;
+        tc_fence_after();
+        for (int p = 0; p < 2; ++p) {
+          scores(p);
+          umma_commit(&s_full[2 * t + p]);
         }
-        for (int j = 0; ok && j < it.tiles; ++j) {
-          for (int g = 0; ok && g < it.groups; ++g) {
-            if (j + 1 < it.tiles && !(ok = scores(g))) break;
-            const uint32_t st = nv % kRing;
-            ok = mbar_wait(&p_full[g], cnt[g] & 1, a.status, kTimeoutMma, abort_flag) &&
-                 mbar_wait(&v_full[st], nv / kRing & 1, a.status, kTimeoutMma, abort_flag);
-            // the accumulator of the group's previous item has been read
-            if (ok && j == 0 && qcnt[g] > 0)
-              ok = mbar_wait(&o_free[g], (qcnt[g] - 1) & 1, a.status, kTimeoutMma, abort_flag);
-            if (!ok) break;
+        umma_commit(&k_empty[nk++ % kRing]);
+        for (int j = 0; ok && j < it.tiles; ++j, ++cnt) {
+          const bool more = j + 1 < it.tiles;
+          // the accumulators of the previous item have been read
+          if (j == 0 && qcnt > 0 && !(ok = wait(&o_free[t], qcnt - 1))) break;
+          if (!(ok = wait(&v_full[nv % kRing], nv / kRing) && (!more || wait(&k_full[nk % kRing], nk / kRing)))) break;
+          for (int p = 0; p < 2; ++p) {
+            const int g = 2 * t + p;
+            if (!(ok = wait(&p_full[g], cnt))) break;
             tc_fence_after();
-            const uint32_t v = smem_u32(sV + st * kTile16);
+            const uint64_t v = dv + nv % kRing * kStage + p * kHalfTile;
 #pragma unroll
-            for (int i = 0; i < kN / 16; ++i)
-              umma_bf16_ts(tmem + kOcol + g * kD, tmem + kPcol + g * (kN / 2) + i * 8,
-                           umma_smem_desc(v + i * 2048, 8192, 1024, 2), idesc_o, (i > 0 || j > 0) ? 1u : 0u);
-            umma_commit(&o_full[g]);
-            ++cnt[g];
-            if (g == it.groups - 1) {
-              umma_commit(&v_empty[st]);
-              ++nv;
-            }
+            for (int i = 0; i < kHalf / 16; ++i)
+              umma_bf16_ts(tmem + kOcol + g * kD, tmem + g * kHalf + i * 8, v + i * 128, idesc_o, (i > 0 || j > 0) ? 1u : 0u);
+            // P V reads the columns that the next scores overwrite: products of one thread run in order
+            if (more) scores(p);
+            umma_commit(&s_full[g]);
           }
+          if (!ok) break;
+          umma_commit(&v_empty[nv++ % kRing]);
+          if (more) umma_commit(&k_empty[nk++ % kRing]);
         }
-        for (int g = 0; g < it.groups; ++g) ++qcnt[g];
+        ++qcnt;
       }
-      umma_commit(done);
-      mbar_wait(done, 0, a.status, kTimeoutMma, nullptr);
+      umma_commit(&done[t]);
+      mbar_wait(&done[t], 0, a.status, kTimeoutMma, nullptr);
     }
   } else if (warp < 4) {
     setmaxnreg_dec<kRegsLow>();
-  } else if (warp >= 12) {
+  } else if (warp < kSoftmaxWarp0) {
     setmaxnreg_dec<kRegsLow>();
     // ------------------------------------------------------------ codes -> fp16 tiles
-    const int tid = threadIdx.x - 12 * 32;
-    const uint32_t units = static_cast<uint32_t>(a.c.stored / 8), inverse = 65536u / units + 1;
-    uint32_t nk = 0, nv = 0;
-    auto widen_tile = [&](const uint8_t* codes, uint8_t* tiles, uint64_t* cfull, uint64_t* cempty, uint64_t* full,
-                          uint64_t* empty, uint32_t& n) -> bool {
-      const uint32_t st = n % kRing, ph = n / kRing & 1;
-      if (!mbar_wait_warp(&cfull[st], ph, a.status, kTimeoutEpilogue, abort_flag)) return false;
-      if (!mbar_wait_warp(&empty[st], ph ^ 1, a.status, kTimeoutEpilogue, abort_flag)) return false;
-      const uint2* src = reinterpret_cast<const uint2*>(codes + st * kTile8);
-      uint8_t* dst = tiles + st * kTile16;
-      // piece i: eight codes of row i / units; eight threads' pieces fill a row of 128 bytes
-#pragma unroll 4
-      for (uint32_t i = tid; i < kN * units; i += kConvertWarps * 32) {
-        const uint32_t row = i * inverse >> 16, c = i - row * units;
-        const uint2 x = src[i];
-        uint4 y;
-        widen<FP8>(biased<FP8>(x.x), y.x, y.y);
-        widen<FP8>(biased<FP8>(x.y), y.z, y.w);
-        *reinterpret_cast<uint4*>(dst + row * 128 + ((c ^ (row & 7)) << 4)) = y;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&cempty[st]);
-        mbar_arrive(&full[st]);
-      }
-      ++n;
-      return true;
-    };
+    // Thread: eight codes (unit c) of rows row0, row0 + 16, ..: fixed steps in both tiles.  The codes
+    // are in registers before the fp16 tile's last reader is waited for.
+    const bool is_v = warp >= 8;
+    const uint32_t units = static_cast<uint32_t>(a.c.stored / 8), tid = threadIdx.x % (kConvertWarps * 32);
+    const uint32_t row0 = tid / units, c = tid - row0 * units;
+    const bool works = row0 < 16;
+    const uint8_t* src = (is_v ? rV : rK) + row0 * a.c.stored + c * 8;
+    uint8_t* dst = (is_v ? sV : sK) + row0 * 128 + ((c ^ (row0 & 7)) << 4);
+    const uint32_t step = 16 * a.c.stored;
+    uint64_t* code_full = is_v ? rv_full : rk_full;
+    uint64_t* code_empty = is_v ? rv_empty : rk_empty;
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
+    uint32_t st = 0, ph = 0;
     bool ok = true;
-    for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+    for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
       const int tiles = item_at(a, w).tiles;
-      if (tiles > 0) ok = widen_tile(rK, sK, rk_full, rk_empty, k_full, k_empty, nk);
-      for (int j = 0; ok && j < tiles; ++j) {
-        if (j + 1 < tiles) ok = widen_tile(rK, sK, rk_full, rk_empty, k_full, k_empty, nk);
-        if (ok) ok = widen_tile(rV, sV, rv_full, rv_empty, v_full, v_empty, nv);
+#pragma unroll 1
+      for (int j = 0; j < tiles; ++j) {
+        if (!(ok = mbar_wait_warp(&code_full[st], ph, a.status, kTimeoutEpilogue, abort_flag))) break;
+        uint2 x[kN / 16];
+        const uint8_t* from = src + st * kTile8;
+        if (works) {
+#pragma unroll
+          for (int e = 0; e < kN / 16; ++e) x[e] = *reinterpret_cast<const uint2*>(from + e * step);
+        }
+        if (!(ok = mbar_wait_warp(&empty[st], ph ^ 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+        uint8_t* to = dst + st * kTile16;
+        if (works) {
+#pragma unroll
+          for (int e = 0; e < kN / 16; ++e) {
+            uint4 y;
+            widen<FP8>(biased<FP8>(x[e].x), y.x, y.y);
+            widen<FP8>(biased<FP8>(x[e].y), y.z, y.w);
+            *reinterpret_cast<uint4*>(to + e * 2048) = y;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          // (only now: with the codes released as soon as their loads were issued, the next copy overtook them)
+          mbar_arrive(&code_empty[st]);
+          mbar_arrive(&full[st]);
+        }
+        if (++st == kRing) st = 0, ph ^= 1;
       }
     }
   } else {
     setmaxnreg_inc<kRegsSoftmax>();
     // ------------------------------------------------------------ softmax
-    const int g = (warp - 4) / 4;
-    const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
-    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + g * kN + lane_off, tP = tmem + kPcol + g * (kN / 2) + lane_off,
-                   tO = tmem + kOcol + g * kD + lane_off;
-    uint8_t* q_row = sQ + g * kTile16 + r * 128;
-    uint32_t cnt = 0;  // tiles of this group so far
+    // Group (query tile qt, half): 64 key columns of every tile; of Q and the result, columns 32 half ..
+    // + 31.  The two warps of the same 32 rows exchange magnitudes of Q and, at the end, (maximum, sum).
+    const int sw = warp - kSoftmaxWarp0, g = sw / 4, qt = g / 2, half = g % 2, quarter = sw % 4;
+    const int r = quarter * 32 + lane;  // row of the tile == TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tS = tmem + g * kHalf + lane_off, tO = tmem + kOcol + g * kD + lane_off,
+                   tO2 = tmem + kOcol + 2 * qt * kD + half * 32 + lane_off;  // this half's columns, both accumulators
+    uint8_t* q_row = sQ + qt * kTile16 + r * 128;
+    uint64_t* bar = &pair[qt * 4 + quarter];
+    uint32_t cnt = 0;  // completions of s_full so far
+    uint32_t xc = 0;   // exchanges so far
     bool ok = true;
-    for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+    auto exchange = [&](float2 x) -> float2 {  // the other half's x for this row (valid if ok)
+      swap[xc & 1][sw][lane] = x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+      ok = mbar_wait_warp(bar, xc & 1, a.status, kTimeoutEpilogue, abort_flag);
+      return swap[xc++ & 1][sw ^ 4][lane];
+    };
+    auto scores_ready = [&]() -> bool {
+      ok = mbar_wait_warp(&s_full[g], cnt++ & 1, a.status, kTimeoutEpilogue, abort_flag);
+      tc_fence_after();
+      return ok;
+    };
+    for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
       const Item it = item_at(a, w);
-      if (g >= it.groups) continue;
-      const int64_t row = it.row0 + g * kM + r;
+      if (qt >= it.groups) continue;
+      const uint32_t row = it.row0 + qt * kM + r;
       const bool there = row < a.rows;
-      const int64_t n = there ? row / a.group : 0;
-      const int head = it.h * a.group + static_cast<int>(there ? row % a.group : 0);
+      const uint32_t n = there ? row / static_cast<uint32_t>(a.group) : 0;
+      const int head = static_cast<int>(it.h * a.group + (there ? row - n * a.group : 0));
       float m = -INFINITY, l = 0.f;
       if (it.tiles > 0) {
-        // ---- the query row as fp16, times a power of two (the group's last scores are done, so
-        // nothing reads its Q any more)
+        // ---- 32 columns of the query row as fp16, times a power of two (the group's last scores are
+        // done, so nothing reads its Q any more)
         float fac;
         {
-          uint32_t x[kD / 2];
-          const uint16_t* src = static_cast<const uint16_t*>(a.q.p) + a.q.offset(it.b, n, head);
+          uint32_t x[16];
+          const uint16_t* src = static_cast<const uint16_t*>(a.q.p) + a.q.offset(it.b, n, head) + half * 32;
+          const int have = there ? a.c.width - half * 32 : 0;
 #pragma unroll
-          for (int i = 0; i < kD / 2; ++i) x[i] = 0;
-          if (there && q_vec) {
+          for (int c = 0; c < 4; ++c) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (q_vec && c * 8 < have) v = __ldg(reinterpret_cast<const uint4*>(src) + c);
+            x[4 * c] = v.x, x[4 * c + 1] = v.y, x[4 * c + 2] = v.z, x[4 * c + 3] = v.w;
+          }
+          if (!q_vec) {
 #pragma unroll
-            for (int c = 0; c < kD / 8; ++c)
-              if (c * 8 < a.c.width) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                x[4 * c] = v.x, x[4 * c + 1] = v.y, x[4 * c + 2] = v.z, x[4 * c + 3] = v.w;
-              }
-          } else if (there) {
-#pragma unroll
-            for (int i = 0; i < kD / 2; ++i) {
-              if (2 * i < a.c.width) x[i] = __ldg(src + 2 * i);
-              if (2 * i + 1 < a.c.width) x[i] |= static_cast<uint32_t>(__ldg(src + 2 * i + 1)) << 16;
+            for (int i = 0; i < 16; ++i) {
+              if (2 * i < have) x[i] = __ldg(src + 2 * i);
+              if (2 * i + 1 < have) x[i] |= static_cast<uint32_t>(__ldg(src + 2 * i + 1)) << 16;
             }
           }
           uint32_t top2 = 0;  // magnitudes order like their bits, infinities and NaN on top
 #pragma unroll
-          for (int i = 0; i < kD / 2; ++i) top2 = __vmaxu2(top2, x[i] & 0x7fff7fffu);
-          const uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
+          for (int i = 0; i < 16; ++i) top2 = __vmaxu2(top2, x[i] & 0x7fff7fffu);
+          uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
+          t16 = max(t16, __float_as_uint(exchange(make_float2(__uint_as_float(t16), 0.f)).x));
+          if (!ok) break;
           const bool bf = a.type == kBF16;
           const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
           float up, down;
           row_scale(top, up, down);
           fac = down * a.scale_log2 * kCodeScale<FP8>;
 #pragma unroll
-          for (int c = 0; c < kD / 8; ++c) {
+          for (int c = 0; c < 4; ++c) {
             uint32_t y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -463,46 +463,48 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
               }
               y[i] = pack_half2(lo * up, hi * up);
             }
-            *reinterpret_cast<uint4*>(q_row + ((c ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(q_row + (((4 * half + c) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[g]);
+          if (lane == 0) mbar_arrive(&q_full[qt]);
         }
         const float* ks = a.c.k_scale + it.bh * a.c.blocks();
         const float* vs = a.c.v_scale + it.bh * a.c.blocks();
-        for (int j = 0; j < it.tiles; ++j, ++cnt) {
-          const int64_t key = it.key0 + static_cast<int64_t>(j) * kN;
-          const int valid = static_cast<int>(min(it.len - key, int64_t{kN}));
-          // lane i holds the scales of keys 32 (i % 4) .. + 31 (a block is 32 keys or more)
-          const int64_t blk = (key + 32 * (lane & 3)) >> a.c.block_log2;
-          const float sk_l = __ldg(ks + blk) , sv_l = safe_scale(__ldg(vs + blk));
-          const float lv_l = log2f(sv_l), inv_l = 1.f / sv_l;
-          if (!(ok = mbar_wait_warp(&s_full[g], cnt & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
-          tc_fence_after();
-          uint32_t s0[32], s1[32], s2[32], s3[32];
+        // scales of the next tile: lane i those of this half's keys 32 (i % 2) .. + 31 (a block is 32 keys or more)
+        const uint32_t key = it.tile0 * kN + kHalf * half + 32 * (lane & 1);
+        float sk = __ldg(ks + (key >> a.c.block_log2)), sv = __ldg(vs + (key >> a.c.block_log2));
+        for (int j = 0; j < it.tiles; ++j) {
+          const int valid = min(it.len - static_cast<int>(it.tile0 + j) * kN, kN) - kHalf * half;
+          float f0, f1, lv0, lv1, inv0, inv1;
+          {
+            const bool none = valid <= 32 * (lane & 1);  // a block behind the last row counts for nothing
+            const float svc = none ? 1.f : safe_scale(sv);
+            const float lv = __log2f(svc), inv = none ? 0.f : __fdividef(1.f, svc);
+            // (never 0: a masked key's -inf stays -inf)
+            f0 = fac * __shfl_sync(0xffffffffu, sk, 0), f1 = fac * __shfl_sync(0xffffffffu, sk, 1);
+            f0 = valid <= 0 ? 1.f : f0 < 1e-38f ? 1e-38f : f0;
+            f1 = valid <= 32 ? 1.f : f1 < 1e-38f ? 1e-38f : f1;
+            lv0 = __shfl_sync(0xffffffffu, lv, 0), lv1 = __shfl_sync(0xffffffffu, lv, 1);
+            inv0 = __shfl_sync(0xffffffffu, inv, 0), inv1 = __shfl_sync(0xffffffffu, inv, 1);
+          }
+          if (j + 1 < it.tiles) {
+            const uint32_t blk = (key + static_cast<uint32_t>(j + 1) * kN) >> a.c.block_log2;
+            sk = __ldg(ks + blk), sv = __ldg(vs + blk);
+          }
+          if (!scores_ready()) break;
+          uint32_t s0[32], s1[32];
           tmem_ld32(tS, s0);
           tmem_ld32(tS + 32, s1);
-          tmem_ld32(tS + 64, s2);
-          tmem_ld32(tS + 96, s3);
           tmem_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[g]);
-          float f[4], lv[4], inv[4];
+          if (valid < kHalf) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            f[c] = fac * __shfl_sync(0xffffffffu, sk_l, c);
-            lv[c] = __shfl_sync(0xffffffffu, lv_l, c);
-            inv[c] = __shfl_sync(0xffffffffu, inv_l, c);
-            if (valid <= 32 * c) inv[c] = 0.f;  // a block behind the last row counts for nothing, whatever its scale
+            for (int i = 0; i < 32; ++i) {
+              if (i >= valid) s0[i] = 0xff800000u;
+              if (32 + i >= valid) s1[i] = 0xff800000u;
+            }
           }
-          float cand = fmaf(max32(s0, valid), f[0], lv[0]);
-          if (valid > 32) cand = fmaxf(cand, fmaf(max32(s1, valid - 32), f[1], lv[1]));
-          if (valid > 64) cand = fmaxf(cand, fmaf(max32(s2, valid - 64), f[2], lv[2]));
-          if (valid > 96) cand = fmaxf(cand, fmaf(max32(s3, valid - 96), f[3], lv[3]));
-          // the group's previous P . V is done: P and O may be written
-          if (cnt > 0 && !(ok = mbar_wait_warp(&o_full[g], (cnt - 1) & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+          const float cand = fmaxf(fmaf(max32(s0), f0, lv0), fmaf(max32(s1), f1, lv1));
           float back = 1.f;
           bool grow = false;
           if (j == 0) {
@@ -512,93 +514,92 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             m = cand;
             grow = true;
           }
-          const float lift = kLift - m;
-          float sum;
-          {
-            uint32_t pk[16];
-            sum = weights32(s0, valid, f[0], lv[0] + lift, pk) * inv[0];
-            tmem_st16(tP, pk);
-            sum = fmaf(weights32(s1, valid - 32, f[1], lv[1] + lift, pk), inv[1], sum);
-            tmem_st16(tP + 16, pk);
-            sum = fmaf(weights32(s2, valid - 64, f[2], lv[2] + lift, pk), inv[2], sum);
-            tmem_st16(tP + 32, pk);
-            sum = fmaf(weights32(s3, valid - 96, f[3], lv[3] + lift, pk), inv[3], sum);
-            tmem_st16(tP + 48, pk);
-          }
+          const float lift = m == -INFINITY ? 0.f : kLift - m;  // (no key of this half is there)
+          float sum = weights32(s0, f0, lv0 + lift, tS) * inv0;
+          sum = fmaf(weights32(s1, f1, lv1 + lift, tS + 16), inv1, sum);
+          l = fmaf(l, back, sum);
+          // (the products before these scores are done: O may be changed)
           if (__any_sync(0xffffffffu, grow)) {
-            tc_fence_after();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              uint32_t o[32];
-              tmem_ld32(tO + half * 32, o);
+            for (int q = 0; q < 4; ++q) {
+              uint32_t o[16];
+              tmem_ld16(tO + q * 16, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * back);
-              tmem_st32(tO + half * 32, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * back);
+              tmem_st16(tO + q * 16, o);
             }
           }
-          l = fmaf(l, back, sum);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[g]);
         }
-        if (!ok) break;
-        if (!(ok = mbar_wait_warp(&o_full[g], (cnt - 1) & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
-        tc_fence_after();
+        if (!ok || !scores_ready()) break;  // the last P V
       }
-      // ---- O (64 columns) to memory
-      uint32_t o0[32], o1[32];
+      // ---- the halves joined: 32 columns of O from both accumulators
+      float o[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o0[i] = o1[i] = 0;
+      for (int i = 0; i < 32; ++i) o[i] = 0.f;
       if (it.tiles > 0) {
-        tmem_ld32(tO, o0);
-        tmem_ld32(tO + 32, o1);
-        tmem_wait_ld();
+        if (!(m < INFINITY)) l = __uint_as_float(0x7fc00000u);  // an infinite score (or a NaN) somewhere
+        const float2 other = exchange(make_float2(m, l));
+        if (!ok) break;
+        const float top = fmaxf(m, other.x);
+        const float f = m == -INFINITY ? 0.f : exp2f(m - top), f2 = other.x == -INFINITY ? 0.f : exp2f(other.x - top);
+        l = l * f + other.y * f2;
+        m = top;
+        const float fa = half ? f2 : f, fb = half ? f : f2;  // of the first and the second half's accumulator
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t x[16], y[16];
+          tmem_ld16(tO2 + 16 * q, x);
+          tmem_ld16(tO2 + kD + 16 * q, y);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[16 * q + i] = __uint_as_float(x[i]) * fa + __uint_as_float(y[i]) * fb;
+        }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[g]);
-        if (!(m < INFINITY)) l = __uint_as_float(0x7fc00000u);  // an infinite score (or a NaN) somewhere
+        if (lane == 0) mbar_arrive(&o_free[qt]);
       }
       if (!there) continue;
       if (a.splits > 1) {
-        const int64_t cell = (it.bh * ((a.rows + kPairRows - 1) / kPairRows) + it.row0 / kPairRows) * a.splits + it.split;
-        const int64_t pr = cell * kPairRows + g * kM + r;
-        a.part_ml[pr] = make_float2(m, l);
+        const int64_t pairs = (static_cast<uint32_t>(a.rows) + kPairRows - 1) / kPairRows;
+        const int64_t cell = (it.bh * pairs + it.pair) * a.splits + it.split;
+        const int64_t pr = cell * kPairRows + qt * kM + r;
+        if (half == 0) a.part_ml[pr] = make_float2(m, l);
         if (it.tiles > 0) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kMaxWidth);
+          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kMaxWidth + half * 32);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            dst[i] = make_float4(__uint_as_float(o0[4 * i]), __uint_as_float(o0[4 * i + 1]), __uint_as_float(o0[4 * i + 2]),
-                                 __uint_as_float(o0[4 * i + 3]));
-            dst[8 + i] = make_float4(__uint_as_float(o1[4 * i]), __uint_as_float(o1[4 * i + 1]),
-                                     __uint_as_float(o1[4 * i + 2]), __uint_as_float(o1[4 * i + 3]));
-          }
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
         continue;
       }
       const float norm = l != 0.f ? kCodeScale<FP8> / l : 0.f;
-      uint16_t* dst = static_cast<uint16_t*>(a.o.p) + a.o.offset(it.b, n, head);
-      uint32_t y[kD / 2];
+      uint16_t* dst = static_cast<uint16_t*>(a.o.p) + a.o.offset(it.b, n, head) + half * 32;
+      const int have = a.c.width - half * 32;
+      uint32_t y[16];
 #pragma unroll
-      for (int i = 0; i < kD / 2; ++i) {
-        const float lo = __uint_as_float(i < 16 ? o0[2 * i] : o1[2 * i - 32]) * norm;
-        const float hi = __uint_as_float(i < 16 ? o0[2 * i + 1] : o1[2 * i - 31]) * norm;
+      for (int i = 0; i < 16; ++i) {
+        const float lo = o[2 * i] * norm, hi = o[2 * i + 1] * norm;
         y[i] = a.type == kBF16 ? pack_bf16x2(lo, hi) : pack_half2(lo, hi);
       }
       if (o_vec) {
 #pragma unroll
-        for (int c = 0; c < kD / 8; ++c)
-          if (c * 8 < a.c.width)
+        for (int c = 0; c < 4; ++c)
+          if (c * 8 < have)
             reinterpret_cast<uint4*>(dst)[c] = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
       } else {
 #pragma unroll
-        for (int i = 0; i < kD / 2; ++i) {
-          if (2 * i < a.c.width) dst[2 * i] = static_cast<uint16_t>(y[i]);
-          if (2 * i + 1 < a.c.width) dst[2 * i + 1] = static_cast<uint16_t>(y[i] >> 16);
+        for (int i = 0; i < 16; ++i) {
+          if (2 * i < have) dst[2 * i] = static_cast<uint16_t>(y[i]);
+          if (2 * i + 1 < have) dst[2 * i + 1] = static_cast<uint16_t>(y[i] >> 16);
         }
       }
-      if (a.lse != nullptr)
+      if (a.lse != nullptr && half == 0)
         a.lse[(static_cast<int64_t>(it.b) * a.c.heads * a.group + head) * a.n + n] = row_lse(m, l);
     }
   }
@@ -618,11 +619,13 @@ bool vectors(const Rows& r, int width) {
 
 template <bool FP8>
 cudaError_t tc_typed(const Attention& a, int ctas, cudaStream_t stream) {
+  if (a.rows > INT32_MAX - kPairRows) return cudaErrorInvalidConfiguration;
   const int64_t items = (a.rows + kPairRows - 1) / kPairRows * a.splits * a.c.batch * a.c.heads;
+  if (items > INT32_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   tc_kernel<FP8><<<static_cast<unsigned>(items < ctas ? items : ctas), kThreads, kSmem, stream>>>(
-      a, items, vectors(a.q, a.c.width), vectors(a.o, a.c.width));
+      a, static_cast<uint32_t>(items), vectors(a.q, a.c.width), vectors(a.o, a.c.width));
   return cudaGetLastError();
 }
 

@@ -117,9 +117,9 @@ __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
   down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 }
 
-// log2 of a V scale and its inverse: a block that was never written has scale 0 and holds zeros,
-// which any small scale says as well.
-__device__ __forceinline__ float safe_scale(float s) { return s < 7.9e-31f ? 7.9e-31f : s; }
+// A V scale whose log2 and inverse are finite: a block that was never written has scale 0 and holds
+// zeros, which the smallest scale of a written block says as well.
+__device__ __forceinline__ float safe_scale(float s) { return s == 0.f ? 7.9e-15f : s; }
 
 // The natural log-sum-exp of a row from its maximum and its sum (which carries kLift).
 __device__ __forceinline__ float row_lse(float m, float l) {

@@ -228,6 +228,18 @@ def test_same_inputs_same_bits(n):
     assert all(torch.equal(ops.block_cache_attention(q, cache, 3000), first) for _ in range(5))
 
 
+@pytest.mark.parametrize("n", [1, 257])
+def test_new_contents_in_every_call(n):
+    """Nothing of an earlier call is left to hide a read that comes too early: other data each time."""
+    for seed in range(12):
+        from synthefy_nori_b200 import ops
+
+        cache, g = make(2, 8, 640, 64, seed=seed, spread=False)
+        q = (2 * torch.randn(2, n, 8, 64, device="cuda", generator=g)).to(torch.float16)
+        for _ in range(3):
+            check(q, cache, [640] * 2, ops.block_cache_attention(q, cache, 640))
+
+
 @pytest.mark.parametrize("n", [1, 200])
 def test_captured_with_appends(n):
     """Append and attend in one graph, replayed as the cache grows; another graph shares nothing with it."""
