@@ -6,10 +6,13 @@
 // of 32 keys, each with a running maximum, sum and output of its own; warps are joined in shared
 // memory, ranges through a workspace by a second kernel.
 //
-// The rows are the M side of m16n8k16 products.  The order of the summed index is free as long as
-// both operands agree, so lanes take whole 8-byte units: in q . k lane (g, t) holds units t and
-// t + 4 of key g; in w . v it holds unit g of four keys, and column c of product j is value
-// 8 c + j.  Loads are 8 bytes, widened to fp16 in registers; nothing goes through shared memory.
+// Keys (of K) and values (of V, transposed) are the M side of m16n8k16 products, the query rows N, 8 or
+// 16 of them.  The order of a summed index is free as long as both operands agree, so lanes take whole
+// 8-byte units: in k . q lane (g, t) holds units t and t + 4 of keys g and g + 8; in v . w it holds unit g
+// of four keys, and rows g, g + 8 of product j are values 8 g + 2 j and 8 g + 2 j + 1.  Weights go from the
+// one product's result to the other's operand by 8 x 8 transposes.  Each warp keeps pieces of 32 keys in
+// flight (contiguous bulk copies into a ring of its own; no warp waits for another), reads them in
+// 8-byte units and widens them to fp16 in registers.
 //
 // Scales cost nothing per value.  With c = scale log2(e) s_k and t = c (q . k) + log2 s_v for the
 // block of a key (one block per piece, since blocks are of 32 rows or more),
@@ -19,6 +22,7 @@
 //
 // Reference counterpart: attention over a quantised context cache (model/layer.py:747-934).
 #include "block_cache.cuh"
+#include "sm100.cuh"
 
 namespace nori {
 namespace bc {
@@ -26,6 +30,8 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 32;  // keys of one step of a warp
+constexpr int kStages = 2;  // pieces of a warp in flight
+constexpr int kPieceBytes = kPiece * kMaxWidth;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -52,13 +58,21 @@ __device__ __forceinline__ void put(void* p, int64_t i, float x, int type) {
   else
     static_cast<__half*>(p)[i] = __float2half_rn(x);
 }
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// over the lanes that hold the same rows (t)
+__device__ __forceinline__ float keys_max(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+__device__ __forceinline__ float keys_sum(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile of 16-bit values
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 struct Row {  // where row r of a K/V head's query rows lies
@@ -68,11 +82,11 @@ struct Row {  // where row r of a K/V head's query rows lies
       : n(r / a.group), head(kv_head * a.group + static_cast<int>(r % a.group)) {}
 };
 
-// TWO: rows g + 8 exist as well.  UNITS: 4 or 8 units of 8 columns.
-template <bool FP8, bool TWO, int UNITS>
-__global__ void __launch_bounds__(kThreads) few_kernel(Attention a) {
-  constexpr int kHalf = UNITS / 4;   // units of a lane in q . k
-  constexpr int kRows = TWO ? 16 : 8;
+// NT: tiles of 8 query rows.  UNITS: 4 or 8 units of 8 columns.
+template <bool FP8, int NT, int UNITS>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attention a) {
+  constexpr int kHalf = UNITS / 4;   // units of a lane in k . q
+  constexpr int kRows = 8 * NT;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int64_t tiles = (a.rows + kRows - 1) / kRows;
   int64_t unit = blockIdx.x;
@@ -89,13 +103,44 @@ __global__ void __launch_bounds__(kThreads) few_kernel(Attention a) {
   const int64_t pieces = (len + kPiece - 1) / kPiece, each = (pieces + a.splits - 1) / a.splits;
   const int64_t p0 = split * each, p1 = min(p0 + each, pieces);
 
-  // query rows g and g + 8: a power of two brings them into fp16's range, exactly
-  uint32_t qf[2 * kHalf][4];
-  float fac[2];
+  const uint8_t* kbase = a.c.k + bh * a.c.cap * a.c.stored;
+  const uint8_t* vbase = a.c.v + bh * a.c.cap * a.c.stored;
+  const float* ks = a.c.k_scale + bh * a.c.blocks();
+  const float* vs = a.c.v_scale + bh * a.c.blocks();
+  const uint32_t koff = g * a.c.stored + t * 8, voff = 2 * t * a.c.stored + g * 8;
+  const uint32_t bytes = kPiece * a.c.stored;
+  const bool kthere[2] = {t < units, t + 4 < units};
+  const bool vthere = g < units;
+
+  // this warp's ring of pieces (K, then V): contiguous copies that lane 0 asks for kStages ahead
+  extern __shared__ __align__(128) uint8_t ring_all[];
+  __shared__ uint64_t bars[kWarps][kStages];
+  uint8_t* ring = ring_all + warp * (kStages * 2 * kPieceBytes);
+  const int64_t first = p0 + warp;
+  const int mine = static_cast<int>(first < p1 ? (p1 - first + kWarps - 1) / kWarps : 0);  // this warp's pieces
+  auto ask = [&](int i) {
+    uint64_t* bar = &bars[warp][i % kStages];
+    uint8_t* dst = ring + i % kStages * (2 * kPieceBytes);
+    const int64_t at = (first + static_cast<int64_t>(i) * kWarps) * bytes;
+    mbar_arrive_expect_tx(bar, 2 * bytes);
+    bulk_load(dst, kbase + at, bytes, bar);
+    bulk_load(dst + kPieceBytes, vbase + at, bytes, bar);
+  };
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&bars[warp][i], 1);
+    fence_barrier_init();
+    for (int i = 0; i < min(mine, kStages); ++i) ask(i);
+  }
+  __syncwarp();
+
+  // the query rows as operand B (lane: row g, its units) while the first pieces arrive; a power of two
+  // brings each into fp16's range, exactly; fac[nt][i]: of row 8 nt + 2 t + i
+  uint32_t qf[NT][2 * kHalf][2];
+  float fac[NT][2];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int64_t r = row0 + g + 8 * half;
-    const bool there = r < a.rows && (TWO || half == 0);
+  for (int nt = 0; nt < NT; ++nt) {
+    const int64_t r = row0 + 8 * nt + g;
+    const bool there = r < a.rows;
     float x[kHalf][8], top = 0.f;
     bool bad = false;
     const Row row(a, h, there ? r : 0);
@@ -109,156 +154,185 @@ __global__ void __launch_bounds__(kThreads) few_kernel(Attention a) {
         top = fmaxf(top, fabsf(x[i][e]));
         bad |= x[i][e] != x[i][e];
       }
-    top = quad_max(bad ? INFINITY : top);
+    if (bad) top = INFINITY;
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     float up, down;
     row_scale(top, up, down);
-    fac[half] = down * a.scale_log2 * kCodeScale<FP8>;
+    down *= a.scale_log2 * kCodeScale<FP8>;
+    fac[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);      // lane (2 t, 0)
+    fac[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);  // lane (2 t + 1, 0)
 #pragma unroll
     for (int i = 0; i < kHalf; ++i)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        qf[2 * i + s][half] = pack_half2(x[i][4 * s] * up, x[i][4 * s + 1] * up);
-        qf[2 * i + s][2 + half] = pack_half2(x[i][4 * s + 2] * up, x[i][4 * s + 3] * up);
+        qf[nt][2 * i + s][0] = pack_half2(x[i][4 * s] * up, x[i][4 * s + 1] * up);
+        qf[nt][2 * i + s][1] = pack_half2(x[i][4 * s + 2] * up, x[i][4 * s + 3] * up);
       }
   }
 
-  float o[8][4];
+  float o[NT][4][4];  // [row tile][product j]: (value 8 g + 2 j, row 2 t), (.., 2 t + 1), (value + 1, 2 t), ..
+  float m[NT][2], l[NT][2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-  const uint8_t* kbase = a.c.k + bh * a.c.cap * a.c.stored;
-  const uint8_t* vbase = a.c.v + bh * a.c.cap * a.c.stored;
-  const float* ks = a.c.k_scale + bh * a.c.blocks();
-  const float* vs = a.c.v_scale + bh * a.c.blocks();
-  const int koff = g * a.c.stored + t * 8, voff = 2 * t * a.c.stored + g * 8;
-  const bool kthere[2] = {t < units, t + 4 < units};
-  const bool vthere = g < units;
-
-  uint2 kq[4][kHalf], vq[2][4];
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+  }
   float sk = 0.f, sv = 0.f;
-  auto load = [&](int64_t p) {
-    const uint8_t* kp = kbase + p * kPiece * a.c.stored + koff;
-    const uint8_t* vp = vbase + p * kPiece * a.c.stored + voff;
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-      for (int i = 0; i < kHalf; ++i)
-        kq[nt][i] = kthere[i] ? __ldg(reinterpret_cast<const uint2*>(kp + nt * 8 * a.c.stored + i * 32)) : make_uint2(0, 0);
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vq[kt][e] = vthere ? __ldg(reinterpret_cast<const uint2*>(vp + (kt * 16 + (e >> 1) * 8 + (e & 1)) * a.c.stored))
-                           : make_uint2(0, 0);
+  auto scales = [&](int64_t p) {
     const int64_t blk = p * kPiece >> a.c.block_log2;
     sk = __ldg(ks + blk);
     sv = __ldg(vs + blk);
   };
+  if (mine > 0) scales(first);
 
-  for (int64_t p = p0 + warp; p < p1; p += kWarps) {
-    load(p);
-    // scores: 4 tiles of 8 keys
-    float s[4][4];
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < kHalf; ++i) {
-        uint32_t b0, b1;
-        widen<FP8>(biased<FP8>(kq[nt][i].x), b0, b1);
-        mma16816(s[nt], qf[2 * i], b0, b1);
-        widen<FP8>(biased<FP8>(kq[nt][i].y), b0, b1);
-        mma16816(s[nt], qf[2 * i + 1], b0, b1);
-      }
+  for (int i = 0; i < mine; ++i) {
+    const int64_t p = first + static_cast<int64_t>(i) * kWarps;
+    const float sk_now = sk, svc = safe_scale(sv);
+    if (i + 1 < mine) scales(p + kWarps);
+    if (!mbar_wait_warp(&bars[warp][i % kStages], i / kStages & 1, a.status, kTimeoutEpilogue, nullptr)) {
+      if (lane == 0)  // own copies in flight
+        for (int k = i; k < min(mine, i + kStages); ++k)
+          mbar_wait(&bars[warp][k % kStages], k / kStages & 1, a.status, kTimeoutEpilogue, nullptr);
+      break;
     }
-    const float svc = safe_scale(sv);
-    const float lv = log2f(svc), inv = 1.f / svc;
+    const uint8_t* kp = ring + i % kStages * (2 * kPieceBytes) + koff;
+    const uint8_t* vp = ring + i % kStages * (2 * kPieceBytes) + kPieceBytes + voff;
+    uint2 kq[4][kHalf], vq[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j)
+        kq[nt][j] = kthere[j] ? *reinterpret_cast<const uint2*>(kp + nt * 8 * a.c.stored + j * 32) : make_uint2(0, 0);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vq[kt][e] = vthere ? *reinterpret_cast<const uint2*>(vp + (kt * 16 + (e >> 1) * 8 + (e & 1)) * a.c.stored)
+                           : make_uint2(0, 0);
+    // scores of keys 16 kt + g (values 0, 1) and + 8 (2, 3), rows 2 t and 2 t + 1
+    float s[NT][2][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][kt][e] = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j) {
+        uint32_t af[4];
+        widen<FP8>(biased<FP8>(kq[2 * kt][j].x), af[0], af[2]);
+        widen<FP8>(biased<FP8>(kq[2 * kt + 1][j].x), af[1], af[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][kt], af, qf[nt][2 * j][0], qf[nt][2 * j][1]);
+        widen<FP8>(biased<FP8>(kq[2 * kt][j].y), af[0], af[2]);
+        widen<FP8>(biased<FP8>(kq[2 * kt + 1][j].y), af[1], af[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][kt], af, qf[nt][2 * j + 1][0], qf[nt][2 * j + 1][1]);
+      }
+    const float lv = __log2f(svc), inv = __fdividef(1.f, svc);
     const int left = static_cast<int>(min(len - p * kPiece, int64_t{kPiece}));  // keys of the piece that are there
     if (left < kPiece) {
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (nt * 8 + 2 * t + (i & 1) >= left) s[nt][i] = -INFINITY;
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * kt + 8 * (e >> 1) + g >= left) s[nt][kt][e] = -INFINITY;
     }
-    float shift[2], back[2];
+    // the maximum moves only where a score is more than 2^kLazy above it: rarely, and only then do the
+    // lanes of a row exchange theirs
+    float cand[NT][2];
     bool grow = false;
 #pragma unroll
-    for (int half = 0; half < (TWO ? 2 : 1); ++half) {
-      float mx = -INFINITY;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
-      mx = quad_max(mx);
-      const float cand = fmaf(mx, fac[half] * sk, lv);
-      back[half] = 1.f;
-      if (cand > m[half] + kLazy || m[half] == -INFINITY) {
-        back[half] = m[half] == -INFINITY ? 0.f : exp2_fast(m[half] - cand);
-        m[half] = cand;
-        grow = true;
+      for (int i2 = 0; i2 < 2; ++i2) {
+        const float mx = fmaxf(fmaxf(s[nt][0][i2], s[nt][0][2 + i2]), fmaxf(s[nt][1][i2], s[nt][1][2 + i2]));
+        cand[nt][i2] = fmaf(mx, fac[nt][i2] * sk_now, lv);
+        grow |= !(cand[nt][i2] <= m[nt][i2] + kLazy);  // (also the first piece, and a NaN)
       }
-      shift[half] = lv - m[half] + kLift;
-    }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        o[j][0] *= back[0], o[j][1] *= back[0];
-        if (TWO) o[j][2] *= back[1], o[j][3] *= back[1];
-      }
-      l[0] *= back[0];
-      if (TWO) l[1] *= back[1];
-    }
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int half = 0; half < (TWO ? 2 : 1); ++half) {
-      const float c = fac[half] * sk;
-      float sum = 0.f;
+        for (int i2 = 0; i2 < 2; ++i2) {
+          const float all = keys_max(cand[nt][i2]);
+          if (all > m[nt][i2] + kLazy || m[nt][i2] == -INFINITY) {
+            const float back = m[nt][i2] == -INFINITY ? 0.f : exp2_fast(m[nt][i2] - all);
+            m[nt][i2] = all;
+            l[nt][i2] *= back;
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float& x = s[nt][2 * half + i];
-          // (a masked key's -inf stays 0 whatever the scale)
-          x = left < kPiece && nt * 8 + 2 * t + i >= left ? 0.f : exp2_fast(fmaf(x, c, shift[half]));
-          sum += x;
+            for (int j = 0; j < 4; ++j) o[nt][j][i2] *= back, o[nt][j][2 + i2] *= back;
+          }
         }
-      l[half] = fmaf(sum, inv, l[half]);
+    }
+    uint32_t pf[NT][4];  // weights as operand B: [keys 8 i ..]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i2 = e & 1;
+          float& x = s[nt][kt][e];
+          x = exp2_fast(fmaf(x, fac[nt][i2] * sk_now, lv - m[nt][i2] + kLift));
+          // (a masked key's weight is 0 whatever the scale)
+          if (left < kPiece && 16 * kt + 8 * (e >> 1) + g >= left) x = 0.f;
+          sum[i2] += x;
+        }
+        pf[nt][2 * kt] = transposed(pack_half2(s[nt][kt][0], s[nt][kt][1]));
+        pf[nt][2 * kt + 1] = transposed(pack_half2(s[nt][kt][2], s[nt][kt][3]));
+      }
+      l[nt][0] = fmaf(sum[0], inv, l[nt][0]);
+      l[nt][1] = fmaf(sum[1], inv, l[nt][1]);
     }
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const uint32_t af[4] = {pack_half2(s[2 * kt][0], s[2 * kt][1]), TWO ? pack_half2(s[2 * kt][2], s[2 * kt][3]) : 0u,
-                              pack_half2(s[2 * kt + 1][0], s[2 * kt + 1][1]),
-                              TWO ? pack_half2(s[2 * kt + 1][2], s[2 * kt + 1][3]) : 0u};
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const uint32_t x0 = biased<FP8>(w ? vq[kt][0].y : vq[kt][0].x), x1 = biased<FP8>(w ? vq[kt][1].y : vq[kt][1].x);
         const uint32_t x2 = biased<FP8>(w ? vq[kt][2].y : vq[kt][2].x), x3 = biased<FP8>(w ? vq[kt][3].y : vq[kt][3].x);
-        uint32_t b0[4], b1[4];  // columns 4w .. 4w + 3: (key, next key)
-        widen<FP8>(__byte_perm(x0, x1, 0x5140), b0[0], b0[1]);
-        widen<FP8>(__byte_perm(x0, x1, 0x7362), b0[2], b0[3]);
-        widen<FP8>(__byte_perm(x2, x3, 0x5140), b1[0], b1[1]);
-        widen<FP8>(__byte_perm(x2, x3, 0x7362), b1[2], b1[3]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma16816(o[4 * w + j], af, b0[j], b1[j]);
+        for (int u = 0; u < 2; ++u) {  // values 4 w + 2 u and + 1 of unit g: (key, next key)
+          uint32_t af[4];
+          widen<FP8>(__byte_perm(x0, x1, u ? 0x7362 : 0x5140), af[0], af[1]);
+          widen<FP8>(__byte_perm(x2, x3, u ? 0x7362 : 0x5140), af[2], af[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * w + u], af, pf[nt][2 * kt], pf[nt][2 * kt + 1]);
+        }
       }
-    }
+    // the codes have been used by every lane: their place may be filled again
+    __syncwarp();
+    if (lane == 0 && i + kStages < mine) ask(i + kStages);
   }
 
   // join the warps
   __shared__ float sm_m[kWarps][16], sm_l[kWarps][16];
-  __shared__ float sm_o[kWarps][kRows][kMaxWidth + 4];
+  auto sm_o = reinterpret_cast<float(*)[kRows][kMaxWidth + 4]>(ring_all);  // (in place of the rings)
+  static_assert(sizeof(float) * kWarps * kRows * (kMaxWidth + 4) <= kWarps * kStages * 2 * kPieceBytes);
+  __syncthreads();
 #pragma unroll
-  for (int half = 0; half < (TWO ? 2 : 1); ++half) {
-    l[half] = quad_sum(l[half]);
-    const int r = g + 8 * half;
-    if (t == 0) sm_m[warp][r] = m[half], sm_l[warp][r] = l[half];
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      const int r = 8 * nt + 2 * t + i;
+      const float sum = keys_sum(l[nt][i]);
+      if (g == 0) sm_m[warp][r] = m[nt][i], sm_l[warp][r] = sum;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sm_o[warp][r][8 * (2 * t + i) + j] = o[j][2 * half + i];
-  }
+      for (int j = 0; j < 4; ++j) {
+        sm_o[warp][r][8 * g + 2 * j] = o[nt][j][i];
+        sm_o[warp][r][8 * g + 2 * j + 1] = o[nt][j][2 + i];
+      }
+    }
   __syncthreads();
   const int64_t cell = (bh * tiles + tile) * a.splits + split;
   for (int i = threadIdx.x; i < kRows * kMaxWidth; i += kThreads) {
@@ -326,12 +400,16 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
     a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(top, sum);
 }
 
-template <bool FP8, bool TWO, int UNITS>
+template <bool FP8, int NT, int UNITS>
 cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
-  constexpr int kRows = TWO ? 16 : 8;
+  constexpr int kRows = 8 * NT;
   const int64_t grid = (a.rows + kRows - 1) / kRows * a.splits * a.c.batch * a.c.heads;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-  few_kernel<FP8, TWO, UNITS><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a);
+  constexpr int kSmem = kWarps * kStages * 2 * kPieceBytes;
+  const cudaError_t e =
+      cudaFuncSetAttribute(few_kernel<FP8, NT, UNITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  few_kernel<FP8, NT, UNITS><<<static_cast<unsigned>(grid), kThreads, kSmem, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -342,11 +420,11 @@ int few_tile_rows(int64_t rows) { return rows > 8 ? 16 : 8; }
 cudaError_t launch_few(const Attention& a, cudaStream_t stream) {
   const bool two = few_tile_rows(a.rows) == 16, wide = a.c.stored > 32;
   if (a.c.fp8) {
-    if (wide) return two ? few_typed<true, true, 8>(a, stream) : few_typed<true, false, 8>(a, stream);
-    return two ? few_typed<true, true, 4>(a, stream) : few_typed<true, false, 4>(a, stream);
+    if (wide) return two ? few_typed<true, 2, 8>(a, stream) : few_typed<true, 1, 8>(a, stream);
+    return two ? few_typed<true, 2, 4>(a, stream) : few_typed<true, 1, 4>(a, stream);
   }
-  if (wide) return two ? few_typed<false, true, 8>(a, stream) : few_typed<false, false, 8>(a, stream);
-  return two ? few_typed<false, true, 4>(a, stream) : few_typed<false, false, 4>(a, stream);
+  if (wide) return two ? few_typed<false, 2, 8>(a, stream) : few_typed<false, 1, 8>(a, stream);
+  return two ? few_typed<false, 2, 4>(a, stream) : few_typed<false, 1, 4>(a, stream);
 }
 
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream) {

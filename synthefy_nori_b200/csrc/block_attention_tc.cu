@@ -55,13 +55,6 @@ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {  // fp16 A and B, 
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // ------------------------------------------------------------------ 2^x
 __device__ __forceinline__ float exp2_mufu(float x) {
   float y;

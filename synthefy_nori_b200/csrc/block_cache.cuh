@@ -80,6 +80,14 @@ template <bool FP8>
 constexpr float kCodeScale = FP8 ? 256.f : 1.f;
 
 #ifdef __CUDACC__
+// A contiguous piece (16-byte aligned, a multiple of 16 bytes) to shared memory; arrives on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(bytes), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
+               : "memory");
+}
+
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
