@@ -173,10 +173,10 @@ void block_cache_write(const torch::Tensor& ck, const torch::Tensor& cv, const t
 std::vector<torch::Tensor> block_cache_read(const torch::Tensor& ck, const torch::Tensor& cv, const torch::Tensor& cks,
                                             const torch::Tensor& cvs, int64_t width, int64_t start, int64_t n,
                                             c10::ScalarType out_type);
-torch::Tensor block_cache_attention(const torch::Tensor& q, const torch::Tensor& ck, const torch::Tensor& cv,
-                                    const torch::Tensor& cks, const torch::Tensor& cvs, int64_t width, int64_t length_all,
-                                    const c10::optional<torch::Tensor>& length_dev, double scale, const torch::Tensor& o,
-                                    bool want_lse, const torch::Tensor& status);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> block_cache_attention(
+    const torch::Tensor& q, const torch::Tensor& ck, const torch::Tensor& cv, const torch::Tensor& cks,
+    const torch::Tensor& cvs, int64_t width, int64_t length_all, const c10::optional<torch::Tensor>& length_dev,
+    double scale, const c10::optional<torch::Tensor>& out, bool want_lse, const torch::Tensor& status);
 }  // namespace nori
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

@@ -4,7 +4,8 @@
 // Bound: every stored byte is read once, 2 W bytes a key, for up to 16 rows.  So the work is split
 // over the keys: a CTA takes a range of one (sequence, K/V head), its four warps every fourth piece
 // of 32 keys, each with a running maximum, sum and output of its own; warps are joined in shared
-// memory, ranges through a workspace by a second kernel.
+// memory, up to eight ranges in their cluster's, and only more than eight through a workspace by a
+// second kernel.
 //
 // Keys (of K) and values (of V, transposed) are the M side of m16n8k16 products, the query rows N, 8 or
 // 16 of them.  The order of a summed index is free as long as both operands agree, so lanes take whole
@@ -21,6 +22,8 @@
 // Sums, maxima and outputs are fp32; w is rounded to fp16 (11 bits) for the product alone.
 //
 // Reference counterpart: attention over a quantised context cache (model/layer.py:747-934).
+#include <cooperative_groups.h>
+
 #include "block_cache.cuh"
 #include "sm100.cuh"
 
@@ -31,6 +34,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kPiece = 32;  // keys of one step of a warp
 constexpr int kStages = 2;  // pieces of a warp in flight
+constexpr int resident(int row_tiles) { return row_tiles == 1 ? 5 : 4; }  // CTAs of an SM (registers)
 constexpr int kPieceBytes = kPiece * kMaxWidth;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -48,9 +52,9 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float to_float(const void* p, int64_t i, int type) {
-  if (type == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
+__device__ __forceinline__ float2 to_float2(uint32_t x, int type) {
+  if (type == kBF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 __device__ __forceinline__ void put(void* p, int64_t i, float x, int type) {
   if (type == kBF16)
@@ -82,35 +86,39 @@ struct Row {  // where row r of a K/V head's query rows lies
       : n(r / a.group), head(kv_head * a.group + static_cast<int>(r % a.group)) {}
 };
 
-// NT: tiles of 8 query rows.  UNITS: 4 or 8 units of 8 columns.
-template <bool FP8, int NT, int UNITS>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attention a) {
-  constexpr int kHalf = UNITS / 4;   // units of a lane in k . q
+// NT: tiles of 8 query rows.  W: bytes of a stored row (with it known at compile time every load has a
+// fixed offset: 171 us for 253 at 168 x 50,000 x 56).  Lanes whose unit lies past the row read what
+// follows it in the ring: q is 0 there, and no result is taken from there (e4m3's NaN is cleared first).
+// Which key of eight stands at place i of a product: lanes t of V's operand then read rows of both
+// parities, which for rows of 64 bytes are different banks.
+__device__ __forceinline__ constexpr int key_at(int i) { return (i & 4) | (i & 1) << 1 | (i >> 1 & 1); }
+
+template <bool FP8, int NT, int W>
+__global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a, bool q_vec) {
+  constexpr int kHalf = W > 32 ? 2 : 1;  // units of a lane in k . q: t and t + 4, or 2 t and 2 t + 1 in one load
+  constexpr bool kPairs = kHalf == 2 && W % 16 == 0;
   constexpr int kRows = 8 * NT;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  const auto unit_of = [&](int i) { return kPairs ? 2 * t + i : t + 4 * i; };
   const int64_t tiles = (a.rows + kRows - 1) / kRows;
-  int64_t unit = blockIdx.x;
-  const int64_t tile = unit % tiles;
-  unit /= tiles;
-  const int split = static_cast<int>(unit % a.splits);
-  const int64_t bh = unit / a.splits;
+  const int split = static_cast<int>(blockIdx.x % a.splits);
+  const int64_t cell = blockIdx.x / a.splits;
+  const int64_t tile = cell % tiles, bh = cell / tiles;
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
   const int64_t row0 = tile * kRows;
-  const int units = a.c.stored / 8;
 
+  asm volatile("griddepcontrol.launch_dependents;");  // (the join of parts may be set up now)
   // this CTA's keys: whole pieces, the same number for every split
   const int64_t len = min(max(a.length.at(b), int64_t{0}), a.c.cap);
   const int64_t pieces = (len + kPiece - 1) / kPiece, each = (pieces + a.splits - 1) / a.splits;
   const int64_t p0 = split * each, p1 = min(p0 + each, pieces);
 
-  const uint8_t* kbase = a.c.k + bh * a.c.cap * a.c.stored;
-  const uint8_t* vbase = a.c.v + bh * a.c.cap * a.c.stored;
+  const uint8_t* kbase = a.c.k + bh * a.c.cap * W;
+  const uint8_t* vbase = a.c.v + bh * a.c.cap * W;
   const float* ks = a.c.k_scale + bh * a.c.blocks();
   const float* vs = a.c.v_scale + bh * a.c.blocks();
-  const uint32_t koff = g * a.c.stored + t * 8, voff = 2 * t * a.c.stored + g * 8;
-  const uint32_t bytes = kPiece * a.c.stored;
-  const bool kthere[2] = {t < units, t + 4 < units};
-  const bool vthere = g < units;
+  constexpr uint32_t bytes = kPiece * W;
+  static_assert((kPiece - 1) * W + kMaxWidth <= kPieceBytes);
 
   // this warp's ring of pieces (K, then V): contiguous copies that lane 0 asks for kStages ahead
   extern __shared__ __align__(128) uint8_t ring_all[];
@@ -146,20 +154,34 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
     const Row row(a, h, there ? r : 0);
     const int64_t at = a.q.offset(b, row.n, row.head);
 #pragma unroll
-    for (int i = 0; i < kHalf; ++i)
+    for (int i = 0; i < kHalf; ++i) {
+      const int d = 8 * unit_of(i);
+      uint32_t w[4] = {0, 0, 0, 0};
+      const uint16_t* src = static_cast<const uint16_t*>(a.q.p) + at + d;
+      if (q_vec) {
+        if (there && d < a.c.width) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+          w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        }
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = 8 * (t + 4 * i) + e;
-        x[i][e] = there && d < a.c.width ? to_float(a.q.p, at + d, a.type) : 0.f;
-        top = fmaxf(top, fabsf(x[i][e]));
-        bad |= x[i][e] != x[i][e];
+        for (int e = 0; e < 8; ++e)
+          if (there && d + e < a.c.width) w[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = to_float2(w[e], a.type);
+        x[i][2 * e] = f.x, x[i][2 * e + 1] = f.y;
+        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        bad |= f.x != f.x || f.y != f.y;
+      }
+    }
     if (bad) top = INFINITY;
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     float up, down;
     row_scale(top, up, down);
-    down *= a.scale_log2 * kCodeScale<FP8>;
+    down *= a.scale_log2;
     fac[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);      // lane (2 t, 0)
     fac[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);  // lane (2 t + 1, 0)
 #pragma unroll
@@ -200,20 +222,39 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
           mbar_wait(&bars[warp][k % kStages], k / kStages & 1, a.status, kTimeoutEpilogue, nullptr);
       break;
     }
-    const uint8_t* kp = ring + i % kStages * (2 * kPieceBytes) + koff;
-    const uint8_t* vp = ring + i % kStages * (2 * kPieceBytes) + kPieceBytes + voff;
+    const uint8_t* kp = ring + i % kStages * (2 * kPieceBytes) + key_at(g) * W + unit_of(0) * 8;
+    const uint8_t* vp = ring + i % kStages * (2 * kPieceBytes) + kPieceBytes + key_at(2 * t) * W + g * 8;
     uint2 kq[4][kHalf], vq[2][4];
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt)
+    for (int nt = 0; nt < 4; ++nt) {
+      if constexpr (kPairs) {
+        const uint4 x = *reinterpret_cast<const uint4*>(kp + nt * 8 * W);
+        kq[nt][0] = make_uint2(x.x, x.y), kq[nt][1] = make_uint2(x.z, x.w);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kHalf; ++j)
-        kq[nt][j] = kthere[j] ? *reinterpret_cast<const uint2*>(kp + nt * 8 * a.c.stored + j * 32) : make_uint2(0, 0);
+        for (int j = 0; j < kHalf; ++j) kq[nt][j] = *reinterpret_cast<const uint2*>(kp + nt * 8 * W + j * 32);
+      }
+      if constexpr (FP8 && W % 32 != 0) {
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) {
+          const uint32_t in_row = unit_of(j) < W / 8 ? 0xffffffffu : 0u;
+          kq[nt][j].x &= in_row, kq[nt][j].y &= in_row;
+        }
+      }
+    }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vq[kt][e] = vthere ? *reinterpret_cast<const uint2*>(vp + (kt * 16 + (e >> 1) * 8 + (e & 1)) * a.c.stored)
-                           : make_uint2(0, 0);
+      for (int e = 0; e < 4; ++e)  // (key_at(2 t + 1) = key_at(2 t) + 2)
+        vq[kt][e] = *reinterpret_cast<const uint2*>(vp + (kt * 16 + (e >> 1) * 8 + (e & 1) * 2) * W);
+    const int left = static_cast<int>(min(len - p * kPiece, int64_t{kPiece}));  // keys of the piece that are there
+    if (FP8 && left < kPiece) {  // codes behind the last row may be NaN (0 x NaN is none of its business)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (kt * 16 + (e >> 1) * 8 + (e & 1) * 2 + key_at(2 * t) >= left) vq[kt][e] = make_uint2(0, 0);
+    }
     // scores of keys 16 kt + g (values 0, 1) and + 8 (2, 3), rows 2 t and 2 t + 1
     float s[NT][2][4];
 #pragma unroll
@@ -237,7 +278,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
         for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][kt], af, qf[nt][2 * j + 1][0], qf[nt][2 * j + 1][1]);
       }
     const float lv = __log2f(svc), inv = __fdividef(1.f, svc);
-    const int left = static_cast<int>(min(len - p * kPiece, int64_t{kPiece}));  // keys of the piece that are there
     if (left < kPiece) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -245,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (16 * kt + 8 * (e >> 1) + g >= left) s[nt][kt][e] = -INFINITY;
+            if (16 * kt + 8 * (e >> 1) + key_at(g) >= left) s[nt][kt][e] = -INFINITY;
     }
     // the maximum moves only where a score is more than 2^kLazy above it: rarely, and only then do the
     // lanes of a row exchange theirs
@@ -286,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
           float& x = s[nt][kt][e];
           x = exp2_fast(fmaf(x, fac[nt][i2] * sk_now, lv - m[nt][i2] + kLift));
           // (a masked key's weight is 0 whatever the scale)
-          if (left < kPiece && 16 * kt + 8 * (e >> 1) + g >= left) x = 0.f;
+          if (left < kPiece && 16 * kt + 8 * (e >> 1) + key_at(g) >= left) x = 0.f;
           sum[i2] += x;
         }
         pf[nt][2 * kt] = transposed(pack_half2(s[nt][kt][0], s[nt][kt][1]));
@@ -334,10 +374,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
       }
     }
   __syncthreads();
-  const int64_t cell = (bh * tiles + tile) * a.splits + split;
-  for (int i = threadIdx.x; i < kRows * kMaxWidth; i += kThreads) {
+  const int64_t left_rows = a.rows - row0;
+  const int rows = static_cast<int>(left_rows < kRows ? left_rows : kRows);
+  __shared__ float2 fin_ml[kRows];
+  float* fin_o = reinterpret_cast<float*>(ring_all) + kWarps * kRows * (kMaxWidth + 4);
+  static_assert(sizeof(float) * kRows * (kWarps * (kMaxWidth + 4) + kMaxWidth) <= kWarps * kStages * 2 * kPieceBytes);
+  // where value d of row r goes: the result, or a part of it
+  auto put_row = [&](int r, int d, float top, float sum, float acc) {
+    if (a.splits > a.cluster) {
+      const int64_t at = (cell * (a.splits / a.cluster) + split / a.cluster) * kRows + r;
+      a.part_o[at * kMaxWidth + d] = acc;
+      if (d == 0) a.part_ml[at] = make_float2(top, sum);
+      return;
+    }
+    const Row row(a, h, row0 + r);
+    if (d < a.c.width) put(a.o.p, a.o.offset(b, row.n, row.head) + d, sum != 0.f ? acc / sum : 0.f, a.type);
+    if (d == 0 && a.lse != nullptr)
+      a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(top, sum);
+  };
+  for (int i = threadIdx.x; i < rows * kMaxWidth; i += kThreads) {
     const int r = i / kMaxWidth, d = i % kMaxWidth;
-    if (row0 + r >= a.rows) break;
     float top = sm_m[0][r];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
@@ -348,90 +404,157 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 5 : 4) few_kernel(Attentio
       sum = fmaf(sm_l[w][r], f, sum);
       acc = fmaf(sm_o[w][r][d], f, acc);
     }
-    if (a.splits > 1) {
-      a.part_o[(cell * kRows + r) * kMaxWidth + d] = acc;
-      if (d == 0) a.part_ml[cell * kRows + r] = make_float2(top, sum);
-      continue;
+    if (a.cluster == 1) {
+      put_row(r, d, top, sum, acc);
+    } else {
+      fin_o[r * kMaxWidth + d] = acc;
+      if (d == 0) fin_ml[r] = make_float2(top, sum);
     }
-    const Row row(a, h, row0 + r);
-    if (d < a.c.width) put(a.o.p, a.o.offset(b, row.n, row.head) + d, sum != 0.f ? acc * kCodeScale<FP8> / sum : 0.f, a.type);
-    if (d == 0 && a.lse != nullptr)
-      a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(top, sum);
   }
+  if (a.cluster == 1) return;
+  // join the cluster: every CTA has written its part; the threads of all share the values
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = static_cast<int>(cluster.block_rank()) * kThreads + threadIdx.x; i < rows * kMaxWidth;
+       i += a.cluster * kThreads) {
+    const int r = i / kMaxWidth, d = i % kMaxWidth;
+    float2 ml[8];
+    float v[8], top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < a.cluster) {
+        ml[c] = cluster.map_shared_rank(fin_ml, c)[r];
+        v[c] = cluster.map_shared_rank(fin_o, c)[i];
+        top = fmaxf(top, ml[c].x);
+      }
+    float sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < a.cluster) {
+        const float f = ml[c].x == -INFINITY && ml[c].y == 0.f ? 0.f : exp2f(ml[c].x - top);
+        sum = fmaf(ml[c].y, f, sum);
+        acc = fmaf(v[c], f, acc);
+      }
+    put_row(r, d, top, sum, acc);
+  }
+  cluster.sync();  // nobody leaves while its shared memory is read
 }
 
-// One CTA joins the splits of one row: each warp a run of them, then the warps.
-constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, float code_scale) {
-  const int64_t r = blockIdx.x % a.rows, bh = blockIdx.x / a.rows;
-  const int64_t tiles = (a.rows + tile_rows - 1) / tile_rows;
-  const int64_t cell0 = (bh * tiles + r / tile_rows) * a.splits;
-  const int tr = static_cast<int>(r % tile_rows);
+// Joins the parts of a row.  Few parts: a warp takes a row, two values a lane; many: a CTA takes a row,
+// each warp a run of its parts.  Started while the kernel before it still runs (its last CTAs leave the
+// launch's latency free), it waits for it before the first read.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+template <bool MANY>
+__global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, int parts) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int64_t unit = MANY ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
+  if (unit >= a.rows * a.c.batch * a.c.heads) return;  // (whole warps; whole CTAs where MANY)
+  const int64_t r = unit % a.rows, bh = unit / a.rows;
+  const int64_t tiles = (a.rows + tile_rows - 1) / tile_rows;
+  const int64_t at = (bh * tiles + r / tile_rows) * parts * tile_rows + r % tile_rows;  // of part 0
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_ml[(cell0 + s) * tile_rows + tr].x);
+  for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.part_ml[at + static_cast<int64_t>(s) * tile_rows].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float sum = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int s = warp; s < a.splits; s += kJoinThreads / 32) {
-    const float2 ml = a.part_ml[(cell0 + s) * tile_rows + tr];
+#pragma unroll 4
+  for (int s = MANY ? warp : 0; s < parts; s += MANY ? kJoinWarps : 1) {
+    const int64_t i = at + static_cast<int64_t>(s) * tile_rows;
+    const float2 ml = a.part_ml[i];
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no keys there (and perhaps no values written)
     const float f = exp2f(ml.x - top);
-    const float2 v = *reinterpret_cast<const float2*>(a.part_o + ((cell0 + s) * tile_rows + tr) * kMaxWidth + 2 * lane);
+    const float2 v = reinterpret_cast<const float2*>(a.part_o + i * kMaxWidth)[lane];
     sum = fmaf(ml.y, f, sum);
     a0 = fmaf(v.x, f, a0);
     a1 = fmaf(v.y, f, a1);
   }
-  __shared__ float sm[kJoinThreads / 32][kMaxWidth + 1];
-  sm[warp][2 * lane] = a0;
-  sm[warp][2 * lane + 1] = a1;
-  if (lane == 0) sm[warp][kMaxWidth] = sum;
-  __syncthreads();
-  if (threadIdx.x >= kMaxWidth) return;
-  const int d = threadIdx.x;
-  float acc = 0.f;
-  sum = 0.f;
+  if constexpr (MANY) {
+    __shared__ float sm[kJoinWarps][kMaxWidth + 1];
+    sm[warp][2 * lane] = a0;
+    sm[warp][2 * lane + 1] = a1;
+    if (lane == 0) sm[warp][kMaxWidth] = sum;
+    __syncthreads();
+    if (warp > 0) return;
+    a0 = a1 = sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) acc += sm[w][d], sum += sm[w][kMaxWidth];
+    for (int w = 0; w < kJoinWarps; ++w) a0 += sm[w][2 * lane], a1 += sm[w][2 * lane + 1], sum += sm[w][kMaxWidth];
+  }
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
   const Row row(a, h, r);
-  if (d < a.c.width) put(a.o.p, a.o.offset(b, row.n, row.head) + d, sum != 0.f ? acc * code_scale / sum : 0.f, a.type);
-  if (d == 0 && a.lse != nullptr)
+  const float norm = sum != 0.f ? 1.f / sum : 0.f;
+  const int64_t out = a.o.offset(b, row.n, row.head) + 2 * lane;
+  if (2 * lane < a.c.width) put(a.o.p, out, a0 * norm, a.type);
+  if (2 * lane + 1 < a.c.width) put(a.o.p, out + 1, a1 * norm, a.type);
+  if (lane == 0 && a.lse != nullptr)
     a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(top, sum);
 }
 
-template <bool FP8, int NT, int UNITS>
+template <bool FP8, int NT, int W>
 cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
   constexpr int kRows = 8 * NT;
   const int64_t grid = (a.rows + kRows - 1) / kRows * a.splits * a.c.batch * a.c.heads;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
   constexpr int kSmem = kWarps * kStages * 2 * kPieceBytes;
   const cudaError_t e =
-      cudaFuncSetAttribute(few_kernel<FP8, NT, UNITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      cudaFuncSetAttribute(few_kernel<FP8, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  few_kernel<FP8, NT, UNITS><<<static_cast<unsigned>(grid), kThreads, kSmem, stream>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(a.cluster);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, few_kernel<FP8, NT, W>, a, vectors(a.q, a.c.width));
 }
 
 }  // namespace
 
 int few_tile_rows(int64_t rows) { return rows > 8 ? 16 : 8; }
+int few_resident(int64_t rows) { return resident(few_tile_rows(rows) / 8); }
 
 cudaError_t launch_few(const Attention& a, cudaStream_t stream) {
-  const bool two = few_tile_rows(a.rows) == 16, wide = a.c.stored > 32;
-  if (a.c.fp8) {
-    if (wide) return two ? few_typed<true, 2, 8>(a, stream) : few_typed<true, 1, 8>(a, stream);
-    return two ? few_typed<true, 2, 4>(a, stream) : few_typed<true, 1, 4>(a, stream);
+  const bool two = few_tile_rows(a.rows) == 16;
+  auto go = [&](auto w) {
+    constexpr int W = w.value;
+    if (a.c.fp8) return two ? few_typed<true, 2, W>(a, stream) : few_typed<true, 1, W>(a, stream);
+    return two ? few_typed<false, 2, W>(a, stream) : few_typed<false, 1, W>(a, stream);
+  };
+  switch (a.c.stored) {
+    case 8: return go(std::integral_constant<int, 8>());
+    case 16: return go(std::integral_constant<int, 16>());
+    case 24: return go(std::integral_constant<int, 24>());
+    case 32: return go(std::integral_constant<int, 32>());
+    case 40: return go(std::integral_constant<int, 40>());
+    case 48: return go(std::integral_constant<int, 48>());
+    case 56: return go(std::integral_constant<int, 56>());
+    case 64: return go(std::integral_constant<int, 64>());
   }
-  if (wide) return two ? few_typed<false, 2, 8>(a, stream) : few_typed<false, 1, 8>(a, stream);
-  return two ? few_typed<false, 2, 4>(a, stream) : few_typed<false, 1, 4>(a, stream);
+  return cudaErrorInvalidValue;
 }
 
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream) {
-  const int64_t grid = a.rows * a.c.batch * a.c.heads;
+  const int parts = a.splits / a.cluster;
+  const bool many = parts > 32;
+  const int64_t rows = a.rows * a.c.batch * a.c.heads, grid = many ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-  combine_kernel<<<static_cast<unsigned>(grid), kJoinThreads, 0, stream>>>(a, tile_rows, a.c.fp8 ? kCodeScale<true> : kCodeScale<false>);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return many ? cudaLaunchKernelEx(&cfg, combine_kernel<true>, a, tile_rows, parts)
+              : cudaLaunchKernelEx(&cfg, combine_kernel<false>, a, tile_rows, parts);
 }
 
 }  // namespace bc

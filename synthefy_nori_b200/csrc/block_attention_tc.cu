@@ -160,7 +160,8 @@ __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
 }
 
 template <bool FP8>
-__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool q_vec,
+__global__ void __launch_bounds__(kThreads, 1)
+    tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool q_vec,
                                                          bool o_vec) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (*reinterpret_cast<volatile int*>(a.status) != 0) return;  // another CTA or kernel timed out
 
+  asm volatile("griddepcontrol.launch_dependents;");  // (the join of parts may be set up now)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&rk_full[i], 1);
@@ -343,7 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     uint32_t st = 0, ph = 0;
     bool ok = true;
     for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
-      const int tiles = item_at(a, w).tiles;
+      const Item it = item_at(a, w);
+      const int tiles = it.tiles;
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         if (!(ok = mbar_wait_warp(&code_full[st], ph, a.status, kTimeoutEpilogue, abort_flag))) break;
@@ -361,6 +364,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             uint4 y;
             widen<FP8>(biased<FP8>(x[e].x), y.x, y.y);
             widen<FP8>(biased<FP8>(x[e].y), y.z, y.w);
+            // codes behind the last row may be NaN (0 x NaN is none of its business)
+            if (FP8 && is_v && static_cast<int>((it.tile0 + j) * kN + row0 + 16 * e) >= it.len) y = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(to + e * 2048) = y;
           }
         }
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
           const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
           float up, down;
           row_scale(top, up, down);
-          fac = down * a.scale_log2 * kCodeScale<FP8>;
+          fac = down * a.scale_log2;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t y[4];
@@ -571,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         }
         continue;
       }
-      const float norm = l != 0.f ? kCodeScale<FP8> / l : 0.f;
+      const float norm = l != 0.f ? 1.f / l : 0.f;
       uint16_t* dst = static_cast<uint16_t*>(a.o.p) + a.o.offset(it.b, n, head) + half * 32;
       const int have = a.c.width - half * 32;
       uint32_t y[16];
@@ -603,11 +608,6 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
-}
-
-bool vectors(const Rows& r, int width) {
-  return width % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.s0 % 8 == 0 && r.s1 % 8 == 0 && r.sn % 8 == 0 &&
-         r.sh % 8 == 0;
 }
 
 template <bool FP8>

@@ -46,6 +46,12 @@ struct Rows {
   }
 };
 
+// Whether 16-bit rows can be read and written 16 bytes at a time.
+inline bool vectors(const Rows& r, int width) {
+  return width % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.s0 % 8 == 0 && r.s1 % 8 == 0 && r.sn % 8 == 0 &&
+         r.sh % 8 == 0;
+}
+
 // One value for all sequences or one of each, on the device.
 struct PerSequence {
   const int* dev;
@@ -64,8 +70,9 @@ struct Attention {
   float scale_log2; // softmax scale * log2(e)
   float* lse;       // [batch, query heads, n] or null
   int splits;       // of the key range
-  float* part_o;    // [units, splits, tile rows, 64], unnormalised
-  float2* part_ml;  // [units, splits, tile rows] (maximum, sum)
+  int cluster;      // splits that are joined on the way (kernel for few rows), a divisor of splits
+  float* part_o;    // [cells, parts, tile rows, 64], unnormalised; parts = splits / cluster
+  float2* part_ml;  // [cells, parts, tile rows] (maximum, sum)
   int* status;
 };
 
@@ -73,11 +80,6 @@ struct Attention {
 // maximum that lags by up to kLazy (no rescale of the sums) stays below fp16's largest value.
 constexpr float kLift = 11.f;
 constexpr float kLazy = 4.f;
-
-// e4m3 codes widen to fp16 by their bits alone, as value * 2^-8 (exponent biases 15 and 7; the
-// subnormals of both formats are linear, so they agree too).
-template <bool FP8>
-constexpr float kCodeScale = FP8 ? 256.f : 1.f;
 
 #ifdef __CUDACC__
 // A contiguous piece (16-byte aligned, a multiple of 16 bytes) to shared memory; arrives on `bar`.
@@ -94,13 +96,15 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
 }
 
 // Four codes (bytes of x, int8 ones biased by 128) -> two fp16 pairs, exact.
-// int8: 0x64uu is the fp16 1024 + u, minus 1152.  e4m3: sign eeee mmm -> sign 0eeee mmm0000000.
+// int8: 0x64uu is the fp16 1024 + u, minus 1152.  e4m3: the conversion instruction (the same by shifts
+// and masks is three times as many instructions: 220 for 180 us a row x 168 x 50,000).
 template <bool FP8>
 __device__ __forceinline__ void widen(uint32_t x, uint32_t& lo, uint32_t& hi) {
   if (FP8) {
-    const uint32_t a = __byte_perm(x, 0, 0x1404), b = __byte_perm(x, 0, 0x3424);
-    lo = ((a >> 1) & 0x3f803f80u) | (a & 0x80008000u);
-    hi = ((b >> 1) & 0x3f803f80u) | (b & 0x80008000u);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(x));
   } else {
     lo = hsub2(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
     hi = hsub2(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
@@ -140,6 +144,7 @@ cudaError_t launch_write(const View& c, const Rows& k, const Rows& v, int type, 
 cudaError_t launch_read(const View& c, void* k, void* v, int type, int64_t start, int64_t n, cudaStream_t stream);
 // rows of a tile of the two attention kernels, and how many splits of the keys they would take
 int few_tile_rows(int64_t rows);
+int few_resident(int64_t rows);  // CTAs that an SM holds
 cudaError_t launch_few(const Attention& a, cudaStream_t stream);
 // rows of a tile pair of the kernel for many rows; one CTA per SM
 constexpr int kPairRows = 256;

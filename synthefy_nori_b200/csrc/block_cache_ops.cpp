@@ -102,8 +102,19 @@ int sm_count(int dev) { return at::cuda::getDeviceProperties(dev)->multiProcesso
 // Up to this many rows of one K/V head run on the kernel that streams the cache through registers.
 constexpr int64_t kFewRows = 16;
 
-int few_splits(int64_t cells, int64_t longest, int sms) {
-  return static_cast<int>(std::clamp<int64_t>(4 * sms / cells, 1, std::max<int64_t>((longest + 255) / 256, 1)));
+// Splits of the keys of each cell for few rows, joined in clusters of up to 8.  A CTA's time goes with its
+// keys and a start and end worth some 400 more (measured), whatever else its SM runs, up to the 5 or
+// 4 CTAs that an SM holds: so the fewest waves of the shortest CTAs, each of 256 keys or more.
+int few_splits(int64_t cells, int64_t longest, int resident) {
+  const int64_t most = std::max<int64_t>((longest + 255) / 256, 1);
+  if (cells * 8 <= resident && most > 8) return static_cast<int>(std::min(resident / cells, most) / 8 * 8);
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int64_t s = 1; s <= std::min<int64_t>(most, 8); ++s) {
+    const int64_t cost = (cells * s + resident - 1) / resident * ((longest + s - 1) / s + 400);
+    if (cost < least) least = cost, best = static_cast<int>(s);
+  }
+  return best;
 }
 
 // Splits of the keys for the persistent kernel: the waves of items, each as long as its key tiles
@@ -159,10 +170,11 @@ std::vector<Tensor> block_cache_read(const Tensor& ck, const Tensor& cv, const T
   return out;
 }
 
-// Returns the log-sum-exp [batch, heads, n] (empty where it is not wanted); o is written.
-Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs,
-                             int64_t width, int64_t length_all, const OptTensor& length_dev, double scale, const Tensor& o,
-                             bool want_lse, const Tensor& status) {
+// (result, log-sum-exp [batch, heads, n] or an undefined tensor)
+std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv, const Tensor& cks,
+                                                    const Tensor& cvs, int64_t width, int64_t length_all,
+                                                    const OptTensor& length_dev, double scale, const OptTensor& out,
+                                                    bool want_lse, const Tensor& status) {
   const char* who = "block_cache_attention";
   bc::Attention a{};
   a.c = view_of(ck, cv, cks, cvs, width, who);
@@ -173,6 +185,9 @@ Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv
               a.c.heads, " K/V heads evenly");
   a.type = float_type(q, false, who, "q");
   a.q = rows_of(q, a.c, a.n, heads, ck.device(), who, "q");
+  const at::cuda::CUDAGuard guard(ck.device());
+  const bool given = out.has_value() && out->defined();
+  const Tensor o = given ? *out : torch::empty(q.sizes(), q.options());
   TORCH_CHECK(o.scalar_type() == q.scalar_type() && o.sizes() == q.sizes(), who, ": out of q's shape and type expected");
   a.o = rows_of(o, a.c, a.n, heads, ck.device(), who, "out");
   a.length = per_sequence(length_dev, length_all, a.c, ck.device(), who, "lengths");
@@ -180,10 +195,10 @@ Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv
     TORCH_CHECK(length_all >= 0 && length_all <= a.c.cap, who, ": length ", length_all, " of a cache of ", a.c.cap);
   TORCH_CHECK(scale > 0.0 && scale < 1e30, who, ": a positive finite scale expected");
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  const at::cuda::CUDAGuard guard(ck.device());
-  Tensor lse = torch::empty({want_lse ? a.c.batch : 0, heads, a.n}, ck.options().dtype(at::kFloat));
-  if (q.numel() == 0) return lse;
-  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  OptTensor lse;
+  if (want_lse) lse = torch::empty({a.c.batch, heads, a.n}, cks.options());
+  if (q.numel() == 0) return {o, lse};
+  a.lse = want_lse ? lse->data_ptr<float>() : nullptr;
   a.group = static_cast<int>(heads / a.c.heads);
   a.rows = a.n * a.group;
   a.status = status.data_ptr<int>();
@@ -193,18 +208,20 @@ Tensor block_cache_attention(const Tensor& q, const Tensor& ck, const Tensor& cv
   const bool few = a.rows <= kFewRows;
   const int tile = few ? bc::few_tile_rows(a.rows) : bc::kPairRows;
   const int64_t cells = (a.rows + tile - 1) / tile * a.c.batch * a.c.heads;
-  a.splits = few ? few_splits(cells, longest, sms) : tc_splits(cells, longest, persistent_sms(sms));
+  a.splits = few ? few_splits(cells, longest, sms * bc::few_resident(a.rows)) : tc_splits(cells, longest, persistent_sms(sms));
+  a.cluster = few ? std::min(a.splits, 8) : 1;
+  const int parts = a.splits / a.cluster;
   Tensor part_o, part_ml;
-  if (a.splits > 1) {
-    part_o = torch::empty({cells * a.splits * tile * bc::kMaxWidth}, lse.options());
-    part_ml = torch::empty({cells * a.splits * tile * 2}, lse.options());
+  if (parts > 1) {
+    part_o = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
+    part_ml = torch::empty({cells * parts * tile * 2}, cks.options());
     a.part_o = part_o.data_ptr<float>();
     a.part_ml = reinterpret_cast<float2*>(part_ml.data_ptr<float>());
   }
   const auto stream = at::cuda::getCurrentCUDAStream();
   C10_CUDA_CHECK(few ? bc::launch_few(a, stream) : bc::launch_tc(a, persistent_sms(sms), stream));
-  if (a.splits > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
-  return lse;
+  if (parts > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
+  return {o, lse};
 }
 
 }  // namespace nori

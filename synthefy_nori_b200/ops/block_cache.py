@@ -15,7 +15,6 @@ operation has a gradient: results have no graph.
 
 from __future__ import annotations
 
-import math
 from typing import NamedTuple
 
 import torch
@@ -123,20 +122,17 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     ``scale`` (default head_dim ** -0.5) is positive.  ``out``, if given, has q's shape and type and shares
     no memory with q or the cache.  With ``return_lse`` also the natural log-sum-exp, fp32 [batch, heads, n].
     Length 0 gives zeros and -inf; a query row with an infinity or a NaN gives NaN."""
-    who = "block_cache_attention"
-    _cuda(cache.k, who, "the cache")
-    _cuda(q, who, "q")
-    given = out is not None
-    if given:
-        _cuda(out, who, "out")
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-            raise ValueError(f"{who}: out must have q's shape, type and device")
-    else:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    length, length_dev = _int_or_tensor(lengths)
-    scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
-    lse = _lib().block_cache_attention(q, *cache[:4], cache.head_dim, length, length_dev, scale, out, bool(return_lse),
-                                       status_word(q.device))
-    if given:
+    k = cache.k
+    if not k.is_cuda or not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("block_cache_attention: q and the cache must be CUDA tensors")
+    if out is not None and not (isinstance(out, torch.Tensor) and out.shape == q.shape and out.dtype == q.dtype
+                                and out.device == q.device):
+        raise ValueError("block_cache_attention: out must have q's shape, type and device")
+    length, length_dev = (0, lengths) if isinstance(lengths, torch.Tensor) else (int(lengths), None)
+    res, lse = _lib().block_cache_attention(q, k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, length, length_dev,
+                                            cache.head_dim ** -0.5 if scale is None else scale, out, return_lse,
+                                            status_word(k.device))
+    if out is not None:
         torch.autograd.graph.increment_version(out)
-    return (out, lse) if return_lse else out
+        res = out
+    return (res, lse) if return_lse else res

@@ -115,16 +115,19 @@ def test_length_zero(n):
     assert not o.any() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("d", [8, 20, 32, 40, 44, 56, 64])
 @pytest.mark.parametrize("n", [1, 20, 260])
-def test_rows_behind_the_length_do_not_count(n):
-    """Whatever codes and scales lie behind the last row (infinities and NaN among the scales)."""
+def test_rows_behind_the_length_do_not_count(n, d):
+    """Whatever codes and scales lie behind the last row (NaN codes, infinities and NaN among the scales)."""
     from synthefy_nori_b200 import ops
 
-    cache, g = make(2, 2, 512, 40, torch.float8_e4m3fn, 32)
-    q = torch.randn(2, n, 2, 40, device="cuda", generator=g).to(torch.bfloat16)
+    cache, g = make(2, 2, 512, d, torch.float8_e4m3fn, 32)
+    q = torch.randn(2, n, 2, d, device="cuda", generator=g).to(torch.bfloat16)
     want = ops.block_cache_attention(q, cache, 161)
     for t in cache[:2]:
-        t.view(torch.int8)[:, :, 161:] = torch.randint(-128, 128, (2, 2, t.shape[2] - 161, 40), device="cuda").to(torch.int8)
+        behind = t.view(torch.int8)[:, :, 161:]
+        behind.copy_(torch.randint(-128, 128, behind.shape, device="cuda"))
+        behind[:, :, :3] = 127  # e4m3's NaN
     for t in cache[2:4]:
         t[:, :, 6:] = torch.tensor([math.nan, math.inf], device="cuda").repeat(5)
     assert torch.equal(ops.block_cache_attention(q, cache, 161), want)
