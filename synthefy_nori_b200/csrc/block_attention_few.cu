@@ -100,12 +100,12 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
   constexpr int kRows = 8 * NT;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const auto unit_of = [&](int i) { return kPairs ? 2 * t + i : t + 4 * i; };
-  const int64_t tiles = (a.rows + kRows - 1) / kRows;
+  const int64_t tiles = (a.rows - a.first + kRows - 1) / kRows;
   const int split = static_cast<int>(blockIdx.x % a.splits);
   const int64_t cell = blockIdx.x / a.splits;
   const int64_t tile = cell % tiles, bh = cell / tiles;
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
-  const int64_t row0 = tile * kRows;
+  const int64_t row0 = a.first + tile * kRows;
 
   asm volatile("griddepcontrol.launch_dependents;");  // (the join of parts may be set up now)
   // this CTA's keys: whole pieces, the same number for every split
@@ -450,9 +450,10 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t unit = MANY ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
-  if (unit >= a.rows * a.c.batch * a.c.heads) return;  // (whole warps; whole CTAs where MANY)
-  const int64_t r = unit % a.rows, bh = unit / a.rows;
-  const int64_t tiles = (a.rows + tile_rows - 1) / tile_rows;
+  const int64_t count = a.rows - a.first;
+  if (unit >= count * a.c.batch * a.c.heads) return;  // (whole warps; whole CTAs where MANY)
+  const int64_t r = unit % count, bh = unit / count;
+  const int64_t tiles = (count + tile_rows - 1) / tile_rows;
   const int64_t at = (bh * tiles + r / tile_rows) * parts * tile_rows + r % tile_rows;  // of part 0
   float top = -INFINITY;
   for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.part_ml[at + static_cast<int64_t>(s) * tile_rows].x);
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
     for (int w = 0; w < kJoinWarps; ++w) a0 += sm[w][2 * lane], a1 += sm[w][2 * lane + 1], sum += sm[w][kMaxWidth];
   }
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
-  const Row row(a, h, r);
+  const Row row(a, h, a.first + r);
   const float norm = sum != 0.f ? 1.f / sum : 0.f;
   const int64_t out = a.o.offset(b, row.n, row.head) + 2 * lane;
   if (2 * lane < a.c.width) put(a.o.p, out, a0 * norm, a.type);
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
 template <bool FP8, int NT, int W>
 cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
   constexpr int kRows = 8 * NT;
-  const int64_t grid = (a.rows + kRows - 1) / kRows * a.splits * a.c.batch * a.c.heads;
+  const int64_t grid = (a.rows - a.first + kRows - 1) / kRows * a.splits * a.c.batch * a.c.heads;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
   constexpr int kSmem = kWarps * kStages * 2 * kPieceBytes;
   const cudaError_t e =
@@ -520,7 +521,7 @@ int few_tile_rows(int64_t rows) { return rows > 8 ? 16 : 8; }
 int few_resident(int64_t rows) { return resident(few_tile_rows(rows) / 8); }
 
 cudaError_t launch_few(const Attention& a, cudaStream_t stream) {
-  const bool two = few_tile_rows(a.rows) == 16;
+  const bool two = few_tile_rows(a.rows - a.first) == 16;
   auto go = [&](auto w) {
     constexpr int W = w.value;
     if (a.c.fp8) return two ? few_typed<true, 2, W>(a, stream) : few_typed<true, 1, W>(a, stream);
@@ -542,7 +543,7 @@ cudaError_t launch_few(const Attention& a, cudaStream_t stream) {
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream) {
   const int parts = a.splits / a.cluster;
   const bool many = parts > 32;
-  const int64_t rows = a.rows * a.c.batch * a.c.heads, grid = many ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
+  const int64_t rows = (a.rows - a.first) * a.c.batch * a.c.heads, grid = many ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));

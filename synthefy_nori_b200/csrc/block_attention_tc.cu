@@ -3,8 +3,10 @@
 //
 // Persistent, one CTA of 28 warps per SM; a work item is 256 query rows (two tiles of 128) against a
 // range of the keys of one (sequence, K/V head).  Roles:
-//   warp 0        copies the codes of 128-key tiles of K and V, each one contiguous piece of the
-//                 cache, into two rings (untiled bulk copies: no stride rules, so any width);
+//   warp 0        takes the next work item (a CTA not yet started is cancelled and its item taken over,
+//                 so sequences of different lengths even out) and tells the others; copies the
+//                 codes of 128-key tiles of K and V, each one contiguous piece of the cache, into
+//                 two rings (untiled bulk copies: no stride rules, so any width);
 //   warps 4..7    widen the codes of K to fp16, exactly, into the swizzled tiles that the products
 //   warps 8..11   read, and those of V: once for 256 query rows;
 //   warps 1, 2    issue the products of one query tile each: S = Q K^T (128 x 64 x 64) and O += P V;
@@ -15,6 +17,9 @@
 // arithmetic, so four of them share an SM: with one thread for all 128 columns of a row and two
 // groups the same arithmetic took 1.3 times as long, with row maxima exchanged between the
 // halves 1.2 times.  The two halves of a query tile are joined once per item.
+//
+// A small kernel before writes the query rows as the fp16 tiles that the products read, so that they
+// are one contiguous copy each (the softmax warps did it at 3 us an item, in which nothing else ran).
 //
 // Scales cost nothing per value: with c = scale log2(e) s_k 2^-e (2^e brings the query row into
 // fp16's range, exactly) and t = c (q . k) + log2 s_v,
@@ -41,13 +46,15 @@ constexpr int kThreads = 896;
 constexpr int kRing = 3;                 // stages of each ring (codes and fp16 tiles, K and V)
 constexpr int kTile16 = kN * kD * 2;     // bytes of an fp16 tile of 128 x 64 (Q, K or V)
 constexpr int kTile8 = kN * kD;          // room for a tile of codes
-constexpr int kSmem = kTile16 * (2 + 2 * kRing) + kTile8 * 2 * kRing + 512 + 1024;
+constexpr int kSmem = kTile16 * (4 + 2 * kRing) + kTile8 * 2 * kRing + 1024 + 1024;
+constexpr int kItems = 4;                // items that are known ahead
+constexpr int kConsumers = 2 + 8 + 16;   // of an item: issuers, converter and softmax warps
 constexpr int kHalf = kN / 2;            // keys of a group's tile
 // S 0..255 (64 a group, P over its first 32), O 256..511 (64 a group)
 constexpr uint32_t kTmemCols = 512, kOcol = 256;
 constexpr int kConvertWarps = 4, kSoftmaxWarp0 = 12;
 // registers of a thread: launch 72 (896 threads); the softmax warps take what the others give up
-constexpr uint32_t kRegsLow = 40, kRegsSoftmax = 96;
+constexpr uint32_t kRegsLow = 56, kRegsSoftmax = 80;
 static_assert(12 * 32 * kRegsLow + 16 * 32 * kRegsSoftmax <= kThreads * 72, "register split over the launch total");
 
 constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {  // fp16 A and B, fp32 D
@@ -100,6 +107,14 @@ __device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
   return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
 }
 
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(x) : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -132,63 +147,77 @@ __device__ __forceinline__ float weights32(const uint32_t (&v)[32], float c, flo
 }
 
 // (everything below 2^31, checked on the host: 64-bit divisions would take a microsecond an item)
-struct Item {
-  uint32_t b, h, split, bh;
-  uint32_t pair, row0;  // pair of query tiles, its first row
-  uint32_t tile0;       // first key tile
-  int len;              // keys of the sequence
-  int tiles;            // key tiles of this item
-  int groups;           // query tiles with rows in them (1 or 2)
+struct alignas(16) Item {
+  uint32_t b, h, bh, part;  // part: of the partial results (pair of tiles and split)
+  uint32_t row0;            // first query row
+  uint32_t tile0;           // first key tile
+  int len;                  // keys of the sequence
+  int tiles;                // key tiles of this item
+  uint32_t pair;            // of query tiles, over all cells
+  int groups;               // query tiles with rows in them (1 or 2; 0: there is no item)
+  uint32_t unused[2];
 };
 
 __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
   Item it;
-  const uint32_t pairs = (static_cast<uint32_t>(a.rows) + kPairRows - 1) / kPairRows;
-  it.pair = w % pairs;
-  it.row0 = it.pair * kPairRows;
-  w /= pairs;
-  it.split = w % static_cast<uint32_t>(a.splits);
-  it.bh = w / static_cast<uint32_t>(a.splits);
+  const uint32_t pairs = (static_cast<uint32_t>(a.rows - a.first) + kPairRows - 1) / kPairRows;
+  const uint32_t cell_split = w / pairs, pair = w - cell_split * pairs;
+  it.row0 = static_cast<uint32_t>(a.first) + pair * kPairRows;
+  it.bh = cell_split / static_cast<uint32_t>(a.splits);
+  const uint32_t split = cell_split - it.bh * static_cast<uint32_t>(a.splits);
+  it.pair = it.bh * pairs + pair;
+  it.part = it.pair * static_cast<uint32_t>(a.splits) + split;
   it.b = it.bh / static_cast<uint32_t>(a.c.heads);
   it.h = it.bh - it.b * static_cast<uint32_t>(a.c.heads);
   it.len = static_cast<int>(min(max(a.length.at(it.b), int64_t{0}), a.c.cap));
   const uint32_t all = (static_cast<uint32_t>(it.len) + kN - 1) / kN, each = (all + a.splits - 1) / static_cast<uint32_t>(a.splits);
-  it.tile0 = min(it.split * each, all);
+  it.tile0 = min(split * each, all);
   it.tiles = static_cast<int>(min(it.tile0 + each, all) - it.tile0);
   it.groups = it.row0 + kM < static_cast<uint32_t>(a.rows) ? 2 : 1;
+  it.unused[0] = it.unused[1] = 0;
   return it;
 }
 
 template <bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
-    tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool q_vec,
-                                                         bool o_vec) {
+    tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool o_vec) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                     // [group]
-  uint8_t* sK = sQ + 2 * kTile16;         // [kRing] fp16, swizzled
+  uint8_t* sQ = smem;                     // [item parity][query tile]
+  uint8_t* sK = sQ + 4 * kTile16;         // [kRing] fp16, swizzled
   uint8_t* sV = sK + kRing * kTile16;     // [kRing]
   uint8_t* rK = sV + kRing * kTile16;     // [kRing] codes
   uint8_t* rV = rK + kRing * kTile8;      // [kRing]
   uint64_t* bars = reinterpret_cast<uint64_t*>(rV + kRing * kTile8);
   uint64_t* rk_full = bars;               // codes have arrived
   uint64_t* rk_empty = rk_full + kRing;   // codes are widened
-  uint64_t* rv_full = rk_empty + kRing;
-  uint64_t* rv_empty = rv_full + kRing;
-  uint64_t* k_full = rv_empty + kRing;    // fp16 tile is there
+  uint64_t* k_full = rk_empty + kRing;    // fp16 tile is there
   uint64_t* k_empty = k_full + kRing;     // the products that read it are done
-  uint64_t* v_full = k_empty + kRing;
+  uint64_t* rv_full = k_empty + kRing;    // the same four for V
+  uint64_t* rv_empty = rv_full + kRing;
+  uint64_t* v_full = rv_empty + kRing;
   uint64_t* v_empty = v_full + kRing;
-  uint64_t* q_full = v_empty + kRing;     // [query tile] per item
-  uint64_t* o_free = q_full + 2;          // [query tile] per item: O is in registers
-  uint64_t* s_full = o_free + 2;          // [group] per tile: scores (and the last P V), and once more per item
+  uint64_t* item_full = v_empty + kRing;  // [kItems]
+  uint64_t* item_empty = item_full + kItems;
+  uint64_t* q_full = item_empty + kItems; // [item parity][query tile]
+  uint64_t* q_empty = q_full + 4;         // the item's scores are done
+  uint64_t* o_free = q_empty + 4;         // [query tile] per item: O is in registers
+  uint64_t* o_full = o_free + 2;          // [group] per item: the last P V is done
+  uint64_t* s_full = o_full + 4;          // [group] per tile: scores are there, the P V before them done
   uint64_t* p_full = s_full + 4;          // [group] per tile: P is in TMEM
   uint64_t* pair = p_full + 4;            // [query tile][lane quarter] the two halves have exchanged
   uint64_t* done = pair + 8;              // [query tile] every product of this CTA
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
+  uint64_t* taken = done + 2;             // the answer to a request for an item
+  uint64_t* answer = taken + 2;           // (16 bytes, 16-byte aligned)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(answer + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ float2 swap[2][16][32];  // [parity of the exchange][softmax warp][row]
-  static_assert((8 * kRing + 22) * 8 + 8 <= 512, "barriers fit their room");
+  __shared__ Item known[kItems];
+  // (s_k, log2 s_v, 1 / s_v) of each 32 keys of a tile, written with its K; a slot is used again four tiles
+  // on, when the scores three tiles before that are done and so the weights of this tile
+  __shared__ float4 scales[4][4];
+  static_assert((8 * kRing + 2 * kItems + 36) * 8 + 8 <= 1024, "barriers fit their room");
+  static_assert((8 * kRing + 2 * kItems + 34) % 2 == 0, "the answer is 16-byte aligned");
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (*reinterpret_cast<volatile int*>(a.status) != 0) return;  // another CTA or kernel timed out
@@ -205,8 +234,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&k_empty[i], 2);
       mbar_init(&v_empty[i], 2);
     }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kConsumers);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(taken, 1);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_full[t], 8);
       mbar_init(&o_free[t], 8);
       mbar_init(&done[t], 1);
     }
@@ -219,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_barrier_init();
   }
   // columns past the width are never written again: zero everywhere (finite, and 0 in Q)
-  for (int i = threadIdx.x; i < kTile16 * (2 + 2 * kRing) / 16; i += kThreads)
+  for (int i = threadIdx.x; i < kTile16 * (4 + 2 * kRing) / 16; i += kThreads)
     reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
@@ -228,14 +266,70 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // The next item, for one thread or a whole warp (`all`): null past the last one or after a timeout.  It
+  // stays in shared memory (registers are scarce) until `done_with`.
+  uint32_t seen = 0;
+  auto next_item = [&](bool all) -> const Item* {
+    const uint32_t i = seen % kItems, ph = seen / kItems & 1;
+    const bool ok = all ? mbar_wait_warp(&item_full[i], ph, a.status, kTimeoutEpilogue, abort_flag)
+                        : mbar_wait(&item_full[i], ph, a.status, kTimeoutMma, abort_flag);
+    return ok && known[i].groups > 0 ? &known[i] : nullptr;
+  };
+  auto done_with = [&](bool all) {
+    if (all) __syncwarp();
+    if (!all || lane == 0) mbar_arrive(&item_empty[seen % kItems]);
+    ++seen;
+  };
+
   if (warp == 0) {
     setmaxnreg_dec<kRegsLow>();
     if (elect_one()) {
       const uint32_t bytes = static_cast<uint32_t>(kN * a.c.stored);
-      uint32_t nk = 0, nv = 0;  // tiles asked for so far
+      uint32_t nk = 0, nv = 0, nq[2] = {0, 0};  // tiles asked for so far
+      uint32_t told = 0, asked = 0;
       bool ok = true;
-      for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
-        const Item it = item_at(a, w);
+      auto tell = [&](uint32_t w) -> bool {  // (`items`: there is none left)
+        const uint32_t i = told % kItems;
+        if (!mbar_wait(&item_empty[i], (told / kItems & 1) ^ 1, a.status, kTimeoutProducer, abort_flag)) return false;
+        known[i] = item_at(a, w < items ? w : 0);
+        if (w >= items) known[i].groups = 0;
+        mbar_arrive(&item_full[i]);
+        ++told;
+        return true;
+      };
+      auto ask = [&] {  // for a CTA that has not started
+        mbar_arrive_expect_tx(taken, 16);
+        asm volatile(
+            "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                smem_u32(answer)),
+            "r"(smem_u32(taken))
+            : "memory");
+        ++asked;
+      };
+      auto answered = [&](uint32_t& w) -> bool {  // the item taken over, `items` where there is none left
+        uint32_t got, id;
+        asm volatile(
+            "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+            "ld.shared.b128 h, [%2];\n\t"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "mov.u32 %1, 0;\n\t"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+            : "=r"(got), "=r"(id)
+            : "r"(smem_u32(answer))
+            : "memory");
+        fence_proxy_async_smem();
+        w = got ? id : items;
+        return true;
+      };
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the query tiles are there
+      uint32_t cur = blockIdx.x, nxt = items;
+      ask();
+      ok = tell(cur);
+      while (ok && cur < items) {
+        const Item& it = known[(told - 1) % kItems];  // (told only now: its slot is not reused before this item is done)
+        const int tiles = it.tiles, groups = it.groups;
+        const int64_t qtile = static_cast<int64_t>(it.pair) * 2;
         const int64_t at = (it.bh * a.c.cap + static_cast<int64_t>(it.tile0) * kN) * a.c.stored;
         auto load = [&](int j, const uint8_t* src, uint8_t* dst, uint64_t* full, uint64_t* empty, uint32_t& n) -> bool {
           const uint32_t st = n % kRing;
@@ -245,13 +339,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++n;
           return true;
         };
-        if (it.tiles > 0) ok = load(0, a.c.k, rK, rk_full, rk_empty, nk);
-        for (int j = 0; ok && j < it.tiles; ++j) {
-          if (j + 1 < it.tiles) ok = load(j + 1, a.c.k, rK, rk_full, rk_empty, nk);
+        if (tiles > 0 && !(ok = load(0, a.c.k, rK, rk_full, rk_empty, nk))) break;
+        for (int t = 0; ok && tiles > 0 && t < groups; ++t) {
+          const uint32_t i = 2 * (nq[t] & 1) + t;
+          if (!(ok = mbar_wait(&q_empty[i], (nq[t] / 2 & 1) ^ 1, a.status, kTimeoutProducer, abort_flag))) break;
+          mbar_arrive_expect_tx(&q_full[i], kTile16);
+          bulk_load(sQ + i * kTile16, a.q_tiles + (qtile + t) * kTile16, kTile16, &q_full[i]);
+          ++nq[t];
+        }
+        if (!ok || !(ok = answered(nxt) && tell(nxt))) break;
+        if (nxt < items) ask();  // (not again after a refusal)
+        for (int j = 0; ok && j < tiles; ++j) {
+          if (j + 1 < tiles) ok = load(j + 1, a.c.k, rK, rk_full, rk_empty, nk);
           if (ok) ok = load(j, a.c.v, rV, rv_full, rv_empty, nv);
         }
+        cur = nxt;
       }
-      // own copies in flight (after an abort nobody else waits for them)
+      // own copies and requests in flight (after an abort nobody else waits for them)
+      if (asked > 0) mbar_wait(taken, (asked - 1) & 1, a.status, kTimeoutProducer, nullptr);
+      for (int t = 0; t < 2; ++t)
+        for (uint32_t i = 0; i < 2; ++i)
+          if (nq[t] > i)
+            mbar_wait(&q_full[2 * ((nq[t] - 1 - i) & 1) + t], (nq[t] - 1 - i) / 2 & 1, a.status, kTimeoutProducer, nullptr);
       for (uint32_t i = 0; i < kRing; ++i) {
         if (nk > i) mbar_wait(&rk_full[(nk - 1 - i) % kRing], (nk - 1 - i) / kRing & 1, a.status, kTimeoutProducer, nullptr);
         if (nv > i) mbar_wait(&rv_full[(nv - 1 - i) % kRing], (nv - 1 - i) / kRing & 1, a.status, kTimeoutProducer, nullptr);
@@ -273,11 +382,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
         return mbar_wait(b, parity & 1, a.status, kTimeoutMma, abort_flag);
       };
-      for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
-        const Item it = item_at(a, w);
-        if (it.tiles == 0) continue;
-        if (t >= it.groups) {  // no rows: the tiles of K and V are the other issuer's
-          for (int j = 0; ok && j < it.tiles; ++j) {
+      while (const Item* it = ok ? next_item(false) : nullptr) {
+        const int tiles = it->tiles;
+        const bool mine = t < it->groups;
+        done_with(false);
+        if (tiles == 0) continue;
+        if (!mine) {  // no rows: the tiles of K and V are the other issuer's
+          for (int j = 0; ok && j < tiles; ++j) {
             if (!(ok = wait(&k_full[nk % kRing], nk / kRing))) break;
             mbar_arrive(&k_empty[nk++ % kRing]);
             if (!(ok = wait(&v_full[nv % kRing], nv / kRing))) break;
@@ -285,21 +396,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           continue;
         }
+        const uint32_t buf = qcnt & 1;
+        const uint64_t q = dq + buf * (2 * kStage);
         auto scores = [&](int p) {  // of K tile nk, for keys 64 p .. + 63
           const uint64_t k = dk + nk % kRing * kStage + p * kHalfTile;
 #pragma unroll
           for (int i = 0; i < kD / 16; ++i)
-            umma_bf16_ss(tmem + (2 * t + p) * kHalf, dq + 2 * i, k + 2 * i, idesc_s, i > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + (2 * t + p) * kHalf, q + 2 * i, k + 2 * i, idesc_s, i > 0 ? 1u : 0u);
         };
-        if (!(ok = wait(&q_full[t], qcnt) && wait(&k_full[nk % kRing], nk / kRing))) break;
+        if (!(ok = wait(&q_full[2 * buf + t], qcnt / 2) && wait(&k_full[nk % kRing], nk / kRing))) break;
         tc_fence_after();
         for (int p = 0; p < 2; ++p) {
           scores(p);
           umma_commit(&s_full[2 * t + p]);
         }
         umma_commit(&k_empty[nk++ % kRing]);
-        for (int j = 0; ok && j < it.tiles; ++j, ++cnt) {
-          const bool more = j + 1 < it.tiles;
+        if (tiles == 1) umma_commit(&q_empty[2 * buf + t]);
+        for (int j = 0; ok && j < tiles; ++j, ++cnt) {
+          const bool more = j + 1 < tiles;
           // the accumulators of the previous item have been read
           if (j == 0 && qcnt > 0 && !(ok = wait(&o_free[t], qcnt - 1))) break;
           if (!(ok = wait(&v_full[nv % kRing], nv / kRing) && (!more || wait(&k_full[nk % kRing], nk / kRing)))) break;
@@ -313,50 +427,54 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_bf16_ts(tmem + kOcol + g * kD, tmem + g * kHalf + i * 8, v + i * 128, idesc_o, (i > 0 || j > 0) ? 1u : 0u);
             // P V reads the columns that the next scores overwrite: products of one thread run in order
             if (more) scores(p);
-            umma_commit(&s_full[g]);
+            umma_commit(more ? &s_full[g] : &o_full[g]);
           }
           if (!ok) break;
           umma_commit(&v_empty[nv++ % kRing]);
           if (more) umma_commit(&k_empty[nk++ % kRing]);
+          if (j + 2 == tiles) umma_commit(&q_empty[2 * buf + t]);  // the item's scores are all issued
         }
         ++qcnt;
       }
       umma_commit(&done[t]);
       mbar_wait(&done[t], 0, a.status, kTimeoutMma, nullptr);
     }
-  } else if (warp < 4) {
-    setmaxnreg_dec<kRegsLow>();
+  } else if (warp == 3) {
+    setmaxnreg_dec<kRegsLow>();  // (its warpgroup's share)
   } else if (warp < kSoftmaxWarp0) {
     setmaxnreg_dec<kRegsLow>();
     // ------------------------------------------------------------ codes -> fp16 tiles
-    // Thread: eight codes (unit c) of rows row0, row0 + 16, ..: fixed steps in both tiles.  The codes
-    // are in registers before the fp16 tile's last reader is waited for.
+    // Thread: eight codes (unit c) of rows row0, row0 + 16, ..: fixed steps in both tiles, and eight threads
+    // a row whatever its width, so that their 16-byte pieces never meet in a bank.  The codes are in
+    // registers before the fp16 tile's last reader is waited for.
     const bool is_v = warp >= 8;
-    const uint32_t units = static_cast<uint32_t>(a.c.stored / 8), tid = threadIdx.x % (kConvertWarps * 32);
-    const uint32_t row0 = tid / units, c = tid - row0 * units;
-    const bool works = row0 < 16;
+    const uint32_t tid = threadIdx.x % (kConvertWarps * 32), row0 = tid / 8, c = tid % 8;
+    const bool works = static_cast<int>(c * 8) < a.c.stored;
     const uint8_t* src = (is_v ? rV : rK) + row0 * a.c.stored + c * 8;
     uint8_t* dst = (is_v ? sV : sK) + row0 * 128 + ((c ^ (row0 & 7)) << 4);
     const uint32_t step = 16 * a.c.stored;
-    uint64_t* code_full = is_v ? rv_full : rk_full;
-    uint64_t* code_empty = is_v ? rv_empty : rk_empty;
-    uint64_t* full = is_v ? v_full : k_full;
-    uint64_t* empty = is_v ? v_empty : k_empty;
-    uint32_t st = 0, ph = 0;
+    uint64_t* bar = is_v ? rv_full : rk_full;  // then code_empty, full, empty, kRing each
+    uint32_t st = 0, ph = 0, n = 0;
     bool ok = true;
-    for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
-      const Item it = item_at(a, w);
-      const int tiles = it.tiles;
+    while (const Item* it = ok ? next_item(true) : nullptr) {
+      const int tiles = it->tiles;
+      // keys of the item from this thread's first row on (warp 4: from chunk lane % 4 on)
+      int left = it->len - static_cast<int>(it->tile0 * kN + (warp == 4 ? 32 * (lane & 3) : row0));
+      const int64_t blk = it->bh * a.c.blocks() + ((it->tile0 * kN + 32 * (lane & 3)) >> a.c.block_log2);
+      const float *ks = a.c.k_scale + blk, *vs = a.c.v_scale + blk;
+      done_with(true);
+      float sk = 0.f, sv = 0.f;
+      if (warp == 4 && tiles > 0) sk = __ldg(ks), sv = __ldg(vs);
 #pragma unroll 1
-      for (int j = 0; j < tiles; ++j) {
-        if (!(ok = mbar_wait_warp(&code_full[st], ph, a.status, kTimeoutEpilogue, abort_flag))) break;
+      for (int j = 0; j < tiles; ++j, ++n, left -= kN) {
+        if (!(ok = mbar_wait_warp(bar + st, ph, a.status, kTimeoutEpilogue, abort_flag))) break;
         uint2 x[kN / 16];
         const uint8_t* from = src + st * kTile8;
         if (works) {
 #pragma unroll
           for (int e = 0; e < kN / 16; ++e) x[e] = *reinterpret_cast<const uint2*>(from + e * step);
         }
-        if (!(ok = mbar_wait_warp(&empty[st], ph ^ 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(bar + 3 * kRing + st, ph ^ 1, a.status, kTimeoutEpilogue, abort_flag))) break;
         uint8_t* to = dst + st * kTile16;
         if (works) {
 #pragma unroll
@@ -365,16 +483,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             widen<FP8>(biased<FP8>(x[e].x), y.x, y.y);
             widen<FP8>(biased<FP8>(x[e].y), y.z, y.w);
             // codes behind the last row may be NaN (0 x NaN is none of its business)
-            if (FP8 && is_v && static_cast<int>((it.tile0 + j) * kN + row0 + 16 * e) >= it.len) y = make_uint4(0, 0, 0, 0);
+            if (FP8 && is_v && 16 * e >= left) y = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(to + e * 2048) = y;
           }
+        }
+        if (warp == 4) {
+          const float svc = safe_scale(sv);
+          // (a block behind the last row counts for nothing, whatever its scale)
+          const float4 y = left > 0 ? make_float4(sk, __log2f(svc), __fdividef(1.f, svc), 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (lane < 4) scales[n & 3][lane] = y;
+          if (j + 1 < tiles) sk = __ldg(ks += kN >> a.c.block_log2), sv = __ldg(vs += kN >> a.c.block_log2);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           // (only now: with the codes released as soon as their loads were issued, the next copy overtook them)
-          mbar_arrive(&code_empty[st]);
-          mbar_arrive(&full[st]);
+          mbar_arrive(bar + kRing + st);
+          mbar_arrive(bar + 2 * kRing + st);
         }
         if (++st == kRing) st = 0, ph ^= 1;
       }
@@ -382,127 +507,55 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     setmaxnreg_inc<kRegsSoftmax>();
     // ------------------------------------------------------------ softmax
-    // Group (query tile qt, half): 64 key columns of every tile; of Q and the result, columns 32 half ..
-    // + 31.  The two warps of the same 32 rows exchange magnitudes of Q and, at the end, (maximum, sum).
+    // Group (query tile qt, half): 64 key columns of every tile, and columns 32 half .. + 31 of the
+    // result.  The two warps of the same 32 rows exchange (maximum, sum) at the end.
     const int sw = warp - kSoftmaxWarp0, g = sw / 4, qt = g / 2, half = g % 2, quarter = sw % 4;
     const int r = quarter * 32 + lane;  // row of the tile == TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + g * kHalf + lane_off, tO = tmem + kOcol + g * kD + lane_off,
                    tO2 = tmem + kOcol + 2 * qt * kD + half * 32 + lane_off;  // this half's columns, both accumulators
-    uint8_t* q_row = sQ + qt * kTile16 + r * 128;
-    uint64_t* bar = &pair[qt * 4 + quarter];
+    uint64_t* pair_bar = &pair[qt * 4 + quarter];
     uint32_t cnt = 0;  // completions of s_full so far
-    uint32_t xc = 0;   // exchanges so far
+    uint32_t nt = 0;   // tiles of all items so far
+    uint32_t xc = 0;   // exchanges, and so items, so far
     bool ok = true;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the query rows are there
     auto exchange = [&](float2 x) -> float2 {  // the other half's x for this row (valid if ok)
       swap[xc & 1][sw][lane] = x;
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-      ok = mbar_wait_warp(bar, xc & 1, a.status, kTimeoutEpilogue, abort_flag);
+      if (lane == 0) mbar_arrive(pair_bar);
+      ok = mbar_wait_warp(pair_bar, xc & 1, a.status, kTimeoutEpilogue, abort_flag);
       return swap[xc++ & 1][sw ^ 4][lane];
     };
-    auto scores_ready = [&]() -> bool {
-      ok = mbar_wait_warp(&s_full[g], cnt++ & 1, a.status, kTimeoutEpilogue, abort_flag);
-      tc_fence_after();
-      return ok;
-    };
-    for (uint32_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
-      const Item it = item_at(a, w);
-      if (qt >= it.groups) continue;
-      const uint32_t row = it.row0 + qt * kM + r;
-      const bool there = row < a.rows;
-      const uint32_t n = there ? row / static_cast<uint32_t>(a.group) : 0;
-      const int head = static_cast<int>(it.h * a.group + (there ? row - n * a.group : 0));
+    while (const Item* it = ok ? next_item(true) : nullptr) {
+      if (qt >= it->groups) {
+        nt += it->tiles;
+        done_with(true);
+        continue;
+      }
+      const int tiles = it->tiles;
       float m = -INFINITY, l = 0.f;
-      if (it.tiles > 0) {
-        // ---- 32 columns of the query row as fp16, times a power of two (the group's last scores are
-        // done, so nothing reads its Q any more)
-        float fac;
-        {
-          uint32_t x[16];
-          const uint16_t* src = static_cast<const uint16_t*>(a.q.p) + a.q.offset(it.b, n, head) + half * 32;
-          const int have = there ? a.c.width - half * 32 : 0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (q_vec && c * 8 < have) v = __ldg(reinterpret_cast<const uint4*>(src) + c);
-            x[4 * c] = v.x, x[4 * c + 1] = v.y, x[4 * c + 2] = v.z, x[4 * c + 3] = v.w;
+      if (tiles > 0) {
+        const float fac = a.q_rows[static_cast<int64_t>(it->pair) * kPairRows + qt * kM + r].factor;  // (anything where no row is)
+        int valid = it->len - static_cast<int>(it->tile0 * kN) - kHalf * half;  // keys from this half's first on
+        for (int j = 0; j < tiles; ++j, ++nt, valid -= kN) {
+          if (!(ok = mbar_wait_warp(&s_full[g], cnt++ & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+          tc_fence_after();
+          if (valid < kHalf) {  // keys behind the last row
+#pragma unroll 1
+            for (int i = max(valid, 0); i < kHalf; ++i) tmem_st1(tS + i, 0xff800000u);
+            tmem_wait_st();
           }
-          if (!q_vec) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (2 * i < have) x[i] = __ldg(src + 2 * i);
-              if (2 * i + 1 < have) x[i] |= static_cast<uint32_t>(__ldg(src + 2 * i + 1)) << 16;
-            }
+          const float4* sc = &scales[nt & 3][2 * half];
+          float cand = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t x[32];
+            tmem_ld32(tS + 32 * c, x);
+            const float f = fac * sc[c].x;  // (never 0: a masked key's -inf stays -inf)
+            tmem_wait_ld();
+            cand = fmaxf(cand, fmaf(max32(x), f < 1e-38f ? 1e-38f : f, sc[c].y));
           }
-          uint32_t top2 = 0;  // magnitudes order like their bits, infinities and NaN on top
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top2 = __vmaxu2(top2, x[i] & 0x7fff7fffu);
-          uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
-          t16 = max(t16, __float_as_uint(exchange(make_float2(__uint_as_float(t16), 0.f)).x));
-          if (!ok) break;
-          const bool bf = a.type == kBF16;
-          const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
-          float up, down;
-          row_scale(top, up, down);
-          fac = down * a.scale_log2;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t v = x[4 * c + i];
-              float lo, hi;
-              if (bf) {
-                lo = __uint_as_float(v << 16), hi = __uint_as_float(v & 0xffff0000u);
-              } else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                lo = f.x, hi = f.y;
-              }
-              y[i] = pack_half2(lo * up, hi * up);
-            }
-            *reinterpret_cast<uint4*>(q_row + (((4 * half + c) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[qt]);
-        }
-        const float* ks = a.c.k_scale + it.bh * a.c.blocks();
-        const float* vs = a.c.v_scale + it.bh * a.c.blocks();
-        // scales of the next tile: lane i those of this half's keys 32 (i % 2) .. + 31 (a block is 32 keys or more)
-        const uint32_t key = it.tile0 * kN + kHalf * half + 32 * (lane & 1);
-        float sk = __ldg(ks + (key >> a.c.block_log2)), sv = __ldg(vs + (key >> a.c.block_log2));
-        for (int j = 0; j < it.tiles; ++j) {
-          const int valid = min(it.len - static_cast<int>(it.tile0 + j) * kN, kN) - kHalf * half;
-          float f0, f1, lv0, lv1, inv0, inv1;
-          {
-            const bool none = valid <= 32 * (lane & 1);  // a block behind the last row counts for nothing
-            const float svc = none ? 1.f : safe_scale(sv);
-            const float lv = __log2f(svc), inv = none ? 0.f : __fdividef(1.f, svc);
-            // (never 0: a masked key's -inf stays -inf)
-            f0 = fac * __shfl_sync(0xffffffffu, sk, 0), f1 = fac * __shfl_sync(0xffffffffu, sk, 1);
-            f0 = valid <= 0 ? 1.f : f0 < 1e-38f ? 1e-38f : f0;
-            f1 = valid <= 32 ? 1.f : f1 < 1e-38f ? 1e-38f : f1;
-            lv0 = __shfl_sync(0xffffffffu, lv, 0), lv1 = __shfl_sync(0xffffffffu, lv, 1);
-            inv0 = __shfl_sync(0xffffffffu, inv, 0), inv1 = __shfl_sync(0xffffffffu, inv, 1);
-          }
-          if (j + 1 < it.tiles) {
-            const uint32_t blk = (key + static_cast<uint32_t>(j + 1) * kN) >> a.c.block_log2;
-            sk = __ldg(ks + blk), sv = __ldg(vs + blk);
-          }
-          if (!scores_ready()) break;
-          uint32_t s0[32], s1[32];
-          tmem_ld32(tS, s0);
-          tmem_ld32(tS + 32, s1);
-          tmem_wait_ld();
-          if (valid < kHalf) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (i >= valid) s0[i] = 0xff800000u;
-              if (32 + i >= valid) s1[i] = 0xff800000u;
-            }
-          }
-          const float cand = fmaxf(fmaf(max32(s0), f0, lv0), fmaf(max32(s1), f1, lv1));
           float back = 1.f;
           bool grow = false;
           if (j == 0) {
@@ -513,12 +566,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             grow = true;
           }
           const float lift = m == -INFINITY ? 0.f : kLift - m;  // (no key of this half is there)
-          float sum = weights32(s0, f0, lv0 + lift, tS) * inv0;
-          sum = fmaf(weights32(s1, f1, lv1 + lift, tS + 16), inv1, sum);
-          l = fmaf(l, back, sum);
+          l *= back;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t x[32];
+            tmem_ld32(tS + 32 * c, x);
+            const float f = fac * sc[c].x;
+            tmem_wait_ld();
+            l = fmaf(weights32(x, f < 1e-38f ? 1e-38f : f, sc[c].y + lift, tS + 16 * c), sc[c].z, l);
+          }
           // (the products before these scores are done: O may be changed)
           if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
+#pragma unroll 1
             for (int q = 0; q < 4; ++q) {
               uint32_t o[16];
               tmem_ld16(tO + q * 16, o);
@@ -533,13 +592,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[g]);
         }
-        if (!ok || !scores_ready()) break;  // the last P V
+        if (!ok || !(ok = mbar_wait_warp(&o_full[g], xc & 1, a.status, kTimeoutEpilogue, abort_flag))) break;  // the last P V
+        tc_fence_after();
       }
-      // ---- the halves joined: 32 columns of O from both accumulators
-      float o[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = 0.f;
-      if (it.tiles > 0) {
+      // ---- the halves joined: 32 columns of O from both accumulators, to memory.  (Once an item, so its
+      // instructions come from far: a loop over 8 columns.)
+      const QueryRow q = a.q_rows[static_cast<int64_t>(it->pair) * kPairRows + qt * kM + r];
+      const bool there = it->row0 + qt * kM + r < static_cast<uint32_t>(a.rows);
+      const int64_t pr = static_cast<int64_t>(it->part) * kPairRows + qt * kM + r;
+      done_with(true);
+      float fa = 0.f, fb = 0.f;  // of the first and the second half's accumulator
+      if (tiles > 0) {
         if (!(m < INFINITY)) l = __uint_as_float(0x7fc00000u);  // an infinite score (or a NaN) somewhere
         const float2 other = exchange(make_float2(m, l));
         if (!ok) break;
@@ -547,58 +610,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float f = m == -INFINITY ? 0.f : exp2f(m - top), f2 = other.x == -INFINITY ? 0.f : exp2f(other.x - top);
         l = l * f + other.y * f2;
         m = top;
-        const float fa = half ? f2 : f, fb = half ? f : f2;  // of the first and the second half's accumulator
+        fa = half ? f2 : f, fb = half ? f : f2;
         tc_fence_after();
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t x[16], y[16];
-          tmem_ld16(tO2 + 16 * q, x);
-          tmem_ld16(tO2 + kD + 16 * q, y);
+      }
+      const bool part = a.splits > 1;
+      if (!part) {
+        const float norm = l != 0.f ? 1.f / l : 0.f;
+        fa *= norm, fb *= norm;
+      }
+      uint16_t* dst = static_cast<uint16_t*>(a.o.p) + q.out + half * 32;
+      float* part_dst = a.part_o + pr * kMaxWidth + half * 32;
+      const int have = there ? a.c.width - half * 32 : 0;
+#pragma unroll 1
+      for (int c = 0; c < 32; c += 8) {
+        float o[8];
+        if (tiles > 0) {
+          uint32_t x[8], y[8];
+          tmem_ld8(tO2 + c, x);
+          tmem_ld8(tO2 + kD + c, y);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[16 * q + i] = __uint_as_float(x[i]) * fa + __uint_as_float(y[i]) * fb;
+          for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(x[i]) * fa + __uint_as_float(y[i]) * fb;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = 0.f;
         }
+        if (part) {
+          if (there) {
+            reinterpret_cast<float4*>(part_dst + c)[0] = make_float4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<float4*>(part_dst + c)[1] = make_float4(o[4], o[5], o[6], o[7]);
+          }
+        } else if (c < have) {
+          uint32_t y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[i] = a.type == kBF16 ? pack_bf16x2(o[2 * i], o[2 * i + 1]) : pack_half2(o[2 * i], o[2 * i + 1]);
+          if (o_vec) {
+            *reinterpret_cast<uint4*>(dst + c) = make_uint4(y[0], y[1], y[2], y[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < have) dst[c + i] = static_cast<uint16_t>(y[i / 2] >> 16 * (i % 2));
+          }
+        }
+      }
+      if (tiles > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free[qt]);
       }
-      if (!there) continue;
-      if (a.splits > 1) {
-        const int64_t pairs = (static_cast<uint32_t>(a.rows) + kPairRows - 1) / kPairRows;
-        const int64_t cell = (it.bh * pairs + it.pair) * a.splits + it.split;
-        const int64_t pr = cell * kPairRows + qt * kM + r;
-        if (half == 0) a.part_ml[pr] = make_float2(m, l);
-        if (it.tiles > 0) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kMaxWidth + half * 32);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        }
-        continue;
+      if (there && half == 0) {
+        if (part)
+          a.part_ml[pr] = make_float2(m, l);
+        else if (a.lse != nullptr)
+          a.lse[q.lse] = row_lse(m, l);
       }
-      const float norm = l != 0.f ? 1.f / l : 0.f;
-      uint16_t* dst = static_cast<uint16_t*>(a.o.p) + a.o.offset(it.b, n, head) + half * 32;
-      const int have = a.c.width - half * 32;
-      uint32_t y[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float lo = o[2 * i] * norm, hi = o[2 * i + 1] * norm;
-        y[i] = a.type == kBF16 ? pack_bf16x2(lo, hi) : pack_half2(lo, hi);
-      }
-      if (o_vec) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c * 8 < have)
-            reinterpret_cast<uint4*>(dst)[c] = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (2 * i < have) dst[2 * i] = static_cast<uint16_t>(y[i]);
-          if (2 * i + 1 < have) dst[2 * i + 1] = static_cast<uint16_t>(y[i] >> 16);
-        }
-      }
-      if (a.lse != nullptr && half == 0)
-        a.lse[(static_cast<int64_t>(it.b) * a.c.heads * a.group + head) * a.n + n] = row_lse(m, l);
     }
   }
 
@@ -610,22 +676,93 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Query rows as the swizzled fp16 tiles of 128 rows x 64 columns that the products read, times a power of
+// two that brings the row into fp16's range (exact); its inverse times the softmax scale, and where
+// the row's results go, are kept beside.  Eight lanes a row, 16 bytes each.
+constexpr int kQueryThreads = 256;
+template <bool VEC>
+__global__ void __launch_bounds__(kQueryThreads) query_kernel(Attention a, int64_t rows_up) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kQueryThreads / 8) + threadIdx.x / 8;
+  const int c = threadIdx.x % 8;
+  const int64_t bh = unit / rows_up, rel = unit - bh * rows_up, row = a.first + rel;  // (whole warps: rows_up % 4 = 0)
+  if (bh >= static_cast<int64_t>(a.c.batch) * a.c.heads) return;
+  const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
+  uint32_t v[4] = {0, 0, 0, 0};
+  if (row < a.rows && c * 8 < a.c.width) {
+    const int64_t n = row / a.group;
+    const uint16_t* src =
+        static_cast<const uint16_t*>(a.q.p) + a.q.offset(b, n, static_cast<int>(h * a.group + row - n * a.group)) + c * 8;
+    if constexpr (VEC) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c * 8 + e < a.c.width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
+    }
+  }
+  // magnitudes order like their bits, infinities and NaN on top
+  uint32_t top2 = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+  const uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
+  const bool bf = a.type == kBF16;
+  const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
+  float up, down;
+  row_scale(top, up, down);
+  uint32_t y[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float2 f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
+    if (!bf) f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+    y[k] = pack_half2(f.x * up, f.y * up);
+  }
+  if (row >= a.rows) return;
+  const int64_t n = row / a.group;
+  const int head = static_cast<int>(h * a.group + row - n * a.group);
+  const int64_t pairs = (a.rows - a.first + kPairRows - 1) / kPairRows, at = bh * pairs * kPairRows + rel;
+  const int r = static_cast<int>(at % kM);
+  *reinterpret_cast<uint4*>(a.q_tiles + at / kM * kTile16 + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+  if (c == 0)
+    a.q_rows[at] = QueryRow{a.o.offset(b, n, head), (static_cast<int64_t>(b) * a.c.heads * a.group + head) * a.n + n,
+                            down * a.scale_log2, 0.f};
+}
+
 template <bool FP8>
-cudaError_t tc_typed(const Attention& a, int ctas, cudaStream_t stream) {
+cudaError_t tc_typed(const Attention& a, cudaStream_t stream) {
   if (a.rows > INT32_MAX - kPairRows) return cudaErrorInvalidConfiguration;
-  const int64_t items = (a.rows + kPairRows - 1) / kPairRows * a.splits * a.c.batch * a.c.heads;
-  if (items > INT32_MAX) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const int64_t cells = (a.rows - a.first + kPairRows - 1) / kPairRows * a.c.batch * a.c.heads, items = cells * a.splits;
+  const int64_t rows_up = (a.rows - a.first + 3) / 4 * 4;
+  const int64_t blocks = (rows_up * a.c.batch * a.c.heads + kQueryThreads / 8 - 1) / (kQueryThreads / 8);
+  if (items > INT32_MAX || blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+  if (vectors(a.q, a.c.width))
+    query_kernel<true><<<static_cast<unsigned>(blocks), kQueryThreads, 0, stream>>>(a, rows_up);
+  else
+    query_kernel<false><<<static_cast<unsigned>(blocks), kQueryThreads, 0, stream>>>(a, rows_up);
+  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  tc_kernel<FP8><<<static_cast<unsigned>(items < ctas ? items : ctas), kThreads, kSmem, stream>>>(
-      a, static_cast<uint32_t>(items), vectors(a.q, a.c.width), vectors(a.o, a.c.width));
-  return cudaGetLastError();
+  e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(items));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};  // set up while the query tiles are written
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tc_kernel<FP8>, a, static_cast<uint32_t>(items), vectors(a.o, a.c.width));
 }
 
 }  // namespace
 
-cudaError_t launch_tc(const Attention& a, int ctas, cudaStream_t stream) {
-  return a.c.fp8 ? tc_typed<true>(a, ctas, stream) : tc_typed<false>(a, ctas, stream);
+int64_t tc_query_bytes(int64_t cells) { return cells * 2 * kTile16; }
+
+cudaError_t launch_tc(const Attention& a, cudaStream_t stream) {
+  return a.c.fp8 ? tc_typed<true>(a, stream) : tc_typed<false>(a, stream);
 }
 
 }  // namespace bc

@@ -8,7 +8,6 @@
 
 #include "block_cache.cuh"
 #include "plain.h"
-#include "tma_host.h"
 
 namespace nori {
 namespace {
@@ -205,22 +204,36 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   // the longest a sequence can be (lengths on the device are not read here)
   const int64_t longest = a.length.dev != nullptr ? a.c.cap : length_all;
   const int sms = sm_count(ck.get_device());
-  const bool few = a.rows <= kFewRows;
-  const int tile = few ? bc::few_tile_rows(a.rows) : bc::kPairRows;
-  const int64_t cells = (a.rows + tile - 1) / tile * a.c.batch * a.c.heads;
-  a.splits = few ? few_splits(cells, longest, sms * bc::few_resident(a.rows)) : tc_splits(cells, longest, persistent_sms(sms));
-  a.cluster = few ? std::min(a.splits, 8) : 1;
-  const int parts = a.splits / a.cluster;
-  Tensor part_o, part_ml;
-  if (parts > 1) {
-    part_o = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
-    part_ml = torch::empty({cells * parts * tile * 2}, cks.options());
-    a.part_o = part_o.data_ptr<float>();
-    a.part_ml = reinterpret_cast<float2*>(part_ml.data_ptr<float>());
-  }
   const auto stream = at::cuda::getCurrentCUDAStream();
-  C10_CUDA_CHECK(few ? bc::launch_few(a, stream) : bc::launch_tc(a, persistent_sms(sms), stream));
-  if (parts > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
+  auto run = [&](int64_t first, int64_t end, bool few) {
+    a.first = first;
+    a.rows = end;
+    const int tile = few ? bc::few_tile_rows(end - first) : bc::kPairRows;
+    const int64_t cells = (end - first + tile - 1) / tile * a.c.batch * a.c.heads;
+    a.splits = few ? few_splits(cells, longest, sms * bc::few_resident(end - first)) : tc_splits(cells, longest, sms);
+    a.cluster = few ? std::min(a.splits, 8) : 1;
+    const int parts = a.splits / a.cluster;
+    Tensor part_o, part_ml, q_tiles, q_rows;
+    if (!few) {
+      q_tiles = torch::empty({bc::tc_query_bytes(cells)}, cks.options().dtype(at::kByte));
+      q_rows = torch::empty({cells * tile * static_cast<int64_t>(sizeof(bc::QueryRow))}, q_tiles.options());
+      a.q_tiles = q_tiles.data_ptr<uint8_t>();
+      a.q_rows = reinterpret_cast<bc::QueryRow*>(q_rows.data_ptr<uint8_t>());
+    }
+    if (parts > 1) {
+      part_o = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
+      part_ml = torch::empty({cells * parts * tile * 2}, cks.options());
+      a.part_o = part_o.data_ptr<float>();
+      a.part_ml = reinterpret_cast<float2*>(part_ml.data_ptr<float>());
+    }
+    C10_CUDA_CHECK(few ? bc::launch_few(a, stream) : bc::launch_tc(a, stream));
+    if (parts > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
+  };
+  // a few rows behind the last whole pair of tiles would cost a pair's time on the tensor cores
+  const int64_t rows = a.rows, whole = rows / bc::kPairRows * bc::kPairRows;
+  const int64_t many = rows - whole > kFewRows ? rows : whole;
+  if (many > 0) run(0, many, false);
+  if (many < rows) run(many, rows, true);
   return {o, lse};
 }
 
