@@ -8,7 +8,8 @@
 //                 codes of 128-key tiles of K and V, each one contiguous piece of the cache, into
 //                 two rings (untiled bulk copies: no stride rules, so any width);
 //   warps 4..7    widen the codes of K to fp16, exactly, into the swizzled tiles that the products
-//   warps 8..11   read, and those of V: once for 256 query rows;
+//   warps 8..11   read, and those of V: once for 256 query rows; before an item's first tile each
+//                 warpgroup brings one of its query tiles to shared memory as fp16;
 //   warps 1, 2    issue the products of one query tile each: S = Q K^T (128 x 64 x 64) and O += P V;
 //   warps 12..27  softmax, four groups: (query tile) x (half of the keys of every tile), each with its
 //                 own maximum, sum and accumulator; thread = query row (its TMEM lane), 64 score columns
@@ -17,9 +18,6 @@
 // arithmetic, so four of them share an SM: with one thread for all 128 columns of a row and two
 // groups the same arithmetic took 1.3 times as long, with row maxima exchanged between the
 // halves 1.2 times.  The two halves of a query tile are joined once per item.
-//
-// A small kernel before writes the query rows as the fp16 tiles that the products read, so that they
-// are one contiguous copy each (the softmax warps did it at 3 us an item, in which nothing else ran).
 //
 // Scales cost nothing per value: with c = scale log2(e) s_k 2^-e (2^e brings the query row into
 // fp16's range, exactly) and t = c (q . k) + log2 s_v,
@@ -146,6 +144,45 @@ __device__ __forceinline__ float weights32(const uint32_t (&v)[32], float c, flo
   return r0 + r1;
 }
 
+// 16 bytes (values 8 c .. 8 c + 7) of query row `row` of a K/V head; zeros where it ends or does not exist.
+__device__ __forceinline__ uint4 query_piece(const Attention& a, int b, int h, uint32_t row, int c, bool vec) {
+  uint32_t v[4] = {0, 0, 0, 0};
+  if (row < static_cast<uint32_t>(a.rows) && c * 8 < a.c.width) {
+    const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group);
+    const uint16_t* src =
+        static_cast<const uint16_t*>(a.q.p) + a.q.offset(b, n, static_cast<int>(h * a.group + row - n * a.group)) + c * 8;
+    if (vec) return __ldg(reinterpret_cast<const uint4*>(src));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c * 8 + e < a.c.width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// The piece as fp16 times the row's power of two (eight neighbouring lanes hold the row), and the
+// factor that its scores take.
+__device__ __forceinline__ uint4 query_fp16(const Attention& a, const uint4& x, float& factor) {
+  const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+  // magnitudes order like their bits, infinities and NaN on top
+  uint32_t top2 = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+  const uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
+  const bool bf = a.type == kBF16;
+  const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
+  float up, down;
+  row_scale(top, up, down);
+  factor = down * a.scale_log2;
+  uint32_t y[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float2 f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
+    if (!bf) f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+    y[k] = pack_half2(f.x * up, f.y * up);
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
+}
+
 // (everything below 2^31, checked on the host: 64-bit divisions would take a microsecond an item)
 struct alignas(16) Item {
   uint32_t b, h, bh, part;  // part: of the partial results (pair of tiles and split)
@@ -155,7 +192,7 @@ struct alignas(16) Item {
   int tiles;                // key tiles of this item
   uint32_t pair;            // of query tiles, over all cells
   int groups;               // query tiles with rows in them (1 or 2; 0: there is no item)
-  uint32_t unused[2];
+  int64_t out;              // where the results of this (sequence, K/V head) begin
 };
 
 __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
@@ -174,13 +211,13 @@ __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
   it.tile0 = min(split * each, all);
   it.tiles = static_cast<int>(min(it.tile0 + each, all) - it.tile0);
   it.groups = it.row0 + kM < static_cast<uint32_t>(a.rows) ? 2 : 1;
-  it.unused[0] = it.unused[1] = 0;
+  it.out = a.o.offset(static_cast<int>(it.b), 0, static_cast<int>(it.h * a.group));
   return it;
 }
 
 template <bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
-    tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool o_vec) {
+    tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool q_vec, bool o_vec) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                     // [item parity][query tile]
@@ -200,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* item_full = v_empty + kRing;  // [kItems]
   uint64_t* item_empty = item_full + kItems;
   uint64_t* q_full = item_empty + kItems; // [item parity][query tile]
-  uint64_t* q_empty = q_full + 4;         // the item's scores are done
+  uint64_t* q_empty = q_full + 4;         // the item's scores are done, its factors read and its results on their way
   uint64_t* o_free = q_empty + 4;         // [query tile] per item: O is in registers
   uint64_t* o_full = o_free + 2;          // [group] per item: the last P V is done
   uint64_t* s_full = o_full + 4;          // [group] per tile: scores are there, the P V before them done
@@ -213,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ float2 swap[2][16][32];  // [parity of the exchange][softmax warp][row]
   __shared__ Item known[kItems];
+  __shared__ float factors[2][2 * kM];  // [item parity][row]: of the row's scores
   // (s_k, log2 s_v, 1 / s_v) of each 32 keys of a tile, written with its K; a slot is used again four tiles
   // on, when the scores three tiles before that are done and so the weights of this tile
   __shared__ float4 scales[4][4];
@@ -239,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&item_empty[i], kConsumers);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_full[i], kConvertWarps);
+      mbar_init(&q_empty[i], 1 + 8);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(taken, 1);
@@ -285,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     setmaxnreg_dec<kRegsLow>();
     if (elect_one()) {
       const uint32_t bytes = static_cast<uint32_t>(kN * a.c.stored);
-      uint32_t nk = 0, nv = 0, nq[2] = {0, 0};  // tiles asked for so far
+      uint32_t nk = 0, nv = 0;  // tiles asked for so far
       uint32_t told = 0, asked = 0;
       bool ok = true;
       auto tell = [&](uint32_t w) -> bool {  // (`items`: there is none left)
@@ -322,14 +360,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         w = got ? id : items;
         return true;
       };
-      asm volatile("griddepcontrol.wait;" ::: "memory");  // the query tiles are there
       uint32_t cur = blockIdx.x, nxt = items;
       ask();
       ok = tell(cur);
       while (ok && cur < items) {
         const Item& it = known[(told - 1) % kItems];  // (told only now: its slot is not reused before this item is done)
-        const int tiles = it.tiles, groups = it.groups;
-        const int64_t qtile = static_cast<int64_t>(it.pair) * 2;
+        const int tiles = it.tiles;
         const int64_t at = (it.bh * a.c.cap + static_cast<int64_t>(it.tile0) * kN) * a.c.stored;
         auto load = [&](int j, const uint8_t* src, uint8_t* dst, uint64_t* full, uint64_t* empty, uint32_t& n) -> bool {
           const uint32_t st = n % kRing;
@@ -340,14 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return true;
         };
         if (tiles > 0 && !(ok = load(0, a.c.k, rK, rk_full, rk_empty, nk))) break;
-        for (int t = 0; ok && tiles > 0 && t < groups; ++t) {
-          const uint32_t i = 2 * (nq[t] & 1) + t;
-          if (!(ok = mbar_wait(&q_empty[i], (nq[t] / 2 & 1) ^ 1, a.status, kTimeoutProducer, abort_flag))) break;
-          mbar_arrive_expect_tx(&q_full[i], kTile16);
-          bulk_load(sQ + i * kTile16, a.q_tiles + (qtile + t) * kTile16, kTile16, &q_full[i]);
-          ++nq[t];
-        }
-        if (!ok || !(ok = answered(nxt) && tell(nxt))) break;
+        if (!(ok = answered(nxt) && tell(nxt))) break;
         if (nxt < items) ask();  // (not again after a refusal)
         for (int j = 0; ok && j < tiles; ++j) {
           if (j + 1 < tiles) ok = load(j + 1, a.c.k, rK, rk_full, rk_empty, nk);
@@ -357,10 +386,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // own copies and requests in flight (after an abort nobody else waits for them)
       if (asked > 0) mbar_wait(taken, (asked - 1) & 1, a.status, kTimeoutProducer, nullptr);
-      for (int t = 0; t < 2; ++t)
-        for (uint32_t i = 0; i < 2; ++i)
-          if (nq[t] > i)
-            mbar_wait(&q_full[2 * ((nq[t] - 1 - i) & 1) + t], (nq[t] - 1 - i) / 2 & 1, a.status, kTimeoutProducer, nullptr);
       for (uint32_t i = 0; i < kRing; ++i) {
         if (nk > i) mbar_wait(&rk_full[(nk - 1 - i) % kRing], (nk - 1 - i) / kRing & 1, a.status, kTimeoutProducer, nullptr);
         if (nv > i) mbar_wait(&rv_full[(nv - 1 - i) % kRing], (nv - 1 - i) / kRing & 1, a.status, kTimeoutProducer, nullptr);
@@ -455,6 +480,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t step = 16 * a.c.stored;
     uint64_t* bar = is_v ? rv_full : rk_full;  // then code_empty, full, empty, kRing each
     uint32_t st = 0, ph = 0, n = 0;
+    const int qt = is_v;  // the query tile that this warpgroup brings
+    uint32_t qcnt = 0;
     bool ok = true;
     while (const Item* it = ok ? next_item(true) : nullptr) {
       const int tiles = it->tiles;
@@ -462,7 +489,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       int left = it->len - static_cast<int>(it->tile0 * kN + (warp == 4 ? 32 * (lane & 3) : row0));
       const int64_t blk = it->bh * a.c.blocks() + ((it->tile0 * kN + 32 * (lane & 3)) >> a.c.block_log2);
       const float *ks = a.c.k_scale + blk, *vs = a.c.v_scale + blk;
+      const bool has_rows = tiles > 0 && qt < it->groups;
+      const uint32_t row_first = it->row0 + qt * kM;
+      const int b = it->b, h = it->h;
       done_with(true);
+      if (has_rows) {
+        // ---- query rows: eight lanes a row, 16 bytes each; a power of two brings the row into fp16's
+        // range, exactly
+        const uint32_t buf = 2 * (qcnt & 1) + qt;
+        if (!(ok = mbar_wait_warp(&q_empty[buf], (qcnt / 2 & 1) ^ 1, a.status, kTimeoutProducer, abort_flag))) break;
+        uint8_t* tile = sQ + buf * kTile16;
+#pragma unroll 1
+        for (int r1 = warp % 4 * 32 + lane / 8; r1 < warp % 4 * 32 + 32; r1 += 16) {
+          uint4 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = query_piece(a, b, h, row_first + r1 + 4 * i, lane % 8, q_vec);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = r1 + 4 * i;
+            float factor;
+            x[i] = query_fp16(a, x[i], factor);
+            *reinterpret_cast<uint4*>(tile + r * 128 + ((lane % 8 ^ (r & 7)) << 4)) = x[i];
+            if (lane % 8 == 0) factors[qcnt & 1][qt * kM + r] = factor;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[buf]);
+        ++qcnt;
+      }
       float sk = 0.f, sv = 0.f;
       if (warp == 4 && tiles > 0) sk = __ldg(ks), sv = __ldg(vs);
 #pragma unroll 1
@@ -519,7 +574,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t nt = 0;   // tiles of all items so far
     uint32_t xc = 0;   // exchanges, and so items, so far
     bool ok = true;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the query rows are there
     auto exchange = [&](float2 x) -> float2 {  // the other half's x for this row (valid if ok)
       swap[xc & 1][sw][lane] = x;
       __syncwarp();
@@ -536,7 +590,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tiles = it->tiles;
       float m = -INFINITY, l = 0.f;
       if (tiles > 0) {
-        const float fac = a.q_rows[static_cast<int64_t>(it->pair) * kPairRows + qt * kM + r].factor;  // (anything where no row is)
+        if (!(ok = mbar_wait_warp(&q_full[2 * (xc & 1) + qt], xc / 2 & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+        const float fac = factors[xc & 1][qt * kM + r];
         int valid = it->len - static_cast<int>(it->tile0 * kN) - kHalf * half;  // keys from this half's first on
         for (int j = 0; j < tiles; ++j, ++nt, valid -= kN) {
           if (!(ok = mbar_wait_warp(&s_full[g], cnt++ & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
@@ -597,9 +652,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // ---- the halves joined: 32 columns of O from both accumulators, to memory.  (Once an item, so its
       // instructions come from far: a loop over 8 columns.)
-      const QueryRow q = a.q_rows[static_cast<int64_t>(it->pair) * kPairRows + qt * kM + r];
-      const bool there = it->row0 + qt * kM + r < static_cast<uint32_t>(a.rows);
+      const uint32_t row = it->row0 + qt * kM + r;
+      const bool there = row < static_cast<uint32_t>(a.rows);
+      const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group), in_group = row - n * a.group;
+      const int64_t out = it->out + n * a.o.sn + in_group * a.o.sh;
       const int64_t pr = static_cast<int64_t>(it->part) * kPairRows + qt * kM + r;
+      const int64_t lse_row = static_cast<int64_t>(it->bh) * a.group + in_group;
       done_with(true);
       float fa = 0.f, fb = 0.f;  // of the first and the second half's accumulator
       if (tiles > 0) {
@@ -618,16 +676,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float norm = l != 0.f ? 1.f / l : 0.f;
         fa *= norm, fb *= norm;
       }
-      uint16_t* dst = static_cast<uint16_t*>(a.o.p) + q.out + half * 32;
+      uint16_t* dst = static_cast<uint16_t*>(a.o.p) + half * 32;
       float* part_dst = a.part_o + pr * kMaxWidth + half * 32;
-      const int have = there ? a.c.width - half * 32 : 0;
+      const int have = a.c.width - half * 32;
+      // the item's query tile becomes the tile of results (nothing reads it any more): a row in pieces of 16 bytes
+      uint8_t* stage = sQ + (2 * ((xc ^ (tiles > 0)) & 1) + qt) * kTile16 + quarter * 32 * 128;
 #pragma unroll 1
-      for (int c = 0; c < 32; c += 8) {
+      for (int c = 0; c < 4; ++c) {
         float o[8];
         if (tiles > 0) {
           uint32_t x[8], y[8];
-          tmem_ld8(tO2 + c, x);
-          tmem_ld8(tO2 + kD + c, y);
+          tmem_ld8(tO2 + 8 * c, x);
+          tmem_ld8(tO2 + kD + 8 * c, y);
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(x[i]) * fa + __uint_as_float(y[i]) * fb;
@@ -637,33 +697,46 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (part) {
           if (there) {
-            reinterpret_cast<float4*>(part_dst + c)[0] = make_float4(o[0], o[1], o[2], o[3]);
-            reinterpret_cast<float4*>(part_dst + c)[1] = make_float4(o[4], o[5], o[6], o[7]);
+            reinterpret_cast<float4*>(part_dst + 8 * c)[0] = make_float4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<float4*>(part_dst + 8 * c)[1] = make_float4(o[4], o[5], o[6], o[7]);
           }
-        } else if (c < have) {
-          uint32_t y[4];
+          continue;
+        }
+        uint32_t y[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            y[i] = a.type == kBF16 ? pack_bf16x2(o[2 * i], o[2 * i + 1]) : pack_half2(o[2 * i], o[2 * i + 1]);
-          if (o_vec) {
-            *reinterpret_cast<uint4*>(dst + c) = make_uint4(y[0], y[1], y[2], y[3]);
-          } else {
+        for (int i = 0; i < 4; ++i)
+          y[i] = a.type == kBF16 ? pack_bf16x2(o[2 * i], o[2 * i + 1]) : pack_half2(o[2 * i], o[2 * i + 1]);
+        if (o_vec && tiles > 0) {
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((4 * half + c) ^ (lane & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+        } else if (there) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c + i < have) dst[c + i] = static_cast<uint16_t>(y[i / 2] >> 16 * (i % 2));
-          }
+          for (int i = 0; i < 8; ++i)
+            if (8 * c + i < have) dst[out + 8 * c + i] = static_cast<uint16_t>(y[i / 2] >> 16 * (i % 2));
         }
       }
       if (tiles > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free[qt]);
+        if (!part && o_vec) {
+          // four lanes a row: a store of the warp meets 8 lines (32 with a lane for each row)
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            const int rr = 8 * i + lane / 4, c = lane % 4;
+            const int64_t to = __shfl_sync(0xffffffffu, out, rr);
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((4 * half + c) ^ (rr & 7)) * 16);
+            if (row - lane + rr < static_cast<uint32_t>(a.rows) && 8 * c < have) *reinterpret_cast<uint4*>(dst + to + 8 * c) = y;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&q_empty[2 * (~xc & 1) + qt]);
       }
       if (there && half == 0) {
         if (part)
           a.part_ml[pr] = make_float2(m, l);
         else if (a.lse != nullptr)
-          a.lse[q.lse] = row_lse(m, l);
+          a.lse[lse_row * a.n + n] = row_lse(m, l);
       }
     }
   }
@@ -676,90 +749,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Query rows as the swizzled fp16 tiles of 128 rows x 64 columns that the products read, times a power of
-// two that brings the row into fp16's range (exact); its inverse times the softmax scale, and where
-// the row's results go, are kept beside.  Eight lanes a row, 16 bytes each.
-constexpr int kQueryThreads = 256;
-template <bool VEC>
-__global__ void __launch_bounds__(kQueryThreads) query_kernel(Attention a, int64_t rows_up) {
-  asm volatile("griddepcontrol.launch_dependents;");
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kQueryThreads / 8) + threadIdx.x / 8;
-  const int c = threadIdx.x % 8;
-  const int64_t bh = unit / rows_up, rel = unit - bh * rows_up, row = a.first + rel;  // (whole warps: rows_up % 4 = 0)
-  if (bh >= static_cast<int64_t>(a.c.batch) * a.c.heads) return;
-  const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
-  uint32_t v[4] = {0, 0, 0, 0};
-  if (row < a.rows && c * 8 < a.c.width) {
-    const int64_t n = row / a.group;
-    const uint16_t* src =
-        static_cast<const uint16_t*>(a.q.p) + a.q.offset(b, n, static_cast<int>(h * a.group + row - n * a.group)) + c * 8;
-    if constexpr (VEC) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
-      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c * 8 + e < a.c.width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
-    }
-  }
-  // magnitudes order like their bits, infinities and NaN on top
-  uint32_t top2 = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
-#pragma unroll
-  for (int o = 1; o < 8; o *= 2) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
-  const uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
-  const bool bf = a.type == kBF16;
-  const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
-  float up, down;
-  row_scale(top, up, down);
-  uint32_t y[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float2 f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
-    if (!bf) f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
-    y[k] = pack_half2(f.x * up, f.y * up);
-  }
-  if (row >= a.rows) return;
-  const int64_t n = row / a.group;
-  const int head = static_cast<int>(h * a.group + row - n * a.group);
-  const int64_t pairs = (a.rows - a.first + kPairRows - 1) / kPairRows, at = bh * pairs * kPairRows + rel;
-  const int r = static_cast<int>(at % kM);
-  *reinterpret_cast<uint4*>(a.q_tiles + at / kM * kTile16 + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-  if (c == 0)
-    a.q_rows[at] = QueryRow{a.o.offset(b, n, head), (static_cast<int64_t>(b) * a.c.heads * a.group + head) * a.n + n,
-                            down * a.scale_log2, 0.f};
-}
-
 template <bool FP8>
 cudaError_t tc_typed(const Attention& a, cudaStream_t stream) {
   if (a.rows > INT32_MAX - kPairRows) return cudaErrorInvalidConfiguration;
-  const int64_t cells = (a.rows - a.first + kPairRows - 1) / kPairRows * a.c.batch * a.c.heads, items = cells * a.splits;
-  const int64_t rows_up = (a.rows - a.first + 3) / 4 * 4;
-  const int64_t blocks = (rows_up * a.c.batch * a.c.heads + kQueryThreads / 8 - 1) / (kQueryThreads / 8);
-  if (items > INT32_MAX || blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
-  if (vectors(a.q, a.c.width))
-    query_kernel<true><<<static_cast<unsigned>(blocks), kQueryThreads, 0, stream>>>(a, rows_up);
-  else
-    query_kernel<false><<<static_cast<unsigned>(blocks), kQueryThreads, 0, stream>>>(a, rows_up);
-  cudaError_t e = cudaGetLastError();
+  const int64_t items = (a.rows - a.first + kPairRows - 1) / kPairRows * a.c.batch * a.c.heads * a.splits;
+  if (items > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const cudaError_t e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(items));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};  // set up while the query tiles are written
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tc_kernel<FP8>, a, static_cast<uint32_t>(items), vectors(a.o, a.c.width));
+  tc_kernel<FP8><<<static_cast<unsigned>(items), kThreads, kSmem, stream>>>(
+      a, static_cast<uint32_t>(items), vectors(a.q, a.c.width), vectors(a.o, a.c.width));
+  return cudaGetLastError();
 }
 
 }  // namespace
-
-int64_t tc_query_bytes(int64_t cells) { return cells * 2 * kTile16; }
 
 cudaError_t launch_tc(const Attention& a, cudaStream_t stream) {
   return a.c.fp8 ? tc_typed<true>(a, stream) : tc_typed<false>(a, stream);

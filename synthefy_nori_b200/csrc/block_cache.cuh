@@ -59,12 +59,6 @@ struct PerSequence {
   __device__ __forceinline__ int64_t at(int b) const { return dev != nullptr ? dev[b] : all; }
 };
 
-struct alignas(8) QueryRow {
-  int64_t out, lse;  // where its results go
-  float factor;      // of its scores
-  float unused;
-};
-
 struct Attention {
   Rows q, o;
   int type;  // of q and o (kBF16, kF16)
@@ -80,8 +74,6 @@ struct Attention {
   int cluster;      // splits that are joined on the way (kernel for few rows), a divisor of splits
   float* part_o;    // [cells, parts, tile rows, 64], unnormalised; parts = splits / cluster
   float2* part_ml;  // [cells, parts, tile rows] (maximum, sum)
-  uint8_t* q_tiles;   // workspace of the kernel for many rows: query tiles, and what belongs to each row
-  QueryRow* q_rows;   // [cells, 256]
   int* status;
 };
 
@@ -157,7 +149,6 @@ int few_resident(int64_t rows);  // CTAs that an SM holds
 cudaError_t launch_few(const Attention& a, cudaStream_t stream);
 // rows of a tile pair of the kernel for many rows; one CTA per SM
 constexpr int kPairRows = 256;
-int64_t tc_query_bytes(int64_t cells);
 cudaError_t launch_tc(const Attention& a, cudaStream_t stream);
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream);
 

@@ -213,13 +213,7 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
     a.splits = few ? few_splits(cells, longest, sms * bc::few_resident(end - first)) : tc_splits(cells, longest, sms);
     a.cluster = few ? std::min(a.splits, 8) : 1;
     const int parts = a.splits / a.cluster;
-    Tensor part_o, part_ml, q_tiles, q_rows;
-    if (!few) {
-      q_tiles = torch::empty({bc::tc_query_bytes(cells)}, cks.options().dtype(at::kByte));
-      q_rows = torch::empty({cells * tile * static_cast<int64_t>(sizeof(bc::QueryRow))}, q_tiles.options());
-      a.q_tiles = q_tiles.data_ptr<uint8_t>();
-      a.q_rows = reinterpret_cast<bc::QueryRow*>(q_rows.data_ptr<uint8_t>());
-    }
+    Tensor part_o, part_ml;
     if (parts > 1) {
       part_o = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
       part_ml = torch::empty({cells * parts * tile * 2}, cks.options());
