@@ -512,7 +512,7 @@ cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = a.cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, few_kernel<FP8, NT, W>, a, vectors(a.q, a.c.width));
+  return cudaLaunchKernelEx(&cfg, few_kernel<FP8, NT, W>, a, access_bytes(a.q, a.c.width) == 16);
 }
 
 }  // namespace

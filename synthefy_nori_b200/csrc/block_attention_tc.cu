@@ -145,16 +145,22 @@ __device__ __forceinline__ float weights32(const uint32_t (&v)[32], float c, flo
 }
 
 // 16 bytes (values 8 c .. 8 c + 7) of query row `row` of a K/V head; zeros where it ends or does not exist.
-__device__ __forceinline__ uint4 query_piece(const Attention& a, int b, int h, uint32_t row, int c, bool vec) {
+__device__ __forceinline__ uint4 query_piece(const Attention& a, int b, int h, uint32_t row, int c, int bytes) {
   uint32_t v[4] = {0, 0, 0, 0};
   if (row < static_cast<uint32_t>(a.rows) && c * 8 < a.c.width) {
     const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group);
     const uint16_t* src =
         static_cast<const uint16_t*>(a.q.p) + a.q.offset(b, n, static_cast<int>(h * a.group + row - n * a.group)) + c * 8;
-    if (vec) return __ldg(reinterpret_cast<const uint4*>(src));
+    if (bytes == 16) return __ldg(reinterpret_cast<const uint4*>(src));
+    if (bytes == 4) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c * 8 + e < a.c.width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
+      for (int e = 0; e < 4; ++e)
+        if (c * 8 + 2 * e < a.c.width) v[e] = __ldg(reinterpret_cast<const uint32_t*>(src) + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c * 8 + e < a.c.width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
+    }
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
@@ -217,7 +223,7 @@ __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
 
 template <bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
-    tc_kernel(const __grid_constant__ Attention a, uint32_t items, bool q_vec, bool o_vec) {
+    tc_kernel(const __grid_constant__ Attention a, uint32_t items, int q_bytes, int o_bytes) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                     // [item parity][query tile]
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int r1 = warp % 4 * 32 + lane / 8; r1 < warp % 4 * 32 + 32; r1 += 16) {
           uint4 x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = query_piece(a, b, h, row_first + r1 + 4 * i, lane % 8, q_vec);
+          for (int i = 0; i < 4; ++i) x[i] = query_piece(a, b, h, row_first + r1 + 4 * i, lane % 8, q_bytes);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = r1 + 4 * i;
@@ -602,15 +608,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_st();
           }
           const float4* sc = &scales[nt & 3][2 * half];
-          float cand = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t x[32];
-            tmem_ld32(tS + 32 * c, x);
-            const float f = fac * sc[c].x;  // (never 0: a masked key's -inf stays -inf)
-            tmem_wait_ld();
-            cand = fmaxf(cand, fmaf(max32(x), f < 1e-38f ? 1e-38f : f, sc[c].y));
-          }
+          uint32_t x0[32], x1[32];
+          tmem_ld32(tS, x0);
+          tmem_ld32(tS + 32, x1);
+          float f0 = fac * sc[0].x, f1 = fac * sc[1].x;  // (never 0: a masked key's -inf stays -inf)
+          f0 = f0 < 1e-38f ? 1e-38f : f0;
+          f1 = f1 < 1e-38f ? 1e-38f : f1;
+          tmem_wait_ld();
+          const float cand = fmaxf(fmaf(max32(x0), f0, sc[0].y), fmaf(max32(x1), f1, sc[1].y));
           float back = 1.f;
           bool grow = false;
           if (j == 0) {
@@ -626,9 +631,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 2; ++c) {
             uint32_t x[32];
             tmem_ld32(tS + 32 * c, x);
-            const float f = fac * sc[c].x;
+            const float f = c ? f1 : f0;
             tmem_wait_ld();
-            l = fmaf(weights32(x, f < 1e-38f ? 1e-38f : f, sc[c].y + lift, tS + 16 * c), sc[c].z, l);
+            l = fmaf(weights32(x, f, sc[c].y + lift, tS + 16 * c), sc[c].z, l);
           }
           // (the products before these scores are done: O may be changed)
           if (__any_sync(0xffffffffu, grow)) {
@@ -706,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           y[i] = a.type == kBF16 ? pack_bf16x2(o[2 * i], o[2 * i + 1]) : pack_half2(o[2 * i], o[2 * i + 1]);
-        if (o_vec && tiles > 0) {
+        if (tiles > 0) {
           *reinterpret_cast<uint4*>(stage + lane * 128 + ((4 * half + c) ^ (lane & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
         } else if (there) {
 #pragma unroll
@@ -718,14 +723,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free[qt]);
-        if (!part && o_vec) {
-          // four lanes a row: a store of the warp meets 8 lines (32 with a lane for each row)
+        if (!part) {
+          // 4 lanes a row (or 16, or 32 where rows are not aligned): a store of the warp meets 8 lines or
+          // fewer (32 with a lane for each row)
+          const int lanes = 64 / o_bytes < 32 ? 64 / o_bytes : 32, col = lane % lanes * (o_bytes / 2);
 #pragma unroll 1
-          for (int i = 0; i < 4; ++i) {
-            const int rr = 8 * i + lane / 4, c = lane % 4;
-            const int64_t to = __shfl_sync(0xffffffffu, out, rr);
-            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((4 * half + c) ^ (rr & 7)) * 16);
-            if (row - lane + rr < static_cast<uint32_t>(a.rows) && 8 * c < have) *reinterpret_cast<uint4*>(dst + to + 8 * c) = y;
+          for (int i = 0; i < lanes; ++i) {
+            const int rr = i * (32 / lanes) + lane / lanes;
+            const int64_t to = __shfl_sync(0xffffffffu, out, rr) + col;
+            const uint8_t* from = stage + rr * 128 + ((4 * half + col / 8) ^ (rr & 7)) * 16 + col % 8 * 2;
+            if (row - lane + rr >= static_cast<uint32_t>(a.rows) || col >= have) continue;
+            if (o_bytes == 16)
+              *reinterpret_cast<uint4*>(dst + to) = *reinterpret_cast<const uint4*>(from);
+            else if (o_bytes == 4)
+              *reinterpret_cast<uint32_t*>(dst + to) = *reinterpret_cast<const uint32_t*>(from);
+            else
+              dst[to] = *reinterpret_cast<const uint16_t*>(from);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -757,7 +770,7 @@ cudaError_t tc_typed(const Attention& a, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   tc_kernel<FP8><<<static_cast<unsigned>(items), kThreads, kSmem, stream>>>(
-      a, static_cast<uint32_t>(items), vectors(a.q, a.c.width), vectors(a.o, a.c.width));
+      a, static_cast<uint32_t>(items), access_bytes(a.q, a.c.width), access_bytes(a.o, a.c.width));
   return cudaGetLastError();
 }
 

@@ -140,17 +140,16 @@ struct Pieces {
 
 template <int TYPE, bool FP8, int ALIGN, int BLOCK>
 __global__ void __launch_bounds__(kWriteThreads)
-    write_kernel(View c, Rows rk, Rows rv, PerSequence start, PerSequence count, int64_t n, int64_t per_seq,
+    write_kernel(View c, Rows rk, Rows rv, PerSequence start, PerSequence count, int64_t n, uint32_t per_seq,
                  Pieces pieces) {
   constexpr int kEach = BLOCK * (kMaxWidth / 8) / kWriteThreads;
   constexpr float kTop = FP8 ? 448.f : 127.f;
-  int64_t unit = blockIdx.x;
-  const int h = static_cast<int>(unit % c.heads);
-  unit /= c.heads;
-  const int which = static_cast<int>(unit & 1);
-  unit >>= 1;
-  const int64_t j = unit % per_seq;
-  const int b = static_cast<int>(unit / per_seq);
+  uint32_t unit = blockIdx.x, rest = unit / static_cast<uint32_t>(c.heads);  // (32 bits: a division in 64 takes longer than the loads)
+  const int h = static_cast<int>(unit - rest * static_cast<uint32_t>(c.heads));
+  const int which = static_cast<int>(rest & 1);
+  rest >>= 1;
+  const int b = static_cast<int>(rest / per_seq);
+  const int64_t j = rest - static_cast<uint32_t>(b) * per_seq;
   const int64_t first = start.at(b), m = min(max(count.at(b), int64_t{0}), n);
   const int64_t lo = max(first, int64_t{0}), hi = min(first + m, c.cap);  // rows of the cache that get values
   const int64_t blk = lo / BLOCK + j, row0 = blk * BLOCK;
@@ -215,6 +214,7 @@ __global__ void __launch_bounds__(kWriteThreads)
 
 // ------------------------------------------------------------------ read back
 constexpr int kReadThreads = 256, kReadEach = 4;
+constexpr int kReadRows = kReadThreads * kReadEach / (kMaxWidth / 8);  // rows of a CTA
 
 template <int TYPE, int ALIGN>
 __device__ __forceinline__ void store8(void* base, int64_t at, const float (&y)[8], int have) {
@@ -254,42 +254,38 @@ __device__ __forceinline__ void store8(void* base, int64_t at, const float (&y)[
   }
 }
 
-// k, v [batch, heads, n, D]; one CTA: kReadThreads * kReadEach pieces of one (sequence, head)
+// k, v [batch, heads, n, D]; one CTA: kReadRows rows of one (sequence, head)
 template <int TYPE, bool FP8, int ALIGN>
 __global__ void __launch_bounds__(kReadThreads)
-    read_kernel(View c, void* k, void* v, int64_t start, int64_t n, int64_t chunks) {
-  int64_t unit = blockIdx.x;
-  const int64_t chunk = unit % chunks;
-  unit /= chunks;
+    read_kernel(View c, void* k, void* v, int64_t start, int64_t n, uint32_t chunks, Pieces pieces) {
+  const uint32_t unit = blockIdx.x / chunks, chunk = blockIdx.x - unit * chunks;
   const int which = static_cast<int>(unit & 1);
-  const int64_t bh = unit >> 1;
-  const int units = c.stored / 8;
-  const int64_t total = n * units;
-  const int64_t i0 = chunk * (kReadThreads * kReadEach) + threadIdx.x;
-  const uint2* src = reinterpret_cast<const uint2*>(c.data(which) + (bh * c.cap + start) * c.stored);
+  const int64_t bh = unit >> 1, row0 = static_cast<int64_t>(chunk) * kReadRows;
+  const int rows = static_cast<int>(min(n - row0, int64_t{kReadRows})), total = rows * pieces.units;
+  const uint2* src = reinterpret_cast<const uint2*>(c.data(which) + (bh * c.cap + start + row0) * c.stored);
   const float* scale = c.scale(which) + bh * c.blocks();
   void* out = which ? v : k;
+  const int64_t to = (bh * n + row0) * c.width;
   uint2 q[kReadEach];
   float s[kReadEach];
+  int row[kReadEach], u[kReadEach];
 #pragma unroll
   for (int e = 0; e < kReadEach; ++e) {
-    const int64_t i = i0 + e * kReadThreads;
+    const int i = threadIdx.x + e * kReadThreads;
+    pieces.at(i, row[e], u[e]);
     if (i < total) {
       q[e] = __ldg(src + i);
-      s[e] = __ldg(scale + ((start + i / units) >> c.block_log2));
+      s[e] = __ldg(scale + ((start + row0 + row[e]) >> c.block_log2));
     }
   }
 #pragma unroll
   for (int e = 0; e < kReadEach; ++e) {
-    const int64_t i = i0 + e * kReadThreads;
-    if (i < total) {
+    if (static_cast<int>(threadIdx.x) + e * kReadThreads < total) {
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         y[j] = __fmul_rn(code_value<FP8>(((j < 4 ? q[e].x : q[e].y) >> 8 * (j & 3)) & 0xffu), s[e]);
-      const int64_t row = i / units;
-      const int u = static_cast<int>(i - row * units);
-      store8<TYPE, ALIGN>(out, (bh * n + row) * c.width + u * 8, y, c.width - u * 8);
+      store8<TYPE, ALIGN>(out, to + row[e] * c.width + u[e] * 8, y, c.width - u[e] * 8);
     }
   }
 }
@@ -320,7 +316,7 @@ cudaError_t write_typed(const View& c, const Rows& k, const Rows& v, const PerSe
   const int units = c.stored / 8;
   const Pieces pieces{units, 65536u / units + 1};
   auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(grid), kWriteThreads, 0, stream>>>(c, k, v, start, count, n, per_seq, pieces);
+    kernel<<<static_cast<unsigned>(grid), kWriteThreads, 0, stream>>>(c, k, v, start, count, n, static_cast<uint32_t>(per_seq), pieces);
   };
   if (block == 32)
     go(write_kernel<TYPE, FP8, ALIGN, 32>);
@@ -333,10 +329,11 @@ cudaError_t write_typed(const View& c, const Rows& k, const Rows& v, const PerSe
 
 template <int TYPE, bool FP8, int ALIGN>
 cudaError_t read_typed(const View& c, void* k, void* v, int64_t start, int64_t n, cudaStream_t stream) {
-  const int64_t pieces = n * (c.stored / 8), chunks = (pieces + kReadThreads * kReadEach - 1) / (kReadThreads * kReadEach);
-  const int64_t grid = chunks * 2 * c.batch * c.heads;
+  const int64_t chunks = (n + kReadRows - 1) / kReadRows, grid = chunks * 2 * c.batch * c.heads;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
-  read_kernel<TYPE, FP8, ALIGN><<<static_cast<unsigned>(grid), kReadThreads, 0, stream>>>(c, k, v, start, n, chunks);
+  const int units = c.stored / 8;
+  read_kernel<TYPE, FP8, ALIGN><<<static_cast<unsigned>(grid), kReadThreads, 0, stream>>>(
+      c, k, v, start, n, static_cast<uint32_t>(chunks), Pieces{units, 65536u / units + 1});
   return cudaGetLastError();
 }
 

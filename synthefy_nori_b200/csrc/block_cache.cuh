@@ -46,10 +46,13 @@ struct Rows {
   }
 };
 
-// Whether 16-bit rows can be read and written 16 bytes at a time.
-inline bool vectors(const Rows& r, int width) {
-  return width % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.s0 % 8 == 0 && r.s1 % 8 == 0 && r.sn % 8 == 0 &&
-         r.sh % 8 == 0;
+// How many bytes of 16-bit rows can be read and written at a time: 16, 4 or 2.
+inline int access_bytes(const Rows& r, int width) {
+  for (int a : {8, 2})
+    if (width % a == 0 && reinterpret_cast<uintptr_t>(r.p) % (2 * a) == 0 && r.s0 % a == 0 && r.s1 % a == 0 &&
+        r.sn % a == 0 && r.sh % a == 0)
+      return 2 * a;
+  return 2;
 }
 
 // One value for all sequences or one of each, on the device.

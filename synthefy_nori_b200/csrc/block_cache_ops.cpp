@@ -99,7 +99,7 @@ bc::PerSequence per_sequence(const OptTensor& dev, int64_t all, const bc::View& 
 int sm_count(int dev) { return at::cuda::getDeviceProperties(dev)->multiProcessorCount; }
 
 // Up to this many rows of one K/V head run on the kernel that streams the cache through registers.
-constexpr int64_t kFewRows = 16;
+constexpr int64_t kFewRows = 32;
 
 // Splits of the keys of each cell for few rows, joined in clusters of up to 8.  A CTA's time goes with its
 // keys and a start and end worth some 400 more (measured), whatever else its SM runs, up to the 5 or
@@ -124,7 +124,7 @@ int tc_splits(int64_t cells, int64_t longest, int ctas) {
   double least = 0;
   for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
     const double waves = static_cast<double>((cells * s + ctas - 1) / ctas);
-    const double cost = waves * (static_cast<double>((tiles + s - 1) / s) + 3.0) + (s > 1 ? 4.0 + 0.04 * cells * s : 0.0);
+    const double cost = waves * (static_cast<double>((tiles + s - 1) / s) + 4.0) + (s > 1 ? 2.0 + 0.016 * cells * s : 0.0);
     if (s == 1 || cost < least) least = cost, best = static_cast<int>(s);
   }
   return best;
