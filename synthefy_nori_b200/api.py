@@ -72,7 +72,7 @@ class NoriRegressor(RegressorMixin, BaseEstimator):
         weights: str | None = None,
         n_estimators: int | None = None,
         inference_config=None,
-        cache_dtype: Literal["bf16", "int8"] | None = None,
+        cache_dtype: Literal["bf16", "int8", "block_int8", "block_fp8"] | None = None,
         memory_policy=None,
         query_chunk_size: int | None = None,
         quantile_collapse: str = "mean",

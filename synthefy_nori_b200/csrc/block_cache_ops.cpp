@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <string>
 
 #include "block_cache.cuh"
 #include "plain.h"
@@ -14,6 +15,10 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
+
+// Numbers in messages as text: streamed as numbers they end the process where the module and torch were
+// linked with different copies of the C++ library's locale facets.
+std::string num(int64_t x) { return std::to_string(x); }
 
 bc::View view_of(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t width, const char* who) {
   for (const Tensor* t : {&k, &v, &ks, &vs}) {
@@ -71,8 +76,8 @@ bc::Rows rows_of(const Tensor& t, const bc::View& c, int64_t n, int64_t heads, c
   const int64_t d = t.dim();
   TORCH_CHECK((d == 4 || d == 5) && t.size(d - 1) == c.width && t.size(d - 2) == heads && t.size(d - 3) == n &&
                   (d == 4 ? t.size(0) : t.size(0) * t.size(1)) == c.batch,
-              who, ": ", what, " must be [batch, n, heads, width] (or two batch dimensions), batch ", c.batch, ", n ", n,
-              ", heads ", heads, ", width ", c.width);
+              who, ": ", what, " must be [batch, n, heads, width] (or two batch dimensions), batch ", num(c.batch), ", n ",
+              num(n), ", heads ", num(heads), ", width ", num(c.width));
   TORCH_CHECK(c.width == 1 || t.stride(d - 1) == 1, who, ": the columns of ", what, " must be contiguous");
   bc::Rows r{};
   r.p = const_cast<void*>(t.const_data_ptr());
@@ -145,8 +150,8 @@ void block_cache_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, co
   const bc::PerSequence start = per_sequence(start_dev, start_all, c, ck.device(), who, "start");
   const bc::PerSequence count = per_sequence(count_dev, n, c, ck.device(), who, "counts");
   if (start.dev == nullptr)
-    TORCH_CHECK(start_all >= 0 && start_all + n <= c.cap, who, ": rows ", start_all, " to ", start_all + n,
-                " of a cache of ", c.cap);
+    TORCH_CHECK(start_all >= 0 && start_all + n <= c.cap, who, ": rows ", num(start_all), " to ",
+                num(start_all + n), " of a cache of ", num(c.cap));
   if (n == 0 || c.batch == 0 || c.heads == 0) return;
   const at::cuda::CUDAGuard guard(ck.device());
   C10_CUDA_CHECK(bc::launch_write(c, rk, rv, type, start, count, n, at::cuda::getCurrentCUDAStream()));
@@ -156,8 +161,8 @@ std::vector<Tensor> block_cache_read(const Tensor& ck, const Tensor& cv, const T
                                      int64_t width, int64_t start, int64_t n, c10::ScalarType out_type) {
   const char* who = "block_cache_read";
   const bc::View c = view_of(ck, cv, cks, cvs, width, who);
-  TORCH_CHECK(start >= 0 && n >= 0 && start <= c.cap && n <= c.cap - start, who, ": rows ", start, " to ", start + n,
-              " of a cache of ", c.cap);
+  TORCH_CHECK(start >= 0 && n >= 0 && start <= c.cap && n <= c.cap - start, who, ": rows ", num(start), " to ", num(start + n),
+              " of a cache of ", num(c.cap));
   const at::cuda::CUDAGuard guard(ck.device());
   std::vector<Tensor> out;
   for (int i = 0; i < 2; ++i)
@@ -180,8 +185,8 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   TORCH_CHECK(q.dim() >= 4, who, ": q [batch, n, heads, width] expected");
   a.n = q.size(-3);
   const int64_t heads = q.size(-2);
-  TORCH_CHECK(a.c.heads > 0 ? heads % a.c.heads == 0 : heads == 0, who, ": ", heads, " query heads do not share ",
-              a.c.heads, " K/V heads evenly");
+  TORCH_CHECK(a.c.heads > 0 ? heads % a.c.heads == 0 : heads == 0, who, ": ", num(heads),
+              " query heads do not share ", num(a.c.heads), " K/V heads evenly");
   a.type = float_type(q, false, who, "q");
   a.q = rows_of(q, a.c, a.n, heads, ck.device(), who, "q");
   const at::cuda::CUDAGuard guard(ck.device());
@@ -191,7 +196,7 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   a.o = rows_of(o, a.c, a.n, heads, ck.device(), who, "out");
   a.length = per_sequence(length_dev, length_all, a.c, ck.device(), who, "lengths");
   if (a.length.dev == nullptr)
-    TORCH_CHECK(length_all >= 0 && length_all <= a.c.cap, who, ": length ", length_all, " of a cache of ", a.c.cap);
+    TORCH_CHECK(length_all >= 0 && length_all <= a.c.cap, who, ": length ", num(length_all), " of a cache of ", num(a.c.cap));
   TORCH_CHECK(scale > 0.0 && scale < 1e30, who, ": a positive finite scale expected");
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   OptTensor lse;

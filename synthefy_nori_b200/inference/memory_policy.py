@@ -19,7 +19,9 @@ permission, on by default; the host budget is a share of the RAM the process may
 use: the smaller of the kernel's available memory and the container's cgroup limit).
 ``stream_*`` (explicit ``stream_context=True``): the cache lives on the host in blocks of
 ``context_row_chunk`` context rows and the device never holds a full layer; query
-attention merges the block partials by their log-sum-exps.  ``context_sharded_int8`` is
+attention merges the block partials by their log-sum-exps.  A cache type
+``"block_int8"`` or ``"block_fp8"`` (8 bits with a scale for each block of rows and head) takes
+the place of int8 on the resident, offload and stream rungs.  ``context_sharded_int8`` is
 this build's multi-GPU rung (the cache split by context rows over the GPUs of one node,
 ``parallel/context_parallel.py``).  ``escalated`` records a rung the caller moved to after
 an out-of-memory error (reference ``MemoryPolicy.escalated``).
@@ -31,7 +33,7 @@ from typing import Literal
 
 from pydantic import BaseModel, ConfigDict, Field, field_validator
 
-CacheDtype = Literal["bf16", "int8"]
+CacheDtype = Literal["bf16", "int8", "block_int8", "block_fp8"]
 MEMORY_PRESETS = ("exact", "max_context", "off")
 RUNGS = ("no_cache", "resident_bf16", "resident_int8", "offload_bf16", "offload_int8", "stream_bf16", "stream_int8",
          "context_sharded_int8", "context_row_chunk", "subsample", "plain_loop")
@@ -85,6 +87,13 @@ def estimate_cache_gb(*, n_context_rows: int, n_groups: int, nlayers: int, embed
 def int8_footprint_gb(est_bf16_gb: float, *, head_dim: int) -> float:
     """The same cache stored int8 with one fp32 scale per (token, head) vector."""
     return est_bf16_gb / 2.0 * (1.0 + 4.0 / max(head_dim, 1))
+
+
+def block_footprint_gb(est_bf16_gb: float, *, head_dim: int, block: int = 64) -> float:
+    """The same cache in 8 bits with one fp32 scale per (block of rows, head); stored head widths are
+    multiples of 8."""
+    d = max(head_dim, 1)
+    return est_bf16_gb / 2.0 * (-(-d // 8) * 8 / d + 4.0 / (block * d))
 
 
 class ContextTooLargeError(RuntimeError, MemoryError):
@@ -167,8 +176,9 @@ class MemoryPolicy(BaseModel):
             raise ValueError("stream_context=True requires offload_to_host=True (the stream lives in host RAM)")
         bf16 = estimate_cache_gb(n_context_rows=n_context_rows, n_groups=n_groups, nlayers=nlayers,
                                  embed_dim=embed_dim)
-        i8 = int8_footprint_gb(bf16, head_dim=head_dim)
-        q_ok = self.cache_dtype == "int8" or self.allow_quantization
+        footprint = block_footprint_gb if self.cache_dtype.startswith("block_") else int8_footprint_gb
+        i8 = footprint(bf16, head_dim=head_dim)
+        q_ok = self.cache_dtype != "bf16" or self.allow_quantization
         budget = self.budget_gb(device_total_gb)
         upd = {"est_cache_gb": bf16, "dropped_context_rows": 0}
         per_layer = bf16 / max(nlayers, 1)
@@ -176,7 +186,7 @@ class MemoryPolicy(BaseModel):
             upd.update(rung="no_cache", resident_gb=0.0)
         elif self.stream_context:
             chunk = self.context_row_chunk or default_stream_row_chunk(device_total_gb)
-            use_i8 = self.cache_dtype == "int8"
+            use_i8 = self.cache_dtype != "bf16"
             host = self.host_budget(host_total_gb)
             size = i8 if use_i8 else bf16
             if size > host:
@@ -244,7 +254,9 @@ class MemoryPolicy(BaseModel):
     def placement(self) -> tuple[str, str, int | None]:
         """(cache dtype, placement, stream block rows) of the resolved rung."""
         r = self.rung or "resident_bf16"
-        dtype = "int8" if (r.endswith("int8") or self.cache_dtype == "int8") else "bf16"
+        dtype = self.cache_dtype
+        if dtype == "bf16" and r.endswith("int8"):
+            dtype = "int8"
         if r in OFFLOAD_RUNGS:
             return dtype, "offload", None
         if r in STREAM_RUNGS:

@@ -106,8 +106,8 @@ class NoriPredictor:
             device = "cuda" if torch.cuda.is_available() else "cpu"
         self.device = torch.device(device)
         self.model = model.to(self.device).eval()
-        if cache_dtype not in ("bf16", "int8"):
-            raise ValueError("cache_dtype must be 'bf16' or 'int8'")
+        if cache_dtype not in ("bf16", "int8", "block_int8", "block_fp8"):
+            raise ValueError("cache_dtype must be 'bf16', 'int8', 'block_int8' or 'block_fp8'")
         if n_estimators is not None and n_estimators < 1:
             raise ValueError("n_estimators must be >= 1")
         self.inference_config = resolve_inference_config(inference_config, model, n_estimators)

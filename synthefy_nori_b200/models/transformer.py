@@ -476,21 +476,25 @@ class FeaturesTransformer(nn.Module):
     # ------------------------------------------------------------------ context cache
     def build_context_cache(self, x_train, y_train, *, cache_dtype: str = "bf16", fit_row_chunk=None,
                             placement: str = "resident", stream_block_rows: int | None = None, **_) -> ContextCache:
-        """Per-layer cross-attention K/V of the context rows.  ``placement``: ``"resident"``
+        """Per-layer cross-attention K/V of the context rows, in bf16, int8 with a scale for each
+        vector, or (``"block_int8"``, ``"block_fp8"``: the native path only) int8 / e4m3 with a
+        scale for each 64 rows and head, which the query attention reads directly.  ``placement``: ``"resident"``
         (device), ``"offload"`` (pinned host, one layer copied in at a time) or
         ``"stream"`` (pinned host in blocks of ``stream_block_rows`` context rows, the
         query attention merging block partials) - the native path only."""
         if not self.supports_context_cache:
             raise NotImplementedError("context caching is not implemented for the two-phase encoder")
-        if cache_dtype not in ("bf16", "int8"):
-            raise ValueError(f"build_context_cache takes cache_dtype 'bf16' or 'int8', got {cache_dtype!r}")
+        if cache_dtype not in ("bf16", "int8", "block_int8", "block_fp8"):
+            raise ValueError("build_context_cache takes cache_dtype 'bf16', 'int8', 'block_int8' or 'block_fp8', got "
+                             f"{cache_dtype!r}")
+        block = cache_dtype.startswith("block_")  # a scale for each block of rows and head
         if self.mask_prediction:
             raise NotImplementedError("build_context_cache requires mask_prediction=False")
         tokens, context = self.context_tokens(x_train, y_train)
         if self.use_native(tokens.device) and _native_cache_available():
             from synthefy_nori_b200.ops.fused_layer import build_stack_cache
 
-            caches = build_stack_cache(self, tokens, quantize=cache_dtype == "int8")
+            caches = build_stack_cache(self, tokens, quantize=cache_dtype if block else cache_dtype == "int8")
             if placement != "resident":
                 from synthefy_nori_b200.ops.fused_layer import place_caches
 
@@ -498,6 +502,8 @@ class FeaturesTransformer(nn.Module):
         else:
             if placement != "resident":
                 raise NotImplementedError("host-offloaded / streamed caches need the native CUDA path")
+            if block:
+                raise NotImplementedError("block-scaled caches need the native CUDA path")
             _, caches = self.transformer_encoder.build_train_cache(tokens, quantize=cache_dtype == "int8")
         context.caches = caches
         return context

@@ -812,6 +812,85 @@ class NativeKV:
         return (self.kv.view(-1, 2, g.H, g.Dp).float() * self.scale.view(-1, 2, g.H, 1)).to(BF16).view(-1, 2 * g.A)
 
 
+#: Cache types with a scale for each block of rows and head (``ops.block_cache``).
+BLOCK_CACHES = {"block_int8": torch.int8, "block_fp8": torch.float8_e4m3fn}
+
+
+class BlockKV:
+    """Cross-attention K/V of one layer for a fixed context as an ``ops.BlockCache``: sequences are
+    (table, token) pairs, int8 or e4m3 codes with one scale for each 64 context rows and head.
+    The query attention reads the codes themselves (no bf16 copy of a layer).  Shared K/V
+    heads are stored once.  Codes and scales lie in one buffer, ``flat``, which moves as a whole."""
+
+    BLOCK = 64
+    quantized = True
+
+    def __init__(self, flat: torch.Tensor, g: Geometry, dtype: str, heads: int):
+        self.flat, self.g, self.dtype, self.heads = flat, g, dtype, heads
+        self.n_rows = g.ep
+        cap, seqs = self._capacity(g), g.B * g.T
+        codes, scales = (seqs, heads, cap, g.Dp), (seqs, heads, cap // self.BLOCK)
+        nc, ns = math.prod(codes), 4 * math.prod(scales)
+        at = (0, nc, 2 * nc, 2 * nc + ns, 2 * nc + 2 * ns)
+        part = [flat[a:b] for a, b in zip(at, at[1:])]
+        self.cache = ops.BlockCache(*(t.view(BLOCK_CACHES[dtype]).view(codes) for t in part[:2]),
+                                    *(t.view(torch.float32).view(scales) for t in part[2:]), g.Dp)
+
+    @staticmethod
+    def _capacity(g: Geometry) -> int:
+        return -(-max(g.ep, 1) // 128) * 128
+
+    @classmethod
+    def empty(cls, g: Geometry, dtype: str, heads: int, device) -> "BlockKV":
+        cap = cls._capacity(g)
+        n = g.B * g.T * heads * (2 * cap * g.Dp + 8 * (cap // cls.BLOCK))
+        return cls(torch.empty(n, dtype=torch.uint8, device=device), g, dtype, heads)
+
+    def write(self, kv: torch.Tensor, start: int = 0) -> "BlockKV":
+        """Context rows ``start ..`` from the projection output ``kv [B * n * T, 2A]`` (any row stride)."""
+        g = self.g
+        rows = kv.view(g.B, -1, g.T, 2, g.H, g.Dp)
+        k, v = (rows[:, :, :, i, : self.heads].permute(0, 2, 1, 3, 4) for i in (0, 1))
+        ops.block_cache_write(self.cache, k, v, start=start)
+        return self
+
+    def attend(self, q: torch.Tensor, o: torch.Tensor, g: Geometry, mult: float, return_lse: bool = False):
+        """``q``, ``o`` [B * nq * T, A] token-major; the log-sum-exp [B * T * H, nq] where it is wanted."""
+        qv, ov = (t.view(g.B, g.nq, g.T, g.H, g.Dp).permute(0, 2, 1, 3, 4) for t in (q, o))
+        r = ops.block_cache_attention(qv, self.cache, g.ep, scale=mult / math.sqrt(g.D), out=ov, return_lse=return_lse)
+        return r[1].view(-1, g.nq) if return_lse else None
+
+    def rows(self, r0: int, r1: int) -> "BlockKV":
+        """Rows ``r0 .. r1`` (``r0`` a multiple of 128) as a cache of their own."""
+        g = self.g
+        part = BlockKV.empty(Geometry(B=g.B, ep=r1 - r0, nq=0, T=g.T, E=g.E, H=g.H), self.dtype, self.heads,
+                             self.flat.device)
+        c0, c1 = r0 // self.BLOCK, (r0 + part.cache.capacity) // self.BLOCK
+        for dst, src in zip(part.cache[:2], self.cache[:2]):
+            dst.view(torch.uint8).copy_(src.view(torch.uint8)[:, :, r0 : r0 + dst.shape[2]])
+        for dst, src in zip(part.cache[2:4], self.cache[2:4]):
+            dst.copy_(src[:, :, c0:c1])
+        return part
+
+    def dequantize(self) -> torch.Tensor:
+        """bf16 ``[B * N * T, 2A]`` (K then V, every head), as the other caches give it."""
+        g = self.g
+        kv = torch.stack(ops.block_cache_read(self.cache, 0, g.ep, dtype=BF16), 2)  # [B T, N, 2, heads, Dp]
+        kv = kv.view(g.B, g.T, g.ep, 2, self.heads, g.Dp).expand(-1, -1, -1, -1, g.H, -1)
+        return kv.transpose(1, 2).reshape(-1, 2 * g.A)
+
+    def nbytes(self) -> int:
+        return self.flat.numel()
+
+
+def _cache_kv(kv: torch.Tensor, g: Geometry, quantize, layer):
+    """The cache of one layer from its projected cross K/V: bf16, int8 per vector (``quantize=True``), or
+    one of ``BLOCK_CACHES`` by name."""
+    if quantize in BLOCK_CACHES:
+        return BlockKV.empty(g, quantize, 1 if layer.cross_share_all_kv_heads else g.H, kv.device).write(kv)
+    return NativeKV.from_bf16(kv, g, bool(quantize))
+
+
 class HostKV:
     """A layer's cross-attention K/V kept in pinned host memory, in row blocks.
 
@@ -823,17 +902,28 @@ class HostKV:
     device never holds a full layer.  Reference: ``model/kv_cache_scaling.py``
     (``ScalableSeqKV`` offload, ``BlockwiseSeqKV`` streaming)."""
 
-    def __init__(self, blocks: list, g: Geometry, quantized: bool):
-        self.blocks = blocks  # [(n_rows, kv_host [B * n_rows * T, 2E], scale_host | None)]
+    def __init__(self, blocks: list, g: Geometry, quantized: bool, block_form: tuple | None = None):
+        self.blocks = blocks  # [(n_rows, kv_host [B * n_rows * T, 2E] (or a BlockKV's buffer), scale_host | None)]
         self.g = g
         self.quantized = quantized
+        self.block_form = block_form  # (type, heads) of a BlockKV
         self.n_rows = g.ep
 
+    def on_device(self, n: int, kd: torch.Tensor, sd: torch.Tensor | None):
+        """A staged block as a cache on the device."""
+        g = Geometry(B=self.g.B, ep=n, nq=0, T=self.g.T, E=self.g.E, H=self.g.H)
+        return NativeKV(kd, g, sd) if self.block_form is None else BlockKV(kd, g, *self.block_form)
+
     @classmethod
-    def from_native(cls, kv: NativeKV, block_rows: int | None) -> "HostKV":
+    def from_native(cls, kv, block_rows: int | None) -> "HostKV":
         g = kv.g
         n = g.ep
         step = n if not block_rows or block_rows >= n else int(block_rows)
+        if isinstance(kv, BlockKV):
+            step = n if step == n else max(128, step // 128 * 128)  # (whole tiles of the cache)
+            blocks = [(min(n, r0 + step) - r0, (kv if step == n else kv.rows(r0, min(n, r0 + step))).flat.cpu().pin_memory(),
+                       None) for r0 in range(0, n, step)]
+            return cls(blocks, g, True, (kv.dtype, kv.heads))
         blocks = []
         kv4 = kv.kv.view(g.B, n, g.T, -1)
         sc4 = kv.scale.view(g.B, n, g.T, -1) if kv.scale is not None else None
@@ -1011,7 +1101,7 @@ def _build_rows_chunk(g: Geometry, hid: int, n_layers: int, quantize: bool, devi
     return max(256, min(g.ep, int(avail // (per_tok_chunk * g.T))))
 
 
-def _seq_ctx_forward_chunked(layer, w, x, g: Geometry, rows: int, quantize: bool):
+def _seq_ctx_forward_chunked(layer, w, x, g: Geometry, rows: int, quantize):
     """``_seq_ctx_forward`` for one table (B = 1) with the row-wise work in chunks of ``rows``
     context rows: only the self-attention K / V ([R, 2E]) exist at full height; queries,
     attention outputs and the cross-attention K / V are formed chunk by chunk, and the
@@ -1027,7 +1117,10 @@ def _seq_ctx_forward_chunked(layer, w, x, g: Geometry, rows: int, quantize: bool
         w_qc = torch.cat((wb["w_ctx"][:A], wb["w_ctx"][3 * A :]), 0).contiguous()
         wb["w_qcross_ctx"] = w_qc
     out = torch.empty_like(x)
-    if quantize:
+    block_kv = None
+    if quantize in BLOCK_CACHES:
+        block_kv = BlockKV.empty(g, quantize, 1 if layer.cross_share_all_kv_heads else g.H, x.device)
+    elif quantize:
         kv_q = torch.empty(R, 2 * A, device=x.device, dtype=torch.int8)
         kv_s = torch.empty(R, 2 * g.H, device=x.device, dtype=torch.float32)
     else:
@@ -1046,7 +1139,9 @@ def _seq_ctx_forward_chunked(layer, w, x, g: Geometry, rows: int, quantize: bool
         _attn(qc, kv_self[:, :A], kv_self[:, A:], oc, lc, l2, lc, BTH, nc, g.ep, g,
               mult=_attn_mult(w.get("info_self"), g.ep))
         ops.gemm_residual(oc, wb["wo_self"], xc, alpha, out=out[r0:r1], w_kn=True)
-        if quantize:
+        if block_kv is not None:
+            block_kv.write(yc[:, A:], start=n0)
+        elif quantize:
             q8, sc = ops.quantize_int8(yc[:, A:].reshape(r1 - r0, 2, g.H, g.Dp))
             kv_q[r0:r1] = q8.reshape(r1 - r0, 2 * A)
             kv_s[r0:r1] = sc.reshape(r1 - r0, 2 * g.H)
@@ -1054,6 +1149,8 @@ def _seq_ctx_forward_chunked(layer, w, x, g: Geometry, rows: int, quantize: bool
             kv_b[r0:r1] = yc[:, A:]
         del yc, qc, oc
     del kv_self
+    if block_kv is not None:
+        return out, block_kv
     kv = NativeKV(kv_q, g, kv_s) if quantize else NativeKV(kv_b, g)
     return out, kv
 
@@ -1069,9 +1166,9 @@ def _rowwise_chunked(fn, x, rows_tok: int):
 
 
 @torch.no_grad()
-def build_stack_cache(model, tokens: torch.Tensor, quantize: bool = False) -> list:
+def build_stack_cache(model, tokens: torch.Tensor, quantize: bool | str = False) -> list:
     """Run the context tokens ``[B, N, T, E]`` through every layer and keep each layer's
-    cross-attention K/V (reference ``LayerStack.build_train_cache``, layer.py:2058-2096).
+    cross-attention K/V, in bf16, int8 per vector (``quantize=True``) or a type of ``BLOCK_CACHES`` by name (reference ``LayerStack.build_train_cache``, layer.py:2058-2096).
     A single long table is processed in row chunks when one layer's full-height
     intermediates would not fit next to the caches (``_build_rows_chunk``)."""
     check_supported(model)
@@ -1079,7 +1176,7 @@ def build_stack_cache(model, tokens: torch.Tensor, quantize: bool = False) -> li
     g = Geometry(B=B, ep=N, nq=0, T=T, E=E, H=model.nhead)
     x = tokens.to(BF16).reshape(-1, E).contiguous()
     hid = int(layer_weights(model.transformer_encoder.layers[0])["w_down"].shape[1])  # SwiGLU hidden width
-    rows = _build_rows_chunk(g, hid, len(model.transformer_encoder.layers), quantize, x.device)
+    rows = _build_rows_chunk(g, hid, len(model.transformer_encoder.layers), bool(quantize), x.device)
     if rows < N:
         caches = []
         for layer in model.transformer_encoder.layers:
@@ -1095,7 +1192,7 @@ def build_stack_cache(model, tokens: torch.Tensor, quantize: bool = False) -> li
         w = layer_weights(layer)
         w["wb"] = _cached_bf16(layer, w)
         x, kv = _seq_ctx_forward(layer, w, x, g)
-        caches.append({"seq_kv": NativeKV.from_bf16(kv, g, quantize)})
+        caches.append({"seq_kv": _cache_kv(kv, g, quantize, layer)})
         x = _mlp_forward(layer, w, x)
         x = _feat_forward(layer, w, x, g)
     return caches
@@ -1127,7 +1224,7 @@ def run_stack_cached(model, tokens: torch.Tensor, caches: list) -> torch.Tensor:
             n, kd, sd = _Stager.wait(pending)
             if li + 1 < len(caches):  # the next layer's copy overlaps this layer
                 pending = stager.issue(caches[li + 1]["seq_kv"].blocks[0])
-            x = _seq_query_forward(layer, w, x, NativeKV(kd, kv.g, sd), g)
+            x = _seq_query_forward(layer, w, x, kv.on_device(n, kd, sd), g)
         elif isinstance(kv, HostKV):
             x = _seq_query_forward_streamed(layer, w, x, kv, g, stager)
         else:
@@ -1159,15 +1256,18 @@ def _seq_query_forward_streamed(layer, w, x, hkv: HostKV, g: Geometry, stager: "
         if bi + 1 < len(blocks):
             nxt = stager.issue(blocks[bi + 1])
         gb = Geometry(B=g.B, ep=n, nq=g.nq, T=g.T, E=E, H=g.H)
-        kvb = NativeKV(kd, gb, sd).dequantize() if sd is not None else kd
-        l2 = _seq_layout(n, gb, 2 * A)
-        _attn(q, kvb[:, :A], kvb[:, A:], o, lq, l2, lq, BTH, g.nq, n, g, lse=lse, mult=mult)
+        if hkv.block_form is not None:
+            lse = hkv.on_device(n, kd, sd).attend(q, o, gb, mult, return_lse=True)
+        else:
+            kvb = NativeKV(kd, gb, sd).dequantize() if sd is not None else kd
+            l2 = _seq_layout(n, gb, 2 * A)
+            _attn(q, kvb[:, :A], kvb[:, A:], o, lq, l2, lq, BTH, g.nq, n, g, lse=lse, mult=mult)
         ops.lib().attn_lse_merge(acc, lse_acc, o, lse, g.T, g.H, g.nq, bi == 0)
     return ops.gemm_residual(acc.to(BF16), w["wb"]["wo_cross"], x, _layer_alpha(layer), w_kn=True)
 
 
 @torch.no_grad()
-def _seq_query_forward(layer, w, x, kv: NativeKV, g: Geometry, lse=None, partial_out=None):
+def _seq_query_forward(layer, w, x, kv, g: Geometry, lse=None, partial_out=None):
     A = g.A
     rs = ops.rms_scale(x, layer.layer_norm_eps)
     yq = ops.gemm(x, w["wb"]["w_q"], row_scale=rs)
@@ -1175,9 +1275,14 @@ def _seq_query_forward(layer, w, x, kv: NativeKV, g: Geometry, lse=None, partial
     o = torch.empty(x.shape[0], A, device=x.device, dtype=BF16)
     lq = _seq_layout(g.nq, g, A)
     BTH = g.B * g.T * g.H
-    scratch = _dequant_scratch(kv) if kv.quantized else None
+    block = isinstance(kv, BlockKV)
+    scratch = _dequant_scratch(kv) if kv.quantized and not block else None
     mult = _attn_mult(w.get("info_cross"), g.ep)
-    if scratch is not None:
+    if block:
+        got = kv.attend(q, o, g, mult, return_lse=lse is not None)
+        if lse is not None:
+            lse.copy_(got.view_as(lse))
+    elif scratch is not None:
         # one GPU: expand the int8 cache to bf16 (a memory-bound pass, ~1/50 of the attention
         # time) so the query attention runs on the tcgen05 kernel; same values as the
         # reference's dequantise-then-attend
