@@ -25,7 +25,7 @@
 // The maximum is lazy (O is rescaled when it grows by more than 2^4); w is kept at up to 2^15 so
 // that fp16 holds 11 bits down to 2^-25 of the largest weight.  Scores, sums and O are fp32.
 // All exponentials run on the MUFU: a polynomial on the FMA pipe for a quarter of them made a tile
-// slower (3634 cycles for 3180), since the warps' issue slots are as scarce as the MUFU.
+// a seventh slower, since the warps' issue slots are as scarce as the MUFU.
 //
 // Every wait is bounded (sm100.cuh); on a timeout the CTA records it in the status word, waits for
 // its own copies and products, frees its TMEM and returns.
@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++asked;
       };
       auto answered = [&](uint32_t& w) -> bool {  // the item taken over, `items` where there is none left
+        if (!mbar_wait(taken, (asked - 1) & 1, a.status, kTimeoutProducer, abort_flag)) return false;
         uint32_t got, id;
         asm volatile(
             "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"

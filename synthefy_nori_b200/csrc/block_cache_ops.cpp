@@ -1,5 +1,6 @@
 // Entry points of the context cache in 8 bits with block scales: checks of the arguments, the
 // choice of kernel and of how far the keys are split.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -122,12 +123,13 @@ int few_splits(int64_t cells, int64_t longest, int resident) {
 }
 
 // Splits of the keys for the persistent kernel: the waves of items, each as long as its key tiles
-// and the start and end of an item; partial results cost a second kernel and their traffic.
+// and the start and end of an item; partial results cost a second kernel and their traffic (and a
+// workspace, held to 16 items an SM: 155 MB).
 int tc_splits(int64_t cells, int64_t longest, int ctas) {
   const int64_t tiles = std::max<int64_t>((longest + bc::kTile - 1) / bc::kTile, 1);
   int best = 1;
   double least = 0;
-  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
+  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64) && (s == 1 || cells * s <= 16 * ctas); ++s) {
     const double waves = static_cast<double>((cells * s + ctas - 1) / ctas);
     const double cost = waves * (static_cast<double>((tiles + s - 1) / s) + 4.0) + (s > 1 ? 2.0 + 0.016 * cells * s : 0.0);
     if (s == 1 || cost < least) least = cost, best = static_cast<int>(s);
@@ -150,8 +152,8 @@ void block_cache_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, co
   const bc::PerSequence start = per_sequence(start_dev, start_all, c, ck.device(), who, "start");
   const bc::PerSequence count = per_sequence(count_dev, n, c, ck.device(), who, "counts");
   if (start.dev == nullptr)
-    TORCH_CHECK(start_all >= 0 && start_all + n <= c.cap, who, ": rows ", num(start_all), " to ",
-                num(start_all + n), " of a cache of ", num(c.cap));
+    TORCH_CHECK(start_all >= 0 && n <= c.cap && start_all <= c.cap - n, who, ": ", num(n), " rows from ", num(start_all),
+                " on of a cache of ", num(c.cap));
   if (n == 0 || c.batch == 0 || c.heads == 0) return;
   const at::cuda::CUDAGuard guard(ck.device());
   C10_CUDA_CHECK(bc::launch_write(c, rk, rv, type, start, count, n, at::cuda::getCurrentCUDAStream()));
@@ -161,8 +163,8 @@ std::vector<Tensor> block_cache_read(const Tensor& ck, const Tensor& cv, const T
                                      int64_t width, int64_t start, int64_t n, c10::ScalarType out_type) {
   const char* who = "block_cache_read";
   const bc::View c = view_of(ck, cv, cks, cvs, width, who);
-  TORCH_CHECK(start >= 0 && n >= 0 && start <= c.cap && n <= c.cap - start, who, ": rows ", num(start), " to ", num(start + n),
-              " of a cache of ", num(c.cap));
+  TORCH_CHECK(start >= 0 && n >= 0 && start <= c.cap && n <= c.cap - start, who, ": ", num(n), " rows from ",
+              num(start), " on of a cache of ", num(c.cap));
   const at::cuda::CUDAGuard guard(ck.device());
   std::vector<Tensor> out;
   for (int i = 0; i < 2; ++i)
@@ -193,6 +195,7 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   const bool given = out.has_value() && out->defined();
   const Tensor o = given ? *out : torch::empty(q.sizes(), q.options());
   TORCH_CHECK(o.scalar_type() == q.scalar_type() && o.sizes() == q.sizes(), who, ": out of q's shape and type expected");
+  TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes, who, ": rows of out share memory");
   a.o = rows_of(o, a.c, a.n, heads, ck.device(), who, "out");
   a.length = per_sequence(length_dev, length_all, a.c, ck.device(), who, "lengths");
   if (a.length.dev == nullptr)
@@ -205,6 +208,7 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   a.lse = want_lse ? lse->data_ptr<float>() : nullptr;
   a.group = static_cast<int>(heads / a.c.heads);
   a.rows = a.n * a.group;
+  TORCH_CHECK(a.rows < INT32_MAX - bc::kPairRows, who, ": 2^31 or more query rows of one K/V head");
   a.status = status.data_ptr<int>();
   // the longest a sequence can be (lengths on the device are not read here)
   const int64_t longest = a.length.dev != nullptr ? a.c.cap : length_all;
