@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       uint32_t cur = blockIdx.x, nxt = items;
-      ask();
       ok = tell(cur);
       while (ok && cur < items) {
         const Item& it = known[(told - 1) % kItems];  // (told only now: its slot is not reused before this item is done)
@@ -383,12 +382,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           return true;
         };
         if (tiles > 0 && !(ok = load(0, a.c.k, rK, rk_full, rk_empty, nk))) break;
-        if (!(ok = answered(nxt) && tell(nxt))) break;
-        if (nxt < items) ask();  // (not again after a refusal)
+        // the next item is asked for two tiles before it is needed and no sooner: it would be held back from
+        // a CTA that is done earlier (never again after a refusal: the loop ends there)
+        if (tiles == 0) ask();
         for (int j = 0; ok && j < tiles; ++j) {
+          if (j == max(tiles - 2, 0)) ask();
           if (j + 1 < tiles) ok = load(j + 1, a.c.k, rK, rk_full, rk_empty, nk);
           if (ok) ok = load(j, a.c.v, rV, rv_full, rv_empty, nv);
         }
+        if (!ok || !(ok = answered(nxt) && tell(nxt))) break;
         cur = nxt;
       }
       // own copies and requests in flight (after an abort nobody else waits for them)
