@@ -411,7 +411,10 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
       if (d == 0) fin_ml[r] = make_float2(top, sum);
     }
   }
-  if (a.cluster == 1) return;
+  // where this kernel was launched beside one that still runs: what follows on the stream waits for this one
+  // alone, so it ends no sooner
+  const auto wait_beside = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+  if (a.cluster == 1) return wait_beside();
   // join the cluster: every CTA has written its part; the threads of all share the values
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -439,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
     put_row(r, d, top, sum, acc);
   }
   cluster.sync();  // nobody leaves while its shared memory is read
+  wait_beside();
 }
 
 // Joins the parts of a row.  Few parts: a warp takes a row, two values a lane; many: a CTA takes a row,
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
 }
 
 template <bool FP8, int NT, int W>
-cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
+cudaError_t few_typed(const Attention& a, bool beside, cudaStream_t stream) {
   constexpr int kRows = 8 * NT;
   const int64_t grid = (a.rows - a.first + kRows - 1) / kRows * a.splits * a.c.batch * a.c.heads;
   if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
@@ -506,12 +510,19 @@ cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(a.cluster);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+  cudaLaunchAttribute attr[2]{};
+  cfg.attrs = attr;
+  if (a.cluster > 1) {
+    cudaLaunchAttribute& x = attr[cfg.numAttrs++];
+    x.id = cudaLaunchAttributeClusterDimension;
+    x.val.clusterDim.x = static_cast<unsigned>(a.cluster);
+    x.val.clusterDim.y = x.val.clusterDim.z = 1;
+  }
+  if (beside) {
+    cudaLaunchAttribute& x = attr[cfg.numAttrs++];
+    x.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    x.val.programmaticStreamSerializationAllowed = 1;
+  }
   return cudaLaunchKernelEx(&cfg, few_kernel<FP8, NT, W>, a, access_bytes(a.q, a.c.width) == 16);
 }
 
@@ -520,12 +531,12 @@ cudaError_t few_typed(const Attention& a, cudaStream_t stream) {
 int few_tile_rows(int64_t rows) { return rows > 8 ? 16 : 8; }
 int few_resident(int64_t rows) { return resident(few_tile_rows(rows) / 8); }
 
-cudaError_t launch_few(const Attention& a, cudaStream_t stream) {
+cudaError_t launch_few(const Attention& a, bool beside, cudaStream_t stream) {
   const bool two = few_tile_rows(a.rows - a.first) == 16;
   auto go = [&](auto w) {
     constexpr int W = w.value;
-    if (a.c.fp8) return two ? few_typed<true, 2, W>(a, stream) : few_typed<true, 1, W>(a, stream);
-    return two ? few_typed<false, 2, W>(a, stream) : few_typed<false, 1, W>(a, stream);
+    if (a.c.fp8) return two ? few_typed<true, 2, W>(a, beside, stream) : few_typed<true, 1, W>(a, beside, stream);
+    return two ? few_typed<false, 2, W>(a, beside, stream) : few_typed<false, 1, W>(a, beside, stream);
   };
   switch (a.c.stored) {
     case 8: return go(std::integral_constant<int, 8>());

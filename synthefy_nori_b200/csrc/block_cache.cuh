@@ -149,7 +149,8 @@ cudaError_t launch_read(const View& c, void* k, void* v, int type, int64_t start
 // rows of a tile of the two attention kernels, and how many splits of the keys they would take
 int few_tile_rows(int64_t rows);
 int few_resident(int64_t rows);  // CTAs that an SM holds
-cudaError_t launch_few(const Attention& a, cudaStream_t stream);
+// beside: it may start while the kernel before it on the stream, which it does not depend on, still runs
+cudaError_t launch_few(const Attention& a, bool beside, cudaStream_t stream);
 // rows of a tile pair of the kernel for many rows; one CTA per SM
 constexpr int kPairRows = 256;
 cudaError_t launch_tc(const Attention& a, cudaStream_t stream);

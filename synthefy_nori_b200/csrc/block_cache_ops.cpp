@@ -214,29 +214,42 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   const int64_t longest = a.length.dev != nullptr ? a.c.cap : length_all;
   const int sms = sm_count(ck.get_device());
   const auto stream = at::cuda::getCurrentCUDAStream();
-  auto run = [&](int64_t first, int64_t end, bool few) {
-    a.first = first;
-    a.rows = end;
+  Tensor part_o[2], part_ml[2];
+  auto plan = [&](int64_t first, int64_t end, bool few) {  // rows first .. end - 1 on one of the kernels
+    bc::Attention p = a;
+    p.first = first;
+    p.rows = end;
     const int tile = few ? bc::few_tile_rows(end - first) : bc::kPairRows;
     const int64_t cells = (end - first + tile - 1) / tile * a.c.batch * a.c.heads;
-    a.splits = few ? few_splits(cells, longest, sms * bc::few_resident(end - first)) : tc_splits(cells, longest, sms);
-    a.cluster = few ? std::min(a.splits, 8) : 1;
-    const int parts = a.splits / a.cluster;
-    Tensor part_o, part_ml;
+    p.splits = few ? few_splits(cells, longest, sms * bc::few_resident(end - first)) : tc_splits(cells, longest, sms);
+    p.cluster = few ? std::min(p.splits, 8) : 1;
+    const int parts = p.splits / p.cluster;
     if (parts > 1) {
-      part_o = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
-      part_ml = torch::empty({cells * parts * tile * 2}, cks.options());
-      a.part_o = part_o.data_ptr<float>();
-      a.part_ml = reinterpret_cast<float2*>(part_ml.data_ptr<float>());
+      part_o[few] = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
+      part_ml[few] = torch::empty({cells * parts * tile * 2}, cks.options());
+      p.part_o = part_o[few].data_ptr<float>();
+      p.part_ml = reinterpret_cast<float2*>(part_ml[few].data_ptr<float>());
     }
-    C10_CUDA_CHECK(few ? bc::launch_few(a, stream) : bc::launch_tc(a, stream));
-    if (parts > 1) C10_CUDA_CHECK(bc::launch_combine(a, tile, stream));
+    return p;
+  };
+  auto join = [&](const bc::Attention& p, bool few) {
+    if (p.splits > p.cluster)
+      C10_CUDA_CHECK(bc::launch_combine(p, few ? bc::few_tile_rows(p.rows - p.first) : bc::kPairRows, stream));
   };
   // a few rows behind the last whole pair of tiles would cost a pair's time on the tensor cores
   const int64_t rows = a.rows, whole = rows / bc::kPairRows * bc::kPairRows;
   const int64_t many = rows - whole > kFewRows ? rows : whole;
-  if (many > 0) run(0, many, false);
-  if (many < rows) run(many, rows, true);
+  bc::Attention tc{}, few{};
+  if (many > 0) {
+    tc = plan(0, many, false);
+    C10_CUDA_CHECK(bc::launch_tc(tc, stream));
+  }
+  if (many < rows) {
+    few = plan(many, rows, true);
+    C10_CUDA_CHECK(bc::launch_few(few, many > 0, stream));
+  }
+  join(tc, false);
+  join(few, true);
   return {o, lse};
 }
 
