@@ -445,55 +445,91 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
   wait_beside();
 }
 
-// Joins the parts of a row.  Few parts: a warp takes a row, two values a lane; many: a CTA takes a row,
-// each warp a run of its parts.  Started while the kernel before it still runs (its last CTAs leave the
+// Joins the parts of a row: 16 lanes, four values each, take its parts four at a time (so that their loads
+// do not wait for one another) under a running maximum.  Few parts: a CTA takes 16 rows; many: a CTA takes a
+// row, its 16 groups of lanes every 16th part.  43,008 rows of 4 parts: a warp for a row, the maximum of all
+// parts first, took 39 us for 14.  Started while the kernel before it still runs (its last CTAs leave the
 // launch's latency free), it waits for it before the first read.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 16;
+__device__ __forceinline__ void fma4(float4& y, const float4& x, float f) {
+  y.x = fmaf(x.x, f, y.x), y.y = fmaf(x.y, f, y.y), y.z = fmaf(x.z, f, y.z), y.w = fmaf(x.w, f, y.w);
+}
+struct Joined {
+  float top = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void rescale(float t) {
+    const float back = top == -INFINITY ? 0.f : exp2f(top - t);
+    top = t, sum *= back;
+    acc.x *= back, acc.y *= back, acc.z *= back, acc.w *= back;
+  }
+};
 template <bool MANY>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, int parts) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t unit = MANY ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
-  const int64_t count = a.rows - a.first;
-  if (unit >= count * a.c.batch * a.c.heads) return;  // (whole warps; whole CTAs where MANY)
-  const int64_t r = unit % count, bh = unit / count;
-  const int64_t tiles = (count + tile_rows - 1) / tile_rows;
-  const int64_t at = (bh * tiles + r / tile_rows) * parts * tile_rows + r % tile_rows;  // of part 0
-  float top = -INFINITY;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.part_ml[at + static_cast<int64_t>(s) * tile_rows].x);
+  const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
+  const uint32_t unit = MANY ? blockIdx.x : blockIdx.x * kJoinRows + group;
+  const uint32_t count = static_cast<uint32_t>(a.rows - a.first), bh = unit / count, r = unit - bh * count;
+  if (bh >= static_cast<uint32_t>(a.c.batch) * a.c.heads) return;  // (not where MANY)
+  const uint32_t tiles = (count + tile_rows - 1) / tile_rows, tile = r / tile_rows;
+  const int64_t at = (static_cast<int64_t>(bh) * tiles + tile) * parts * tile_rows + (r - tile * tile_rows);  // of part 0
+  const float4* part_o = reinterpret_cast<const float4*>(a.part_o) + lane;
+  constexpr int kStride = MANY ? kJoinRows : 1;
+  Joined j;
+  for (int s0 = MANY ? group : 0; s0 < parts; s0 += 4 * kStride) {
+    float2 ml[4];
+    float4 v[4];
+    float t = j.top;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f, a0 = 0.f, a1 = 0.f;
-#pragma unroll 4
-  for (int s = MANY ? warp : 0; s < parts; s += MANY ? kJoinWarps : 1) {
-    const int64_t i = at + static_cast<int64_t>(s) * tile_rows;
-    const float2 ml = a.part_ml[i];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no keys there (and perhaps no values written)
-    const float f = exp2f(ml.x - top);
-    const float2 v = reinterpret_cast<const float2*>(a.part_o + i * kMaxWidth)[lane];
-    sum = fmaf(ml.y, f, sum);
-    a0 = fmaf(v.x, f, a0);
-    a1 = fmaf(v.y, f, a1);
+    for (int k = 0; k < 4; ++k) {
+      const int s = s0 + k * kStride;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s < parts) {
+        const int64_t i = at + static_cast<int64_t>(s) * tile_rows;
+        ml[k] = a.part_ml[i];
+        v[k] = part_o[i * (kMaxWidth / 4)];
+      }
+      t = fmaxf(t, ml[k].x);
+    }
+    j.rescale(t);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // no keys there (and perhaps no values written)
+      const float f = exp2f(ml[k].x - t);
+      j.sum = fmaf(ml[k].y, f, j.sum);
+      fma4(j.acc, v[k], f);
+    }
   }
   if constexpr (MANY) {
-    __shared__ float sm[kJoinWarps][kMaxWidth + 1];
-    sm[warp][2 * lane] = a0;
-    sm[warp][2 * lane + 1] = a1;
-    if (lane == 0) sm[warp][kMaxWidth] = sum;
+    __shared__ float4 sm_o[kJoinRows][16];
+    __shared__ float2 sm_ml[kJoinRows];
+    sm_o[group][lane] = j.acc;
+    if (lane == 0) sm_ml[group] = make_float2(j.top, j.sum);
     __syncthreads();
-    if (warp > 0) return;
-    a0 = a1 = sum = 0.f;
+    if (group > 0) return;
+    float t = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) a0 += sm[w][2 * lane], a1 += sm[w][2 * lane + 1], sum += sm[w][kMaxWidth];
+    for (int w = 0; w < kJoinRows; ++w) t = fmaxf(t, sm_ml[w].x);
+    j = Joined();
+    j.top = t;
+#pragma unroll
+    for (int w = 0; w < kJoinRows; ++w) {
+      if (sm_ml[w].x == -INFINITY && sm_ml[w].y == 0.f) continue;
+      const float f = exp2f(sm_ml[w].x - t);
+      j.sum = fmaf(sm_ml[w].y, f, j.sum);
+      fma4(j.acc, sm_o[w][lane], f);
+    }
   }
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
   const Row row(a, h, a.first + r);
-  const float norm = sum != 0.f ? 1.f / sum : 0.f;
-  const int64_t out = a.o.offset(b, row.n, row.head) + 2 * lane;
-  if (2 * lane < a.c.width) put(a.o.p, out, a0 * norm, a.type);
-  if (2 * lane + 1 < a.c.width) put(a.o.p, out + 1, a1 * norm, a.type);
+  const float norm = j.sum != 0.f ? 1.f / j.sum : 0.f;
+  const int64_t out = a.o.offset(b, row.n, row.head) + 4 * lane;
+  const float y[4] = {j.acc.x * norm, j.acc.y * norm, j.acc.z * norm, j.acc.w * norm};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (4 * lane + i < a.c.width) put(a.o.p, out + i, y[i], a.type);
   if (lane == 0 && a.lse != nullptr)
-    a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(top, sum);
+    a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(j.top, j.sum);
 }
 
 template <bool FP8, int NT, int W>
@@ -554,8 +590,8 @@ cudaError_t launch_few(const Attention& a, bool beside, cudaStream_t stream) {
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream) {
   const int parts = a.splits / a.cluster;
   const bool many = parts > 32;
-  const int64_t rows = (a.rows - a.first) * a.c.batch * a.c.heads, grid = many ? rows : (rows + kJoinWarps - 1) / kJoinWarps;
-  if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const int64_t rows = (a.rows - a.first) * a.c.batch * a.c.heads, grid = many ? rows : (rows + kJoinRows - 1) / kJoinRows;
+  if (rows > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kJoinThreads);
