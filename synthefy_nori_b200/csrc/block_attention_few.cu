@@ -467,11 +467,13 @@ template <bool MANY>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, int parts) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
-  const uint32_t unit = MANY ? blockIdx.x : blockIdx.x * kJoinRows + group;
-  const uint32_t count = static_cast<uint32_t>(a.rows - a.first), bh = unit / count, r = unit - bh * count;
-  if (bh >= static_cast<uint32_t>(a.c.batch) * a.c.heads) return;  // (not where MANY)
-  const uint32_t tiles = (count + tile_rows - 1) / tile_rows, tile = r / tile_rows;
-  const int64_t at = (static_cast<int64_t>(bh) * tiles + tile) * parts * tile_rows + (r - tile * tile_rows);  // of part 0
+  const uint32_t unit = MANY ? blockIdx.x : blockIdx.x * kJoinRows + group;  // rows of the cells that are split
+  const uint32_t count = static_cast<uint32_t>(a.rows - a.first), tiles = (count + tile_rows - 1) / tile_rows;
+  const uint32_t split_cell = unit / tile_rows, in_tile = unit - split_cell * tile_rows;
+  const uint32_t cell = static_cast<uint32_t>(a.whole) + split_cell, bh = cell / tiles;
+  const uint32_t r = (cell - bh * tiles) * tile_rows + in_tile;
+  if (bh >= static_cast<uint32_t>(a.c.batch) * a.c.heads || r >= count) return;  // (a whole CTA where MANY)
+  const int64_t at = static_cast<int64_t>(split_cell) * parts * tile_rows + in_tile;  // of part 0
   const float4* part_o = reinterpret_cast<const float4*>(a.part_o) + lane;
   constexpr int kStride = MANY ? kJoinRows : 1;
   Joined j;
@@ -590,7 +592,8 @@ cudaError_t launch_few(const Attention& a, bool beside, cudaStream_t stream) {
 cudaError_t launch_combine(const Attention& a, int tile_rows, cudaStream_t stream) {
   const int parts = a.splits / a.cluster;
   const bool many = parts > 32;
-  const int64_t rows = (a.rows - a.first) * a.c.batch * a.c.heads, grid = many ? rows : (rows + kJoinRows - 1) / kJoinRows;
+  const int64_t cells = (a.rows - a.first + tile_rows - 1) / tile_rows * a.c.batch * a.c.heads - a.whole;
+  const int64_t rows = cells * tile_rows, grid = many ? rows : (rows + kJoinRows - 1) / kJoinRows;
   if (rows > INT32_MAX) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));

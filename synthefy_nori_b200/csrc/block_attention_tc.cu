@@ -190,13 +190,13 @@ __device__ __forceinline__ uint4 query_fp16(const Attention& a, const uint4& x, 
 }
 
 // (everything below 2^31, checked on the host: 64-bit divisions would take a microsecond an item)
+constexpr uint32_t kNoPart = 0xffffffffu;
 struct alignas(16) Item {
-  uint32_t b, h, bh, part;  // part: of the partial results (pair of tiles and split)
+  uint32_t b, h, bh, part;  // part: of the partial results, or kNoPart
   uint32_t row0;            // first query row
   uint32_t tile0;           // first key tile
   int len;                  // keys of the sequence
   int tiles;                // key tiles of this item
-  uint32_t pair;            // of query tiles, over all cells
   int groups;               // query tiles with rows in them (1 or 2; 0: there is no item)
   int64_t out;              // where the results of this (sequence, K/V head) begin
 };
@@ -204,16 +204,20 @@ struct alignas(16) Item {
 __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
   Item it;
   const uint32_t pairs = (static_cast<uint32_t>(a.rows - a.first) + kPairRows - 1) / kPairRows;
-  const uint32_t cell_split = w / pairs, pair = w - cell_split * pairs;
-  it.row0 = static_cast<uint32_t>(a.first) + pair * kPairRows;
-  it.bh = cell_split / static_cast<uint32_t>(a.splits);
-  const uint32_t split = cell_split - it.bh * static_cast<uint32_t>(a.splits);
-  it.pair = it.bh * pairs + pair;
-  it.part = it.pair * static_cast<uint32_t>(a.splits) + split;
+  const uint32_t whole = static_cast<uint32_t>(a.whole), n = w < whole ? 1u : static_cast<uint32_t>(a.splits);
+  uint32_t cell = w, split = 0;  // cell: (sequence, K/V head) and pair of query tiles
+  it.part = kNoPart;
+  if (n > 1) {
+    it.part = w - whole;
+    split = it.part % n;
+    cell = whole + it.part / n;
+  }
+  it.bh = cell / pairs;
+  it.row0 = static_cast<uint32_t>(a.first) + (cell - it.bh * pairs) * kPairRows;
   it.b = it.bh / static_cast<uint32_t>(a.c.heads);
   it.h = it.bh - it.b * static_cast<uint32_t>(a.c.heads);
   it.len = static_cast<int>(min(max(a.length.at(it.b), int64_t{0}), a.c.cap));
-  const uint32_t all = (static_cast<uint32_t>(it.len) + kN - 1) / kN, each = (all + a.splits - 1) / static_cast<uint32_t>(a.splits);
+  const uint32_t all = (static_cast<uint32_t>(it.len) + kN - 1) / kN, each = n > 1 ? (all + n - 1) / n : all;
   it.tile0 = min(split * each, all);
   it.tiles = static_cast<int>(min(it.tile0 + each, all) - it.tile0);
   it.groups = it.row0 + kM < static_cast<uint32_t>(a.rows) ? 2 : 1;
@@ -664,6 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool there = row < static_cast<uint32_t>(a.rows);
       const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group), in_group = row - n * a.group;
       const int64_t out = it->out + n * a.o.sn + in_group * a.o.sh;
+      const bool part = it->part != kNoPart;
       const int64_t pr = static_cast<int64_t>(it->part) * kPairRows + qt * kM + r;
       const int64_t lse_row = static_cast<int64_t>(it->bh) * a.group + in_group;
       done_with(true);
@@ -679,7 +684,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         fa = half ? f2 : f, fb = half ? f : f2;
         tc_fence_after();
       }
-      const bool part = a.splits > 1;
       if (!part) {
         const float norm = l != 0.f ? 1.f / l : 0.f;
         fa *= norm, fb *= norm;
@@ -768,7 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <bool FP8>
 cudaError_t tc_typed(const Attention& a, cudaStream_t stream) {
   if (a.rows > INT32_MAX - kPairRows) return cudaErrorInvalidConfiguration;
-  const int64_t items = (a.rows - a.first + kPairRows - 1) / kPairRows * a.c.batch * a.c.heads * a.splits;
+  const int64_t cells = (a.rows - a.first + kPairRows - 1) / kPairRows * a.c.batch * a.c.heads;
+  const int64_t items = a.whole + (cells - a.whole) * a.splits;
   if (items > INT32_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = cudaFuncSetAttribute(tc_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;

@@ -73,10 +73,11 @@ struct Attention {
   int64_t first;
   float scale_log2; // softmax scale * log2(e)
   float* lse;       // [batch, query heads, n] or null
-  int splits;       // of the key range
+  int64_t whole;    // cells, a (sequence, K/V head) and a tile of query rows each, that one CTA takes whole
+  int splits;       // of the key range of the others
   int cluster;      // splits that are joined on the way (kernel for few rows), a divisor of splits
-  float* part_o;    // [cells, parts, tile rows, 64], unnormalised; parts = splits / cluster
-  float2* part_ml;  // [cells, parts, tile rows] (maximum, sum)
+  float* part_o;    // [cells - whole, parts, tile rows, 64], unnormalised; parts = splits / cluster
+  float2* part_ml;  // [cells - whole, parts, tile rows] (maximum, sum)
   int* status;
 };
 

@@ -122,17 +122,28 @@ int few_splits(int64_t cells, int64_t longest, int resident) {
   return best;
 }
 
-// Splits of the keys for the persistent kernel: the waves of items, each as long as its key tiles
-// and the start and end of an item; partial results cost a second kernel and their traffic (and a
-// workspace, held to 16 items an SM: 155 MB).
-int tc_splits(int64_t cells, int64_t longest, int ctas) {
+// Cells that the persistent kernel takes whole, and splits of the keys of the others: as many whole ones as
+// fill every SM some number of times, so that only a last, partial wave is split.  The time is the waves of
+// items, each as long as its key tiles and the start and end of an item; partial results cost a second
+// kernel and their traffic (and a workspace, held to 16 items an SM: 155 MB).  A split has to promise 3%, since
+// long runs of items even out by themselves (4096 rows x 1000 of 168 cells: 378 us whole, 395 split for 1%;
+// 256 rows x 10,000: 234 us with every cell split, 196 with the last 20).
+struct Split {
+  int64_t whole;
+  int splits;
+};
+Split tc_splits(int64_t cells, int64_t longest, int ctas) {
   const int64_t tiles = std::max<int64_t>((longest + bc::kTile - 1) / bc::kTile, 1);
-  int best = 1;
-  double least = 0;
-  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64) && (s == 1 || cells * s <= 16 * ctas); ++s) {
-    const double waves = static_cast<double>((cells * s + ctas - 1) / ctas);
-    const double cost = waves * (static_cast<double>((tiles + s - 1) / s) + 4.0) + (s > 1 ? 2.0 + 0.016 * cells * s : 0.0);
-    if (s == 1 || cost < least) least = cost, best = static_cast<int>(s);
+  Split best{cells, 1};
+  double least = 0.97 * static_cast<double>((cells + ctas - 1) / ctas) * (static_cast<double>(tiles) + 4.0);
+  for (int64_t waves = cells / ctas, tried = 0; waves >= 0 && tried < 3; --waves, ++tried) {
+    const int64_t whole = waves * ctas, rest = cells - whole;
+    for (int64_t s = 2; rest > 0 && s <= std::min<int64_t>(tiles, 64) && rest * s <= 16 * ctas; ++s) {
+      const double cost = waves * (static_cast<double>(tiles) + 4.0) +
+                          static_cast<double>((rest * s + ctas - 1) / ctas) * (static_cast<double>((tiles + s - 1) / s) + 4.0) +
+                          4.0 + 0.012 * rest * s;
+      if (cost < least) least = cost, best = Split{whole, static_cast<int>(s)};
+    }
   }
   return best;
 }
@@ -221,12 +232,15 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
     p.rows = end;
     const int tile = few ? bc::few_tile_rows(end - first) : bc::kPairRows;
     const int64_t cells = (end - first + tile - 1) / tile * a.c.batch * a.c.heads;
-    p.splits = few ? few_splits(cells, longest, sms * bc::few_resident(end - first)) : tc_splits(cells, longest, sms);
+    const Split by = few ? Split{0, few_splits(cells, longest, sms * bc::few_resident(end - first))} : tc_splits(cells, longest, sms);
+    p.whole = by.whole;
+    p.splits = by.splits;
     p.cluster = few ? std::min(p.splits, 8) : 1;
     const int parts = p.splits / p.cluster;
     if (parts > 1) {
-      part_o[few] = torch::empty({cells * parts * tile * bc::kMaxWidth}, cks.options());
-      part_ml[few] = torch::empty({cells * parts * tile * 2}, cks.options());
+      const int64_t part_rows = (cells - by.whole) * parts * tile;
+      part_o[few] = torch::empty({part_rows * bc::kMaxWidth}, cks.options());
+      part_ml[few] = torch::empty({part_rows * 2}, cks.options());
       p.part_o = part_o[few].data_ptr<float>();
       p.part_ml = reinterpret_cast<float2*>(part_ml[few].data_ptr<float>());
     }

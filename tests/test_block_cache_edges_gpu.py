@@ -191,3 +191,17 @@ def test_small_contexts_of_the_model(rows, dtype):
         b = m.apply_context_cache(x[:, rows:], m.build_context_cache(x[:, :rows], y[:, :rows], cache_dtype=dtype))
     assert torch.isfinite(b).all()
     assert torch.nn.functional.cosine_similarity(a.float().flatten(), b.float().flatten(), dim=0) > 0.998
+
+
+@pytest.mark.parametrize("b,h,group,n,rows", [(19, 8, 1, 200, 3000), (25, 2, 3, 290, 1700), (5, 1, 1, 9000, 2000)])
+@pytest.mark.parametrize("device_lengths", [False, True])
+def test_more_work_than_one_wave(b, h, group, n, rows, device_lengths):
+    """A little more work than there are SMs: some cells are taken whole, the keys of the last ones are split."""
+    from synthefy_nori_b200 import ops
+
+    cache, g = make(b, h, rows, 56, seed=b)
+    q = torch.randn(b, n, h * group, 56, device="cuda", generator=g).to(torch.bfloat16)
+    lengths = [rows - 100 * (i % 7) for i in range(b)] if device_lengths else [rows] * b
+    given = torch.tensor(lengths, dtype=torch.int32, device="cuda") if device_lengths else rows
+    o, lse = ops.block_cache_attention(q, cache, given, return_lse=True)
+    check(q, cache, lengths, o, lse)
