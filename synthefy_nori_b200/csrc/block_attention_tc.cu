@@ -12,8 +12,10 @@
 //                 warpgroup brings one of its query tiles to shared memory as fp16;
 //   warps 1, 2    issue the products of one query tile each: S = Q K^T (128 x 64 x 64) and O += P V;
 //   warps 12..27  softmax, four groups: (query tile) x (half of the keys of every tile), each with its
-//                 own maximum, sum and accumulator; thread = query row (its TMEM lane), 64 score columns
-//                 in registers; P (fp16 pairs) goes over S in TMEM and is the A operand of P V.
+//                 own maximum, sum and accumulator; thread = query row (its TMEM lane), 32 scores of a chunk
+//                 in registers; P (fp16 pairs) goes over S in TMEM and is the A operand of P V.  A group has
+//                 two chunks: products of the one run while it works on the other (with one chunk of 64
+//                 that was waited for, 1024 rows x 10,000 took 691 us for 680).
 // A group's tile is a chain (scores, maximum, weights, two products) whose latency is several times its
 // arithmetic, so four of them share an SM: with one thread for all 128 columns of a row and two
 // groups the same arithmetic took 1.3 times as long, with row maxima exchanged between the
@@ -22,8 +24,8 @@
 // Scales cost nothing per value: with c = scale log2(e) s_k 2^-e (2^e brings the query row into
 // fp16's range, exactly) and t = c (q . k) + log2 s_v,
 //   w = 2^(t - max t),  O = sum w v_code,  l = sum over blocks of (sum of w) / s_v.
-// The maximum is lazy (O is rescaled when it grows by more than 2^4); w is kept at up to 2^15 so
-// that fp16 holds 11 bits down to 2^-25 of the largest weight.  Scores, sums and O are fp32.
+// The maximum is lazy (O is rescaled when it grows by more than 2^8); w is kept at up to 2^15 so
+// that fp16 holds 11 bits down to 2^-21 of the largest weight.  Scores, sums and O are fp32.
 // All exponentials run on the MUFU: a polynomial on the FMA pipe for a quarter of them made a tile
 // a seventh slower, since the warps' issue slots are as scarce as the MUFU.
 //
@@ -48,7 +50,8 @@ constexpr int kSmem = kTile16 * (4 + 2 * kRing) + kTile8 * 2 * kRing + 1024 + 10
 constexpr int kItems = 4;                // items that are known ahead
 constexpr int kConsumers = 2 + 8 + 16;   // of an item: issuers, converter and softmax warps
 constexpr int kHalf = kN / 2;            // keys of a group's tile
-// S 0..255 (64 a group, P over its first 32), O 256..511 (64 a group)
+constexpr int kChunk = kHalf / 2;        // keys of a step of its softmax
+// S 0..255 (64 a group, P of each 32 over its first 16), O 256..511 (64 a group)
 constexpr uint32_t kTmemCols = 512, kOcol = 256;
 constexpr int kConvertWarps = 4, kSoftmaxWarp0 = 12;
 // registers of a thread: launch 72 (896 threads); the softmax warps take what the others give up
@@ -145,12 +148,11 @@ __device__ __forceinline__ float weights32(const uint32_t (&v)[32], float c, flo
 }
 
 // 16 bytes (values 8 c .. 8 c + 7) of query row `row` of a K/V head; zeros where it ends or does not exist.
-__device__ __forceinline__ uint4 query_piece(const Attention& a, int b, int h, uint32_t row, int c, int bytes) {
+__device__ __forceinline__ uint4 query_piece(const Attention& a, int64_t begin, uint32_t row, int c, int bytes) {
   uint32_t v[4] = {0, 0, 0, 0};
   if (row < static_cast<uint32_t>(a.rows) && c * 8 < a.c.width) {
     const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group);
-    const uint16_t* src =
-        static_cast<const uint16_t*>(a.q.p) + a.q.offset(b, n, static_cast<int>(h * a.group + row - n * a.group)) + c * 8;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q.p) + begin + n * a.q.sn + (row - n * a.group) * a.q.sh + c * 8;
     if (bytes == 16) return __ldg(reinterpret_cast<const uint4*>(src));
     if (bytes == 4) {
 #pragma unroll
@@ -198,7 +200,7 @@ struct alignas(16) Item {
   int len;                  // keys of the sequence
   int tiles;                // key tiles of this item
   int groups;               // query tiles with rows in them (1 or 2; 0: there is no item)
-  int64_t out;              // where the results of this (sequence, K/V head) begin
+  int64_t in, out;          // where the query rows and the results of this (sequence, K/V head) begin
 };
 
 __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
@@ -221,6 +223,7 @@ __device__ __forceinline__ Item item_at(const Attention& a, uint32_t w) {
   it.tile0 = min(split * each, all);
   it.tiles = static_cast<int>(min(it.tile0 + each, all) - it.tile0);
   it.groups = it.row0 + kM < static_cast<uint32_t>(a.rows) ? 2 : 1;
+  it.in = a.q.offset(static_cast<int>(it.b), 0, static_cast<int>(it.h * a.group));
   it.out = a.o.offset(static_cast<int>(it.b), 0, static_cast<int>(it.h * a.group));
   return it;
 }
@@ -249,10 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = item_empty + kItems; // [item parity][query tile]
   uint64_t* q_empty = q_full + 4;         // the item's scores are done, its factors read and its results on their way
   uint64_t* o_free = q_empty + 4;         // [query tile] per item: O is in registers
-  uint64_t* o_full = o_free + 2;          // [group] per item: the last P V is done
-  uint64_t* s_full = o_full + 4;          // [group] per tile: scores are there, the P V before them done
-  uint64_t* p_full = s_full + 4;          // [group] per tile: P is in TMEM
-  uint64_t* pair = p_full + 4;            // [query tile][lane quarter] the two halves have exchanged
+  uint64_t* s_full = o_free + 2;          // [group][chunk] per tile and at the end: scores are there, the P V before them done
+  uint64_t* p_full = s_full + 8;          // [group][chunk] per tile: P is in TMEM
+  uint64_t* pair = p_full + 8;            // [query tile][lane quarter] the two halves have exchanged
   uint64_t* done = pair + 8;              // [query tile] every product of this CTA
   uint64_t* taken = done + 2;             // the answer to a request for an item
   uint64_t* answer = taken + 2;           // (16 bytes, 16-byte aligned)
@@ -264,8 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // (s_k, log2 s_v, 1 / s_v) of each 32 keys of a tile, written with its K; a slot is used again four tiles
   // on, when the scores three tiles before that are done and so the weights of this tile
   __shared__ float4 scales[4][4];
-  static_assert((8 * kRing + 2 * kItems + 36) * 8 + 8 <= 1024, "barriers fit their room");
-  static_assert((8 * kRing + 2 * kItems + 34) % 2 == 0, "the answer is 16-byte aligned");
+  static_assert((8 * kRing + 2 * kItems + 40) * 8 + 8 <= 1024, "barriers fit their room");
+  static_assert((8 * kRing + 2 * kItems + 38) % 2 == 0, "the answer is 16-byte aligned");
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (*reinterpret_cast<volatile int*>(a.status) != 0) return;  // another CTA or kernel timed out
@@ -289,16 +291,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(&q_full[i], kConvertWarps);
       mbar_init(&q_empty[i], 1 + 8);
-      mbar_init(&o_full[i], 1);
     }
     mbar_init(taken, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&o_free[t], 8);
       mbar_init(&done[t], 1);
     }
-    for (int g = 0; g < 4; ++g) {
-      mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 4);
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&pair[i], 2);
     *abort_flag = 0;
@@ -407,12 +408,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp <= 2) {
     setmaxnreg_dec<kRegsLow>();
     if (elect_one()) {
-      constexpr uint32_t idesc_s = idesc_f16(kM, kHalf, false), idesc_o = idesc_f16(kM, kD, true);
+      constexpr uint32_t idesc_s = idesc_f16(kM, kChunk, false), idesc_o = idesc_f16(kM, kD, true);
       const int t = warp - 1;          // query tile
       // operands: 32 bytes further for each 16 columns of Q and K, 2048 for each 16 keys of V
       const uint64_t dq = umma_desc_kmajor_sw128(smem_u32(sQ + t * kTile16));
       const uint64_t dk = umma_desc_kmajor_sw128(smem_u32(sK)), dv = umma_smem_desc(smem_u32(sV), 8192, 1024, 2);
-      constexpr uint32_t kStage = kTile16 >> 4, kHalfTile = kStage / 2;
+      constexpr uint32_t kStage = kTile16 >> 4, kHalfTile = kStage / 2, kChunkTile = kStage / 4;
       uint32_t nk = 0, nv = 0;         // ring positions
       uint32_t cnt = 0;                // tiles of this query tile so far
       uint32_t qcnt = 0;               // items of this query tile so far
@@ -436,18 +437,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const uint32_t buf = qcnt & 1;
         const uint64_t q = dq + buf * (2 * kStage);
-        auto scores = [&](int p) {  // of K tile nk, for keys 64 p .. + 63
-          const uint64_t k = dk + nk % kRing * kStage + p * kHalfTile;
+        auto scores = [&](int p, int u) {  // of K tile nk, for keys 64 p + 32 u .. + 31
+          const uint64_t k = dk + nk % kRing * kStage + p * kHalfTile + u * kChunkTile;
 #pragma unroll
           for (int i = 0; i < kD / 16; ++i)
-            umma_bf16_ss(tmem + (2 * t + p) * kHalf, q + 2 * i, k + 2 * i, idesc_s, i > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + (2 * t + p) * kHalf + u * kChunk, q + 2 * i, k + 2 * i, idesc_s, i > 0 ? 1u : 0u);
         };
         if (!(ok = wait(&q_full[2 * buf + t], qcnt / 2) && wait(&k_full[nk % kRing], nk / kRing))) break;
         tc_fence_after();
-        for (int p = 0; p < 2; ++p) {
-          scores(p);
-          umma_commit(&s_full[2 * t + p]);
-        }
+        for (int u = 0; u < 2; ++u)
+          for (int p = 0; p < 2; ++p) {
+            scores(p, u);
+            umma_commit(&s_full[2 * (2 * t + p) + u]);
+          }
         umma_commit(&k_empty[nk++ % kRing]);
         if (tiles == 1) umma_commit(&q_empty[2 * buf + t]);
         for (int j = 0; ok && j < tiles; ++j, ++cnt) {
@@ -455,17 +457,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the accumulators of the previous item have been read
           if (j == 0 && qcnt > 0 && !(ok = wait(&o_free[t], qcnt - 1))) break;
           if (!(ok = wait(&v_full[nv % kRing], nv / kRing) && (!more || wait(&k_full[nk % kRing], nk / kRing)))) break;
-          for (int p = 0; p < 2; ++p) {
-            const int g = 2 * t + p;
-            if (!(ok = wait(&p_full[g], cnt))) break;
+          for (int i = 0; ok && i < 4; ++i) {
+            const int u = i / 2, p = i % 2, g = 2 * t + p;
+            if (!(ok = wait(&p_full[2 * g + u], cnt))) break;
             tc_fence_after();
-            const uint64_t v = dv + nv % kRing * kStage + p * kHalfTile;
+            const uint64_t v = dv + nv % kRing * kStage + p * kHalfTile + u * kChunkTile;
 #pragma unroll
-            for (int i = 0; i < kHalf / 16; ++i)
-              umma_bf16_ts(tmem + kOcol + g * kD, tmem + g * kHalf + i * 8, v + i * 128, idesc_o, (i > 0 || j > 0) ? 1u : 0u);
+            for (int k = 0; k < kChunk / 16; ++k)
+              umma_bf16_ts(tmem + kOcol + g * kD, tmem + g * kHalf + u * kChunk + k * 8, v + k * 128, idesc_o,
+                           (k > 0 || u > 0 || j > 0) ? 1u : 0u);
             // P V reads the columns that the next scores overwrite: products of one thread run in order
-            if (more) scores(p);
-            umma_commit(more ? &s_full[g] : &o_full[g]);
+            if (more) scores(p, u);
+            umma_commit(&s_full[2 * g + u]);
           }
           if (!ok) break;
           umma_commit(&v_empty[nv++ % kRing]);
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float *ks = a.c.k_scale + blk, *vs = a.c.v_scale + blk;
       const bool has_rows = tiles > 0 && qt < it->groups;
       const uint32_t row_first = it->row0 + qt * kM;
-      const int b = it->b, h = it->h;
+      const int64_t begin = it->in;
       done_with(true);
       if (has_rows) {
         // ---- query rows: eight lanes a row, 16 bytes each; a power of two brings the row into fp16's
@@ -516,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int r1 = warp % 4 * 32 + lane / 8; r1 < warp % 4 * 32 + 32; r1 += 16) {
           uint4 x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = query_piece(a, b, h, row_first + r1 + 4 * i, lane % 8, q_bytes);
+          for (int i = 0; i < 4; ++i) x[i] = query_piece(a, begin, row_first + r1 + 4 * i, lane % 8, q_bytes);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = r1 + 4 * i;
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = tmem + g * kHalf + lane_off, tO = tmem + kOcol + g * kD + lane_off,
                    tO2 = tmem + kOcol + 2 * qt * kD + half * 32 + lane_off;  // this half's columns, both accumulators
     uint64_t* pair_bar = &pair[qt * 4 + quarter];
-    uint32_t cnt = 0;  // completions of s_full so far
+    uint32_t cnt = 0;  // completions of each s_full so far
     uint32_t nt = 0;   // tiles of all items so far
     uint32_t xc = 0;   // exchanges, and so items, so far
     bool ok = true;
@@ -606,26 +609,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = mbar_wait_warp(&q_full[2 * (xc & 1) + qt], xc / 2 & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
         const float fac = factors[xc & 1][qt * kM + r];
         int valid = it->len - static_cast<int>(it->tile0 * kN) - kHalf * half;  // keys from this half's first on
-        for (int j = 0; j < tiles; ++j, ++nt, valid -= kN) {
-          if (!(ok = mbar_wait_warp(&s_full[g], cnt++ & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
-          tc_fence_after();
-          if (valid < kHalf) {  // keys behind the last row
+        uint64_t* bar = &s_full[2 * g];
 #pragma unroll 1
-            for (int i = max(valid, 0); i < kHalf; ++i) tmem_st1(tS + i, 0xff800000u);
+        for (int step = 0; step < 2 * tiles; ++step) {  // (tile, chunk)
+          const int u = step & 1;
+          if (!(ok = mbar_wait_warp(bar + u, cnt + step / 2 & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+          tc_fence_after();
+          const uint32_t tC = tS + u * kChunk;
+          if (valid < kChunk) {  // keys behind the last row
+#pragma unroll 1
+            for (int i = max(valid, 0); i < kChunk; ++i) tmem_st1(tC + i, 0xff800000u);
             tmem_wait_st();
           }
-          const float4* sc = &scales[nt & 3][2 * half];
-          uint32_t x0[32], x1[32];
-          tmem_ld32(tS, x0);
-          tmem_ld32(tS + 32, x1);
-          float f0 = fac * sc[0].x, f1 = fac * sc[1].x;  // (never 0: a masked key's -inf stays -inf)
-          f0 = f0 < 1e-38f ? 1e-38f : f0;
-          f1 = f1 < 1e-38f ? 1e-38f : f1;
+          valid -= u ? kN - kChunk : kChunk;
+          uint32_t x[32];
+          tmem_ld32(tC, x);
+          const float4 sc = scales[(nt + step / 2) & 3][2 * half + u];
+          const float f0 = fac * sc.x, f = f0 < 1e-38f ? 1e-38f : f0;  // (never 0: a masked key's -inf stays -inf)
           tmem_wait_ld();
-          const float cand = fmaxf(fmaf(max32(x0), f0, sc[0].y), fmaf(max32(x1), f1, sc[1].y));
+          const float cand = fmaf(max32(x), f, sc.y);
           float back = 1.f;
           bool grow = false;
-          if (j == 0) {
+          if (step == 0) {
             m = cand;
           } else if (cand > m + kLazy) {
             back = exp2_mufu(m - cand);
@@ -633,17 +638,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             grow = true;
           }
           const float lift = m == -INFINITY ? 0.f : kLift - m;  // (no key of this half is there)
-          l *= back;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t x[32];
-            tmem_ld32(tS + 32 * c, x);
-            const float f = c ? f1 : f0;
-            tmem_wait_ld();
-            l = fmaf(weights32(x, f, sc[c].y + lift, tS + 16 * c), sc[c].z, l);
-          }
-          // (the products before these scores are done: O may be changed)
+          l = fmaf(weights32(x, f, sc.y + lift, tC), sc.z, l * back);
           if (__any_sync(0xffffffffu, grow)) {
+            // the other chunk's product may still be under way: its next scores come behind it
+            if (!(ok = mbar_wait_warp(bar + (u ^ 1), cnt + (step + 1) / 2 & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
               uint32_t o[16];
@@ -657,9 +656,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[g]);
+          if (lane == 0) mbar_arrive(&p_full[2 * g + u]);
         }
-        if (!ok || !(ok = mbar_wait_warp(&o_full[g], xc & 1, a.status, kTimeoutEpilogue, abort_flag))) break;  // the last P V
+        nt += tiles;
+        cnt += tiles;
+        for (int u = 0; u < 2 && ok; ++u)  // the last P V
+          ok = mbar_wait_warp(bar + u, cnt & 1, a.status, kTimeoutEpilogue, abort_flag);
+        ++cnt;
+        if (!ok) break;
         tc_fence_after();
       }
       // ---- the halves joined: 32 columns of O from both accumulators, to memory.  (Once an item, so its

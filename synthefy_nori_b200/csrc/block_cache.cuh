@@ -81,10 +81,12 @@ struct Attention {
   int* status;
 };
 
-// Weights are 2^(t - m + kLift): fp16 keeps 11 bits of them down to 2^-25 of the largest, and a
-// maximum that lags by up to kLazy (no rescale of the sums) stays below fp16's largest value.
-constexpr float kLift = 11.f;
-constexpr float kLazy = 4.f;
+// Weights are 2^(t - m + kLift): fp16 keeps 11 bits of them down to 2^-21 of the largest, and below that its
+// values are 2^-31 of the largest apart (a million keys off by half of that: 2^-12 at most).  A maximum that
+// lags by up to kLazy (no rescale of the sums) stays below fp16's largest value.  4 and 11 instead rescale a
+// dozen times a row where scores spread by a few units: 1024 rows x 10,000 733 us for 698.
+constexpr float kLift = 7.f;
+constexpr float kLazy = 8.f;
 
 #ifdef __CUDACC__
 // A contiguous piece (16-byte aligned, a multiple of 16 bytes) to shared memory; arrives on `bar`.
