@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float fac = factors[xc & 1][qt * kM + r];
         int valid = it->len - static_cast<int>(it->tile0 * kN) - kHalf * half;  // keys from this half's first on
         uint64_t* bar = &s_full[2 * g];
-#pragma unroll 1
+#pragma unroll 2
         for (int step = 0; step < 2 * tiles; ++step) {  // (tile, chunk)
           const int u = step & 1;
           if (!(ok = mbar_wait_warp(bar + u, cnt + step / 2 & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int have = a.c.width - half * 32;
       // the item's query tile becomes the tile of results (nothing reads it any more): a row in pieces of 16 bytes
       uint8_t* stage = sQ + (2 * ((xc ^ (tiles > 0)) & 1) + qt) * kTile16 + quarter * 32 * 128;
-#pragma unroll 1
+#pragma unroll 2
       for (int c = 0; c < 4; ++c) {
         float o[8];
         if (tiles > 0) {
