@@ -147,48 +147,73 @@ __device__ __forceinline__ float weights32(const uint32_t (&v)[32], float c, flo
   return r0 + r1;
 }
 
-// 16 bytes (values 8 c .. 8 c + 7) of query row `row` of a K/V head; zeros where it ends or does not exist.
-__device__ __forceinline__ uint4 query_piece(const Attention& a, int64_t begin, uint32_t row, int c, int bytes) {
+// 16 bytes (values 8 c .. 8 c + 7) of the query row at src, in pieces of 4 or 2 bytes; zeros where it ends.
+__device__ __forceinline__ uint4 query_piece(const uint16_t* src, int c, int width, int bytes) {
   uint32_t v[4] = {0, 0, 0, 0};
-  if (row < static_cast<uint32_t>(a.rows) && c * 8 < a.c.width) {
-    const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group);
-    const uint16_t* src = static_cast<const uint16_t*>(a.q.p) + begin + n * a.q.sn + (row - n * a.group) * a.q.sh + c * 8;
-    if (bytes == 16) return __ldg(reinterpret_cast<const uint4*>(src));
-    if (bytes == 4) {
+  if (bytes == 4) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c * 8 + 2 * e < a.c.width) v[e] = __ldg(reinterpret_cast<const uint32_t*>(src) + e);
-    } else {
+    for (int e = 0; e < 4; ++e)
+      if (c * 8 + 2 * e < width) v[e] = __ldg(reinterpret_cast<const uint32_t*>(src) + e);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c * 8 + e < a.c.width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
-    }
+    for (int e = 0; e < 8; ++e)
+      if (c * 8 + e < width) v[e / 2] |= static_cast<uint32_t>(__ldg(src + e)) << 16 * (e % 2);
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// The piece as fp16 times the row's power of two (eight neighbouring lanes hold the row), and the
-// factor that its scores take.
-__device__ __forceinline__ uint4 query_fp16(const Attention& a, const uint4& x, float& factor) {
-  const uint32_t v[4] = {x.x, x.y, x.z, x.w};
-  // magnitudes order like their bits, infinities and NaN on top
-  uint32_t top2 = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
+// Four query rows, r0 and every fourth after it, to the tile as fp16 times each row's power of two, and the
+// factors that their scores take.  Eight neighbouring lanes hold a row, 16 bytes (unit c) each.  The four go
+// through every step side by side: one after the other they took twice as long.
+__device__ __forceinline__ void query_rows(const Attention& a, int64_t begin, uint32_t row_first, int r0, int c, int bytes,
+                                           uint8_t* tile, float* factors) {
+  uint4 x[4];
+  auto source = [&](int i) -> const uint16_t* {  // null where there is no such row or unit
+    const uint32_t row = row_first + r0 + 4 * i;
+    if (row >= static_cast<uint32_t>(a.rows) || c * 8 >= a.c.width) return nullptr;
+    const uint32_t n = a.group == 1 ? row : row / static_cast<uint32_t>(a.group);
+    return static_cast<const uint16_t*>(a.q.p) + begin + n * a.q.sn + (row - n * a.group) * a.q.sh + c * 8;
+  };
 #pragma unroll
-  for (int o = 1; o < 8; o *= 2) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
-  const uint32_t t16 = max(top2 & 0xffffu, top2 >> 16);
-  const bool bf = a.type == kBF16;
-  const float top = bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16)));
-  float up, down;
-  row_scale(top, up, down);
-  factor = down * a.scale_log2;
-  uint32_t y[4];
+  for (int i = 0; i < 4; ++i) x[i] = make_uint4(0, 0, 0, 0);
+  if (bytes == 16) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float2 f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
-    if (!bf) f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
-    y[k] = pack_half2(f.x * up, f.y * up);
+    for (int i = 0; i < 4; ++i)
+      if (const uint16_t* src = source(i)) x[i] = __ldg(reinterpret_cast<const uint4*>(src));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (const uint16_t* src = source(i)) x[i] = query_piece(src, c, a.c.width, bytes);
   }
-  return make_uint4(y[0], y[1], y[2], y[3]);
+  // magnitudes order like their bits, infinities and NaN on top
+  uint32_t top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    top[i] = __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+  const bool bf = a.type == kBF16;
+  float mine = 0.f;  // lane c keeps the factor of row c
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t16 = max(top[i] & 0xffffu, top[i] >> 16);
+    float up, down;
+    row_scale(bf ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(t16))), up, down);
+    mine = c == i ? down * a.scale_log2 : mine;
+    const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float2 f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
+      if (!bf) f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+      y[k] = pack_half2(f.x * up, f.y * up);
+    }
+    const int r = r0 + 4 * i;
+    *reinterpret_cast<uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+  if (c < 4) factors[r0 + 4 * c] = mine;
 }
 
 // (everything below 2^31, checked on the host: 64-bit divisions would take a microsecond an item)
@@ -252,9 +277,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = item_empty + kItems; // [item parity][query tile]
   uint64_t* q_empty = q_full + 4;         // the item's scores are done, its factors read and its results on their way
   uint64_t* o_free = q_empty + 4;         // [query tile] per item: O is in registers
-  uint64_t* s_full = o_free + 2;          // [group][chunk] per tile and at the end: scores are there, the P V before them done
+  uint64_t* s_full = o_free + 2;          // [group][chunk] per tile: scores are there, the P V before them done
   uint64_t* p_full = s_full + 8;          // [group][chunk] per tile: P is in TMEM
-  uint64_t* pair = p_full + 8;            // [query tile][lane quarter] the two halves have exchanged
+  uint64_t* o_full = p_full + 8;          // [group][chunk] per item: the last P V is done (not another phase of
+                                          // s_full: the next item's scores do not wait for the warps that wait for it)
+  uint64_t* pair = o_full + 8;            // [query tile][lane quarter] the two halves have exchanged
   uint64_t* done = pair + 8;              // [query tile] every product of this CTA
   uint64_t* taken = done + 2;             // the answer to a request for an item
   uint64_t* answer = taken + 2;           // (16 bytes, 16-byte aligned)
@@ -266,11 +293,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   // (s_k, log2 s_v, 1 / s_v) of each 32 keys of a tile, written with its K; a slot is used again four tiles
   // on, when the scores three tiles before that are done and so the weights of this tile
   __shared__ float4 scales[4][4];
-  static_assert((8 * kRing + 2 * kItems + 40) * 8 + 8 <= 1024, "barriers fit their room");
-  static_assert((8 * kRing + 2 * kItems + 38) % 2 == 0, "the answer is 16-byte aligned");
+  static_assert((8 * kRing + 2 * kItems + 48) * 8 + 8 <= 1024, "barriers fit their room");
+  static_assert((8 * kRing + 2 * kItems + 46) % 2 == 0, "the answer is 16-byte aligned");
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (*reinterpret_cast<volatile int*>(a.status) != 0) return;  // another CTA or kernel timed out
+  const int failed = *reinterpret_cast<volatile int*>(a.status);  // (looked at below)
 
   asm volatile("griddepcontrol.launch_dependents;");  // (the join of parts may be set up now)
   if (threadIdx.x == 0) {
@@ -300,14 +327,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 8; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&pair[i], 2);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  // columns past the width are never written again: zero everywhere (finite, and 0 in Q)
-  for (int i = threadIdx.x; i < kTile16 * (4 + 2 * kRing) / 16; i += kThreads)
-    reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  // columns of K and V past the width are never written: zero (finite; Q is 0 there)
+  const int unit0 = a.c.stored / 8, units = 8 - unit0;
+  for (int i = threadIdx.x; i < 2 * kRing * kN * units; i += kThreads) {
+    const int row = i / units, c = unit0 + i - row * units;
+    *reinterpret_cast<uint4*>(sK + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+  }
+  if (threadIdx.x == 0) known[0] = item_at(a, blockIdx.x);  // (while the others write)
+  if (failed != 0) return;  // another CTA or kernel timed out
   fence_proxy_async_smem();
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
@@ -340,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto tell = [&](uint32_t w) -> bool {  // (`items`: there is none left)
         const uint32_t i = told % kItems;
         if (!mbar_wait(&item_empty[i], (told / kItems & 1) ^ 1, a.status, kTimeoutProducer, abort_flag)) return false;
-        known[i] = item_at(a, w < items ? w : 0);
+        if (told > 0) known[i] = item_at(a, w < items ? w : 0);  // (the first is there)
         if (w >= items) known[i].groups = 0;
         mbar_arrive(&item_full[i]);
         ++told;
@@ -468,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                            (k > 0 || u > 0 || j > 0) ? 1u : 0u);
             // P V reads the columns that the next scores overwrite: products of one thread run in order
             if (more) scores(p, u);
-            umma_commit(&s_full[2 * g + u]);
+            umma_commit(more ? &s_full[2 * g + u] : &o_full[2 * g + u]);
           }
           if (!ok) break;
           umma_commit(&v_empty[nv++ % kRing]);
@@ -516,19 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = mbar_wait_warp(&q_empty[buf], (qcnt / 2 & 1) ^ 1, a.status, kTimeoutProducer, abort_flag))) break;
         uint8_t* tile = sQ + buf * kTile16;
 #pragma unroll 1
-        for (int r1 = warp % 4 * 32 + lane / 8; r1 < warp % 4 * 32 + 32; r1 += 16) {
-          uint4 x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = query_piece(a, begin, row_first + r1 + 4 * i, lane % 8, q_bytes);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = r1 + 4 * i;
-            float factor;
-            x[i] = query_fp16(a, x[i], factor);
-            *reinterpret_cast<uint4*>(tile + r * 128 + ((lane % 8 ^ (r & 7)) << 4)) = x[i];
-            if (lane % 8 == 0) factors[qcnt & 1][qt * kM + r] = factor;
-          }
-        }
+        for (int r1 = warp % 4 * 32 + lane / 8; r1 < warp % 4 * 32 + 32; r1 += 16)
+          query_rows(a, begin, row_first, r1, lane % 8, q_bytes, tile, &factors[qcnt & 1][qt * kM]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[buf]);
@@ -640,8 +662,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float lift = m == -INFINITY ? 0.f : kLift - m;  // (no key of this half is there)
           l = fmaf(weights32(x, f, sc.y + lift, tC), sc.z, l * back);
           if (__any_sync(0xffffffffu, grow)) {
-            // the other chunk's product may still be under way: its next scores come behind it
-            if (!(ok = mbar_wait_warp(bar + (u ^ 1), cnt + (step + 1) / 2 & 1, a.status, kTimeoutEpilogue, abort_flag))) break;
+            // the other chunk's product may still be under way: its next scores, if there are any, come behind it
+            const bool last = step == 2 * tiles - 1;
+            if (!(ok = mbar_wait_warp(last ? &o_full[2 * g] : bar + (u ^ 1), (last ? xc : cnt + (step + 1) / 2) & 1, a.status,
+                                      kTimeoutEpilogue, abort_flag)))
+              break;
             tc_fence_after();
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
@@ -661,8 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         nt += tiles;
         cnt += tiles;
         for (int u = 0; u < 2 && ok; ++u)  // the last P V
-          ok = mbar_wait_warp(bar + u, cnt & 1, a.status, kTimeoutEpilogue, abort_flag);
-        ++cnt;
+          ok = mbar_wait_warp(&o_full[2 * g + u], xc & 1, a.status, kTimeoutEpilogue, abort_flag);
         if (!ok) break;
         tc_fence_after();
       }

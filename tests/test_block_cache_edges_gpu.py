@@ -205,3 +205,22 @@ def test_more_work_than_one_wave(b, h, group, n, rows, device_lengths):
     given = torch.tensor(lengths, dtype=torch.int32, device="cuda") if device_lengths else rows
     o, lse = ops.block_cache_attention(q, cache, given, return_lse=True)
     check(q, cache, lengths, o, lse)
+
+
+@pytest.mark.parametrize("b,h,n,rows", [(21, 8, 1024, 1000), (21, 8, 600, 130), (40, 8, 257, 700)])
+def test_many_items_again_and_again(b, h, n, rows):
+    """Short items in long rows of calls, a cold cache before some: every wait ends, every result is the first."""
+    from synthefy_nori_b200 import ops
+
+    cache, g = make(b, h, rows, 56, seed=n)
+    q = (3 * torch.randn(b, n, h, 56, device="cuda", generator=g)).to(torch.bfloat16)
+    first = ops.block_cache_attention(q, cache, rows)
+    cold = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for i in range(400):
+        if i % 8 == 0:
+            cold.fill_(i & 255)
+        o = ops.block_cache_attention(q, cache, rows)
+        if i % 50 == 0:
+            assert torch.equal(o, first)
+    assert torch.equal(o, first)
+    ops.check_status(q.device)
