@@ -6,12 +6,12 @@
 //   q  = round(x * (1 / s)),   rows that stay: q' = round(q * (s_old * (1 / s)))
 // every operation in fp32 with one rounding, ties to even.  A block with an infinity or a NaN gets
 // a NaN scale: all of it reads as NaN, rather than as something finite.
-// A CTA takes 64 rows (128 for blocks of 128) of one (sequence, head) of K or V, twice as many threads a
+// A CTA takes 64 rows (128 for blocks of 128) of one (sequence, head), K and V, twice as many threads a
 // block as it has rows, its new rows in registers between the maximum and the rounding: each new value
-// is read once (2 bytes, or 4) and written once (1 byte).  K and V and all heads of a row are
-// neighbouring CTAs, so the pieces of a cache line that different heads own are read together.
-// Bound by latency between load, maximum and store: CTAs of 128 rows for every block length take 275 us
-// for 222 at 168 x 2048 x 8 x 56 bf16.
+// is read once (2 bytes, or 4) and written once (1 byte).  All heads of a row are neighbouring CTAs, so the
+// pieces of a cache line that different heads own are read together.  168 x 2048 x 8 x 56 bf16 take
+// 155 us, 6.0 TB/s; a CTA each for K and V spent its instructions on finding its place (222 us, issue slots
+// 81% taken), CTAs of 128 rows for every block length left too few loads in flight (275 us).
 //
 // Read.  x = q * s, rounded once to the result's type: 8 values a thread and step.
 //
@@ -148,8 +148,6 @@ __global__ void __launch_bounds__(2 * write_rows(BLOCK))
   constexpr float kTop = FP8 ? 448.f : 127.f;
   uint32_t rest = blockIdx.x / static_cast<uint32_t>(c.heads);  // (32 bits: a division in 64 takes longer than the loads)
   const int h = static_cast<int>(blockIdx.x - rest * static_cast<uint32_t>(c.heads));
-  const int which = static_cast<int>(rest & 1);
-  rest >>= 1;
   const int b = static_cast<int>(rest / per_seq);
   const int64_t j = rest - static_cast<uint32_t>(b) * per_seq;
   const int64_t first = start.at(b), m = min(max(count.at(b), int64_t{0}), n);
@@ -161,63 +159,80 @@ __global__ void __launch_bounds__(2 * write_rows(BLOCK))
   const int r1 = static_cast<int>(min(max(hi - row0, int64_t{0}), int64_t{BLOCK}));
   const bool touched = r0 < r1;
   const int64_t bh = static_cast<int64_t>(b) * c.heads + h;
-  uint8_t* dst = c.data(which) + (bh * c.cap + row0) * c.stored;
-  float* scale = c.scale(which) + bh * c.blocks() + (row0 >> c.block_log2);
-  const int64_t from = which ? rv.offset(b, row0 - first, h) : rk.offset(b, row0 - first, h);
-  const int64_t stride = which ? rv.sn : rk.sn;
-  const void* src = which ? rv.p : rk.p;
+  const int64_t dst_at = (bh * c.cap + row0) * c.stored, scale_at = bh * c.blocks() + (row0 >> c.block_log2);
 
-  Raw<TYPE> x[kEach];
-  uint32_t top = 0;
+  // K, then V: all their values in flight together
+  Raw<TYPE> x[2][kEach];
+  uint32_t top[2] = {0, 0};
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    int row, u;
-    pieces.at(t + e * kGroup, row, u);
-    if (row >= r0 && row < r1) {
-      x[e] = load8<TYPE, ALIGN>(src, from + row * stride + u * 8, c.width - u * 8);
-      top = top_bits<TYPE>(x[e], top);
+  for (int w = 0; w < 2; ++w) {
+    const Rows& src = w ? rv : rk;
+    const int64_t from = src.offset(b, row0 - first, h);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      int row, u;
+      pieces.at(t + e * kGroup, row, u);
+      if (row >= r0 && row < r1) x[w][e] = load8<TYPE, ALIGN>(src.p, from + row * src.sn + u * 8, c.width - u * 8);
     }
   }
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      int row, u;
+      pieces.at(t + e * kGroup, row, u);
+      if (row >= r0 && row < r1) top[w] = top_bits<TYPE>(x[w][e], top[w]);
+    }
   // over the block: magnitudes order like their bits
-  const float old = touched && r0 > 0 ? *scale : 0.f;  // rows before r0 stay
-  uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(top_value<TYPE>(top)));
-  __shared__ uint32_t tops[2 * kRows / 32];
-  if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = w;
+  float old[2] = {0.f, 0.f};
+  if (touched && r0 > 0) old[0] = c.k_scale[scale_at], old[1] = c.v_scale[scale_at];  // rows before r0 stay
+  __shared__ uint32_t tops[2][2 * kRows / 32];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    top[w] = __reduce_max_sync(0xffffffffu, __float_as_uint(top_value<TYPE>(top[w])));
+    if (threadIdx.x % 32 == 0) tops[w][threadIdx.x / 32] = top[w];
+  }
   __syncthreads();
+  if (!touched) return;
   const int w0 = threadIdx.x / kGroup * (kGroup / 32);
 #pragma unroll
-  for (int i = 0; i < kGroup / 32; ++i) w = max(w, tops[w0 + i]);
-  if (!touched) return;
-  const float amax = __uint_as_float(w);
-  float s = __fdiv_rn(fmaxf(amax, 1e-12f), kTop);
-  s = old > s ? old : s;
-  if (!(amax < INFINITY) || old != old) s = __uint_as_float(0x7fc00000u);
-  const float inv = __frcp_rn(s);
+  for (int w = 0; w < 2; ++w) {
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    int row, u;
-    pieces.at(t + e * kGroup, row, u);
-    if (row >= r0 && row < r1) {
-      float y[8];
+    for (int i = 0; i < kGroup / 32; ++i) top[w] = max(top[w], tops[w][w0 + i]);
+    const float amax = __uint_as_float(top[w]), was = old[w];
+    float s = __fdiv_rn(fmaxf(amax, 1e-12f), kTop);
+    s = was > s ? was : s;
+    if (!(amax < INFINITY) || was != was) s = __uint_as_float(0x7fc00000u);
+    const float inv = __frcp_rn(s);
+    uint8_t* dst = c.data(w) + dst_at;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(value<TYPE>(x[e], i), inv);
-      *reinterpret_cast<uint2*>(dst + row * c.stored + u * 8) =
-          make_uint2(codes4<FP8>(y[0], y[1], y[2], y[3]), codes4<FP8>(y[4], y[5], y[6], y[7]));
+    for (int e = 0; e < kEach; ++e) {
+      int row, u;
+      pieces.at(t + e * kGroup, row, u);
+      if (row >= r0 && row < r1) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(value<TYPE>(x[w][e], i), inv);
+        // (W = 8 units: piece t + e * kGroup of the block lies at 8 times that)
+        *reinterpret_cast<uint2*>(dst + (t + e * kGroup) * 8) =
+            make_uint2(codes4<FP8>(y[0], y[1], y[2], y[3]), codes4<FP8>(y[4], y[5], y[6], y[7]));
+      }
     }
-  }
-  if (r0 > 0 && s != old) {  // the rows that stay, under the new scale
-    const float ratio = __fmul_rn(old, inv);
-    for (int i = t; i < r0 * pieces.units; i += kGroup) {
-      uint2* p = reinterpret_cast<uint2*>(dst) + i;  // W = 8 units: pieces are contiguous
-      const uint2 q = *p;
-      float y[8];
+    if (r0 > 0 && s != was) {  // the rows that stay, under the new scale
+      const float ratio = __fmul_rn(was, inv);
+#pragma unroll 1
+      for (int i = t; i < r0 * pieces.units; i += kGroup) {
+        uint2* p = reinterpret_cast<uint2*>(dst) + i;
+        const uint2 q = *p;
+        float y[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        y[k] = __fmul_rn(code_value<FP8>(((k < 4 ? q.x : q.y) >> 8 * (k & 3)) & 0xffu), ratio);
-      *p = make_uint2(codes4<FP8>(y[0], y[1], y[2], y[3]), codes4<FP8>(y[4], y[5], y[6], y[7]));
+        for (int k = 0; k < 8; ++k)
+          y[k] = __fmul_rn(code_value<FP8>(((k < 4 ? q.x : q.y) >> 8 * (k & 3)) & 0xffu), ratio);
+        *p = make_uint2(codes4<FP8>(y[0], y[1], y[2], y[3]), codes4<FP8>(y[4], y[5], y[6], y[7]));
+      }
     }
+    if (t == 0) c.scale(w)[scale_at] = s;
   }
-  if (t == 0) *scale = s;
 }
 
 // ------------------------------------------------------------------ read back
@@ -321,7 +336,7 @@ cudaError_t write_typed(const View& c, const Rows& k, const Rows& v, const PerSe
     // runs of kRows rows that n rows can touch, wherever they begin
     const int64_t most = c.cap / kRows;
     const int64_t span = start.dev == nullptr ? (start.all + n - 1) / kRows - start.all / kRows + 1 : (n - 1) / kRows + 2;
-    const int64_t per_seq = span < most ? span : most, grid = static_cast<int64_t>(c.batch) * per_seq * 2 * c.heads;
+    const int64_t per_seq = span < most ? span : most, grid = static_cast<int64_t>(c.batch) * per_seq * c.heads;
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
     write_kernel<TYPE, FP8, ALIGN, block.value><<<static_cast<unsigned>(grid), 2 * kRows, 0, stream>>>(
         c, k, v, start, count, n, static_cast<uint32_t>(per_seq), pieces);
