@@ -224,3 +224,32 @@ def test_many_items_again_and_again(b, h, n, rows):
             assert torch.equal(o, first)
     assert torch.equal(o, first)
     ops.check_status(q.device)
+
+
+@pytest.mark.parametrize("n,group", [(257, 1), (100, 8), (33, 8)])
+def test_captured_attention_write_attention(n, group):
+    """Both kernels of a call and its joins, a write behind them and a second call, in one graph, replayed: what
+    follows waits for all of them."""
+    from synthefy_nori_b200 import ops
+
+    cache, g = make(6, 2, 5000, 56, seed=n)
+    q = torch.randn(6, n, 2 * group, 56, device="cuda", generator=g).to(torch.bfloat16)
+    k, v = (torch.randn(6, 5000, 2, 56, device="cuda", generator=g) for _ in "kv")
+    kept = [t.clone() for t in cache[:4]]
+
+    def both():
+        a = ops.block_cache_attention(q, cache, 5000)
+        ops.block_cache_write(cache, k, v)
+        return a, ops.block_cache_attention(q, cache, 5000)
+
+    want = both()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for _ in range(5):
+        for dst, src in zip(cache[:4], kept):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert not torch.equal(want[0], want[1])
