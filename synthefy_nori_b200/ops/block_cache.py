@@ -121,7 +121,7 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     contiguous columns; its heads are a multiple of the cache's, neighbours sharing a K/V head.
     ``scale`` (default head_dim ** -0.5) is positive.  ``out``, if given, has q's shape and type and shares
     no memory with q or the cache.  With ``return_lse`` also the natural log-sum-exp, fp32 [batch, heads, n].
-    Length 0 gives zeros and -inf; a query row with an infinity or a NaN gives NaN."""
+    Length 0 gives zeros and -inf; a query row with an infinity or a NaN, or scores past fp32's range, give NaN."""
     k = cache.k
     if not k.is_cuda or not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("block_cache_attention: q and the cache must be CUDA tensors")
