@@ -340,13 +340,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     *reinterpret_cast<uint4*>(sK + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
   }
   if (threadIdx.x == 0) known[0] = item_at(a, blockIdx.x);  // (while the others write)
-  if (failed != 0) return;  // another CTA or kernel timed out
   fence_proxy_async_smem();
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
-  __syncthreads();
+  // Another CTA or kernel timed out: nothing is written.  The word can change at any time, so the threads settle
+  // on one answer; with some gone and some not, tensor memory would be used without its address.
+  const bool stop = __syncthreads_or(failed) != 0;
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (stop) {
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
 
   // The next item, for one thread or a whole warp (`all`): null past the last one or after a timeout.  It
   // stays in shared memory (registers are scarce) until `done_with`.
