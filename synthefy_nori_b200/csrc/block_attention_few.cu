@@ -480,6 +480,7 @@ struct Joined {
 template <bool MANY>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, int parts) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int failed = *reinterpret_cast<const volatile int*>(a.status);
   const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
   const uint32_t unit = MANY ? blockIdx.x : blockIdx.x * kJoinRows + group;  // rows of the cells that are split
   const uint32_t count = static_cast<uint32_t>(a.rows - a.first), tiles = (count + tile_rows - 1) / tile_rows;
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
       fma4(j.acc, sm_o[w][lane], f);
     }
   }
+  if (failed != 0) return;  // a wait has run out: the parts may never have been written
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
   const Row row(a, h, a.first + r);
   const float norm = j.sum != 0.f ? 1.f / j.sum : 0.f;

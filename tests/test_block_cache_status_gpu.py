@@ -29,3 +29,22 @@ def test_after_a_timeout_many_rows_are_left_alone(n, rows):
     for _ in range(3):
         check(q, cache, [rows] * 3, ops.block_cache_attention(q, cache, rows, out=out))
     ops.check_status(q.device)
+
+
+@pytest.mark.parametrize("n,rows", [(200, 700), (1100, 3000), (1, 100003)])
+def test_after_a_timeout_no_parts_are_joined(n, rows):
+    """Where the keys are split, the join does not read parts that were never written."""
+    from synthefy_nori_b200 import ops
+
+    cache, g = make(1, 2, rows, 56)
+    q = torch.randn(1, n, 2, 56, device="cuda", generator=g).to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    word = ops.status_word(q.device)
+    try:
+        word.fill_(2)
+        for _ in range(3):
+            ops.block_cache_attention(q, cache, rows, out=out)
+    finally:
+        word.zero_()
+    assert (out == 7.0).all()
+    check(q, cache, [rows], ops.block_cache_attention(q, cache, rows, out=out))
