@@ -234,6 +234,8 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
       if (lane == 0)  // own copies in flight
         for (int k = i; k < min(mine, i + kStages); ++k)
           mbar_wait(&bars[warp][k % kStages], k / kStages & 1, a.status, kTimeoutEpilogue, nullptr);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __uint_as_float(0x7fc00000u);  // no result of a part of the keys
       break;
     }
     const uint8_t* kp = ring + i % kStages * (2 * kPieceBytes) + key_at(g) * W + unit_of(0) * 8;
