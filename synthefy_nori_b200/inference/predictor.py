@@ -130,6 +130,13 @@ class NoriPredictor:
         if self.placement != "resident":
             self.cuda_graphs = False  # host-staged caches copy per query pass
 
+    def _check_device(self) -> None:
+        """Raises if a bounded wait of a kernel has run out: rows may never have been written."""
+        if self.device.type == "cuda":
+            from synthefy_nori_b200 import ops
+
+            ops.check_status(self.device)
+
     # ------------------------------------------------------------------ context
     def _members(self) -> list[MemberPipeline]:
         return [MemberPipeline(c, s, o) for c, s, o in zip(self.inference_config, self.seeds, self.offsets)]
@@ -165,6 +172,7 @@ class NoriPredictor:
                                                    stream_block_rows=self.stream_block_rows)
             fc.groups.append(MemberGroup(members=[m for m, _ in items], cache=cache))
         if key is not None:
+            self._check_device()  # (nothing is kept of a build that failed)
             self.store.put(key, fc)
         return fc
 
@@ -191,9 +199,9 @@ class NoriPredictor:
                 continue
             outs.append(self.model.apply_context_cache(xq, g.cache, row_chunk_size=self.query_chunk_size,
                                                        return_hidden=return_hidden).float())
-        if return_hidden:
-            return torch.cat(outs, 0)
-        return torch.cat(outs, 0).sum(0) / ctx.n_members
+        out = torch.cat(outs, 0)
+        self._check_device()
+        return out if return_hidden else out.sum(0) / ctx.n_members
 
     @torch.no_grad()
     def context_embeddings(self, X, y, *, categorical=None) -> torch.Tensor:
@@ -209,6 +217,7 @@ class NoriPredictor:
             yy = torch.cat([y, y[:1]], 0).unsqueeze(0)
             h = self.model(xx, yy, eval_pos=X.shape[0], task_type="reg", return_embeddings=True)
             outs.append(h[0, : X.shape[0]].float())
+        self._check_device()
         return torch.stack(outs, 0)
 
     @torch.no_grad()

@@ -48,3 +48,43 @@ def test_after_a_timeout_no_parts_are_joined(n, rows):
         word.zero_()
     assert (out == 7.0).all()
     check(q, cache, [rows], ops.block_cache_attention(q, cache, rows, out=out))
+
+
+@pytest.mark.parametrize("call", ["predict", "embeddings", "build"])
+def test_a_timeout_reaches_who_predicts(call, monkeypatch):
+    """A wait that ran out in a query pass or a build is an error, and nothing of that build is kept."""
+    import numpy as np
+
+    from synthefy_nori_b200 import NoriRegressor, ops
+
+    rng = np.random.default_rng(0)
+    X = rng.normal(size=(200, 4)).astype(np.float32)
+    r = NoriRegressor(model="nori-tiny", weights="random", device="cuda", n_estimators=1, cache_dtype="block_int8")
+    r.fit(X[:150], X[:150, 0])
+    want = r.predict(X[150:])
+    pred, word = r.predictor_, ops.status_word(torch.device("cuda", torch.cuda.current_device()))
+    name = "build_context_cache" if call == "build" else "apply_context_cache"
+    stock = getattr(pred.model, name)
+
+    def fails(*a, **kw):
+        res = stock(*a, **kw)
+        word.fill_(3)  # as a kernel of the call would have set it
+        return res
+
+    try:
+        with monkeypatch.context() as m:
+            m.setattr(pred.model, name, fails)
+            with pytest.raises(RuntimeError, match="timeout"):
+                if call == "build":
+                    pred.fit_context(X[:100], X[:100, 0])
+                elif call == "predict":
+                    r.predict(X[150:])
+                else:
+                    r.get_embeddings(X[150:])
+    finally:
+        word.zero_()
+    if call == "build":
+        hits = pred.store.hits
+        pred.fit_context(X[:100], X[:100, 0])
+        assert pred.store.hits == hits
+    assert np.array_equal(r.predict(X[150:]), want)
