@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(ff::kThreads, 1)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t n_items = p.n_items;
-  if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int failed = read_status(p.status);  // (looked at below)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -117,9 +117,13 @@ __global__ void __launch_bounds__(ff::kThreads, 1)
   }
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
-  __syncthreads();
+  const bool stop = __syncthreads_or(failed) != 0;  // a CTA that starts after another one timed out returns at once
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (stop) {
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   const uint32_t tS = tmem, tO = tmem + 256;
 
   if (warp == 0) {
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(fbw::kThreads, 1)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t n_items = p.n_items;
-  if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int failed = read_status(p.status);  // (looked at below)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -364,9 +368,13 @@ __global__ void __launch_bounds__(fbw::kThreads, 1)
   }
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
-  __syncthreads();
+  const bool stop = __syncthreads_or(failed) != 0;  // a CTA that starts after another one timed out returns at once
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (stop) {
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   const uint32_t tS = tmem, tDP = tmem + 128, tDV = tmem + 256, tDK = tmem + 320, tDQ = tmem + 384,
                  tDS = tmem + 448;
   const int T = p.T;

@@ -252,8 +252,7 @@ __global__ void __launch_bounds__(fa::kThreads, 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int n_tiles = (p.Nk + kN - 1) / kN;
   const int64_t n_items = p.n_items;
-  // a CTA that starts after another one timed out returns at once
-  if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int failed = read_status(p.status);  // (looked at below)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -276,9 +275,13 @@ __global__ void __launch_bounds__(fa::kThreads, 1)
   }
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
-  __syncthreads();
+  const bool stop = __syncthreads_or(failed) != 0;  // a CTA that starts after another one timed out returns at once
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (stop) {
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   const uint32_t tS = tmem;            // S buffers (one per group) at columns 0, 128
   // O accumulators: two sets (item parity) of one per group, at columns 256 + 128 set + 64 group,
   // so the next item's P . V products overlap this item's epilogue
@@ -636,7 +639,7 @@ __global__ void __launch_bounds__(fb::kThreads, 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int n_qt = (p.Nq + kM - 1) / kM;
   const int64_t n_items = p.n_items;
-  if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int failed = read_status(p.status);  // (looked at below)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -658,9 +661,13 @@ __global__ void __launch_bounds__(fb::kThreads, 1)
   }
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
-  __syncthreads();
+  const bool stop = __syncthreads_or(failed) != 0;  // a CTA that starts after another one timed out returns at once
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (stop) {
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   const uint32_t tS = tmem, tDP = tmem + 128, tDV = tmem + 256, tDK = tmem + 320, tDQ = tmem + 384;
   const uint32_t tPT = tmem + 448;  // P^T: key row = lane, queries 2c, 2c + 1 in column c
 

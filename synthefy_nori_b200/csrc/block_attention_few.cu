@@ -482,7 +482,7 @@ struct Joined {
 template <bool MANY>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, int parts) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int failed = *reinterpret_cast<const volatile int*>(a.status);
+  const int failed = read_status(a.status);
   const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
   const uint32_t unit = MANY ? blockIdx.x : blockIdx.x * kJoinRows + group;  // rows of the cells that are split
   const uint32_t count = static_cast<uint32_t>(a.rows - a.first), tiles = (count + tile_rows - 1) / tile_rows;

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   static_assert((8 * kRing + 2 * kItems + 46) % 2 == 0, "the answer is 16-byte aligned");
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int failed = *reinterpret_cast<volatile int*>(a.status);  // (looked at below)
+  const int failed = read_status(a.status);  // (looked at below)
 
   asm volatile("griddepcontrol.launch_dependents;");  // (the join of parts may be set up now)
   if (threadIdx.x == 0) {
@@ -343,9 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_proxy_async_smem();
   if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
-  // Another CTA or kernel timed out: nothing is written.  The word can change at any time, so the threads settle
-  // on one answer; with some gone and some not, tensor memory would be used without its address.
-  const bool stop = __syncthreads_or(failed) != 0;
+  const bool stop = __syncthreads_or(failed) != 0;  // another CTA or kernel timed out: nothing is written
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (stop) {

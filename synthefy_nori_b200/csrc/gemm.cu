@@ -123,8 +123,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int num_n = (p.N + BN - 1) / BN;
   const int num_kb = (p.K + kBK - 1) / kBK;
   const int items = num_m * num_n * p.k_splits;
-  // a CTA that starts after another one timed out returns at once
-  if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int failed = read_status(p.status);  // (looked at below)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -147,9 +146,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   }
   if (warp == 1) tmem_alloc(tmem_slot, Cfg::kTmemCols);
   tc_fence_before();
-  __syncthreads();
+  const bool stop = __syncthreads_or(failed) != 0;  // a CTA that starts after another one timed out returns at once
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (stop) {
+    if (warp == 1) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    return;
+  }
 
   // item -> (mb, nb, ks); N-tiles of one M block are adjacent so the A block stays in L2
   auto decode = [&](int t, int& mb, int& nb, int& ks) {

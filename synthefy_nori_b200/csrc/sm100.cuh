@@ -42,6 +42,13 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// Whether the status word says that a wait of another CTA or kernel has run out.  The word can change at any
+// time, so a CTA whose threads share barriers or tensor memory settles on one answer (__syncthreads_or): with
+// some threads gone and some not, tensor memory would be used without its address.
+__device__ __forceinline__ int read_status(const int* status) {
+  return status != nullptr ? *reinterpret_cast<const volatile int*>(status) : 0;
+}
+
 // ------------------------------------------------------------------ mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
