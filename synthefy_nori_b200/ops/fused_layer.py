@@ -1168,7 +1168,8 @@ def _rowwise_chunked(fn, x, rows_tok: int):
 @torch.no_grad()
 def build_stack_cache(model, tokens: torch.Tensor, quantize: bool | str = False) -> list:
     """Run the context tokens ``[B, N, T, E]`` through every layer and keep each layer's
-    cross-attention K/V, in bf16, int8 per vector (``quantize=True``) or a type of ``BLOCK_CACHES`` by name (reference ``LayerStack.build_train_cache``, layer.py:2058-2096).
+    cross-attention K/V, in bf16, int8 per vector (``quantize=True``) or a type of ``BLOCK_CACHES`` by name
+    (reference ``LayerStack.build_train_cache``, layer.py:2058-2096).
     A single long table is processed in row chunks when one layer's full-height
     intermediates would not fit next to the caches (``_build_rows_chunk``)."""
     check_supported(model)
@@ -1177,6 +1178,10 @@ def build_stack_cache(model, tokens: torch.Tensor, quantize: bool | str = False)
     x = tokens.to(BF16).reshape(-1, E).contiguous()
     hid = int(layer_weights(model.transformer_encoder.layers[0])["w_down"].shape[1])  # SwiGLU hidden width
     rows = _build_rows_chunk(g, hid, len(model.transformer_encoder.layers), bool(quantize), x.device)
+    if quantize in BLOCK_CACHES and rows < N:
+        # whole blocks a chunk: one that a chunk's end cuts would be quantised twice, and the cache would hang on
+        # how much memory was free
+        rows = max(BlockKV.BLOCK, rows // BlockKV.BLOCK * BlockKV.BLOCK)
     if rows < N:
         caches = []
         for layer in model.transformer_encoder.layers:
