@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
     m[nt][0] = m[nt][1] = -INFINITY;
     l[nt][0] = l[nt][1] = 0.f;
   }
-  float sk = 0.f, sv = 0.f;
+  float sk = 0.f, sv = 0.f, least = kLeastScale;
   // (a warp's pieces are 128 keys apart, a whole number of blocks)
   const int64_t blk = first * kPiece >> a.c.block_log2;
   const int blk_step = kWarps * kPiece >> a.c.block_log2;
@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
   int rest = static_cast<int>(len - first * kPiece);  // keys from this piece's first on
 
   for (int i = 0; i < mine; ++i, rest -= kWarps * kPiece) {
-    const float sk_now = sk, svc = safe_scale(sv);
+    raise_floor(least, sv);
+    const float sk_now = sk, svc = safe_scale(sv, least);
     if (i + 1 < mine) sk = __ldg(ks += blk_step), sv = __ldg(vs += blk_step);
     if (!mbar_wait_warp(&bars[warp][i % kStages], i / kStages & 1, a.status, kTimeoutEpilogue, nullptr)) {
       if (lane == 0)  // own copies in flight
@@ -322,9 +323,9 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
         for (int i2 = 0; i2 < 2; ++i2) {
           const float all = keys_max(cand[nt][i2]);
           if (all > m[nt][i2] + kLazy || m[nt][i2] == -INFINITY) {
-            const float back = m[nt][i2] == -INFINITY ? 0.f : exp2_fast(m[nt][i2] - all);
+            const float h = m[nt][i2] == -INFINITY ? 0.f : exp2_fast(0.5f * (m[nt][i2] - all)), back = h * h;
             m[nt][i2] = all;
-            l[nt][i2] *= back;
+            l[nt][i2] = lowered(l[nt][i2], h);
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[nt][j][i2] *= back, o[nt][j][2 + i2] *= back;
           }
@@ -416,9 +417,9 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
     float sum = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f ? 0.f : exp2f(sm_m[w][r] - top);
-      sum = fmaf(sm_l[w][r], f, sum);
-      acc = fmaf(sm_o[w][r][d], f, acc);
+      const float h = sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f ? 0.f : exp2f(0.5f * (sm_m[w][r] - top));
+      sum = fmaf(sm_l[w][r] * h, h, sum);
+      acc = fmaf(sm_o[w][r][d], h * h, acc);
     }
     if (a.cluster == 1) {
       put_row(r, d, top, sum, acc);
@@ -451,9 +452,9 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       if (c < a.cluster) {
-        const float f = ml[c].x == -INFINITY && ml[c].y == 0.f ? 0.f : exp2f(ml[c].x - top);
-        sum = fmaf(ml[c].y, f, sum);
-        acc = fmaf(v[c], f, acc);
+        const float h = ml[c].x == -INFINITY && ml[c].y == 0.f ? 0.f : exp2f(0.5f * (ml[c].x - top));
+        sum = fmaf(ml[c].y * h, h, sum);
+        acc = fmaf(v[c], h * h, acc);
       }
     put_row(r, d, top, sum, acc);
   }
@@ -474,8 +475,8 @@ struct Joined {
   float top = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   __device__ __forceinline__ void rescale(float t) {
-    const float back = top == -INFINITY ? 0.f : exp2f(top - t);
-    top = t, sum *= back;
+    const float h = top == -INFINITY ? 0.f : exp2f(0.5f * (top - t)), back = h * h;
+    top = t, sum = lowered(sum, h);
     acc.x *= back, acc.y *= back, acc.z *= back, acc.w *= back;
   }
 };
@@ -514,9 +515,9 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // no keys there (and perhaps no values written)
-      const float f = exp2f(ml[k].x - t);
-      j.sum = fmaf(ml[k].y, f, j.sum);
-      fma4(j.acc, v[k], f);
+      const float h = exp2f(0.5f * (ml[k].x - t));
+      j.sum = fmaf(ml[k].y * h, h, j.sum);
+      fma4(j.acc, v[k], h * h);
     }
   }
   if constexpr (MANY) {
@@ -534,9 +535,9 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
 #pragma unroll
     for (int w = 0; w < kJoinRows; ++w) {
       if (sm_ml[w].x == -INFINITY && sm_ml[w].y == 0.f) continue;
-      const float f = exp2f(sm_ml[w].x - t);
-      j.sum = fmaf(sm_ml[w].y, f, j.sum);
-      fma4(j.acc, sm_o[w][lane], f);
+      const float h = exp2f(0.5f * (sm_ml[w].x - t));
+      j.sum = fmaf(sm_ml[w].y * h, h, j.sum);
+      fma4(j.acc, sm_o[w][lane], h * h);
     }
   }
   if (failed != 0) return;  // a wait has run out: the parts may never have been written

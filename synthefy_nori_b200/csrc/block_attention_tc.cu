@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&q_full[buf]);
         ++qcnt;
       }
-      float sk = 0.f, sv = 0.f;
+      float sk = 0.f, sv = 0.f, least = kLeastScale;
       if (warp == 4 && tiles > 0) sk = __ldg(ks), sv = __ldg(vs);
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j, ++n, left -= kN) {
@@ -584,7 +584,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (warp == 4) {
-          const float svc = safe_scale(sv);
+          float top = left > 0 ? sv : 0.f;  // of the tile's four chunks (fmaxf passes over a NaN)
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          raise_floor(least, fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
+          const float svc = safe_scale(sv, least);
           // (a block behind the last row counts for nothing, whatever its scale)
           const float4 y = left > 0 ? make_float4(sk, __log2f(svc), __fdividef(1.f, svc), 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
           if (lane < 4) scales[n & 3][lane] = y;
@@ -658,12 +661,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (step == 0) {
             m = cand;
           } else if (cand > m + kLazy) {
-            back = exp2_mufu(m - cand);
+            const float h = exp2_mufu(0.5f * (m - cand));
+            back = h * h;
+            l = lowered(l, h);
             m = cand;
             grow = true;
           }
           const float lift = m == -INFINITY ? 0.f : kLift - m;  // (no key of this half is there)
-          l = fmaf(weights32(x, f, sc.y + lift, tC), sc.z, l * back);
+          l = fmaf(weights32(x, f, sc.y + lift, tC), sc.z, l);
           if (__any_sync(0xffffffffu, grow)) {
             // the other chunk's product may still be under way: its next scores, if there are any, come behind it
             const bool last = step == 2 * tiles - 1;
@@ -709,10 +714,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 other = exchange(make_float2(m, l));
         if (!ok) break;
         const float top = fmaxf(m, other.x);
-        const float f = m == -INFINITY ? 0.f : exp2f(m - top), f2 = other.x == -INFINITY ? 0.f : exp2f(other.x - top);
-        l = l * f + other.y * f2;
+        const float h1 = m == -INFINITY ? 0.f : exp2f(0.5f * (m - top));
+        const float h2 = other.x == -INFINITY ? 0.f : exp2f(0.5f * (other.x - top));
+        l = lowered(l, h1) + lowered(other.y, h2);
         m = top;
-        fa = half ? f2 : f, fb = half ? f : f2;
+        fa = half ? h2 * h2 : h1 * h1, fb = half ? h1 * h1 : h2 * h2;
         tc_fence_after();
       }
       if (!part) {

@@ -136,9 +136,22 @@ __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
   down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 }
 
-// A V scale whose log2 and inverse are finite: a block that was never written has scale 0 and holds
-// zeros, which the smallest scale of a written block says as well.
-__device__ __forceinline__ float safe_scale(float s) { return s == 0.f ? 7.9e-15f : s; }
+// The V scale that a block counts with: one whose log2 and inverse are finite (a block that was never written has
+// scale 0 and holds zeros), and 2^-100 of the largest so far at least.  Weights carry the scale (t = score + log2 s_v)
+// and the sum divides by it, so keys of a block whose values are tiny beside the largest can be all of the sum and
+// nothing of the result: with a log2 further below, 2^t would leave fp32's range.  The sum does not mind which scale
+// it is; the result is off by 2^-100 of the largest value at most.
+constexpr float kLeastScale = 0x1p-80f;  // (written ones are 2^-49 or more)
+__device__ __forceinline__ void raise_floor(float& least, float s) { least = fmaxf(least, s * 0x1p-100f); }  // (not by a NaN)
+__device__ __forceinline__ float safe_scale(float s, float least) {  // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(s), "f"(least));
+  return r;
+}
+
+// A sum times h^2 = 2^d, d <= 0, in two steps: 2^d alone may lie below fp32's range where the sum, which divides by
+// scales down to 2^-47, lies as far above 1.
+__device__ __forceinline__ float lowered(float sum, float h) { return sum * h * h; }
 
 // The natural log-sum-exp of a row from its maximum and its sum (which carries kLift).
 __device__ __forceinline__ float row_lse(float m, float l) {

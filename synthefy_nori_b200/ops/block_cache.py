@@ -121,7 +121,12 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     contiguous columns; its heads are a multiple of the cache's, neighbours sharing a K/V head.
     ``scale`` (default head_dim ** -0.5) is positive.  ``out``, if given, has q's shape and type and shares
     no memory with q or the cache.  With ``return_lse`` also the natural log-sum-exp, fp32 [batch, heads, n].
-    Length 0 gives zeros and -inf; a query row with an infinity or a NaN, or scores past fp32's range, give NaN."""
+    Length 0 gives zeros and -inf; a query row with an infinity or a NaN, or scores past fp32's range, give NaN.
+
+    Sums, maxima and results are held in fp32; weights are rounded to fp16 for the product with V, relative to the
+    largest weight times its block's scale of V (11 bits down to 2^-21 of that).  A block's scale of V counts as
+    2^-80 and as 2^-100 of the largest at least: the result is off by 2^-100 of the largest value of V at most, the
+    log-sum-exp not at all."""
     k = cache.k
     if not k.is_cuda or not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("block_cache_attention: q and the cache must be CUDA tensors")
