@@ -1,6 +1,8 @@
 // Python bindings of the native operator library (module synthefy_nori_b200._C).
 #include <torch/extension.h>
 
+#include "plain.h"
+
 namespace nori {
 torch::Tensor gemm_bf16(const torch::Tensor& A, const torch::Tensor& W, const c10::optional<torch::Tensor>& row_scale,
                         const c10::optional<torch::Tensor>& bias, const torch::Tensor& status, int64_t bn, bool w_kn,
@@ -253,4 +255,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_cache_write", &nori::block_cache_write);
   m.def("block_cache_read", &nori::block_cache_read);
   m.def("block_cache_attention", &nori::block_cache_attention);
+  m.def("shares_memory", [](const torch::Tensor& a, const c10::optional<torch::Tensor>& b) {  // b: none for a itself
+    return b.has_value() ? nori::shares_memory(a, *b) : nori::shares_memory(a, a, true);
+  }, py::arg("a"), py::arg("b") = py::none());
 }

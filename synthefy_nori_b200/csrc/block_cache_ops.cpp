@@ -1,6 +1,5 @@
 // Entry points of the context cache in 8 bits with block scales: checks of the arguments, the
 // choice of kernel and of how far the keys are split.
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -166,6 +165,11 @@ void block_cache_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, co
     TORCH_CHECK(start_all >= 0 && n <= c.cap && start_all <= c.cap - n, who, ": ", num(n), " rows from ", num(start_all),
                 " on of a cache of ", num(c.cap));
   if (n == 0 || c.batch == 0 || c.heads == 0) return;
+  const Tensor* parts[] = {&ck, &cv, &cks, &cvs};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < i; ++j) TORCH_CHECK(!overlap(*parts[i], *parts[j]), who, ": the cache's tensors share memory");
+    TORCH_CHECK(!shares_memory(*parts[i], k) && !shares_memory(*parts[i], v), who, ": k or v shares memory with the cache");
+  }
   const at::cuda::CUDAGuard guard(ck.device());
   C10_CUDA_CHECK(bc::launch_write(c, rk, rv, type, start, count, n, at::cuda::getCurrentCUDAStream()));
 }
@@ -206,9 +210,14 @@ std::tuple<Tensor, OptTensor> block_cache_attention(const Tensor& q, const Tenso
   const bool given = out.has_value() && out->defined();
   const Tensor o = given ? *out : torch::empty(q.sizes(), q.options());
   TORCH_CHECK(o.scalar_type() == q.scalar_type() && o.sizes() == q.sizes(), who, ": out of q's shape and type expected");
-  TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes, who, ": rows of out share memory");
   a.o = rows_of(o, a.c, a.n, heads, ck.device(), who, "out");
   a.length = per_sequence(length_dev, length_all, a.c, ck.device(), who, "lengths");
+  if (given) {
+    TORCH_CHECK(!shares_memory(o, o, true), who, ": rows of out share memory");
+    for (const Tensor* t : {&q, &ck, &cv, &cks, &cvs})
+      TORCH_CHECK(!shares_memory(o, *t), who, ": out shares memory with q or the cache");
+    TORCH_CHECK(a.length.dev == nullptr || !shares_memory(o, *length_dev), who, ": out shares memory with the lengths");
+  }
   if (a.length.dev == nullptr)
     TORCH_CHECK(length_all >= 0 && length_all <= a.c.cap, who, ": length ", num(length_all), " of a cache of ", num(a.c.cap));
   TORCH_CHECK(scale > 0.0 && scale < 1e30, who, ": a positive finite scale expected");

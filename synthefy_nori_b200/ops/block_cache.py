@@ -87,7 +87,7 @@ def block_cache_write(cache: BlockCache, k: torch.Tensor, v: torch.Tensor, start
     any strides with contiguous columns) into rows ``start .. start + n`` of each sequence.
 
     ``start`` is an int or int32 [batch] on the device, ``counts`` (int32 [batch], default n) how many
-    of the n rows of a sequence are there.  A block's scale is its largest magnitude over 127 (int8)
+    of the n rows of a sequence are there.  ``k`` and ``v`` share no memory with the cache.  A block's scale is its largest magnitude over 127 (int8)
     or 448 (e4m3).  Where earlier rows of the first block stay (``start`` inside a block), its scale
     only grows, and they are quantised again under it when it does (half a step more error).  Rows
     at or behind ``start + counts`` in the last block end there: their codes stay, but under its new scale.
@@ -120,7 +120,7 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     ``q`` is bf16 or fp16 [batch, n, heads, head_dim] (or two batch dimensions) with any strides and
     contiguous columns; its heads are a multiple of the cache's, neighbours sharing a K/V head.
     ``scale`` (default head_dim ** -0.5) is positive.  ``out``, if given, has q's shape and type and shares
-    no memory with q or the cache.  With ``return_lse`` also the natural log-sum-exp, fp32 [batch, heads, n].
+    no memory with q, the cache or the lengths (columns of one buffer side by side share none).  With ``return_lse`` also the natural log-sum-exp, fp32 [batch, heads, n].
     Length 0 gives zeros and -inf; a query row with an infinity or a NaN, or scores past fp32's range, give NaN.
 
     Sums, maxima and results are held in fp32; weights are rounded to fp16 for the product with V, relative to the
