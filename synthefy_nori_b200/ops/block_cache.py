@@ -15,6 +15,7 @@ operation has a gradient: results have no graph.
 
 from __future__ import annotations
 
+from operator import index
 from typing import NamedTuple
 
 import torch
@@ -57,17 +58,18 @@ def block_cache(batch: int, heads: int, capacity: int, head_dim: int, *, dtype=t
     """An empty cache (zeros) for ``capacity`` rows of ``batch`` sequences (made a multiple of 128)."""
     if dtype not in BLOCK_CACHE_TYPES:
         raise ValueError(f"block_cache: int8 or float8_e4m3fn expected, got {dtype}")
+    batch, heads, capacity, head_dim, block = (index(x) for x in (batch, heads, capacity, head_dim, block))
     if block not in (32, 64, 128):
         raise ValueError(f"block_cache: blocks of 32, 64 or 128 rows expected, got {block}")
     if not 1 <= head_dim <= 64:
         raise ValueError(f"block_cache: head widths of 1 to 64 expected, got {head_dim}")
     if batch < 0 or heads < 0 or capacity < 0:
         raise ValueError("block_cache: negative size")
-    cap = max(_ROWS, -(-int(capacity) // _ROWS) * _ROWS)
-    width = -(-int(head_dim) // 8) * 8
+    cap = max(_ROWS, -(-capacity // _ROWS) * _ROWS)
+    width = -(-head_dim // 8) * 8
     k, v = (torch.zeros(batch, heads, cap, width, dtype=dtype, device=device) for _ in "kv")
     ks, vs = (torch.zeros(batch, heads, cap // block, dtype=torch.float32, device=device) for _ in "kv")
-    return BlockCache(k, v, ks, vs, int(head_dim))
+    return BlockCache(k, v, ks, vs, head_dim)
 
 
 def _cuda(t, who: str, what: str) -> None:
@@ -79,7 +81,7 @@ def _int_or_tensor(x):
     """(value, device tensor or None) of an int or an int32 tensor."""
     if isinstance(x, torch.Tensor):
         return 0, x
-    return int(x), None
+    return index(x), None
 
 
 def block_cache_write(cache: BlockCache, k: torch.Tensor, v: torch.Tensor, start=0, counts=None) -> None:
@@ -107,8 +109,8 @@ def block_cache_read(cache: BlockCache, start: int = 0, end: int | None = None, 
     _cuda(cache.k, "block_cache_read", "the cache")
     if dtype not in _FLOATS:
         raise ValueError(f"block_cache_read: fp32, bf16 or fp16 expected, got {dtype}")
-    end = cache.capacity if end is None else int(end)
-    k, v = _lib().block_cache_read(*cache[:4], cache.head_dim, int(start), end - int(start), dtype)
+    start, end = index(start), cache.capacity if end is None else index(end)
+    k, v = _lib().block_cache_read(*cache[:4], cache.head_dim, start, end - start, dtype)
     return k, v
 
 
@@ -133,7 +135,7 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     if out is not None and not (isinstance(out, torch.Tensor) and out.shape == q.shape and out.dtype == q.dtype
                                 and out.device == q.device):
         raise ValueError("block_cache_attention: out must have q's shape, type and device")
-    length, length_dev = (0, lengths) if isinstance(lengths, torch.Tensor) else (int(lengths), None)
+    length, length_dev = _int_or_tensor(lengths)
     res, lse = _lib().block_cache_attention(q, k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, length, length_dev,
                                             cache.head_dim ** -0.5 if scale is None else scale, out, return_lse,
                                             status_word(k.device))

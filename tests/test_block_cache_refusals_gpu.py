@@ -69,3 +69,22 @@ def test_writes_that_share_memory():
     same = ops.BlockCache(c.k, c.k, c.k_scale, c.k_scale, 16)
     q = torch.ones(1, 1, 2, 16, device="cuda", dtype=torch.bfloat16)
     assert (ops.block_cache_attention(q, same, 10) == 1).all()
+
+
+def test_lengths_and_places_are_whole_numbers():
+    """A fraction is refused, not cut off; numpy's whole numbers are taken."""
+    import numpy as np
+
+    from synthefy_nori_b200 import ops
+
+    c, g = make(1, 2, 200, 16)
+    x = torch.randn(1, 10, 2, 16, device="cuda", generator=g)
+    q = x.bfloat16()
+    before = [t.clone() for t in c[:4]]
+    _refused(
+        lambda: ops.block_cache_attention(q, c, 10.9), lambda: ops.block_cache_attention(q, c, "10"),
+        lambda: ops.block_cache_attention(q, c, np.float64(10.0)), lambda: ops.block_cache_write(c, x, x, start=0.5),
+        lambda: ops.block_cache_read(c, 0.5, 10), lambda: ops.block_cache_read(c, 0, 9.5),
+    )
+    assert all(torch.equal(a, b) for a, b in zip(before, c[:4]))
+    assert torch.equal(ops.block_cache_attention(q, c, np.int64(10)), ops.block_cache_attention(q, c, 10))
