@@ -21,7 +21,7 @@ use: the smaller of the kernel's available memory and the container's cgroup lim
 ``context_row_chunk`` context rows and the device never holds a full layer; query
 attention merges the block partials by their log-sum-exps.  A cache type
 ``"block_int8"`` or ``"block_fp8"`` (8 bits with a scale for each block of rows and head) takes
-the place of int8 on the resident, offload and stream rungs.  ``context_sharded_int8`` is
+the place of int8 on the resident, offload and stream rungs, not on the sharded one.  ``context_sharded_int8`` is
 this build's multi-GPU rung (the cache split by context rows over the GPUs of one node,
 ``parallel/context_parallel.py``).  ``escalated`` records a rung the caller moved to after
 an out-of-memory error (reference ``MemoryPolicy.escalated``).
@@ -180,6 +180,8 @@ class MemoryPolicy(BaseModel):
         i8 = footprint(bf16, head_dim=head_dim)
         q_ok = self.cache_dtype != "bf16" or self.allow_quantization
         budget = self.budget_gb(device_total_gb)
+        # the shards of several GPUs hold int8 with a scale for each vector, whatever the type asked for
+        sharded = int8_footprint_gb(bf16, head_dim=head_dim)
         upd = {"est_cache_gb": bf16, "dropped_context_rows": 0}
         per_layer = bf16 / max(nlayers, 1)
         if not self.cache:
@@ -201,8 +203,8 @@ class MemoryPolicy(BaseModel):
             upd.update(rung="resident_bf16", resident_gb=bf16)
         elif q_ok and i8 <= budget:
             upd.update(rung="resident_int8", resident_gb=i8)
-        elif n_gpus > 1 and q_ok and i8 / n_gpus <= budget:  # NVLink beats the host link
-            upd.update(rung="context_sharded_int8", resident_gb=i8 / n_gpus)
+        elif n_gpus > 1 and q_ok and sharded / n_gpus <= budget:  # NVLink beats the host link
+            upd.update(rung="context_sharded_int8", resident_gb=sharded / n_gpus)
         elif self.offload_to_host and self.cache_dtype == "bf16" and bf16 <= self.host_budget(host_total_gb) \
                 and 2 * per_layer <= budget:
             upd.update(rung="offload_bf16", resident_gb=2 * per_layer)
@@ -255,7 +257,7 @@ class MemoryPolicy(BaseModel):
         """(cache dtype, placement, stream block rows) of the resolved rung."""
         r = self.rung or "resident_bf16"
         dtype = self.cache_dtype
-        if dtype == "bf16" and r.endswith("int8"):
+        if r == "context_sharded_int8" or (dtype == "bf16" and r.endswith("int8")):
             dtype = "int8"
         if r in OFFLOAD_RUNGS:
             return dtype, "offload", None

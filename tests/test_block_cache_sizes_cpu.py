@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from synthefy_nori_b200 import ops
+from synthefy_nori_b200.inference.memory_policy import MemoryPolicy, int8_footprint_gb
 
 
 @pytest.mark.parametrize("kw", [dict(capacity=100.5), dict(head_dim=16.5), dict(batch=1.5), dict(heads=2.0), dict(block=64.0)])
@@ -16,3 +17,16 @@ def test_fractions_are_refused(kw):
 def test_whole_numbers_of_numpy():
     c = ops.block_cache(*(np.int64(x) for x in (2, 3, 100, 20)), device="cpu")
     assert c.k.shape == (2, 3, 128, 24) and c.head_dim == 20 and type(c.head_dim) is int
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int8", "block_int8", "block_fp8"])
+def test_shards_of_several_gpus_hold_int8(dtype):
+    """The sharded rung has one form, int8 with a scale for each vector: it is sized and named as that."""
+    table = dict(n_context_rows=100_000, n_groups=21, nlayers=26, embed_dim=448, head_dim=56, device_total_gb=20.0,
+                 host_total_gb=0.0)
+    got = MemoryPolicy(cache_dtype=dtype).resolve(**table, n_gpus=8)
+    assert got.rung == "context_sharded_int8" and got.placement() == ("int8", "resident", None)
+    assert got.resident_gb == pytest.approx(int8_footprint_gb(got.est_cache_gb, head_dim=56) / 8)
+    # a budget that block scales would meet (1 + 4 / 3584) and a scale for each vector (1 + 4 / 56) does not
+    tight = MemoryPolicy(cache_dtype=dtype, gpu_budget_absolute_gb=got.est_cache_gb / 16 * 1.03)
+    assert tight.resolve(**table, n_gpus=8).rung == "subsample"
