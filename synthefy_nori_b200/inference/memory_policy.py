@@ -89,11 +89,12 @@ def int8_footprint_gb(est_bf16_gb: float, *, head_dim: int) -> float:
     return est_bf16_gb / 2.0 * (1.0 + 4.0 / max(head_dim, 1))
 
 
-def block_footprint_gb(est_bf16_gb: float, *, head_dim: int, block: int = 64) -> float:
+def block_footprint_gb(est_bf16_gb: float, *, head_dim: int, block: int = 64, n_context_rows: int | None = None) -> float:
     """The same cache in 8 bits with one fp32 scale per (block of rows, head); stored head widths are
-    multiples of 8."""
+    multiples of 8, and rows (where their number is given) of 128."""
     d = max(head_dim, 1)
-    return est_bf16_gb / 2.0 * (-(-d // 8) * 8 / d + 4.0 / (block * d))
+    rows = 1.0 if not n_context_rows else -(-n_context_rows // 128) * 128 / n_context_rows
+    return est_bf16_gb / 2.0 * (-(-d // 8) * 8 / d + 4.0 / (block * d)) * rows
 
 
 class ContextTooLargeError(RuntimeError, MemoryError):
@@ -176,8 +177,9 @@ class MemoryPolicy(BaseModel):
             raise ValueError("stream_context=True requires offload_to_host=True (the stream lives in host RAM)")
         bf16 = estimate_cache_gb(n_context_rows=n_context_rows, n_groups=n_groups, nlayers=nlayers,
                                  embed_dim=embed_dim)
-        footprint = block_footprint_gb if self.cache_dtype.startswith("block_") else int8_footprint_gb
-        i8 = footprint(bf16, head_dim=head_dim)
+        block = self.cache_dtype.startswith("block_")
+        i8 = (block_footprint_gb(bf16, head_dim=head_dim, n_context_rows=n_context_rows) if block
+              else int8_footprint_gb(bf16, head_dim=head_dim))
         q_ok = self.cache_dtype != "bf16" or self.allow_quantization
         budget = self.budget_gb(device_total_gb)
         # the shards of several GPUs hold int8 with a scale for each vector, whatever the type asked for
@@ -214,8 +216,12 @@ class MemoryPolicy(BaseModel):
         elif self.allow_subsample:
             per_row = (i8 if q_ok else bf16) / max(n_context_rows, 1)
             keep = int(budget / per_row) if per_row > 0 else n_context_rows
+            if block:  # (capacities are multiples of 128 rows)
+                per_row = i8 / (-(-n_context_rows // 128) * 128)
+                keep = int(budget / per_row) // 128 * 128
             keep = max(1, min(keep, n_context_rows))
-            upd.update(rung="subsample", resident_gb=per_row * keep, dropped_context_rows=n_context_rows - keep)
+            upd.update(rung="subsample", resident_gb=per_row * (-(-keep // 128) * 128 if block else keep),
+                       dropped_context_rows=n_context_rows - keep)
         else:
             raise ContextTooLargeError(f"context cache needs {i8:.1f} GiB even as int8 (budget {budget:.1f} GiB) "
                                        "and subsampling is disabled: raise elements_budget / the device budget, or "
