@@ -179,6 +179,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> block_cache_attention(
     const torch::Tensor& q, const torch::Tensor& ck, const torch::Tensor& cv, const torch::Tensor& cks,
     const torch::Tensor& cvs, int64_t width, int64_t length_all, const c10::optional<torch::Tensor>& length_dev,
     double scale, const c10::optional<torch::Tensor>& out, bool want_lse, const torch::Tensor& status);
+torch::Tensor status_word_beside_capture(int64_t device);
 }  // namespace nori
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -255,6 +256,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_cache_write", &nori::block_cache_write);
   m.def("block_cache_read", &nori::block_cache_read);
   m.def("block_cache_attention", &nori::block_cache_attention);
+  m.def("status_word_beside_capture", &nori::status_word_beside_capture);
   m.def("shares_memory", [](const torch::Tensor& a, const c10::optional<torch::Tensor>& b) {  // b: none for a itself
     return b.has_value() ? nori::shares_memory(a, *b) : nori::shares_memory(a, a, true);
   }, py::arg("a"), py::arg("b") = py::none());

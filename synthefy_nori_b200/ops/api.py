@@ -70,7 +70,10 @@ def status_word(device: torch.device) -> torch.Tensor:
         if torch._C._len_torch_dispatch_stack():  # a fake word would stay for every later call
             with torch.utils._python_dispatch._disable_current_modes():
                 return status_word(device)
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        if torch.cuda.is_current_stream_capturing():  # the graph would own the word and clear it with every replay
+            t = _lib().status_word_beside_capture(idx)
+        else:
+            t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
         _STATUS[idx] = t
     return t
 

@@ -88,3 +88,40 @@ def test_a_timeout_reaches_who_predicts(call, monkeypatch):
         pred.fit_context(X[:100], X[:100, 0])
         assert pred.store.hits == hits
     assert np.array_equal(r.predict(X[150:]), want)
+
+
+FIRST_CALL = """
+import torch
+from synthefy_nori_b200 import ops
+
+cache = ops.block_cache(2, 2, 640, 32)
+x = torch.randn(2, 640, 2, 32, device="cuda")
+ops.block_cache_write(cache, x, x)
+q = torch.randn(2, 200, 2, 32, device="cuda").to(torch.bfloat16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):  # the first call that takes the word
+    o = ops.block_cache_attention(q, cache, 640)
+assert int(ops.status_word(q.device).item()) == 0
+graph.replay()
+want = ops.block_cache_attention(q, cache, 640)
+assert torch.equal(o, want)
+word = ops.status_word(q.device)
+word.fill_(7)
+o.zero_()
+graph.replay()
+assert int(word.item()) == 7 and not o.any()
+word.zero_()
+graph.replay()
+assert torch.equal(o, want)
+print("fine")
+"""
+
+
+def test_the_first_call_may_be_captured():
+    """The status word is not part of the graph that happens to make the first call: replays do not clear it."""
+    import subprocess
+    import sys
+
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "fine" in run.stdout, run.stderr[-2000:]
