@@ -3,7 +3,8 @@
 A ``BlockCache`` holds keys and values as int8 or e4m3 codes ``[batch, heads, capacity, W]`` (``W`` the
 head width up to a multiple of 8) with one fp32 scale per (sequence, head, block of 32, 64 or 128
 rows); a value is code * scale.  ``block_cache_write`` quantises rows as they are written, at the end of
-what a sequence holds or anywhere; ``block_cache_read`` gives them back; ``block_cache_attention`` runs
+what a sequence holds (rows behind them in the same block keep their codes and get the block's new scale,
+so rows in the middle are rewritten by whole blocks); ``block_cache_read`` gives them back; ``block_cache_attention`` runs
 query rows against the codes themselves (any number of rows, a single one included; shared K/V
 heads).  Against one scale per (row, head) vector (``quantize_int8``) the scales take 4 / (block D)
 instead of 4 / D of the codes, and the attention needs no bf16 copy of the cache.
@@ -91,7 +92,9 @@ def block_cache_write(cache: BlockCache, k: torch.Tensor, v: torch.Tensor, start
     ``start`` is an int or int32 [batch] on the device, ``counts`` (int32 [batch], default n) how many
     of the n rows of a sequence are there.  ``k`` and ``v`` share no memory with the cache.  A block's scale is its largest magnitude over 127 (int8)
     or 448 (e4m3).  Where earlier rows of the first block stay (``start`` inside a block), its scale
-    only grows, and they are quantised again under it when it does (half a step more error).  Rows
+    only grows, and they are quantised again under it when it does: each growth rounds them once more (half a
+    step of the new scale in int8, up to 2^-4 of the value in e4m3), up to block - 1 times where rows come one
+    by one.  Rows written by whole blocks are rounded once.  Rows
     at or behind ``start + counts`` in the last block end there: their codes stay, but under its new scale.
     With device values, rows outside the capacity are not written.  A block that gets an infinity or
     a NaN reads as NaN."""
@@ -126,7 +129,7 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     Length 0 gives zeros and -inf; a query row with an infinity or a NaN, or scores past fp32's range, give NaN.
 
     Sums, maxima and results are held in fp32; weights are rounded to fp16 for the product with V, relative to the
-    largest weight times its block's scale of V (11 bits down to 2^-21 of that).  A block's scale of V counts as
+    largest weight times its block's scale of V (11 bits down to 2^-21 of that, 2^-32 of it below).  A block's scale of V counts as
     2^-80 and as 2^-100 of the largest at least: the result is off by 2^-100 of the largest value of V at most, the
     log-sum-exp not at all."""
     k = cache.k
