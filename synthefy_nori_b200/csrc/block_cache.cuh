@@ -162,9 +162,9 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 cudaError_t launch_write(const View& c, const Rows& k, const Rows& v, int type, const PerSequence& start,
                          const PerSequence& count, int64_t n, cudaStream_t stream);
 cudaError_t launch_read(const View& c, void* k, void* v, int type, int64_t start, int64_t n, cudaStream_t stream);
-// rows of a tile of the two attention kernels, and how many splits of the keys they would take
+// rows of a tile of the kernel for few rows, and how many of its CTAs an SM holds
 int few_tile_rows(int64_t rows);
-int few_resident(int64_t rows);  // CTAs that an SM holds
+int few_resident(int64_t rows);
 // beside: it may start while the kernel before it on the stream, which it does not depend on, still runs
 cudaError_t launch_few(const Attention& a, bool beside, cudaStream_t stream);
 // rows of a tile pair of the kernel for many rows; one CTA per SM

@@ -103,7 +103,11 @@ bc::PerSequence per_sequence(const OptTensor& dev, int64_t all, const bc::View& 
 
 int sm_count(int dev) { return at::cuda::getDeviceProperties(dev)->multiProcessorCount; }
 
-// Up to this many rows of one K/V head run on the kernel that streams the cache through registers.
+// Up to this many rows of one K/V head run on the kernel that streams the cache through registers, 16 of them a
+// pass: 168 heads x 10,000 keys take 84 us with 16 rows, 119 with 32 and 147 with 33, where the kernel for many rows
+// takes 147 with any number up to 64; 21 x 6001 keys of 56: 22 for 29, and 27 with 33.  Few heads with a long
+// context, which that one splits over all SMs, meet earlier (2 x 100,003 keys of 64: 33 for 35 with 16 rows, 43 for
+// 35 with 32).
 constexpr int64_t kFewRows = 32;
 
 // Splits of the keys of each cell for few rows, joined in clusters of up to 8.  A CTA's time goes with its

@@ -480,8 +480,8 @@ class FeaturesTransformer(nn.Module):
         vector, or (``"block_int8"``, ``"block_fp8"``: the native path only) int8 / e4m3 with a
         scale for each 64 rows and head, which the query attention reads directly.  ``placement``: ``"resident"``
         (device), ``"offload"`` (pinned host, one layer copied in at a time) or
-        ``"stream"`` (pinned host in blocks of ``stream_block_rows`` context rows, the
-        query attention merging block partials) - the native path only."""
+        ``"stream"`` (pinned host in blocks of ``stream_block_rows`` context rows, of whole 128s for the
+        block types, the query attention merging block partials) - the native path only."""
         if not self.supports_context_cache:
             raise NotImplementedError("context caching is not implemented for the two-phase encoder")
         if cache_dtype not in ("bf16", "int8", "block_int8", "block_fp8"):
