@@ -483,7 +483,7 @@ struct Joined {
 template <bool MANY>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int tile_rows, int parts) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int failed = read_status(a.status);
+  const bool written = read_status(a.status) == 0;  // (the parts may never have been, after a wait that ran out)
   const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
   const uint32_t unit = MANY ? blockIdx.x : blockIdx.x * kJoinRows + group;  // rows of the cells that are split
   const uint32_t count = static_cast<uint32_t>(a.rows - a.first), tiles = (count + tile_rows - 1) / tile_rows;
@@ -540,7 +540,6 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
       fma4(j.acc, sm_o[w][lane], h * h);
     }
   }
-  if (failed != 0) return;  // a wait has run out: the parts may never have been written
   const int b = static_cast<int>(bh / a.c.heads), h = static_cast<int>(bh % a.c.heads);
   const Row row(a, h, a.first + r);
   const float norm = j.sum != 0.f ? 1.f / j.sum : 0.f;
@@ -548,8 +547,8 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(Attention a, int 
   const float y[4] = {j.acc.x * norm, j.acc.y * norm, j.acc.z * norm, j.acc.w * norm};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (4 * lane + i < a.c.width) put(a.o.p, out + i, y[i], a.type);
-  if (lane == 0 && a.lse != nullptr)
+    if (written && 4 * lane + i < a.c.width) put(a.o.p, out + i, y[i], a.type);
+  if (written && lane == 0 && a.lse != nullptr)
     a.lse[(static_cast<int64_t>(b) * a.c.heads * a.group + row.head) * a.n + row.n] = row_lse(j.top, j.sum);
 }
 

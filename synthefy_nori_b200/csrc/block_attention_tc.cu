@@ -584,9 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (warp == 4) {
-          float top = left > 0 ? sv : 0.f;  // of the tile's four chunks (fmaxf passes over a NaN)
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          raise_floor(least, fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
+          const float there = left > 0 ? sv : 0.f;  // (the other chunk of a group is the next lane's)
+          raise_floor(least, fmaxf(there, __shfl_xor_sync(0xffffffffu, there, 1)));
           const float svc = safe_scale(sv, least);
           // (a block behind the last row counts for nothing, whatever its scale)
           const float4 y = left > 0 ? make_float4(sk, __log2f(svc), __fdividef(1.f, svc), 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -656,19 +655,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float f0 = fac * sc.x, f = f0 < 1e-38f ? 1e-38f : f0;  // (never 0: a masked key's -inf stays -inf)
           tmem_wait_ld();
           const float cand = fmaf(max32(x), f, sc.y);
-          float back = 1.f;
+          float h = 1.f;  // its square rescales the sums (lowered())
           bool grow = false;
           if (step == 0) {
             m = cand;
           } else if (cand > m + kLazy) {
-            const float h = exp2_mufu(0.5f * (m - cand));
-            back = h * h;
-            l = lowered(l, h);
+            h = exp2_mufu(0.5f * (m - cand));
+            l *= h;
             m = cand;
             grow = true;
           }
           const float lift = m == -INFINITY ? 0.f : kLift - m;  // (no key of this half is there)
-          l = fmaf(weights32(x, f, sc.y + lift, tC), sc.z, l);
+          l = fmaf(weights32(x, f, sc.y + lift, tC), sc.z, l * h);
           if (__any_sync(0xffffffffu, grow)) {
             // the other chunk's product may still be under way: its next scores, if there are any, come behind it
             const bool last = step == 2 * tiles - 1;
@@ -682,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_ld16(tO + q * 16, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * back);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * (h * h));
               tmem_st16(tO + q * 16, o);
             }
           }
