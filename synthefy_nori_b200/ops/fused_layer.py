@@ -857,7 +857,9 @@ class BlockKV:
     def attend(self, q: torch.Tensor, o: torch.Tensor, g: Geometry, mult: float, return_lse: bool = False):
         """``q``, ``o`` [B * nq * T, A] token-major; the log-sum-exp [B * T * H, nq] where it is wanted."""
         qv, ov = (t.view(g.B, g.nq, g.T, g.H, g.Dp).permute(0, 2, 1, 3, 4) for t in (q, o))
-        r = ops.block_cache_attention(qv, self.cache, g.ep, scale=mult / math.sqrt(g.D), out=ov, return_lse=return_lse)
+        # (a temperature of 0 makes all keys equal, as so small a scale does; the operator takes positive ones)
+        scale = max(mult / math.sqrt(g.D), 1e-30)
+        r = ops.block_cache_attention(qv, self.cache, g.ep, scale=scale, out=ov, return_lse=return_lse)
         return r[1].view(-1, g.nq) if return_lse else None
 
     def rows(self, r0: int, r1: int) -> "BlockKV":
