@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) few_kernel(Attention a
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][kt], af, qf[nt][2 * j + 1][0], qf[nt][2 * j + 1][1]);
       }
+    // (approximate: 2^-22 of a log2 that reaches -49 is 1e-5 of a weight, 1 / 30 of its rounding to fp16)
     const float lv = log2_fast(svc), inv = rcp_fast(svc);
     if (left < kPiece) {
 #pragma unroll

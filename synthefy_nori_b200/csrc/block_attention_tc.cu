@@ -587,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float there = left > 0 ? sv : 0.f;  // (the other chunk of a group is the next lane's)
           raise_floor(least, fmaxf(there, __shfl_xor_sync(0xffffffffu, there, 1)));
           const float svc = safe_scale(sv, least);
-          // (a block behind the last row counts for nothing, whatever its scale)
+          // (a block behind the last row counts for nothing, whatever its scale; log2 and reciprocal approximate, 1e-5 of
+          // a weight at most: 1 / 30 of its rounding to fp16)
           const float4 y = left > 0 ? make_float4(sk, __log2f(svc), __fdividef(1.f, svc), 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
           if (lane < 4) scales[n & 3][lane] = y;
           if (j + 1 < tiles) sk = __ldg(ks += kN >> a.c.block_log2), sv = __ldg(vs += kN >> a.c.block_log2);

@@ -131,7 +131,8 @@ def block_cache_attention(q: torch.Tensor, cache: BlockCache, lengths, *, scale:
     Sums, maxima and results are held in fp32; weights are rounded to fp16 for the product with V, relative to the
     largest weight times its block's scale of V (11 bits down to 2^-21 of that, 2^-32 of it below).  A block's scale of V counts as
     2^-80 and as 2^-100 of the largest at least: the result is off by 2^-100 of the largest value of V at most, the
-    log-sum-exp not at all."""
+    log-sum-exp not at all.  Where keys are split over SMs, partial results take up to 160 MB while a call runs.
+    After a wait on the device has run out (``ops.check_status`` raises) rows may not have been written."""
     k = cache.k
     if not k.is_cuda or not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("block_cache_attention: q and the cache must be CUDA tensors")
