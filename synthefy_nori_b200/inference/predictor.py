@@ -135,7 +135,7 @@ class NoriPredictor:
         if self.device.type == "cuda":
             from synthefy_nori_b200 import ops
 
-            ops.check_status(self.device)
+            ops.check_status(self.taus.device)  # (self.device may be "cuda" without a number)
 
     # ------------------------------------------------------------------ context
     def _members(self) -> list[MemberPipeline]:
